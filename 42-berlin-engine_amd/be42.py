@@ -33,6 +33,12 @@ SIGNATURES = {
     "be42_quant_rows_fp8": (i32, [vp, vp, vp, i32, i32, vp]),
     "be42_dequant_rows_int8": (i32, [vp, vp, vp, i32, i32, vp]),
     "be42_fp8_decode": (i32, [vp, vp, sz, vp]),
+    "be42_norm_quant_rows_int8": (i32, [vp, vp, vp, vp, i32, vp, i32, i32, vp, i32, i32, f32, vp]),
+    "be42_norm_quant_rows_fp8": (i32, [vp, vp, vp, vp, i32, vp, i32, i32, vp, i32, i32, f32, vp]),
+    "be42_prefix_attention_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32]),
+    "be42_prefix_attention": (i32, [vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, i32, f32, vp, vp, sz, vp]),
+    "be42_logprobs_workspace_bytes": (sz, [i32, i32, i32]),
+    "be42_logprobs": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, i32, f32, vp, i32, i32, vp, sz, vp]),
     "be42_gemv_q8": (i32, [vp, vp, vp, vp, i32, i32, i32, vp]),
     "be42_gemv_fp8": (i32, [vp, vp, vp, vp, i32, i32, i32, vp]),
     "be42_gemv_xdig_bytes": (sz, [i32, i32, i32]),
@@ -181,6 +187,39 @@ class Lib:
         self.init()
         self.check(getattr(self.lib, name)(*args), name)
 
+    def _device_call(self, dev, name, *args):
+        """_call on device `dev` (that of the call's tensors) and its current
+        stream, which is the call's last argument."""
+        t = self.torch
+        if dev.type != "cuda":
+            raise Be42Error(f"{name}: tensors on {dev}, not on a GPU")
+        if dev.index == t.cuda.current_device():
+            return self._call(name, *args, self.stream())
+        with t.cuda.device(dev):
+            self._call(name, *args, self.stream())
+
+    @staticmethod
+    def _want(name, what, x, dtypes, shape=None, dev=None):
+        """x has one of `dtypes`, that shape (None: any size) and lies dense on
+        the device of the call."""
+        if x.dtype not in dtypes:
+            raise Be42Error(f"{name}: {what} is {x.dtype}")
+        if dev is not None and x.device != dev:
+            raise Be42Error(f"{name}: {what} is on {x.device}, not on {dev}")
+        if shape is not None and (x.dim() != len(shape) or any(w is not None and w != n for w, n in zip(shape, x.shape))):
+            raise Be42Error(f"{name}: {what} has shape {tuple(x.shape)}")
+        if not x.is_contiguous():
+            raise Be42Error(f"{name}: {what} is not contiguous")
+
+    def _rows(self, name, what, x, dtypes, cols=None, dev=None):
+        """Element stride of the rows of a 2-d tensor whose rows are dense."""
+        if x.dim() != 2 or x.dtype not in dtypes or (cols is not None and x.shape[1] != cols) or \
+                (dev is not None and x.device != dev):
+            raise Be42Error(f"{name}: {what} is {x.dtype} {tuple(x.shape)} on {x.device}")
+        if x.shape[1] > 1 and x.stride(1) != 1:
+            raise Be42Error(f"{name}: {what} has rows that are not dense")
+        return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
     # -- quant codecs ---------------------------------------------------------
     def quant_rows_int8(self, x):
         t = self.torch
@@ -197,6 +236,34 @@ class Lib:
         s = t.empty(rows, dtype=t.float32, device=x.device)
         self._call("be42_quant_rows_fp8", self.p(q), self.p(s), self.p(x), rows, cols, self.stream())
         return q, s
+
+    def norm_quant_rows(self, x, w, eps, kind, residual=None, sum=None):
+        """Residual addition + RMS norm + row codes: x (and residual) [rows][cols]
+        float32 or bfloat16, w [cols] bfloat16 -> (codes [rows][cols] int8 or,
+        kind "fp8", uint8 E4M3, scales [rows], x + residual).  Rows may be
+        strided.  sum: where the new stream goes (x or residual itself to
+        replace it); by default a new tensor with a residual, none without."""
+        t, name = self.torch, "be42_norm_quant_rows_" + kind
+        if kind not in ("int8", "fp8"):
+            raise Be42Error(f"norm_quant_rows: kind {kind!r}")
+        dev, dt = x.device, x.dtype
+        xs = self._rows(name, "x", x, (t.float32, t.bfloat16))
+        rows, cols = x.shape
+        rs = cols
+        if residual is not None:
+            rs = self._rows(name, "residual", residual, (dt,), cols, dev)
+            if residual.shape[0] != rows:
+                raise Be42Error(f"{name}: residual has {residual.shape[0]} rows, x {rows}")
+            if sum is None:
+                sum = t.empty((rows, cols), dtype=dt, device=dev)
+        if sum is not None:
+            self._want(name, "sum", sum, (dt,), (rows, cols), dev)
+        self._want(name, "w", w, (t.bfloat16,), (cols,), dev)
+        q = t.empty((rows, cols), dtype=t.int8 if kind == "int8" else t.uint8, device=dev)
+        s = t.empty(rows, dtype=t.float32, device=dev)
+        self._device_call(dev, name, self.p(q), self.p(s), self.p(sum), self.p(x), xs, self.p(residual), rs,
+                          int(dt == t.bfloat16), self.p(w), rows, cols, float(eps))
+        return q, s, sum
 
     def dequant_rows_int8(self, q, s):
         t = self.torch
@@ -336,6 +403,34 @@ class Lib:
                    float(temp), float(top_p), self.p(u), self.stream())
         return out
 
+    def logprobs(self, logits, tokens=None, temp=1.0, top_k=0, entropy=False, workspace=None):
+        """Of logits [rows][n] (float32 or bfloat16, rows may be strided): a dict
+        of "logprobs" [rows][j] for the given tokens [rows][j] (int32), "entropy"
+        [rows], "top_ids" and "top_logprobs" [rows][top_k], as far as asked for."""
+        t, name = self.torch, "be42_logprobs"
+        dev = logits.device
+        ls = self._rows(name, "logits", logits, (t.float32, t.bfloat16))
+        rows, n = logits.shape
+        got, given = {}, 0
+        if tokens is not None:
+            self._want(name, "tokens", tokens, (t.int32,), (rows, None), dev)
+            given = tokens.shape[1]
+            got["logprobs"] = t.empty((rows, given), dtype=t.float32, device=dev)
+        if entropy:
+            got["entropy"] = t.empty(rows, dtype=t.float32, device=dev)
+        if top_k:
+            got["top_ids"] = t.empty((rows, top_k), dtype=t.int32, device=dev)
+            got["top_logprobs"] = t.empty((rows, top_k), dtype=t.float32, device=dev)
+        ws, wsb = None, 0
+        if workspace is not None:
+            self._want(name, "workspace", workspace, (t.uint8,), (None,), dev)
+            ws, wsb = self.p(workspace), workspace.numel()
+        self._device_call(dev, name, self.p(got.get("logprobs")), self.p(got.get("entropy")),
+                          self.p(got.get("top_ids")), self.p(got.get("top_logprobs")), self.p(logits),
+                          int(logits.dtype == t.bfloat16), ls, n, rows, float(temp), self.p(tokens), given, int(top_k),
+                          ws, wsb)
+        return got
+
     def kv_pool(self, kind, n_layers, n_kv, head_dim, max_logical, hpT=None):
         return KVPool(self, kind, n_layers, n_kv, head_dim, max_logical, hpT)
 
@@ -374,6 +469,38 @@ class Lib:
         ws, wsb = (self.p(workspace), workspace.numel()) if workspace is not None else (None, 0)
         self._call("be42_paged_attention", pool.handle, self.p(q), B, H, self.p(sel), self.p(nsel),
                    sel.shape[1], max_sel, float(scale), self.p(out), n_split, ws, wsb, self.stream())
+        return out
+
+    def prefix_attention(self, pool, q, prefix_slot, prefix_len, scale, slots=None, lens=None, max_len=None, out=None,
+                         workspace=None):
+        """Attention of queries q [n][n_heads][head_dim] (float32 or bfloat16,
+        queries may be strided) over the first prefix_len tokens of slot
+        prefix_slot, read once for all, and the first lens[b] tokens of slot
+        slots[b] (None: slot b / all its tokens).  max_len bounds lens (None:
+        what a slot can hold; the closer, the better the work is split)."""
+        t, name = self.torch, "be42_prefix_attention"
+        if q.dim() != 3 or q.shape[2] != pool.head_dim or q.dtype not in (t.float32, t.bfloat16):
+            raise Be42Error(f"{name}: q is {q.dtype} {tuple(q.shape)}")
+        B, H, hd = q.shape
+        if B and ((hd > 1 and q.stride(2) != 1) or (H > 1 and q.stride(1) != hd)):
+            raise Be42Error(f"{name}: q has rows that are not dense")
+        qs = q.stride(0) if B > 1 else H * hd
+        for what, x in (("slots", slots), ("lens", lens)):
+            if x is not None:
+                self._want(name, what, x, (t.int32,), (B,), q.device)
+        if out is None:
+            out = t.empty((B, H, hd), dtype=q.dtype, device=q.device)
+        else:
+            self._want(name, "out", out, (q.dtype,), (B, H, hd), q.device)
+        if max_len is None:
+            max_len = pool.max_logical * 16
+        ws, wsb = None, 0
+        if workspace is not None:
+            self._want(name, "workspace", workspace, (t.uint8,), (None,), q.device)
+            ws, wsb = self.p(workspace), workspace.numel()
+        self._device_call(q.device, name, pool.handle, self.p(q), int(q.dtype == t.bfloat16), qs, B, H,
+                          int(prefix_slot), int(prefix_len), self.p(slots), self.p(lens), int(max_len), float(scale),
+                          self.p(out), ws, wsb)
         return out
 
     # -- linear KV cache [T][n_kv][head_dim] bf16 (kv_cache.c) ------------------

@@ -174,6 +174,111 @@ static bool launch_quant_vec(uint8_t *q, float *scales, const float *x, int rows
     return true;
 }
 
+// ---- residual + RMS norm + codes -----------------------------------------------
+// h = x + residual in the stream's type, y = fp32(h / sqrt(mean h^2 + eps) * w)
+// and the codec's code of y.  The sum of squares and the product are formed in
+// 64 bits and rounded once to fp32, so y, and with it every code, is the same
+// for any split of the row over threads.
+
+// element i of a row of the residual stream (fp32 or bf16) as fp32
+template <bool BF16>
+__device__ __forceinline__ float act_load(const void *p, size_t i)
+{
+    return BF16 ? bf16_to_f32(((const uint16_t *)p)[i]) : ((const float *)p)[i];
+}
+
+template <bool BF16>
+__device__ __forceinline__ void act_store(void *p, size_t i, float v)
+{
+    if (BF16)
+        ((uint16_t *)p)[i] = f32_to_bf16(v);
+    else
+        ((float *)p)[i] = v;
+}
+
+// x + r as the stream holds it
+template <bool BF16>
+__device__ __forceinline__ float act_add(float x, float r)
+{
+    return BF16 ? bf16_to_f32(f32_to_bf16(x + r)) : x + r;
+}
+
+__device__ __forceinline__ double wave_sum_d(double v)
+{
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+        v += __shfl_xor(v, o, kWave);
+    return v;
+}
+
+__device__ __forceinline__ float norm_value(float h, double r, uint16_t w)
+{
+    return (float)((double)h * r * (double)bf16_to_f32(w));
+}
+
+// Any row: three passes over it, one element a thread.
+template <bool FP8, bool BF16>
+__global__ __launch_bounds__(256) void k_norm_quant_rows(uint8_t *q, float *scales, void *sum, const void *x,
+                                                         size_t x_stride, const void *res, size_t res_stride,
+                                                         const uint16_t *w, int cols, float eps)
+{
+    __shared__ double redd[4];
+    __shared__ float red[4];
+    const size_t row = blockIdx.x;
+    auto load = [&](int i) {
+        const float v = act_load<BF16>(x, row * x_stride + i);
+        return res ? act_add<BF16>(v, act_load<BF16>(res, row * res_stride + i)) : v;
+    };
+    // after the first pass the new stream is read where it was written (it may
+    // have replaced x or the residual)
+    auto again = [&](int i) { return sum ? act_load<BF16>(sum, row * cols + i) : load(i); };
+    double ss = 0.0;
+    for (int i = threadIdx.x; i < cols; i += 256) {
+        const float h = load(i);
+        if (sum)
+            act_store<BF16>(sum, row * cols + i, h);
+        ss = fma((double)h, (double)h, ss);
+    }
+    ss = wave_sum_d(ss);
+    if ((threadIdx.x & 63) == 0)
+        redd[threadIdx.x >> 6] = ss;
+    __syncthreads();
+    const double r = 1.0 / sqrt(((redd[0] + redd[1]) + (redd[2] + redd[3])) / cols + (double)eps);
+    float m = 0.0f;
+    for (int i = threadIdx.x; i < cols; i += 256)
+        m = fmaxf(m, fabsf(norm_value(again(i), r, w[i])));
+    m = wave_max(m);
+    if ((threadIdx.x & 63) == 0)
+        red[threadIdx.x >> 6] = m;
+    __syncthreads();
+    const float amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    float scale = 1.0f, inv = 1.0f;
+    if (amax > 0.0f) {
+        scale = amax / (FP8 ? 224.0f : 127.0f);
+        inv = FP8 ? 1.0f / scale : 127.0f / amax;
+    }
+    if (threadIdx.x == 0)
+        scales[row] = scale;
+    for (int i = threadIdx.x; i < cols; i += 256) {
+        const float y = norm_value(again(i), r, w[i]);
+        q[row * cols + i] = FP8 ? f32_to_fp8(y * inv) : (uint8_t)f32_to_int8(y, inv);
+    }
+}
+
+template <bool FP8>
+static void launch_norm_quant(uint8_t *q, float *scales, void *sum, const void *x, size_t x_stride, const void *res,
+                              size_t res_stride, bool bf16, const uint16_t *w, int rows, int cols, float eps,
+                              hipStream_t s)
+{
+    const dim3 g(rows), b(256);
+    if (bf16)
+        hipLaunchKernelGGL((k_norm_quant_rows<FP8, true>), g, b, 0, s, q, scales, sum, x, x_stride, res, res_stride,
+                           w, cols, eps);
+    else
+        hipLaunchKernelGGL((k_norm_quant_rows<FP8, false>), g, b, 0, s, q, scales, sum, x, x_stride, res, res_stride,
+                           w, cols, eps);
+}
+
 __global__ void k_dequant_rows_int8(float *out, const int8_t *q, const float *scales, int cols,
                                     size_t total)
 {
@@ -263,6 +368,53 @@ extern "C" int be42_quant_rows_fp8(uint8_t *q, float *scales, const float *x, in
         hipLaunchKernelGGL(k_quant_rows_fp8, dim3(rows), dim3(256), 0, as_stream(stream), q, scales, x, cols);
     BE42_LAUNCH_CHECK();
     return BE42_OK;
+}
+
+static int norm_quant_rows(const char *name, bool fp8, uint8_t *q, float *scales, void *sum, const void *x,
+                           int x_stride, const void *residual, int residual_stride, int act_bf16, const uint16_t *w,
+                           int rows, int cols, float eps, void *stream)
+{
+    BE42_CHECK(rows >= 0 && cols > 0, "%s: bad shape %d x %d", name, rows, cols);
+    BE42_CHECK(x_stride >= cols && (!residual || residual_stride >= cols), "%s: rows of %d at strides %d, %d", name,
+               cols, x_stride, residual_stride);
+    BE42_CHECK(eps >= 0.0f, "%s: eps %g", name, (double)eps);
+    if (rows == 0)
+        return BE42_OK;
+    BE42_CHECK(q && scales && x && w, "%s: null pointer", name);
+    // a row is written where it was read only if both lie at the same place
+    BE42_CHECK(!sum || ((sum != x || x_stride == cols) && (sum != residual || residual_stride == cols)),
+               "%s: sum replaces rows that are not contiguous", name);
+    const uintptr_t unit = act_bf16 ? 1 : 3;
+    BE42_CHECK(!(((uintptr_t)x | (uintptr_t)residual | (uintptr_t)sum) & unit) && !((uintptr_t)w & 1) &&
+                   !((uintptr_t)scales & 3), "%s: unaligned pointer", name);
+    if (fp8) {
+        const int rc = ensure_thresholds();
+        if (rc)
+            return rc;
+        launch_norm_quant<true>(q, scales, sum, x, x_stride, residual, residual_stride, act_bf16 != 0, w, rows, cols,
+                                eps, as_stream(stream));
+    } else {
+        launch_norm_quant<false>(q, scales, sum, x, x_stride, residual, residual_stride, act_bf16 != 0, w, rows, cols,
+                                 eps, as_stream(stream));
+    }
+    BE42_LAUNCH_CHECK();
+    return BE42_OK;
+}
+
+extern "C" int be42_norm_quant_rows_int8(int8_t *q, float *scales, void *sum, const void *x, int x_stride,
+                                         const void *residual, int residual_stride, int act_bf16, const uint16_t *w,
+                                         int rows, int cols, float eps, void *stream)
+{
+    return norm_quant_rows("be42_norm_quant_rows_int8", false, (uint8_t *)q, scales, sum, x, x_stride, residual,
+                           residual_stride, act_bf16, w, rows, cols, eps, stream);
+}
+
+extern "C" int be42_norm_quant_rows_fp8(uint8_t *q, float *scales, void *sum, const void *x, int x_stride,
+                                        const void *residual, int residual_stride, int act_bf16, const uint16_t *w,
+                                        int rows, int cols, float eps, void *stream)
+{
+    return norm_quant_rows("be42_norm_quant_rows_fp8", true, q, scales, sum, x, x_stride, residual, residual_stride,
+                           act_bf16, w, rows, cols, eps, stream);
 }
 
 extern "C" int be42_dequant_rows_int8(float *out, const int8_t *q, const float *scales, int rows,

@@ -54,6 +54,24 @@ int         be42_memset(void *dst, int value, size_t bytes, void *stream);
  * Codes and scales are bit-identical to the reference. */
 int be42_quant_rows_int8(int8_t *q, float *scales, const float *x, int rows, int cols, void *stream);
 int be42_quant_rows_fp8(uint8_t *q, float *scales, const float *x, int rows, int cols, void *stream);
+/* Residual addition + RMS norm + row codes: the step before a per-token-quantized
+ * product (be42_gemm_i8 / be42_gemm_fp8).  For each of `rows` rows of `cols`:
+ *   h = x + residual (h = x without one), in the rows' type;
+ *   y = fp32(h / sqrt(mean(h^2) + eps) * w), formed in 64 bits and rounded once;
+ *   (q, scales) = the codes and the scale that be42_quant_rows_int8 / _fp8 give
+ *   for y, bit for bit.
+ * x and residual are fp32, or bf16 with act_bf16 (the sum is then rounded to bf16
+ * before the norm reads it); row r begins at element r * x_stride / r *
+ * residual_stride.  sum (may be NULL) takes h, [rows][cols] in the rows' type;
+ * it may be x or residual itself where that one's rows are contiguous, and
+ * overlaps neither otherwise.  w: [cols] bf16.  A row whose h holds an infinity
+ * or a NaN gets unspecified codes; other rows are not touched by it. */
+int be42_norm_quant_rows_int8(int8_t *q, float *scales, void *sum, const void *x, int x_stride,
+                              const void *residual, int residual_stride, int act_bf16, const uint16_t *w, int rows,
+                              int cols, float eps, void *stream);
+int be42_norm_quant_rows_fp8(uint8_t *q, float *scales, void *sum, const void *x, int x_stride,
+                             const void *residual, int residual_stride, int act_bf16, const uint16_t *w, int rows,
+                             int cols, float eps, void *stream);
 /* (float)q * scale[row], dequant_int8_to_f32_avx2 (ops_quant.c:275-305) row-wise */
 int be42_dequant_rows_int8(float *out, const int8_t *q, const float *scales, int rows, int cols,
                            void *stream);
@@ -250,6 +268,33 @@ int  be42_lsh_attention(const be42_kv_pool *pool, const float *q, const int *slo
  * word it reads is the device's, shared by every stream, and is cleared. */
 int  be42_lsh_attention_status(void *stream);
 
+/* Attention of a batch that shares a prefix: query b [n_heads][head_dim] (row b
+ * at element b * q_stride of q) attends to the first prefix_len tokens of slot
+ * prefix_slot, which are read once for all queries, and to the first lens[b]
+ * tokens of its own slot slots[b] (slots NULL: slot b; lens NULL: every token the
+ * slot holds).  Several queries may name one slot with different lens: tokens of
+ * one continuation, each seeing the cache as of its own position.  Slots are the
+ * pool's page tables (be42_kv_append); query head h reads KV head
+ * h / (n_heads / n_kv), any group size; head_dim 64 or 128; INT8 or bf16 pages.
+ *   out[b][h] = sum_t softmax_t(scale * q[b][h] . k_t) v_t
+ * with the exact exponential (not fast_expf as be42_paged_attention); a query
+ * that sees no token gets zeros.  q and out are fp32, or both bf16 with q_bf16;
+ * out is [n_queries][n_heads][head_dim].  K, V (as the pages hold them) and fp32
+ * queries and weights enter the products with their full precision; bf16 queries
+ * are used as they are.
+ * max_len bounds lens: own tokens from max_len on are not seen.  prefix_len,
+ * lens and a slot's pages are cut at the tokens the slot holds, and a slot
+ * outside the pool holds none.  The launch depends on prefix_len and max_len
+ * alone, so slots and lens may change between replays of a captured graph.
+ * workspace NULL: the library's (grow-only), else a device buffer of
+ * be42_prefix_attention_workspace_bytes() bytes, 16-byte aligned. */
+size_t be42_prefix_attention_workspace_bytes(int n_queries, int n_heads, int n_kv, int head_dim, int prefix_len,
+                                             int max_len);
+int    be42_prefix_attention(const be42_kv_pool *pool, const void *q, int q_bf16, int q_stride, int n_queries,
+                             int n_heads, int prefix_slot, int prefix_len, const int *slots, const int *lens,
+                             int max_len, float scale, void *out, void *workspace, size_t workspace_bytes,
+                             void *stream);
+
 /* ---- linear (non-paged) bf16 KV cache -----------------------------------------------
  * The cache layout of kv_cache.h:19-27: rows [T][n_kv][head_dim] bf16.
  *   be42_kv_linear_append: row `pos` of K and V from fp32 [row] (float_to_bf16,
@@ -399,6 +444,26 @@ int be42_sample_temperature_dt(int *out, const void *logits, int logits_bf16, in
                                const float *r, void *stream);
 int be42_sample_top_p_dt(int *out, const void *logits, int logits_bf16, int n, int batch, float temp, float top_p,
                          const float *u, void *stream);
+
+/* ---- log probabilities ---------------------------------------------------------
+ * For `rows` rows of n logits (fp32, or bf16 with logits_bf16; row r begins at
+ * element r * row_stride) and z = (x - max) / temp, log s = log(sum exp(z)):
+ *   logprobs[r][j] = z[tokens[r][j]] - log s for the n_tokens given tokens of the
+ *     row (device [rows][n_tokens]; an id outside [0, n) gets -infinity);
+ *   entropy[r] = -sum p log p (may be NULL);
+ *   top_ids / top_logprobs [r][0 .. top_k): the top_k <= 64 (and <= n) largest
+ *     logits in descending order, equal ones (and +0, -0) in ascending id order,
+ *     and their log probabilities.
+ * Logits of -infinity are tokens of probability zero.  A row without a
+ * distribution (it holds a NaN or +infinity, or nothing but -infinity) gets NaN
+ * log probabilities and entropy; its top_ids take a NaN for -infinity.
+ * n_tokens and top_k may be 0 (their arrays are then not used).
+ * workspace NULL: the library's (grow-only), else a device buffer of
+ * be42_logprobs_workspace_bytes() bytes, 16-byte aligned. */
+size_t be42_logprobs_workspace_bytes(int n, int rows, int top_k);
+int    be42_logprobs(float *logprobs, float *entropy, int *top_ids, float *top_logprobs, const void *logits,
+                     int logits_bf16, int row_stride, int n, int rows, float temp, const int *tokens, int n_tokens,
+                     int top_k, void *workspace, size_t workspace_bytes, void *stream);
 
 /* ---- checkpoints --------------------------------------------------------------
  * A decoder from a safetensors checkpoint and an HF config.json: load_config

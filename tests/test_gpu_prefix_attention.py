@@ -1,0 +1,299 @@
+"""Attention behind a shared prefix (be42_prefix_attention) against float64 over
+the pages' own values.
+
+Tolerance: a score is a sum of hd products of exact factors in fp32 (three
+products of parts for an fp32 query), so its error d is at most
+hd * 2^-22 * scale * max_t sum_i |q_i k_ti| / sqrt(hd) in norm terms (random
+signs; 16 of those standard deviations), plus 2^-22 of the score itself in the
+exponential's argument; weights then are off by d relatively, the output by
+2 d max|v|, and by 2^-20 max|v| for the sums.  bf16 queries add the rounding
+of the weights and of the output, 2^-8 max|v| each."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+PAGE = 16
+
+
+def make_pool(be, kind, n_slots, kvh, hd, held, seed, order=None):
+    """A pool whose slot s holds held[s] tokens; slots are filled a page at a
+    time in turn, so that their pages interleave.  -> (pool, k, v): the values
+    the pages hold, per slot [tokens][kvh][hd] float64."""
+    import be42
+    rng = np.random.default_rng(seed)
+    pool = be.kv_pool(be42.KV_BF16 if kind == "bf16" else be42.KV_INT8, n_slots, kvh, hd, max(1, -(-max(held) // PAGE)) + 1)
+    k = [rng.standard_normal((n, kvh, hd)).astype(np.float32) for n in held]
+    v = [rng.standard_normal((n, kvh, hd)).astype(np.float32) for n in held]
+    dk, dv = [torch.from_numpy(a).cuda() for a in k], [torch.from_numpy(a).cuda() for a in v]
+    step = 3 * PAGE
+    for at in range(0, max(held), step):
+        for s, n in enumerate(held):
+            if at < n:
+                m = min(step, n - at)
+                pool.append(s, dk[s][at:at + m].reshape(m, -1), dv[s][at:at + m].reshape(m, -1), at)
+
+    def stored(a):
+        if kind == "bf16":
+            return torch.from_numpy(a).bfloat16().double().numpy()
+        amax = np.abs(a).max(-1, keepdims=True)
+        sc, inv = (amax / np.float32(127)).astype(np.float32), (np.float32(127) / amax).astype(np.float32)
+        x = a * inv
+        return np.trunc(x + np.copysign(np.float32(0.5), x)).clip(-127, 127).astype(np.float64) * sc
+
+    return pool, [stored(a) for a in k], [stored(a) for a in v]
+
+
+def reference(q, k, v, n_heads, scale, prefix_slot, prefix_len, slots, lens, max_len):
+    """float64 out [B][H][hd] and the tolerance of each query and head."""
+    B, H, hd = q.shape
+    out, tol = np.zeros((B, H, hd)), np.zeros((B, H))
+    for b in range(B):
+        own = slots[b]
+        n = min(lens[b], max_len)
+        n = min(n, len(k[own])) if 0 <= own < len(k) else 0
+        p = min(prefix_len, len(k[prefix_slot]))
+        kk = np.concatenate([k[prefix_slot][:p]] + ([k[own][:n]] if n > 0 else []))
+        vv = np.concatenate([v[prefix_slot][:p]] + ([v[own][:n]] if n > 0 else []))
+        if not len(kk):
+            continue
+        g = H // kk.shape[1]
+        for h in range(H):
+            K, V = kk[:, h // g], vv[:, h // g]
+            s = K @ q[b, h] * scale
+            w = np.exp(s - s.max())
+            out[b, h] = (w / w.sum()) @ V
+            d = hd * 2.0 ** -22 * abs(scale) * (np.abs(K) @ np.abs(q[b, h])).max() / math.sqrt(hd) + 2.0 ** -22 * np.abs(s).max()
+            tol[b, h] = (2 * d + 2.0 ** -20) * np.abs(V).max()
+    return out, tol, [np.abs(np.concatenate([a.reshape(-1) for a in v] + [np.zeros(1)])).max()]
+
+
+def run(be, pool, q, k, v, prefix_slot, prefix_len, slots, lens, max_len, scale=None, give_slots=True, give_lens=True,
+        q_dev=None, **kw):
+    B, H, hd = q.shape
+    scale = 1.0 / math.sqrt(hd) if scale is None else scale
+    bf16 = q.dtype == torch.bfloat16
+    st = torch.tensor(list(slots), dtype=torch.int32, device="cuda") if give_slots else None
+    lt = torch.tensor(list(lens), dtype=torch.int32, device="cuda") if give_lens else None
+    got = be.prefix_attention(pool, q.cuda() if q_dev is None else q_dev, prefix_slot, prefix_len, scale, slots=st,
+                              lens=lt, max_len=max_len, **kw)
+    assert got.dtype == q.dtype and got.shape == q.shape
+    want, tol, vmax = reference(q.double().numpy(), k, v, H, scale, prefix_slot, prefix_len, slots, lens, max_len)
+    tol = tol + (2.0 ** -7 * vmax[0] if bf16 else 0.0)
+    off = np.abs(got.cpu().double().numpy() - want).max(-1)
+    assert np.isfinite(got.float().cpu().numpy()).all()
+    assert (off <= tol).all(), (np.unravel_index((off - tol).argmax(), off.shape), off.max(), tol.min())
+    return got
+
+
+def queries(seed, B, H, hd, bf16):
+    q = torch.randn(B, H, hd, generator=torch.Generator().manual_seed(seed))
+    return q.bfloat16() if bf16 else q
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("heads,kvh,hd", [(8, 8, 64), (6, 2, 128), (4, 1, 64), (20, 1, 128), (3, 3, 128), (72, 2, 64)])
+def test_heads(be, kind, bf16, heads, kvh, hd):
+    held = [0, 5, 40, 100, 333]
+    pool, k, v = make_pool(be, kind, 5, kvh, hd, held, 1)
+    run(be, pool, queries(2, 4, heads, hd, bf16), k, v, 4, 333, [0, 1, 2, 3], [0, 5, 40, 100], 100)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("prefix", [0, 1, 15, 16, 17, 31, 32, 33, 47, 64, 100, 127, 128, 129, 500, 1000, 2049, 5003])
+def test_prefix_lengths(be, kind, prefix):
+    held = [17, 1, 0, max(prefix, 1)]
+    pool, k, v = make_pool(be, kind, 4, 2, 128, held, 3 + prefix)
+    run(be, pool, queries(4, 3, 8, 128, False), k, v, 3, prefix, [0, 1, 2], [17, 1, 0], 17)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("own", [0, 1, 15, 16, 17, 32, 33, 63, 64, 65, 130, 700, 1500])
+def test_own_lengths(be, kind, own):
+    """No prefix, a short one; a query that sees less than its slot holds."""
+    held = [max(own, 1), 20, 50]
+    pool, k, v = make_pool(be, kind, 3, 2, 64, held, 5 + own)
+    for prefix in (0, 50):
+        run(be, pool, queries(6, 3, 4, 64, False), k, v, 2, prefix, [0, 1, 0], [own, 0, max(own - 3, 0)], max(own, 1))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("B", [1, 2, 9, 16, 17, 33, 70, 129])
+def test_batches(be, kind, bf16, B):
+    held = [(b * 7) % 50 for b in range(B)] + [1203]
+    pool, k, v = make_pool(be, kind, B + 1, 2, 128, held, 7 + B)
+    run(be, pool, queries(8, B, 8, 128, bf16), k, v, B, 1203, range(B), held[:B], 50)
+
+
+def test_query_with_nothing_to_see_gets_zeros(be):
+    pool, k, v = make_pool(be, "bf16", 3, 2, 64, [0, 30, 0], 9)
+    q = queries(10, 2, 4, 64, False)
+    got = run(be, pool, q, k, v, 2, 0, [0, 1], [0, 30], 30)
+    assert not got[0].any() and got[1].any()
+    assert not be.prefix_attention(pool, q.cuda(), 1, 0, 0.1, max_len=0).any()
+    # a prefix of a slot that holds nothing
+    assert not be.prefix_attention(pool, q.cuda(), 2, 40, 0.1, max_len=0).any()
+
+
+def test_lengths_are_cut_at_what_the_slot_holds(be):
+    pool, k, v = make_pool(be, "bf16", 4, 2, 64, [20, 7, 33, 100], 11)
+    q = queries(12, 3, 4, 64, False)
+    run(be, pool, q, k, v, 3, 112, [0, 1, 2], [112, 8, 40], 112)          # more than held
+    run(be, pool, q, k, v, 3, 100, [0, 1, 2], [20, 7, 33], 10)            # more than max_len
+    run(be, pool, q, k, v, 3, 100, [0, -1, 4], [20, 7, 33], 40)           # slots outside the pool hold nothing
+    run(be, pool, q, k, v, 3, 100, [0, 1, 2], [-5, -2 ** 31, 2 ** 31 - 1], 40)
+    run(be, pool, q, k, v, 3, 100, [0, 1, 2], [20, 7, 33], 40, give_slots=False, give_lens=False)
+    # the same slot as prefix and as own tokens, and twice as own
+    run(be, pool, q, k, v, 3, 60, [3, 3, 0], [100, 100, 3], 100)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+def test_unwritten_token_slots_are_not_read(be, kind):
+    """Page slots past a slot's tokens, and pages nobody holds, full of NaN
+    patterns: the result does not move."""
+    held = [5, 18, 0, 35]
+    pool, k, v = make_pool(be, kind, 4, 2, 128, held, 13)
+    q = queries(14, 3, 6, 128, False)
+    want = run(be, pool, q, k, v, 3, 35, [0, 1, 2], [5, 18, 0], 18)
+    used = {}
+    for s, n in enumerate(held):
+        for i, ph in enumerate(pool.layer_pages(s)):
+            used[int(ph)] = min(PAGE, n - i * PAGE)
+    cap, kvh, hd = pool.s.capacity, 2, 128
+    if kind == "bf16":
+        K, V = pool.fetch("k", cap * kvh * PAGE * hd, np.uint16), pool.fetch("v", cap * kvh * PAGE * hd, np.uint16)
+        Kr, Vr = K.reshape(cap, kvh, PAGE, hd), V.reshape(cap, kvh, hd, PAGE)
+        for ph in range(cap):
+            Kr[ph, :, used.get(ph, 0):], Vr[ph, :, :, used.get(ph, 0):] = 0x7FC0, 0x7FC0
+        put = (("k", K), ("v", V))
+    else:
+        put = []
+        for f in ("k_scale", "v_scale"):
+            S = pool.fetch(f, cap * kvh * PAGE, np.float32)
+            for ph in range(cap):
+                S.reshape(cap, kvh, PAGE)[ph, :, used.get(ph, 0):] = np.nan
+            put.append((f, S))
+    for f, a in put:
+        be.check(be.lib.be42_memcpy_h2d(getattr(pool.s, f), a.ctypes.data, a.nbytes, None), "h2d")
+    torch.cuda.synchronize()
+    assert torch.equal(run(be, pool, q, k, v, 3, 35, [0, 1, 2], [5, 18, 0], 18), want)
+
+
+def test_nan_of_one_query_stays_there(be):
+    pool, k, v = make_pool(be, "bf16", 4, 2, 64, [5, 9, 3, 300], 15)
+    q = queries(16, 3, 4, 64, False)
+    want = run(be, pool, q, k, v, 3, 300, [0, 1, 2], [5, 9, 3], 9)
+    q[1, 2, 7] = math.nan
+    got = be.prefix_attention(pool, q.cuda(), 3, 300, 0.125, slots=torch.arange(3, dtype=torch.int32, device="cuda"),
+                              lens=torch.tensor([5, 9, 3], dtype=torch.int32, device="cuda"), max_len=9)
+    assert torch.isnan(got[1, 2]).all()
+    got[1, 2] = want[1, 2]
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+def test_large_scores_and_small_values(be, kind):
+    """Scores hundreds apart (weights of zero), queries far from one."""
+    pool, k, v = make_pool(be, kind, 3, 1, 64, [40, 3, 700], 17)
+    for mul in (300.0, 1e-30, 0.0):
+        q = queries(18, 2, 4, 64, False) * mul
+        run(be, pool, q, k, v, 2, 700, [0, 1], [40, 3], 40)
+    run(be, pool, queries(18, 2, 4, 64, False), k, v, 2, 700, [0, 1], [40, 3], 40, scale=-3.0)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_continuations_of_several_tokens(be, kind, bf16):
+    """Queries of one slot at consecutive positions, each as if alone."""
+    held = [9, 30, 400]
+    pool, k, v = make_pool(be, kind, 3, 2, 128, held, 19)
+    slots, lens = [0] * 9 + [1] * 30, list(range(1, 10)) + list(range(1, 31))
+    run(be, pool, queries(20, 39, 6, 128, bf16), k, v, 2, 400, slots, lens, 30)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_strided_queries(be, bf16):
+    """The q part of rows that hold q, k and v side by side, off 16 bytes."""
+    pool, k, v = make_pool(be, "bf16", 4, 2, 64, [5, 9, 3, 100], 21)
+    for pad, off in ((256, 0), (7, 1), (2, 2)):
+        q = queries(22, 3, 4, 64, bf16)
+        wide = torch.full((3, 256 + pad + off), math.nan, dtype=q.dtype, device="cuda")
+        wide[:, off:off + 256] = q.reshape(3, 256).cuda()
+        run(be, pool, q, k, v, 3, 100, [0, 1, 2], [5, 9, 3], 9, q_dev=wide[:, off:off + 256].unflatten(1, (4, 64)))
+
+
+@pytest.mark.parametrize("B,heads,prefix,max_len", [(1, 4, 50, 9), (3, 8, 3000, 40), (70, 8, 900, 0), (5, 4, 0, 300)])
+def test_workspace_of_the_caller(be, B, heads, prefix, max_len):
+    """Exactly the bytes asked for, full of NaN patterns, nothing behind them touched."""
+    held = [min(max_len, 3 + b) for b in range(B)] + [max(prefix, 1)]
+    pool, k, v = make_pool(be, "bf16", B + 1, 2, 64, held, 23)
+    size = be.lib.be42_prefix_attention_workspace_bytes(B, heads, 2, 64, prefix, max_len)
+    ws = torch.full((size + 256,), 255, dtype=torch.uint8, device="cuda")
+    out = torch.full((B, heads, 64), math.nan, device="cuda")
+    got = run(be, pool, queries(24, B, heads, 64, False), k, v, B, prefix, range(B), held[:B], max_len,
+              workspace=ws[:size], out=out)
+    assert got is out and (ws[size:] == 255).all()
+
+
+def test_repeats_to_the_bit(be):
+    pool, k, v = make_pool(be, "int8", 9, 2, 128, [50] * 8 + [4000], 25)
+    q = queries(26, 8, 8, 128, False)
+    a = run(be, pool, q, k, v, 8, 4000, range(8), [50] * 8, 50)
+    for _ in range(3):
+        assert torch.equal(run(be, pool, q, k, v, 8, 4000, range(8), [50] * 8, 50), a)
+
+
+def test_refusals(be):
+    import be42
+    pool, k, v = make_pool(be, "bf16", 3, 2, 64, [5, 9, 30], 27)
+    q = torch.zeros(2, 4, 64, device="cuda")
+    i = torch.zeros(2, dtype=torch.int32, device="cuda")
+    for kw in (dict(q=q.half()), dict(q=q[:, :, :32]), dict(q=q[0]), dict(q=q.cpu()), dict(q=q[:, :3]),
+               dict(q=q.transpose(0, 1)), dict(prefix_slot=3), dict(prefix_len=1000), dict(slots=i.long()),
+               dict(lens=i[:1]), dict(lens=i.cpu()), dict(out=q.bfloat16()), dict(out=q[:1]), dict(max_len=-1),
+               dict(scale=math.nan), dict(workspace=q), dict(workspace=torch.zeros(1, dtype=torch.uint8, device="cuda"))):
+        a = dict(q=q, prefix_slot=2, prefix_len=30, scale=0.1, slots=i, lens=i, max_len=9)
+        a.update(kw)
+        with pytest.raises(be42.Be42Error):
+            be.prefix_attention(pool, **a)
+    assert be.prefix_attention(pool, q[:0], 2, 30, 0.1).shape == (0, 4, 64)
+
+
+def test_graph_decodes_on(be):
+    """Captured once, replayed while slots grow and the batch's slots change
+    places: each replay equals the eager call and float64."""
+    B, kvh, hd = 3, 2, 64
+    pool, k, v = make_pool(be, "bf16", 4, kvh, hd, [4, 1, 0, 200], 29)
+    q = torch.zeros(B, 4, hd, device="cuda")
+    slots = torch.arange(B, dtype=torch.int32, device="cuda")
+    lens = torch.tensor([4, 1, 0], dtype=torch.int32, device="cuda")
+    ws = torch.empty(be.lib.be42_prefix_attention_workspace_bytes(B, 4, kvh, hd, 200, 12), dtype=torch.uint8, device="cuda")
+    call = lambda: be.prefix_attention(pool, q, 3, 200, 0.125, slots=slots, lens=lens, max_len=12, workspace=ws)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    g, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(g, stream=side):
+        got = call()
+    held = [4, 1, 0]
+    rng = np.random.default_rng(30)
+    for step in range(5):
+        place = rng.permutation(B)
+        for s in range(B):
+            a, b = (rng.standard_normal((1, kvh, hd)).astype(np.float32) for _ in range(2))
+            pool.append(s, torch.from_numpy(a).cuda().reshape(1, -1), torch.from_numpy(b).cuda().reshape(1, -1), held[s])
+            k[s] = np.concatenate([k[s], torch.from_numpy(a).bfloat16().double().numpy()])
+            v[s] = np.concatenate([v[s], torch.from_numpy(b).bfloat16().double().numpy()])
+            held[s] += 1
+        qc = queries(31 + step, B, 4, hd, False)
+        q.copy_(qc)
+        slots.copy_(torch.from_numpy(place.astype(np.int32)))
+        lens.copy_(torch.tensor([held[p] for p in place], dtype=torch.int32))
+        g.replay()
+        torch.cuda.synchronize()
+        again = run(be, pool, qc, k, v, 3, 200, [int(p) for p in place], [held[p] for p in place], 12, scale=0.125)
+        assert torch.equal(again, got), step

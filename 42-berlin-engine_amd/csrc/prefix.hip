@@ -4,6 +4,13 @@
 //   out[b][h] = sum_t softmax_t(scale * q[b][h] . k_t) v_t
 // over the first prefix_len tokens of slot prefix_slot and the first lens[b]
 // tokens of slot slots[b].
+//
+// Tokens are cut into parts, some of the prefix and some of each query's own
+// tokens; one workgroup forms, for up to 16 rows (query, head) of one KV head
+// and one part, m = max s, l = sum 2^(s - m) and o = sum 2^(s - m) v with
+// s = log2(e) * scale * q.k, and k_prefix_join adds the parts of a row with
+// weights 2^(m - max m).  Rows of the prefix are those of all queries, so its
+// pages are read once for 16 rows.
 #include <algorithm>
 #include <cmath>
 
@@ -12,14 +19,21 @@
 
 namespace be42 {
 
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+
 struct PrefixArgs {
     const void *q;
     void *out;
     const int *slots, *lens;
-    float *part;              // workspace
+    float *part_o, *part_ml;  // [parts][rows][head_dim], [parts][rows][2]; rows = n_queries * n_heads
     size_t q_stride;
     int n_queries, n_heads, prefix_slot, prefix_len, max_len;
     float scale;
+    // the cut: parts of the prefix and of the own tokens, tokens of each, and
+    // tiles of 16 rows that a KV head has over the prefix and over one query
+    int parts_p, parts_o, chunk_p, chunk_o, tiles_p, tiles_o;
 };
 
 // tokens a slot holds (0 for a slot outside the pool)
@@ -36,57 +50,437 @@ __device__ __forceinline__ int slot_tokens(const be42_kv_pool &P, int slot)
     return (pages - 1) * kPage + min(P.ntok[last], kPage);
 }
 
-template <bool BF16>
-__device__ __forceinline__ float kv_elem(const be42_kv_pool &P, bool v, size_t page_head, int t, int d)
+// Eight fp32 as N bf16 parts: each part the rest rounded to bf16, so that three
+// hold all 24 bits and one is a plain rounding.
+template <int N>
+__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&p)[N])
 {
-    const void *p = v ? P.v : P.k;
-    if (BF16)
-        return bf16_to_f32(((const uint16_t *)p)[v ? (page_head * P.head_dim + d) * kPage + t
-                                                   : (page_head * kPage + t) * P.head_dim + d]);
-    return (float)((const int8_t *)p)[(page_head * kPage + t) * P.head_dim + d] *
-           (v ? P.v_scale : P.k_scale)[page_head * kPage + t];
-}
-
-// one wave per (query, head), one token at a time
-template <bool BF16, bool QB>
-__global__ __launch_bounds__(64) void k_prefix_attn(const be42_kv_pool P, const PrefixArgs a)
-{
-    const int b = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-    const int hd = P.head_dim, per = hd / kWave, kvh = h / (a.n_heads / P.n_kv);
-    float q[2], o[2] = {0.0f, 0.0f};
-    for (int i = 0; i < per; i++) {
-        const size_t at = (size_t)b * a.q_stride + (size_t)h * hd + lane + i * kWave;
-        q[i] = QB ? bf16_to_f32(((const uint16_t *)a.q)[at]) : ((const float *)a.q)[at];
-    }
-    float m = -INFINITY, l = 0.0f;
-    for (int part = 0; part < 2; part++) {
-        const int slot = part ? (a.slots ? a.slots[b] : b) : a.prefix_slot;
-        int n = slot_tokens(P, slot);
-        n = min(n, part ? (a.lens ? min(a.lens[b], a.max_len) : a.max_len) : a.prefix_len);
-        for (int t = 0; t < n; t++) {
-            const int phys = P.page_table[(size_t)slot * P.max_logical + t / kPage];
-            if (phys < 0 || phys >= P.capacity)
-                continue;
-            const size_t ph = (size_t)phys * P.n_kv + kvh;
-            float s = 0.0f;
-            for (int i = 0; i < per; i++)
-                s = __fmaf_rn(q[i], kv_elem<BF16>(P, false, ph, t % kPage, lane + i * kWave), s);
-            s = wave_sum(s) * a.scale;
-            const float mn = fmaxf(m, s), c = expf(m - mn), p = expf(s - mn);
-            l = l * c + p;
-            for (int i = 0; i < per; i++)
-                o[i] = __fmaf_rn(p, kv_elem<BF16>(P, true, ph, t % kPage, lane + i * kWave), o[i] * c);
-            m = mn;
+    uint32_t w[N][4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        v2f r = {x[2 * j], x[2 * j + 1]};
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            w[n][j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, bf16x2));
+            if (n + 1 < N) {
+                r[0] -= __uint_as_float(w[n][j] << 16);
+                r[1] -= __uint_as_float(w[n][j] & 0xFFFF0000u);
+            }
         }
     }
-    for (int i = 0; i < per; i++) {
-        const size_t at = ((size_t)b * a.n_heads + h) * hd + lane + i * kWave;
-        const float v = l == 0.0f ? 0.0f : o[i] / l;
-        if (QB)
-            ((uint16_t *)a.out)[at] = f32_to_bf16(v);
-        else
-            ((float *)a.out)[at] = v;
+#pragma unroll
+    for (int n = 0; n < N; n++)
+        p[n] = __builtin_bit_cast(bf16x8, make_uint4(w[n][0], w[n][1], w[n][2], w[n][3]));
+}
+
+// bytes 0 .. 7 of two words as bf16 (exact)
+__device__ __forceinline__ bf16x8 codes8(uint32_t a, uint32_t b)
+{
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const uint32_t u = j < 2 ? a : b;
+        const v2f r = {(float)(int8_t)(u >> (16 * (j & 1))), (float)(int8_t)(u >> (16 * (j & 1) + 8))};
+        w[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, bf16x2));
     }
+    return __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+}
+
+__device__ __forceinline__ v4f mfma16(bf16x8 a, bf16x8 b, v4f c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+constexpr int kPartWaves = 4;
+constexpr int kStep = 32;         // tokens of a wave's step: two pages
+
+template <int HD>
+struct PartShared {
+    float o[kPartWaves][16][HD + 4];
+    float m[kPartWaves][16], l[kPartWaves][16];
+};
+
+// Rows of a part in 16x16 tiles.  Both products are formed transposed, S^T =
+// K Q^T (operand rows are tokens, columns are query rows) and O^T = V^T P^T, so
+// that a lane keeps one query row from the scores to the output: column c =
+// lane % 16, and with g = lane / 16 the lane's eight scores of a step of 32
+// tokens are tokens 8 g .. 8 g + 7 -- row 4 g + i of score tile t is given to
+// token 8 g + 4 t + i -- which is the operand the second product takes from
+// it.  Weights go from one product to the other in registers.
+template <bool KV8, int HD, int NP, int PP>
+__device__ __forceinline__ void part16(const be42_kv_pool &P, const PrefixArgs &a, PartShared<HD> &S, int slot,
+                                       int lo, int hi, int kvh, int b0, int row0, int rows)
+{
+    constexpr int NK = HD / 32, NE = HD / 16;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+    const int G = a.n_heads / P.n_kv;
+    const int ns = (hi - lo + kStep - 1) / kStep;
+    const int mine = ns > wave ? (ns - wave + kPartWaves - 1) / kPartWaves : 0;   // steps wave, wave + 4, ..
+
+    // the lane's query row, eight elements a k block: bf16 pages take element
+    // 32 kb + 8 g + j there, INT8 pages (16 codes a load) 64 (kb / 2) + 16 g + 8 (kb % 2) + j
+    bf16x8 Q[NK][NP];
+    {
+        const int ri = min(row0 + c, rows - 1);
+        const size_t at = (size_t)(b0 + ri / G) * a.q_stride + (size_t)(kvh * G + ri % G) * HD;
+        const bool flip = a.scale < 0.0f;
+#pragma unroll
+        for (int kb = 0; kb < NK; kb++) {
+            const int d = KV8 ? 64 * (kb / 2) + 16 * g + 8 * (kb % 2) : 32 * kb + 8 * g;
+            if constexpr (NP == 1) {
+                uint32_t w[4];
+                __builtin_memcpy(w, (const uint16_t *)a.q + at + d, 16);
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    w[j] ^= flip ? 0x80008000u : 0u;
+                Q[kb][0] = __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+            } else {
+                float x[8];
+                __builtin_memcpy(x, (const float *)a.q + at + d, 32);
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    x[j] = flip ? -x[j] : x[j];
+                split8<NP>(x, Q[kb]);
+            }
+        }
+    }
+    const float sc = fabsf(a.scale) * 1.44269504088896340736f;
+
+    v4f O[NE];
+#pragma unroll
+    for (int e = 0; e < NE; e++)
+        O[e] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;
+
+    uint4 K[2][KV8 ? NK / 2 : NK];
+    uint4 V[KV8 ? 1 : NE];
+    uint32_t V8[KV8 ? 8 : 1][HD / 64];
+    float4 ks[2], vs[2];
+    // physical pages of the wave's next 32 steps: lane 2 i + e holds page e of step i
+    int pages = 0;
+    auto load_pages = [&](int i0) {
+        const int e = lane & 1, lp = lo / kPage + 2 * (wave + kPartWaves * (i0 + lane / 2)) + e;
+        // a step's second page may lie past the part: its first one stands in (masked)
+        const int at = lp * kPage < hi ? lp : lp - e;
+        pages = at * kPage < hi ? P.page_table[(size_t)slot * P.max_logical + at] : 0;
+        pages = min(max(pages, 0), P.capacity - 1);
+    };
+    auto head_of = [&](int i, int e) {
+        return (size_t)__builtin_amdgcn_readlane(pages, 2 * (i & 31) + e) * P.n_kv + kvh;
+    };
+    const int kg = c >> 2, ktok = 8 * (kg & 1) + (c & 3);      // token (of its page) that operand row c of tile 0 is
+    auto load_k = [&](int i) {
+        const size_t h0 = head_of(i, 0), h1 = head_of(i, 1), hk = kg >> 1 ? h1 : h0, hv = g >> 1 ? h1 : h0;
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const size_t row = (hk * kPage + ktok + 4 * t) * HD;
+#pragma unroll
+            for (int x = 0; x < (KV8 ? NK / 2 : NK); x++)
+                K[t][x] = KV8 ? *(const uint4 *)((const int8_t *)P.k + row + 64 * x + 16 * g)
+                              : *(const uint4 *)((const uint16_t *)P.k + row + 32 * x + 8 * g);
+        }
+        if constexpr (KV8)
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+                ks[t] = *(const float4 *)(P.k_scale + hv * kPage + 8 * (g & 1) + 4 * t);
+    };
+    auto load_v = [&](int i) {
+        const size_t h0 = head_of(i, 0), h1 = head_of(i, 1), hv = g >> 1 ? h1 : h0;
+        if constexpr (KV8) {
+            // eight tokens of NE dims: tile e's row r is dim NE r + e
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                __builtin_memcpy(V8[j], (const int8_t *)P.v + (hv * kPage + 8 * (g & 1) + j) * HD + NE * c, HD / 16);
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+                vs[t] = *(const float4 *)(P.v_scale + hv * kPage + 8 * (g & 1) + 4 * t);
+        } else {
+#pragma unroll
+            for (int e = 0; e < NE; e++)
+                V[e] = *(const uint4 *)((const uint16_t *)P.v + (hv * HD + 16 * e + c) * kPage + 8 * (g & 1));
+        }
+    };
+
+    if (mine) {
+        load_pages(0);
+        load_k(0);
+        load_v(0);
+    }
+    for (int i = 0; i < mine; i++) {
+        const int left = hi - lo - (wave + kPartWaves * i) * kStep;      // tokens from this step on
+        v4f s[2] = {v4f{0.0f, 0.0f, 0.0f, 0.0f}, v4f{0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+        for (int kb = 0; kb < NK; kb++)
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const bf16x8 k = KV8 ? (kb & 1 ? codes8(K[t][kb / 2].z, K[t][kb / 2].w) : codes8(K[t][kb / 2].x, K[t][kb / 2].y))
+                                     : __builtin_bit_cast(bf16x8, K[t][KV8 ? 0 : kb]);
+#pragma unroll
+                for (int n = NP - 1; n >= 0; n--)
+                    s[t] = mfma16(k, Q[kb][n], s[t]);
+            }
+        float p[8], vsc[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            p[j] = s[j >> 2][j & 3];
+            if constexpr (KV8) {
+                p[j] *= ((const float *)&ks[j >> 2])[j & 3];
+                vsc[j] = ((const float *)&vs[j >> 2])[j & 3];
+            }
+        }
+        const bool more = i + 1 < mine;
+        if (more) {
+            if (((i + 1) & 31) == 0)
+                load_pages(i + 1);
+            load_k(i + 1);
+        }
+        if (left < kStep)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const bool out = 8 * g + j >= left;
+                p[j] = out ? -INFINITY : p[j];
+                if (KV8)
+                    vsc[j] = out ? 0.0f : vsc[j];
+            }
+        float top = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
+        top = fmaxf(top, __shfl_xor(top, 16, kWave));
+        top = fmaxf(top, __shfl_xor(top, 32, kWave));
+        const float mn = fmaxf(m, top * sc);
+        if (__any(mn > m)) {
+            const float f = __builtin_amdgcn_exp2f(m - mn);
+            l *= f;
+#pragma unroll
+            for (int e = 0; e < NE; e++)
+                O[e] *= f;
+            m = mn;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            p[j] = __builtin_amdgcn_exp2f(__fmaf_rn(p[j], sc, -m));
+            l += p[j];
+            if (KV8)
+                p[j] *= vsc[j];
+        }
+        bf16x8 W[PP];
+        split8<PP>(p, W);
+        // V of tokens past the part is whatever the page held: a weight of zero
+        // times a NaN pattern would be NaN
+        if (!KV8 && left < kStep) {
+            uint32_t keep[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                keep[j] = (8 * g + 2 * j < left ? 0xFFFFu : 0u) | (8 * g + 2 * j + 1 < left ? 0xFFFF0000u : 0u);
+#pragma unroll
+            for (int e = 0; e < (KV8 ? 0 : NE); e++) {
+                V[e].x &= keep[0];
+                V[e].y &= keep[1];
+                V[e].z &= keep[2];
+                V[e].w &= keep[3];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < NE; e++) {
+            bf16x8 v;
+            if constexpr (KV8) {
+                uint32_t w[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int word = e >> 2, at = 8 * (e & 3);
+                    const v2f r = {(float)(int8_t)(V8[2 * j][word] >> at), (float)(int8_t)(V8[2 * j + 1][word] >> at)};
+                    w[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, bf16x2));
+                }
+                v = __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+            } else {
+                v = __builtin_bit_cast(bf16x8, V[KV8 ? 0 : e]);
+            }
+#pragma unroll
+            for (int n = PP - 1; n >= 0; n--)
+                O[e] = mfma16(v, W[n], O[e]);
+        }
+        if (more)
+            load_v(i + 1);
+    }
+
+    // the four waves' sums of the part
+    l += __shfl_xor(l, 16, kWave);
+    l += __shfl_xor(l, 32, kWave);
+    if (g == 0) {
+        S.m[wave][c] = m;
+        S.l[wave][c] = l;
+    }
+#pragma unroll
+    for (int e = 0; e < NE; e++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            S.o[wave][c][KV8 ? NE * (4 * g + i) + e : 16 * e + 4 * g + i] = O[e][i];
+    __syncthreads();
+}
+
+// Weight of a partial result whose maximum is m against the maximum of all; one
+// without tokens weighs nothing.
+__device__ __forceinline__ float part_weight(float m, float l, float top)
+{
+    return l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+}
+
+template <bool QB>
+__device__ __forceinline__ void store_out4(void *out, size_t at, float4 v)
+{
+    if constexpr (QB) {
+        const v2f a = {v.x, v.y}, b = {v.z, v.w};
+        const uint2 w = make_uint2(__builtin_bit_cast(uint32_t, __builtin_convertvector(a, bf16x2)),
+                                   __builtin_bit_cast(uint32_t, __builtin_convertvector(b, bf16x2)));
+        __builtin_memcpy((uint16_t *)out + at, &w, 8);
+    } else {
+        __builtin_memcpy((float *)out + at, &v, 16);
+    }
+}
+
+// block: (KV head, row tile, part) of the prefix, then (KV head, row tile,
+// query, part) of the own tokens
+template <bool KV8, int HD, bool QB>
+__global__ __launch_bounds__(64 * kPartWaves, 2) void k_prefix_part(const be42_kv_pool P, const PrefixArgs a)
+{
+    __shared__ PartShared<HD> S;
+    const int G = a.n_heads / P.n_kv;
+    const unsigned of_prefix = (unsigned)P.n_kv * a.tiles_p * a.parts_p;
+    unsigned id = blockIdx.x;
+    int slot, lo, n, chunk, part, b0, row0, rows;
+    const bool own = id >= of_prefix;
+    if (own)
+        id -= of_prefix;
+    const int kvh = (int)(id % (unsigned)P.n_kv);
+    id /= (unsigned)P.n_kv;
+    if (own) {
+        row0 = 16 * (int)(id % (unsigned)a.tiles_o);
+        id /= (unsigned)a.tiles_o;
+        b0 = (int)(id % (unsigned)a.n_queries);
+        part = (int)(id / (unsigned)a.n_queries);
+        rows = G;
+        slot = a.slots ? a.slots[b0] : b0;
+        n = min(slot_tokens(P, slot), a.max_len);
+        if (a.lens)
+            n = min(n, a.lens[b0]);
+        chunk = a.chunk_o;
+    } else {
+        row0 = 16 * (int)(id % (unsigned)a.tiles_p);
+        part = (int)(id / (unsigned)a.tiles_p);
+        b0 = 0;
+        rows = a.n_queries * G;
+        slot = a.prefix_slot;
+        n = min(slot_tokens(P, slot), a.prefix_len);
+        chunk = a.chunk_p;
+    }
+    lo = part * chunk;
+    part += own ? a.parts_p : 0;
+    const int hi = max(lo, min(n, lo + chunk));
+    part16<KV8, HD, QB ? 1 : 3, QB ? 1 : 3>(P, a, S, slot, lo, hi, kvh, b0, row0, rows);
+
+    const int c = threadIdx.x >> 4, d4 = threadIdx.x & 15, ri = row0 + c;
+    if (ri >= rows)
+        return;
+    float top = S.m[0][c], w[kPartWaves], l = 0.0f;
+#pragma unroll
+    for (int x = 1; x < kPartWaves; x++)
+        top = fmaxf(top, S.m[x][c]);
+#pragma unroll
+    for (int x = 0; x < kPartWaves; x++) {
+        w[x] = part_weight(S.m[x][c], S.l[x][c], top);
+        l += w[x] * S.l[x][c];
+    }
+    const size_t row = (size_t)(b0 + ri / G) * a.n_heads + kvh * G + ri % G;
+    const size_t all = (size_t)a.n_queries * a.n_heads;
+    const bool last = a.parts_p + a.parts_o == 1;
+    if (!last && d4 == 0)
+        *(float2 *)(a.part_ml + 2 * (part * all + row)) = make_float2(top, l);
+    if (!last && l == 0.0f)
+        return;                    // k_prefix_join reads no values of a part without tokens
+    const float inv = last ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+#pragma unroll
+    for (int x = 0; x < HD / 64; x++) {
+        const int d = 64 * x + 4 * d4;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int y = 0; y < kPartWaves; y++) {
+            const float4 o = *(const float4 *)&S.o[y][c][d];
+            v.x = __fmaf_rn(w[y], o.x, v.x);
+            v.y = __fmaf_rn(w[y], o.y, v.y);
+            v.z = __fmaf_rn(w[y], o.z, v.z);
+            v.w = __fmaf_rn(w[y], o.w, v.w);
+        }
+        if (last)
+            store_out4<QB>(a.out, row * HD + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+        else
+            *(float4 *)(a.part_o + (part * all + row) * HD + d) = v;
+    }
+}
+
+// one wave per row: its parts by weight; lanes of head_dim / 4 words take the
+// parts in turn
+template <int HD, bool QB>
+__global__ __launch_bounds__(256) void k_prefix_join(const PrefixArgs a, int parts)
+{
+    constexpr int L = HD / 4, PER = kWave / L;
+    const size_t all = (size_t)a.n_queries * a.n_heads, row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, sub = lane / L;
+    if (row >= all)
+        return;
+    const float2 *ml = (const float2 *)a.part_ml;
+    float top = -INFINITY;
+    for (int p = lane; p < parts; p += kWave)
+        top = fmaxf(top, ml[p * all + row].x);
+    top = wave_max(top);
+    float l = 0.0f;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int p = sub; p < parts; p += PER) {
+        const float2 x = ml[p * all + row];
+        if (x.y == 0.0f)
+            continue;
+        const float w = part_weight(x.x, x.y, top);
+        const float4 o = *(const float4 *)(a.part_o + (p * all + row) * HD + 4 * (lane % L));
+        l = __fmaf_rn(w, x.y, l);
+        v.x = __fmaf_rn(w, o.x, v.x);
+        v.y = __fmaf_rn(w, o.y, v.y);
+        v.z = __fmaf_rn(w, o.z, v.z);
+        v.w = __fmaf_rn(w, o.w, v.w);
+    }
+#pragma unroll
+    for (int o = L; o < kWave; o <<= 1) {
+        l += __shfl_xor(l, o, kWave);
+        v.x += __shfl_xor(v.x, o, kWave);
+        v.y += __shfl_xor(v.y, o, kWave);
+        v.z += __shfl_xor(v.z, o, kWave);
+        v.w += __shfl_xor(v.w, o, kWave);
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    if (sub == 0)
+        store_out4<QB>(a.out, row * HD + 4 * lane, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+}
+
+// Tokens of a slot that a call may name: their sums stay within 32 bits.
+constexpr int kMaxTokens = 1 << 30;
+
+// The cut of the tokens.  A part has at least 128 tokens (a step for each of the
+// workgroup's waves); prefix and own tokens are each cut into as many parts as
+// give them two workgroups a CU.
+static void cut(int tokens, long tiles, int *parts, int *chunk)
+{
+    *parts = *chunk = 0;
+    if (!tokens)
+        return;
+    const int unit = kPartWaves * kStep, units = (int)(((long)tokens + unit - 1) / unit);
+    const int want = (int)std::min<long>(units, std::max<long>(1, (512 + tiles - 1) / tiles));
+    *chunk = (units + want - 1) / want * unit;
+    *parts = (int)(((long)tokens + *chunk - 1) / *chunk);
+}
+
+static void plan_prefix(PrefixArgs &a, int n_kv)
+{
+    const int G = a.n_heads / n_kv;
+    a.tiles_p = (int)(((long)a.n_queries * G + 15) / 16);
+    a.tiles_o = (G + 15) / 16;
+    cut(a.prefix_len, (long)a.tiles_p * n_kv, &a.parts_p, &a.chunk_p);
+    cut(a.max_len, (long)a.tiles_o * n_kv * a.n_queries, &a.parts_o, &a.chunk_o);
 }
 
 }  // namespace be42
@@ -97,9 +491,15 @@ extern "C" size_t be42_prefix_attention_workspace_bytes(int n_queries, int n_hea
                                                         int prefix_len, int max_len)
 {
     if (n_queries <= 0 || n_heads <= 0 || n_kv <= 0 || n_heads % n_kv || (head_dim != 64 && head_dim != 128) ||
-        prefix_len < 0 || max_len < 0)
+        prefix_len < 0 || prefix_len > kMaxTokens || max_len < 0 || max_len > kMaxTokens)
         return 0;
-    return 16;
+    PrefixArgs a = {};
+    a.n_queries = n_queries;
+    a.n_heads = n_heads;
+    a.prefix_len = prefix_len;
+    a.max_len = max_len;
+    plan_prefix(a, n_kv);
+    return 16 + (size_t)(a.parts_p + a.parts_o) * n_queries * n_heads * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int be42_prefix_attention(const be42_kv_pool *pool, const void *q, int q_bf16, int q_stride, int n_queries,
@@ -117,7 +517,7 @@ extern "C" int be42_prefix_attention(const be42_kv_pool *pool, const void *q, in
     BE42_CHECK(prefix_slot >= 0 && prefix_slot < P.n_layers, "be42_prefix_attention: prefix slot %d of %d", prefix_slot,
                P.n_layers);
     const long held = (long)P.max_logical * kPage;
-    BE42_CHECK(prefix_len >= 0 && prefix_len <= held && max_len >= 0,
+    BE42_CHECK(prefix_len >= 0 && prefix_len <= std::min(held, (long)kMaxTokens) && max_len >= 0 && max_len <= kMaxTokens,
                "be42_prefix_attention: prefix %d, max_len %d (a slot holds %ld tokens)", prefix_len, max_len, held);
     BE42_CHECK(std::isfinite(scale), "be42_prefix_attention: scale %g", (double)scale);
     BE42_CHECK(!(((uintptr_t)q | (uintptr_t)out) & (q_bf16 ? 1 : 3)), "be42_prefix_attention: unaligned pointer");
@@ -126,21 +526,40 @@ extern "C" int be42_prefix_attention(const be42_kv_pool *pool, const void *q, in
                n_queries, P.n_layers);
     if (n_queries == 0)
         return BE42_OK;
+    PrefixArgs a = {q, out, slots, lens, nullptr, nullptr, (size_t)q_stride, n_queries, n_heads, prefix_slot, prefix_len,
+                    max_len, scale};
+    plan_prefix(a, P.n_kv);
+    const int parts = a.parts_p + a.parts_o;
+    const long blocks = (long)P.n_kv * ((long)a.tiles_p * a.parts_p + (long)a.tiles_o * n_queries * a.parts_o);
+    const size_t rows = (size_t)n_queries * n_heads;
+    BE42_CHECK(blocks <= 0x7FFFFFFF && (long)n_queries * (n_heads / P.n_kv) <= 0x7FFFFFFF - 16,
+               "be42_prefix_attention: %d queries of %d heads", n_queries, n_heads);
     const size_t need = be42_prefix_attention_workspace_bytes(n_queries, n_heads, P.n_kv, P.head_dim, prefix_len,
                                                               max_len);
     BE42_CHECK(!workspace || (!((uintptr_t)workspace & 15) && workspace_bytes >= need),
                "be42_prefix_attention: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, need);
-    PrefixArgs a = {q, out, slots, lens, nullptr, (size_t)q_stride, n_queries, n_heads, prefix_slot, prefix_len,
-                    max_len, scale};
-    const dim3 g(n_queries, n_heads), b(64);
     hipStream_t s = as_stream(stream);
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, g, b, 0, s, P, a); };
-    if (P.kind == BE42_KV_BF16) {
-        if (q_bf16) go(k_prefix_attn<true, true>);
-        else go(k_prefix_attn<true, false>);
+    if (parts > 1) {
+        if (!workspace)
+            workspace = be42::workspace(need, s);
+        if (!workspace)
+            return BE42_ENOMEM;
+        a.part_o = (float *)workspace;
+        a.part_ml = a.part_o + (size_t)parts * rows * P.head_dim;
+    }
+    auto go = [&](auto part, auto join) {
+        if (parts)
+            hipLaunchKernelGGL(part, dim3((unsigned)blocks), dim3(64 * kPartWaves), 0, s, P, a);
+        if (parts != 1)
+            hipLaunchKernelGGL(join, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a, parts);
+    };
+    const bool i8 = P.kind == BE42_KV_INT8;
+    if (P.head_dim == 64) {
+        if (q_bf16) i8 ? go(k_prefix_part<true, 64, true>, k_prefix_join<64, true>) : go(k_prefix_part<false, 64, true>, k_prefix_join<64, true>);
+        else i8 ? go(k_prefix_part<true, 64, false>, k_prefix_join<64, false>) : go(k_prefix_part<false, 64, false>, k_prefix_join<64, false>);
     } else {
-        if (q_bf16) go(k_prefix_attn<false, true>);
-        else go(k_prefix_attn<false, false>);
+        if (q_bf16) i8 ? go(k_prefix_part<true, 128, true>, k_prefix_join<128, true>) : go(k_prefix_part<false, 128, true>, k_prefix_join<128, true>);
+        else i8 ? go(k_prefix_part<true, 128, false>, k_prefix_join<128, false>) : go(k_prefix_part<false, 128, false>, k_prefix_join<128, false>);
     }
     BE42_LAUNCH_CHECK();
     return BE42_OK;

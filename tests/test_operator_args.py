@@ -103,6 +103,7 @@ def prefix(lib, p=None, **kw):
     (dict(n_heads=0), "heads"), (dict(n_queries=-1), "queries"), (dict(q_stride=255), "stride"),
     (dict(prefix_slot=4), "slot"), (dict(prefix_slot=-1), "slot"), (dict(prefix_len=129), "holds"),
     (dict(prefix_len=-1), "holds"), (dict(max_len=-1), "holds"),
+    (dict(max_len=(1 << 30) + 1), "holds"),
     (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(q=PTR + 2), "unaligned"),
     (dict(out=PTR + 2), "unaligned"), (dict(q=PTR + 1, q_bf16=1), "unaligned"),
     (dict(slots=None, n_queries=5), "slots"), (dict(workspace=PTR + 8, bytes=1 << 30), "workspace"),
@@ -124,7 +125,7 @@ def test_prefix_attention_no_queries(lib):
 def test_prefix_attention_workspace(lib):
     f = lib.lib.be42_prefix_attention_workspace_bytes
     assert f(0, 4, 2, 64, 10, 10) == 0 and f(1, 3, 2, 64, 10, 10) == 0 and f(1, 4, 2, 96, 10, 10) == 0
-    assert f(1, 4, 2, 64, -1, 10) == 0 and f(1, 4, 2, 64, 10, -1) == 0
+    assert f(1, 4, 2, 64, 1, INT_MAX) == 0 and f(1, 4, 2, 64, -1, 10) == 0 and f(1, 4, 2, 64, 10, -1) == 0
     assert f(1, 4, 2, 64, 0, 0) > 0 and f(128, 32, 8, 128, 32768, 1024) > 0
     # sizes past 32 bits do not wrap
     assert f(1 << 20, 64, 8, 128, 1 << 20, 1 << 20) >= f(1 << 10, 64, 8, 128, 1 << 20, 1 << 20) > 0

@@ -58,6 +58,7 @@ def score(lib, **kw):
 
 @pytest.mark.parametrize("kw,word", [
     (dict(logits=None), "null"), (dict(n=0), "rows of"), (dict(rows=-1), "rows of"), (dict(row_stride=99), "stride"),
+    (dict(n=(1 << 30) + 1, row_stride=INT_MAX), "rows of"),
     (dict(temp=0.0), "temperature"), (dict(temp=-1.0), "temperature"), (dict(temp=float("inf")), "temperature"),
     (dict(temp=float("nan")), "temperature"), (dict(temp=1e-40), "temperature"),
     (dict(n_tokens=-1), "tokens"), (dict(tokens=None), "tokens"), (dict(logprobs=None), "tokens"),

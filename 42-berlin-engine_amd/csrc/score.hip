@@ -16,6 +16,7 @@ namespace be42 {
 constexpr int kTopMax = 64;
 constexpr int kScoreT = 256, kScoreW = kScoreT / kWave;
 constexpr int kScoreE = 32;                 // entries a thread holds
+constexpr int kGroup = 8;                   // entries that are looked through together
 constexpr int kSlice = kScoreT * kScoreE;
 constexpr int kScoreCand = 512;             // candidates of a slice that are ranked together
 constexpr int kJoinCand = 1024;             // of a row's slices
@@ -78,13 +79,33 @@ __device__ __forceinline__ float log_prob(const ScoreArgs &a, const RowSums &r, 
     return r.ls != r.ls ? NAN : (float)(((double)x - r.m) / (double)a.temp - r.ls);
 }
 
+// the wave's largest value, in every lane (lane moves)
+__device__ __forceinline__ float wave_top(float v)
+{
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wave_prefix_max(v)), 63));
+}
+template <int CTRL, int ROWMASK = 0xF>
+__device__ __forceinline__ uint32_t dpp_max_u(uint32_t v)
+{
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWMASK, 0xF, false));
+}
+__device__ __forceinline__ uint32_t wave_top_u(uint32_t v)
+{
+    v = dpp_max_u<0x111>(v);          // row_shr:1, 2, 4, 8
+    v = dpp_max_u<0x112>(v);
+    v = dpp_max_u<0x114>(v);
+    v = dpp_max_u<0x118>(v);
+    v = dpp_max_u<0x142, 0xA>(v);     // row_bcast:15 into rows 1, 3
+    v = dpp_max_u<0x143, 0xC>(v);     // row_bcast:31 into rows 2, 3
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
 // One set of entries' m, s and t as they count under the maximum `top` of several.
 __device__ __forceinline__ void rebase(const ScoreArgs &a, const float4 &p, float top, double &s, double &t)
 {
-    const double d = p.x == -INFINITY ? 0.0 : ((double)p.x - (double)top) * (1.44269504088896340736 / (double)a.temp);
-    const double w = exp2(d);
-    s = w * p.y;
-    t = w * (p.z + d * p.y);
+    const float d = p.x == -INFINITY ? 0.0f : (p.x - top) * a.c, w = __builtin_amdgcn_exp2f(d);
+    s = (double)w * p.y;
+    t = (double)w * ((double)p.z + (double)fmaxf(d, -200.0f) * p.y);
 }
 
 // the given tokens and the entropy of a row
@@ -163,37 +184,60 @@ __global__ __launch_bounds__(kScoreT) void k_score_slice(const ScoreArgs a)
     // words lie on 16 bytes of memory: word w of the row holds entries VE w - off ..
     const int off = (int)((uintptr_t)xr / (BF16 ? 2 : 4) % VE);
     float x[kScoreE];
-    auto id_of = [&](int i) { return ((slice * U + i / VE) * kScoreT + tid) * VE - off + i % VE; };
+    const int first = slice * kSlice - off;
+    auto id_of = [&](int i) { return first + (i / VE * kScoreT + tid) * VE + i % VE; };
+    // every thread loads whole words, all in flight together (one that is not
+    // wholly of the row reads the row's first whole word instead); entries of
+    // the words that the row's ends cut are then loaded singly
+    const bool inside = first >= 0 && first <= a.n - kSlice;
+    const int whole = off ? VE - off : 0;
+    auto is_whole = [&](int e0) { return inside || (e0 >= 0 && e0 <= a.n - VE); };
+    uint4 w[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const int e0 = id_of(u * VE);
-        if (e0 >= 0 && e0 <= a.n - VE) {
-            if constexpr (BF16) {
-                const uint4 w = *(const uint4 *)((const uint16_t *)xr + e0);
-                const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+        w[u] = make_uint4(0, 0, 0, 0);
+        if (inside || whole <= a.n - VE)
+            w[u] = *(const uint4 *)((const char *)xr + (ptrdiff_t)(is_whole(e0) ? e0 : whole) * (BF16 ? 2 : 4));
+    }
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    x[u * VE + 2 * j] = __uint_as_float(v[j] << 16);
-                    x[u * VE + 2 * j + 1] = __uint_as_float(v[j] & 0xFFFF0000u);
-                }
+    for (int u = 0; u < U; u++) {
+        const int e0 = id_of(u * VE);
+        const uint32_t v[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if constexpr (BF16) {
+                x[u * VE + 2 * j] = __uint_as_float(v[j] << 16);
+                x[u * VE + 2 * j + 1] = __uint_as_float(v[j] & 0xFFFF0000u);
             } else {
-                const float4 w = *(const float4 *)((const float *)xr + e0);
-                x[u * VE] = w.x;
-                x[u * VE + 1] = w.y;
-                x[u * VE + 2] = w.z;
-                x[u * VE + 3] = w.w;
+                x[u * VE + j] = __uint_as_float(v[j]);
             }
-        } else {
+        }
+        if (!inside && !is_whole(e0)) {
 #pragma unroll
             for (int j = 0; j < VE; j++)
-                x[u * VE + j] = e0 + j >= 0 && e0 + j < a.n ? logit<BF16>(xr, e0 + j) : -INFINITY;
+                x[u * VE + j] = -INFINITY;
+            if (e0 > -VE && e0 < a.n) {
+                float y[VE];
+#pragma unroll
+                for (int j = 0; j < VE; j++)
+                    y[j] = logit<BF16>(xr, min(max(e0 + j, 0), a.n - 1));
+#pragma unroll
+                for (int j = 0; j < VE; j++)
+                    x[u * VE + j] = e0 + j >= 0 && e0 + j < a.n ? y[j] : -INFINITY;
+            }
         }
     }
-    float mt = -INFINITY;
+    float mg[kScoreE / kGroup], mt = -INFINITY;     // maxima of groups of entries, and of all
 #pragma unroll
-    for (int i = 0; i < kScoreE; i++)
-        mt = fmaxf(mt, x[i]);
-    const float m = wave_max(mt), mf = m == -INFINITY ? 0.0f : m;
+    for (int g = 0; g < kScoreE / kGroup; g++) {
+        mg[g] = x[g * kGroup];
+#pragma unroll
+        for (int i = 1; i < kGroup; i++)
+            mg[g] = fmaxf(mg[g], x[g * kGroup + i]);
+        mt = fmaxf(mt, mg[g]);
+    }
+    const float m = wave_top(mt), mf = m == -INFINITY ? 0.0f : m;
     float s = 0.0f, t = 0.0f;
 #pragma unroll
     for (int i = 0; i < kScoreE; i++) {
@@ -202,8 +246,8 @@ __global__ __launch_bounds__(kScoreT) void k_score_slice(const ScoreArgs a)
         s += e;
         t = __fmaf_rn(e, fmaxf(z, -200.0f), t);
     }
-    s = wave_sum(s);
-    t = wave_sum(t);
+    s = wave_sum_dpp(s);
+    t = wave_sum_dpp(t);
     if (lane == 0)
         part[wave] = make_float4(m, s, t, 0.0f);
     tops[tid] = order_bits(mt);
@@ -239,13 +283,8 @@ __global__ __launch_bounds__(kScoreT) void k_score_slice(const ScoreArgs a)
         lo = min(lo, q[w]);
         hi = max(hi, q[w]);
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        lo = min(lo, (uint32_t)__shfl_xor((int)lo, o, kWave));
-        hi = max(hi, (uint32_t)__shfl_xor((int)hi, o, kWave));
-    }
-    lo = __builtin_amdgcn_readfirstlane(lo);
-    hi = __builtin_amdgcn_readfirstlane(hi) + 1;
+    lo = ~wave_top_u(~lo);
+    hi = wave_top_u(hi) + 1;
     int reach = kScoreT;
     while (hi - lo > 1 && reach > k + k / 4) {
         const uint32_t mid = lo + (hi - lo) / 2;
@@ -260,18 +299,20 @@ __global__ __launch_bounds__(kScoreT) void k_score_slice(const ScoreArgs a)
             hi = mid;
         }
     }
-    if (order_bits(mt) >= lo) {
-        const float bound = key_value((unsigned long long)lo << 32);
+    const float bound = key_value((unsigned long long)lo << 32);
 #pragma unroll
-        for (int i = 0; i < kScoreE; i++) {
-            const int id = id_of(i);
-            if (!(x[i] < bound) && id >= 0 && id < a.n) {
-                const int at = atomicAdd(&n_cand, 1);
-                if (at < kScoreCand)
-                    cand[at] = order_key(x[i], id);
+    for (int g = 0; g < kScoreE / kGroup; g++)
+        // (a group of nothing but NaN has the maximum NaN)
+        if (!(mg[g] < bound))
+#pragma unroll
+            for (int i = g * kGroup; i < (g + 1) * kGroup; i++) {
+                const int id = id_of(i);
+                if (!(x[i] < bound) && (inside || (id >= 0 && id < a.n))) {
+                    const int at = atomicAdd(&n_cand, 1);
+                    if (at < kScoreCand)
+                        cand[at] = order_key(x[i], id);
+                }
             }
-        }
-    }
     __syncthreads();
     const int found = n_cand;
     auto out = [&](int rank, unsigned long long key) {
@@ -319,7 +360,7 @@ __global__ __launch_bounds__(kScoreT) void k_score_join(const ScoreArgs a)
         if (k)
             bound = larger(bound, keys[(size_t)i * k + k - 1]);
     }
-    m = wave_max(m);
+    m = wave_top(m);
     for (int o = 32; o > 0; o >>= 1)
         bound = larger(bound, __shfl_xor(bound, o, kWave));
     if (lane == 0) {

@@ -187,16 +187,21 @@ class Lib:
         self.init()
         self.check(getattr(self.lib, name)(*args), name)
 
-    def _device_call(self, dev, name, *args):
-        """_call on device `dev` (that of the call's tensors) and its current
-        stream, which is the call's last argument."""
-        t = self.torch
-        if dev.type != "cuda":
-            raise Be42Error(f"{name}: tensors on {dev}, not on a GPU")
-        if dev.index == t.cuda.current_device():
-            return self._call(name, *args, self.stream())
-        with t.cuda.device(dev):
-            self._call(name, *args, self.stream())
+    def _device_call(self, x, name, *args):
+        """Entry point `name` on x's device and that device's current stream,
+        which is its last argument.  (Plain integers for pointers and the raw
+        stream: made of objects a call takes 4 us longer than its kernel.)"""
+        if not x.is_cuda:
+            raise Be42Error(f"{name}: tensors on {x.device}, not on a GPU")
+        self.init()
+        dev, t = x.get_device(), self.torch
+        if dev == t._C._cuda_getDevice():
+            rc = getattr(self.lib, name)(*args, t._C._cuda_getCurrentRawStream(dev))
+        else:
+            with t.cuda.device(dev):
+                rc = getattr(self.lib, name)(*args, t._C._cuda_getCurrentRawStream(dev))
+        if rc != BE42_OK:
+            self.check(rc, name)
 
     @staticmethod
     def _want(name, what, x, dtypes, shape=None, dev=None):
@@ -206,7 +211,7 @@ class Lib:
             raise Be42Error(f"{name}: {what} is {x.dtype}")
         if dev is not None and x.device != dev:
             raise Be42Error(f"{name}: {what} is on {x.device}, not on {dev}")
-        if shape is not None and (x.dim() != len(shape) or any(w is not None and w != n for w, n in zip(shape, x.shape))):
+        if shape is not None and x.shape != shape:
             raise Be42Error(f"{name}: {what} has shape {tuple(x.shape)}")
         if not x.is_contiguous():
             raise Be42Error(f"{name}: {what} is not contiguous")
@@ -261,8 +266,9 @@ class Lib:
         self._want(name, "w", w, (t.bfloat16,), (cols,), dev)
         q = t.empty((rows, cols), dtype=t.int8 if kind == "int8" else t.uint8, device=dev)
         s = t.empty(rows, dtype=t.float32, device=dev)
-        self._device_call(dev, name, self.p(q), self.p(s), self.p(sum), self.p(x), xs, self.p(residual), rs,
-                          int(dt == t.bfloat16), self.p(w), rows, cols, float(eps))
+        self._device_call(x, name, q.data_ptr(), s.data_ptr(), None if sum is None else sum.data_ptr(), x.data_ptr(), xs,
+                          None if residual is None else residual.data_ptr(), rs, dt == t.bfloat16, w.data_ptr(), rows,
+                          cols, eps)
         return q, s, sum
 
     def dequant_rows_int8(self, q, s):
@@ -413,8 +419,10 @@ class Lib:
         rows, n = logits.shape
         got, given = {}, 0
         if tokens is not None:
-            self._want(name, "tokens", tokens, (t.int32,), (rows, None), dev)
+            if tokens.dim() != 2:
+                raise Be42Error(f"{name}: tokens has shape {tuple(tokens.shape)}")
             given = tokens.shape[1]
+            self._want(name, "tokens", tokens, (t.int32,), (rows, given), dev)
             got["logprobs"] = t.empty((rows, given), dtype=t.float32, device=dev)
         if entropy:
             got["entropy"] = t.empty(rows, dtype=t.float32, device=dev)
@@ -423,12 +431,12 @@ class Lib:
             got["top_logprobs"] = t.empty((rows, top_k), dtype=t.float32, device=dev)
         ws, wsb = None, 0
         if workspace is not None:
-            self._want(name, "workspace", workspace, (t.uint8,), (None,), dev)
-            ws, wsb = self.p(workspace), workspace.numel()
-        self._device_call(dev, name, self.p(got.get("logprobs")), self.p(got.get("entropy")),
-                          self.p(got.get("top_ids")), self.p(got.get("top_logprobs")), self.p(logits),
-                          int(logits.dtype == t.bfloat16), ls, n, rows, float(temp), self.p(tokens), given, int(top_k),
-                          ws, wsb)
+            self._want(name, "workspace", workspace, (t.uint8,), None, dev)
+            ws, wsb = workspace.data_ptr(), workspace.numel()
+        at = {k: v.data_ptr() for k, v in got.items()}
+        self._device_call(logits, name, at.get("logprobs"), at.get("entropy"), at.get("top_ids"), at.get("top_logprobs"),
+                          logits.data_ptr(), logits.dtype == t.bfloat16, ls, n, rows, temp,
+                          None if tokens is None else tokens.data_ptr(), given, top_k, ws, wsb)
         return got
 
     def kv_pool(self, kind, n_layers, n_kv, head_dim, max_logical, hpT=None):
@@ -496,11 +504,11 @@ class Lib:
             max_len = pool.max_logical * 16
         ws, wsb = None, 0
         if workspace is not None:
-            self._want(name, "workspace", workspace, (t.uint8,), (None,), q.device)
-            ws, wsb = self.p(workspace), workspace.numel()
-        self._device_call(q.device, name, pool.handle, self.p(q), int(q.dtype == t.bfloat16), qs, B, H,
-                          int(prefix_slot), int(prefix_len), self.p(slots), self.p(lens), int(max_len), float(scale),
-                          self.p(out), ws, wsb)
+            self._want(name, "workspace", workspace, (t.uint8,), None, q.device)
+            ws, wsb = workspace.data_ptr(), workspace.numel()
+        self._device_call(q, name, pool.handle, q.data_ptr(), q.dtype == t.bfloat16, qs, B, H, prefix_slot, prefix_len,
+                          None if slots is None else slots.data_ptr(), None if lens is None else lens.data_ptr(), max_len,
+                          scale, out.data_ptr(), ws, wsb)
         return out
 
     # -- linear KV cache [T][n_kv][head_dim] bf16 (kv_cache.c) ------------------

@@ -1,11 +1,19 @@
 // score.hip -- log probabilities of given tokens, entropy and the top
 // alternatives of logits rows.
 //
-// With z = (x - m) / T, m the row's maximum, s = sum e^z and t = sum z e^z:
-//   log p(i) = z_i - log s,   H = log s - t / s.
-// A row is cut into slices that one workgroup holds in registers, so that it
-// is read once: each slice leaves its m, s, t and its top_k largest entries,
-// and a second launch (none where a row is one slice) joins a row's slices.
+// With exponents to base 2, c = log2(e) / T, z = (x - m) c for the largest entry
+// m, s = sum 2^z and t = sum 2^z z:
+//   log p(i) = ln 2 (z_i - log2 s),   H = ln 2 (log2 s - t / s).
+// A workgroup reads a run of a row once.  Its waves take chunks of 64 x 8 words
+// of 16 bytes in turn and keep s and t of each lane and the largest entries so
+// far; they share a bound that top_k entries are known to reach, so that few
+// entries past the first chunks are looked at again.  A second launch (none
+// where a row is one run) joins the runs of a row.  Sums of lanes, waves and
+// runs are joined in 64 bits.
+//
+// Instruction bound for bf16 (an entry costs a shift or mask, half a maximum, a
+// difference, a product, the exponential -- four times as long as another
+// instruction --, an add and an fma), memory bound for fp32.
 #include <algorithm>
 #include <cmath>
 
@@ -14,12 +22,11 @@
 namespace be42 {
 
 constexpr int kTopMax = 64;
-constexpr int kScoreT = 256, kScoreW = kScoreT / kWave;
-constexpr int kScoreE = 32;                 // entries a thread holds
-constexpr int kGroup = 8;                   // entries that are looked through together
-constexpr int kSlice = kScoreT * kScoreE;
-constexpr int kScoreCand = 512;             // candidates of a slice that are ranked together
-constexpr int kJoinCand = 1024;             // of a row's slices
+constexpr int kScoreW = 4;                  // waves of a workgroup, each on its own
+constexpr int kScoreU = 8;                  // words of 16 bytes a lane holds
+constexpr int kChunkBytes = kWave * kScoreU * 16;
+constexpr int kTopCap = 576;                // a wave's candidates: top_k, and the entries of 64 words
+constexpr int kJoinKeys = 8;                // keys of the runs that a lane of the joining wave holds
 
 // One number per (value, id) that is larger for a larger value, then for a
 // lower id: the value's bits as an order-preserving integer, then ~id.  -0 is
@@ -39,6 +46,14 @@ __device__ __forceinline__ float key_value(unsigned long long k)
     const uint32_t o = (uint32_t)(k >> 32);
     return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
 }
+__device__ __forceinline__ unsigned long long larger(unsigned long long p, unsigned long long q) { return p > q ? p : q; }
+
+// s and t of a set of entries and m c, which they count from (-infinity: no
+// entry but -infinity)
+struct Sums {
+    double ref;
+    float s, t;
+};
 
 struct ScoreArgs {
     const void *logits;
@@ -46,10 +61,11 @@ struct ScoreArgs {
     float *lp, *entropy, *top_lp;
     int *top_ids;
     const int *tokens;
-    int n_tokens, top_k, n, slices;
-    float temp, c;                          // c = log2(e) / T: exponents are kept in base 2
-    float4 *stats;                          // [rows][slices]: m, s, t (of base-2 exponents)
-    unsigned long long *keys;               // [rows][slices][top_k], descending
+    int n_tokens, top_k, n;
+    float c;
+    int chunks, per, runs;                  // chunks of a row, of a run, runs of a row
+    Sums *sums;                             // [rows][runs]
+    unsigned long long *keys;               // [rows][runs][top_k], descending, 0 past the last entry
 };
 
 template <bool BF16>
@@ -64,19 +80,19 @@ __device__ __forceinline__ const void *row_of(const ScoreArgs &a, int row)
     return (const char *)a.logits + (size_t)row * a.row_stride * (BF16 ? 2 : 4);
 }
 
-// What a row's sums say: log s is NaN for a row without a distribution (s is
-// NaN where an entry was NaN or +infinity).
+// What a row's sums say: NaN for a row without a distribution (s is NaN or
+// infinite where an entry was NaN or +infinity).
 struct RowSums {
-    double m, ls, H;
+    double base, H;                         // log p(x) = ln 2 (x c - base)
 };
-__device__ __forceinline__ RowSums row_sums(float m, double s, double t)
+__device__ __forceinline__ RowSums row_sums(double ref, double s, double t)
 {
-    const double ls = m == -INFINITY ? (double)NAN : log(s);
-    return {m, ls, ls - t / s * 0.69314718055994530942};
+    const double ls = ref > -INFINITY && s < INFINITY ? log2(s) : (double)NAN;
+    return {ref + ls, (ls - t / s) * 0.69314718055994530942};
 }
 __device__ __forceinline__ float log_prob(const ScoreArgs &a, const RowSums &r, float x)
 {
-    return r.ls != r.ls ? NAN : (float)(((double)x - r.m) / (double)a.temp - r.ls);
+    return r.base != r.base ? NAN : (float)(((double)x * (double)a.c - r.base) * 0.69314718055994530942);
 }
 
 // the wave's largest value, in every lane (lane moves)
@@ -84,41 +100,47 @@ __device__ __forceinline__ float wave_top(float v)
 {
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wave_prefix_max(v)), 63));
 }
-template <int CTRL, int ROWMASK = 0xF>
-__device__ __forceinline__ uint32_t dpp_max_u(uint32_t v)
+
+// s and t under the reference `top` >= p.ref
+__device__ __forceinline__ void rebase(const Sums &p, double top, double &s, double &t)
 {
-    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWMASK, 0xF, false));
-}
-__device__ __forceinline__ uint32_t wave_top_u(uint32_t v)
-{
-    v = dpp_max_u<0x111>(v);          // row_shr:1, 2, 4, 8
-    v = dpp_max_u<0x112>(v);
-    v = dpp_max_u<0x114>(v);
-    v = dpp_max_u<0x118>(v);
-    v = dpp_max_u<0x142, 0xA>(v);     // row_bcast:15 into rows 1, 3
-    v = dpp_max_u<0x143, 0xC>(v);     // row_bcast:31 into rows 2, 3
-    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+    const double d = p.ref == -INFINITY ? 0.0 : p.ref - top;
+    const double w = (double)__builtin_amdgcn_exp2f((float)d);
+    s = w * p.s;
+    t = w * ((double)p.t + fmax(d, -1000.0) * p.s);
 }
 
-// One set of entries' m, s and t as they count under the maximum `top` of several.
-__device__ __forceinline__ void rebase(const ScoreArgs &a, const float4 &p, float top, double &s, double &t)
+// joins the lanes' sums; every lane gets the reference and the sums
+__device__ __forceinline__ void join_lanes(const Sums &mine, double &ref, double &s, double &t)
 {
-    const float d = p.x == -INFINITY ? 0.0f : (p.x - top) * a.c, w = __builtin_amdgcn_exp2f(d);
-    s = (double)w * p.y;
-    t = (double)w * ((double)p.z + (double)fmaxf(d, -200.0f) * p.y);
-}
-
-// the given tokens and the entropy of a row
-template <bool BF16>
-__device__ __forceinline__ void write_row(const ScoreArgs &a, int row, const RowSums &r, int tid, int threads)
-{
-    if (tid == 0 && a.entropy)
-        a.entropy[row] = (float)r.H;
-    for (int j = tid; j < a.n_tokens; j += threads) {
-        const int id = a.tokens[(size_t)row * a.n_tokens + j];
-        a.lp[(size_t)row * a.n_tokens + j] =
-            log_prob(a, r, id >= 0 && id < a.n ? logit<BF16>(row_of<BF16>(a, row), id) : -INFINITY);
+    ref = mine.ref;
+    for (int o = 32; o > 0; o >>= 1)
+        ref = fmax(ref, __shfl_xor(ref, o, kWave));
+    rebase(mine, ref, s, t);
+    for (int o = 32; o > 0; o >>= 1) {
+        s += __shfl_xor(s, o, kWave);
+        t += __shfl_xor(t, o, kWave);
     }
+}
+
+// the logit of given token j of a row (one outside the row: -infinity)
+template <bool BF16>
+__device__ __forceinline__ float given_logit(const ScoreArgs &a, int row, int j)
+{
+    const int id = a.tokens[(size_t)row * a.n_tokens + j];
+    return id >= 0 && id < a.n ? logit<BF16>(row_of<BF16>(a, row), id) : -INFINITY;
+}
+
+// the given tokens (x0: the logit of token `lane`) and the entropy of a row, by one wave
+template <bool BF16>
+__device__ __forceinline__ void write_row(const ScoreArgs &a, int row, const RowSums &r, int lane, float x0)
+{
+    if (lane == 0 && a.entropy)
+        a.entropy[row] = (float)r.H;
+    if (lane < a.n_tokens)
+        a.lp[(size_t)row * a.n_tokens + lane] = log_prob(a, r, x0);
+    for (int j = kWave + lane; j < a.n_tokens; j += kWave)
+        a.lp[(size_t)row * a.n_tokens + j] = log_prob(a, r, given_logit<BF16>(a, row, j));
 }
 
 __device__ __forceinline__ void write_top(const ScoreArgs &a, int row, const RowSums &r, int rank,
@@ -128,170 +150,183 @@ __device__ __forceinline__ void write_top(const ScoreArgs &a, int row, const Row
     a.top_lp[(size_t)row * a.top_k + rank] = log_prob(a, r, key_value(key));
 }
 
-__device__ __forceinline__ unsigned long long larger(unsigned long long p, unsigned long long q) { return p > q ? p : q; }
-
-// Calls out(rank, key) for the k largest of n distinct keys in LDS: a key's
-// rank is the number of larger ones.
-template <class F>
-__device__ __forceinline__ void rank_keys(const unsigned long long *cand, int n, int k, F &&out)
+// LDS written by other lanes of the wave before this point may be read after it
+__device__ __forceinline__ void wave_lds()
 {
-    for (int i = threadIdx.x; i < n; i += kScoreT) {
-        const unsigned long long mine = cand[i];
-        int rank = 0;
-        for (int j = 0; j < n; j++)
-            rank += cand[j] > mine;
-        if (rank < k)
-            out(rank, mine);
-    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
-// The same where there are too many keys to rank together: one after the
-// other, best(last) being the thread's largest key below `last` (0: none).
-template <class B, class F>
-__device__ __forceinline__ void pull_keys(unsigned long long *sh, int k, B &&best, F &&out)
+// Calls out(rank, key) for the k largest of the n <= N * 64 distinct keys that a
+// wave keeps in LDS (with room for 8 more): a key's rank is the number of larger
+// ones.  All keys are read before the first call.
+template <int N, class F>
+__device__ __forceinline__ void rank_keys(unsigned long long *cand, int n, int k, int lane, F &&out)
 {
-    unsigned long long last = ~0ull;
-    for (int r = 0; r < k; r++) {
-        unsigned long long b = best(last);
-        for (int o = 32; o > 0; o >>= 1)
-            b = larger(b, __shfl_xor(b, o, kWave));
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0)
-            sh[threadIdx.x >> 6] = b;
-        __syncthreads();
-        last = larger(larger(sh[0], sh[1]), larger(sh[2], sh[3]));
-        if (threadIdx.x == 0)
-            out(r, last);
-        if (last == 0)
-            last = 1;                       // nothing is left: the other ranks are 0 too
+    if (lane < 8)
+        cand[n + lane] = 0;
+    wave_lds();
+    unsigned long long mine[N];
+    int rank[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        mine[i] = lane + i * kWave < n ? cand[lane + i * kWave] : 0;
+        rank[i] = mine[i] ? 0 : k;
     }
+    for (int j = 0; j < n; j += 8)
+#pragma unroll
+        for (int x = 0; x < 8; x++) {
+            const unsigned long long other = cand[j + x];
+#pragma unroll
+            for (int i = 0; i < N; i++)
+                rank[i] += other > mine[i];
+        }
+    wave_lds();
+#pragma unroll
+    for (int i = 0; i < N; i++)
+        if (rank[i] < k)
+            out(rank[i], mine[i]);
+    wave_lds();
 }
 
-// One slice of a row: block (row, slice).  The candidates of the slice's top_k
-// are the entries not below a bound that at least top_k threads' maxima reach:
-// the bound is bisected over the 256 maxima until few more than top_k do.
+// A wave's run of a row.  Places past the row's ends are set to -1e30, which
+// adds nothing to the sums, and are left out of the maxima.
 template <bool BF16>
-__global__ __launch_bounds__(kScoreT) void k_score_slice(const ScoreArgs a)
-{
-    constexpr int VE = BF16 ? 8 : 4, U = kScoreE / VE;     // entries of a 16-byte word, words a thread
-    __shared__ float4 part[kScoreW];
-    __shared__ uint32_t tops[kScoreT];
-    __shared__ unsigned long long cand[kScoreCand];
-    __shared__ int n_cand;
-    const int row = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, k = a.top_k;
-    const void *xr = row_of<BF16>(a, row);
+struct Run {
+    static constexpr int VE = BF16 ? 8 : 4;    // entries of a word
+    static constexpr int kEntries = kWave * kScoreU * VE;
+    const void *xr;
+    int n, off, lane;
     // words lie on 16 bytes of memory: word w of the row holds entries VE w - off ..
-    const int off = (int)((uintptr_t)xr / (BF16 ? 2 : 4) % VE);
-    float x[kScoreE];
-    const int first = slice * kSlice - off;
-    auto id_of = [&](int i) { return first + (i / VE * kScoreT + tid) * VE + i % VE; };
-    // every thread loads whole words, all in flight together (one that is not
-    // wholly of the row reads the row's first whole word instead); entries of
-    // the words that the row's ends cut are then loaded singly
-    const bool inside = first >= 0 && first <= a.n - kSlice;
-    const int whole = off ? VE - off : 0;
-    auto is_whole = [&](int e0) { return inside || (e0 >= 0 && e0 <= a.n - VE); };
-    uint4 w[U];
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int e0 = id_of(u * VE);
-        w[u] = make_uint4(0, 0, 0, 0);
-        if (inside || whole <= a.n - VE)
-            w[u] = *(const uint4 *)((const char *)xr + (ptrdiff_t)(is_whole(e0) ? e0 : whole) * (BF16 ? 2 : 4));
+    __device__ __forceinline__ Run(const ScoreArgs &a, int row, int ln) : xr(row_of<BF16>(a, row)), n(a.n), lane(ln)
+    {
+        off = (int)((uintptr_t)xr / (BF16 ? 2 : 4) % VE);
     }
+    __device__ __forceinline__ int id(int chunk, int u, int j) const
+    {
+        return chunk * kEntries - off + (u * kWave + lane) * VE + j;
+    }
+    __device__ __forceinline__ bool inside(int chunk) const
+    {
+        return chunk * kEntries - off >= 0 && chunk * kEntries - off <= n - kEntries;
+    }
+    // All words in flight together.  One that is not wholly of the row reads the
+    // row's first whole word instead; entries of words that the row's ends cut
+    // are then loaded singly.
+    __device__ __forceinline__ void load(int chunk, uint4 (&w)[kScoreU]) const
+    {
+        const char *base = (const char *)xr;
+        if (inside(chunk)) {
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int e0 = id_of(u * VE);
-        const uint32_t v[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+            for (int u = 0; u < kScoreU; u++)
+                w[u] = *(const uint4 *)(base + (ptrdiff_t)id(chunk, u, 0) * (BF16 ? 2 : 4));
+            return;
+        }
+        const int whole = off ? VE - off : 0;
+        auto is_whole = [&](int e0) { return e0 >= 0 && e0 <= n - VE; };
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if constexpr (BF16) {
-                x[u * VE + 2 * j] = __uint_as_float(v[j] << 16);
-                x[u * VE + 2 * j + 1] = __uint_as_float(v[j] & 0xFFFF0000u);
+        for (int u = 0; u < kScoreU; u++) {
+            const int e0 = id(chunk, u, 0);
+            w[u] = make_uint4(0, 0, 0, 0);
+            if (whole <= n - VE)
+                w[u] = *(const uint4 *)(base + (ptrdiff_t)(is_whole(e0) ? e0 : whole) * (BF16 ? 2 : 4));
+        }
+        constexpr uint32_t none = BF16 ? 0xF14AF14Au : 0xF149F2CAu;
+#pragma unroll
+        for (int u = 0; u < kScoreU; u++) {
+            const int e0 = id(chunk, u, 0);
+            if (is_whole(e0))
+                continue;
+            w[u] = make_uint4(none, none, none, none);
+            if (e0 > -VE && e0 < n) {
+                uint32_t y[VE], z[4];
+#pragma unroll
+                for (int j = 0; j < VE; j++)
+                    y[j] = __float_as_uint(logit<BF16>(xr, min(max(e0 + j, 0), n - 1)));
+#pragma unroll
+                for (int j = 0; j < VE; j++)
+                    y[j] = e0 + j >= 0 && e0 + j < n ? y[j] : BF16 ? none & 0xFFFF0000u : none;
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    z[j] = BF16 ? y[2 * j % VE] >> 16 | y[(2 * j + 1) % VE] : y[j];
+                w[u] = make_uint4(z[0], z[1], z[2], z[3]);
+            }
+        }
+    }
+    // entry j of a word; of a bf16 pair's upper entry, `raw` leaves the lower one's bits behind it
+    static __device__ __forceinline__ float entry(const uint4 &v, int j, bool raw = false)
+    {
+        const int at = BF16 ? j / 2 : j;
+        const uint32_t part = at == 0 ? v.x : at == 1 ? v.y : at == 2 ? v.z : v.w;
+        return __uint_as_float(!BF16 || (raw && (j & 1)) ? part : j & 1 ? part & 0xFFFF0000u : part << 16);
+    }
+    // Maxima of a lane's words, and of all of them; raw: an infinity among bf16
+    // entries may be passed over (the bits behind an upper entry do not change
+    // which entry is the largest, but make an infinity a NaN).
+    __device__ __forceinline__ float tops(int chunk, const uint4 (&w)[kScoreU], float (&mg)[kScoreU], bool raw) const
+    {
+        float top = -INFINITY;
+        raw = raw && inside(chunk);
+#pragma unroll
+        for (int u = 0; u < kScoreU; u++) {
+            mg[u] = -INFINITY;
+            if (raw) {
+#pragma unroll
+                for (int j = 0; j < VE; j++)
+                    mg[u] = fmaxf(mg[u], entry(w[u], j, true));
+                if (BF16)
+                    mg[u] = __uint_as_float(__float_as_uint(mg[u]) & 0xFFFF0000u);
             } else {
-                x[u * VE + j] = __uint_as_float(v[j]);
-            }
-        }
-        if (!inside && !is_whole(e0)) {
-#pragma unroll
-            for (int j = 0; j < VE; j++)
-                x[u * VE + j] = -INFINITY;
-            if (e0 > -VE && e0 < a.n) {
-                float y[VE];
 #pragma unroll
                 for (int j = 0; j < VE; j++)
-                    y[j] = logit<BF16>(xr, min(max(e0 + j, 0), a.n - 1));
-#pragma unroll
-                for (int j = 0; j < VE; j++)
-                    x[u * VE + j] = e0 + j >= 0 && e0 + j < a.n ? y[j] : -INFINITY;
+                    mg[u] = fmaxf(mg[u], (unsigned)id(chunk, u, j) < (unsigned)n ? entry(w[u], j) : -INFINITY);
             }
+            top = fmaxf(top, mg[u]);
         }
+        return top;
     }
-    float mg[kScoreE / kGroup], mt = -INFINITY;     // maxima of groups of entries, and of all
-#pragma unroll
-    for (int g = 0; g < kScoreE / kGroup; g++) {
-        mg[g] = x[g * kGroup];
-#pragma unroll
-        for (int i = 1; i < kGroup; i++)
-            mg[g] = fmaxf(mg[g], x[g * kGroup + i]);
-        mt = fmaxf(mt, mg[g]);
-    }
-    const float m = wave_top(mt), mf = m == -INFINITY ? 0.0f : m;
-    float s = 0.0f, t = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kScoreE; i++) {
-        // an entry of -infinity adds 0 to t, not 0 * -infinity
-        const float z = (x[i] - mf) * a.c, e = __builtin_amdgcn_exp2f(z);
-        s += e;
-        t = __fmaf_rn(e, fmaxf(z, -200.0f), t);
-    }
-    s = wave_sum_dpp(s);
-    t = wave_sum_dpp(t);
-    if (lane == 0)
-        part[wave] = make_float4(m, s, t, 0.0f);
-    tops[tid] = order_bits(mt);
-    if (tid == 0)
-        n_cand = 0;
-    __syncthreads();
+};
 
-    const float top = fmaxf(fmaxf(part[0].x, part[1].x), fmaxf(part[2].x, part[3].x));
-    double bs = 0.0, bt = 0.0;
-    const bool single = a.slices == 1;
-    if (tid == 0 || single)
-        for (int w = 0; w < kScoreW; w++) {
-            double sw, tw;
-            rebase(a, part[w], top, sw, tw);
-            bs += sw;
-            bt += tw;
-        }
-    RowSums r = {};
-    if (single) {
-        r = row_sums(top, bs, bt);
-        write_row<BF16>(a, row, r, tid, kScoreT);
-    } else if (tid == 0) {
-        a.stats[blockIdx.x] = make_float4(top, (float)bs, (float)bt, 0.0f);
-    }
-    if (!k)
-        return;
-
-    // every wave bisects by itself: at least k maxima are >= lo, fewer than k >= hi
-    uint32_t q[kScoreW], lo = ~0u, hi = 0;
+// Makes the compiler take a chunk's words apart again at their next use: kept
+// apart, 64 bf16 entries a lane take 165 registers.
+__device__ __forceinline__ void keep_packed(uint4 (&w)[kScoreU])
+{
 #pragma unroll
-    for (int w = 0; w < kScoreW; w++) {
-        q[w] = tops[w * kWave + lane];
-        lo = min(lo, q[w]);
-        hi = max(hi, q[w]);
+    for (int u = 0; u < kScoreU; u++)
+        asm volatile("" : "+v"(w[u].x), "+v"(w[u].y), "+v"(w[u].z), "+v"(w[u].w));
+}
+
+// The largest entries of a wave's chunks, so far, in the wave's part of LDS: keys
+// of entries, words that have yet to be looked through, and a bound that top_k
+// entries of the run are known to reach, shared by the workgroup's waves as the
+// order bits of a value.  (They read and raise it without waiting for each
+// other: which entries are looked at depends on that, which are found does not.)
+// Only words are noted where they are seen, and read again in batches of 64:
+// looking into a word's entries there and then kept 64 bf16 entries apart in
+// 207 registers (2000 rows of 128256 with 5 alternatives 300 us).
+struct TopKeys {
+    unsigned long long *cand, least;        // candidates have keys > least
+    int *words;                             // indexes of 16-byte words of the row
+    uint32_t *shared;
+    int n, n_words;
+    __device__ __forceinline__ float bound() const
+    {
+        // (the lowest order bits of a number are those of -infinity)
+        return (uint32_t)(least >> 32) < 0x007FFFFFu ? -INFINITY : key_value(least);
     }
-    lo = ~wave_top_u(~lo);
-    hi = wave_top_u(hi) + 1;
-    int reach = kScoreT;
+};
+
+// The largest value, or one with few more above, that at least k of the lanes'
+// N order bits reach (N * 64 >= k; lowest: one that they all reach).
+template <int N>
+__device__ __forceinline__ uint32_t reached(const uint32_t (&q)[N], int k, uint32_t lo, uint32_t hi)
+{
+    int reach = N * kWave;                  // at least k are >= lo, fewer than k >= hi
     while (hi - lo > 1 && reach > k + k / 4) {
         const uint32_t mid = lo + (hi - lo) / 2;
         int c = 0;
 #pragma unroll
-        for (int w = 0; w < kScoreW; w++)
-            c += __popcll(__ballot(q[w] >= mid));
+        for (int i = 0; i < N; i++)
+            c += __popcll(__ballot(q[i] >= mid));
         if (c >= k) {
             lo = mid;
             reach = c;
@@ -299,126 +334,281 @@ __global__ __launch_bounds__(kScoreT) void k_score_slice(const ScoreArgs a)
             hi = mid;
         }
     }
-    const float bound = key_value((unsigned long long)lo << 32);
+    return lo;
+}
+
+__device__ __forceinline__ void raise(TopKeys &T, unsigned long long least, int lane)
+{
+    if (least <= T.least)
+        return;
+    T.least = least;
+    if (lane == 0)
+        atomicMax(T.shared, (uint32_t)(least >> 32));
+}
+
+// leaves the k largest
+__device__ __forceinline__ void compress(TopKeys &T, int k, int lane)
+{
+    auto keep = [&](int rank, unsigned long long key) { T.cand[rank] = key; };
+    if (T.n <= kWave)
+        rank_keys<1>(T.cand, T.n, k, lane, keep);
+    else if (T.n <= 4 * kWave)
+        rank_keys<4>(T.cand, T.n, k, lane, keep);
+    else
+        rank_keys<kTopCap / kWave>(T.cand, T.n, k, lane, keep);
+    T.n = min(T.n, k);
+    if (T.n == k)
+        raise(T, T.cand[k - 1], lane);
+}
+
+// notes the words of a chunk that hold entries at the bound or above
+__device__ __forceinline__ void note(TopKeys &T, int chunk, const float (&mg)[kScoreU], float top, int k, int lane)
+{
+    T.least = larger(T.least, (unsigned long long)*(volatile uint32_t *)T.shared << 32);
+    float bound = T.bound();
+    const int reach = __popcll(__ballot(!(top < bound)));
+    if (!reach)
+        return;
+    if (reach > k + k / 4) {                // the first chunk, rising entries
+        const uint32_t q[1] = {order_bits(top)};
+        raise(T, (unsigned long long)reached<1>(q, k, 0, ~0u) << 32, lane);
+        bound = T.bound();
+    }
 #pragma unroll
-    for (int g = 0; g < kScoreE / kGroup; g++)
-        // (a group of nothing but NaN has the maximum NaN)
-        if (!(mg[g] < bound))
+    for (int u = 0; u < kScoreU; u++) {
+        const bool in = !(mg[u] < bound);
+        const unsigned long long who = __ballot(in);
+        if (in)
+            T.words[T.n_words + __popcll(who & ((1ull << lane) - 1))] = (chunk * kScoreU + u) * kWave + lane;
+        T.n_words += __popcll(who);
+    }
+}
+
+// looks through the noted words
+template <bool BF16>
+__device__ __forceinline__ void look(TopKeys &T, const Run<BF16> &run, int k, int lane)
+{
+    constexpr int VE = Run<BF16>::VE;
+    wave_lds();
+    for (int i0 = 0; i0 < T.n_words; i0 += kWave) {
+        const int first = i0 + lane < T.n_words ? T.words[i0 + lane] * VE - run.off : run.n;
+        float x[VE];
 #pragma unroll
-            for (int i = g * kGroup; i < (g + 1) * kGroup; i++) {
-                const int id = id_of(i);
-                if (!(x[i] < bound) && (inside || (id >= 0 && id < a.n))) {
-                    const int at = atomicAdd(&n_cand, 1);
-                    if (at < kScoreCand)
-                        cand[at] = order_key(x[i], id);
-                }
-            }
+        for (int j = 0; j < VE; j++)
+            x[j] = logit<BF16>(run.xr, min(max(first + j, 0), run.n - 1));
+#pragma unroll
+        for (int j = 0; j < VE; j++) {
+            const unsigned long long key = (unsigned)(first + j) < (unsigned)run.n ? order_key(x[j], first + j) : 0;
+            const unsigned long long who = __ballot(key > T.least);
+            if (key > T.least)
+                T.cand[T.n + __popcll(who & ((1ull << lane) - 1))] = key;
+            T.n += __popcll(who);
+        }
+        if (T.n > k)
+            compress(T, k, lane);
+    }
+    T.n_words = 0;
+}
+
+// block: (row, run)
+template <bool BF16>
+__global__ __launch_bounds__(kWave *kScoreW) void k_score_run(const ScoreArgs a)
+{
+    __shared__ unsigned long long lds[kScoreW][kTopCap + 8];
+    __shared__ int words[kScoreW][(kScoreU + 1) * kWave];
+    __shared__ unsigned long long merged[kScoreW * kTopMax + 8];
+    __shared__ Sums sums[kScoreW];
+    __shared__ uint32_t shared;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), k = a.top_k;
+    const int row = (int)(blockIdx.x / (unsigned)a.runs), part = (int)(blockIdx.x % (unsigned)a.runs);
+    const int c0 = part * a.per, c1 = min(c0 + a.per, a.chunks);
+    const Run<BF16> run(a, row, lane);
+    const bool single = a.runs == 1;
+    const float x0 = single && wave == 0 && lane < a.n_tokens ? given_logit<BF16>(a, row, lane) : 0.0f;
+    if (threadIdx.x == 0)
+        shared = 0;
     __syncthreads();
-    const int found = n_cand;
+    TopKeys T = {lds[wave], 0, words[wave], &shared, 0, 0};
+    uint4 w[kScoreU];
+    float mg[kScoreU];
+    // each lane by itself: its largest entry and its sums, z = (x - m) c
+    float m = -INFINITY, ref = 0.0f, s = 0.0f, t = 0.0f;
+    for (int c = c0 + wave; c < c1; c += kScoreW) {
+        run.load(c, w);
+        const float top = run.tops(c, w, mg, true);
+        keep_packed(w);
+        if (__any(top > m)) {
+            const float r2 = top > m ? top : ref, d = m == -INFINITY ? 0.0f : (ref - r2) * a.c;
+            const float f = __builtin_amdgcn_exp2f(d);
+            t = f * __fmaf_rn(fmaxf(d, -200.0f), s, t);
+            s *= f;
+            ref = r2;
+            m = fmaxf(m, top);
+        }
+        const float s0 = s, t0 = t;
+#pragma unroll
+        for (int u = 0; u < kScoreU; u++)
+#pragma unroll
+            for (int j = 0; j < Run<BF16>::VE; j++) {
+                const float z = (Run<BF16>::entry(w[u], j) - ref) * a.c, e = __builtin_amdgcn_exp2f(z);
+                s += e;
+                t = __fmaf_rn(e, z, t);
+            }
+        keep_packed(w);
+        if (__any(!(fabsf(t) < INFINITY))) {
+            // an entry of -infinity (0 * -infinity), or what has no distribution:
+            // again, exponents held where they underflow
+            s = s0;
+            t = t0;
+#pragma unroll
+            for (int u = 0; u < kScoreU; u++)
+#pragma unroll
+                for (int j = 0; j < Run<BF16>::VE; j++) {
+                    const float z = (Run<BF16>::entry(w[u], j) - ref) * a.c, e = __builtin_amdgcn_exp2f(z);
+                    s += e;
+                    t = __fmaf_rn(e, fmaxf(z, -200.0f), t);
+                }
+            keep_packed(w);
+        }
+        if (k) {
+            note(T, c, mg, top, k, lane);
+            if (T.n_words >= kWave || c + kScoreW >= c1)
+                look<BF16>(T, run, k, lane);
+        }
+    }
+    if (BF16 && k && __any(!(s < INFINITY))) {
+        // the maxima may have passed over +infinity
+        T = {lds[wave], 0, words[wave], &shared, 0, 0};
+        for (int c = c0 + wave; c < c1; c += kScoreW) {
+            run.load(c, w);
+            const float top = run.tops(c, w, mg, false);
+            note(T, c, mg, top, k, lane);
+            look<BF16>(T, run, k, lane);
+        }
+    }
+    const Sums mine = {(double)m * (double)a.c, s, t};
+    double rs, ss, tt;
+    join_lanes(mine, rs, ss, tt);
+    if (lane == 0)
+        sums[wave] = {rs, (float)ss, (float)tt};
+    if (lane < k)
+        merged[wave * k + lane] = lane < T.n ? T.cand[lane] : 0;
+    __syncthreads();
+    if (wave)
+        return;
+    join_lanes(lane < kScoreW ? sums[lane] : Sums{-INFINITY, 0.0f, 0.0f}, rs, ss, tt);
+    RowSums r = {};
+    if (single) {
+        r = row_sums(rs, ss, tt);
+        write_row<BF16>(a, row, r, lane, x0);
+    } else if (lane == 0) {
+        a.sums[blockIdx.x] = {rs, (float)ss, (float)tt};
+    }
+    if (!k)
+        return;
+    if (!single && lane < k)
+        a.keys[(size_t)blockIdx.x * k + lane] = 0;      // a row's last run may hold fewer than k entries
     auto out = [&](int rank, unsigned long long key) {
         if (single)
             write_top(a, row, r, rank, key);
         else
             a.keys[(size_t)blockIdx.x * k + rank] = key;
     };
-    if (found <= kScoreCand) {
-        rank_keys(cand, found, k, out);
-        for (int i = found + tid; i < k; i += kScoreT)
-            out(i, 0);                      // a row's last slice may hold fewer entries (a single one holds k)
-        return;
-    }
-    // ties, or large entries of few threads
-    pull_keys(cand, k,
-              [&](unsigned long long last) {
-                  unsigned long long best = 0;
-#pragma unroll
-                  for (int i = 0; i < kScoreE; i++) {
-                      const int id = id_of(i);
-                      const unsigned long long key = order_key(x[i], id);
-                      best = id >= 0 && id < a.n && key < last ? larger(best, key) : best;
-                  }
-                  return best;
-              },
-              out);
+    if (kScoreW * k <= kWave)
+        rank_keys<1>(merged, kScoreW * k, k, lane, out);
+    else if (kScoreW * k <= 2 * kWave)
+        rank_keys<2>(merged, kScoreW * k, k, lane, out);
+    else
+        rank_keys<kScoreW>(merged, kScoreW * k, k, lane, out);
 }
 
-// The slices of a row, one block a row.
+// The runs of a row, one wave a row.
 template <bool BF16>
-__global__ __launch_bounds__(kScoreT) void k_score_join(const ScoreArgs a)
+__global__ __launch_bounds__(kWave) void k_score_join(const ScoreArgs a)
 {
-    __shared__ double sums[2][kScoreW];
-    __shared__ float maxs[kScoreW];
-    __shared__ unsigned long long bounds[kScoreW], cand[kJoinCand];
-    __shared__ int n_cand;
-    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, k = a.top_k;
-    const float4 *st = a.stats + (size_t)row * a.slices;
-    const unsigned long long *keys = a.keys + (size_t)row * a.slices * k;
-    float m = -INFINITY;
-    unsigned long long bound = 0;           // the best slice's last key: k keys of the row reach it
-    for (int i = tid; i < a.slices; i += kScoreT) {
-        m = fmaxf(m, st[i].x);
-        if (k)
-            bound = larger(bound, keys[(size_t)i * k + k - 1]);
+    __shared__ unsigned long long cand[kJoinKeys * kWave + 8];
+    const int row = blockIdx.x, lane = threadIdx.x, k = a.top_k, all = a.runs * k;
+    const Sums *st = a.sums + (size_t)row * a.runs;
+    const unsigned long long *keys = a.keys + (size_t)row * all;
+    // a chain of dependent loads would be most of a short call: what the first
+    // 64 runs, 512 keys and 64 tokens need is asked for at once
+    Sums mine = {-INFINITY, 0.0f, 0.0f};
+    if (lane < a.runs)
+        mine = st[lane];
+    unsigned long long key[kJoinKeys];
+#pragma unroll
+    for (int x = 0; x < kJoinKeys; x++)
+        key[x] = x * kWave + lane < all ? keys[x * kWave + lane] : 0;
+    const float x0 = lane < a.n_tokens ? given_logit<BF16>(a, row, lane) : 0.0f;
+
+    for (int i = lane + kWave; i < a.runs; i += kWave) {
+        const Sums b = st[i];
+        const double top = fmax(mine.ref, b.ref);
+        double s, t, s2, t2;
+        rebase(mine, top, s, t);
+        rebase(b, top, s2, t2);
+        mine = {top, (float)(s + s2), (float)(t + t2)};
     }
-    m = wave_top(m);
-    for (int o = 32; o > 0; o >>= 1)
-        bound = larger(bound, __shfl_xor(bound, o, kWave));
-    if (lane == 0) {
-        maxs[wave] = m;
-        bounds[wave] = bound;
-    }
-    if (tid == 0)
-        n_cand = 0;
-    __syncthreads();
-    m = fmaxf(fmaxf(maxs[0], maxs[1]), fmaxf(maxs[2], maxs[3]));
-    bound = larger(larger(bounds[0], bounds[1]), larger(bounds[2], bounds[3]));
-    double s = 0.0, t = 0.0;
-    for (int i = tid; i < a.slices; i += kScoreT) {
-        double si, ti;
-        rebase(a, st[i], m, si, ti);
-        s += si;
-        t += ti;
-    }
-    for (int o = 32; o > 0; o >>= 1) {
-        s += __shfl_xor(s, o, kWave);
-        t += __shfl_xor(t, o, kWave);
-    }
-    if (lane == 0) {
-        sums[0][wave] = s;
-        sums[1][wave] = t;
-    }
-    const int all = a.slices * k;
-    for (int i = tid; i < all; i += kScoreT) {
-        const unsigned long long key = keys[i];
-        if (key && key >= bound) {
-            const int at = atomicAdd(&n_cand, 1);
-            if (at < kJoinCand)
-                cand[at] = key;
-        }
-    }
-    __syncthreads();
-    const RowSums r = row_sums(m, (sums[0][0] + sums[0][1]) + (sums[0][2] + sums[0][3]),
-                               (sums[1][0] + sums[1][1]) + (sums[1][2] + sums[1][3]));
-    write_row<BF16>(a, row, r, tid, kScoreT);
+    double ref, s, t;
+    join_lanes(mine, ref, s, t);
+    const RowSums r = row_sums(ref, s, t);
+    write_row<BF16>(a, row, r, lane, x0);
     if (!k)
         return;
-    const int found = n_cand;
-    auto out = [&](int rank, unsigned long long key) { write_top(a, row, r, rank, key); };
-    if (found <= kJoinCand)
-        rank_keys(cand, found, k, out);
-    else
-        pull_keys(cand, k,
-                  [&](unsigned long long last) {
-                      unsigned long long best = 0;
-                      for (int i = tid; i < all; i += kScoreT)
-                          best = keys[i] < last ? larger(best, keys[i]) : best;
-                      return best;
-                  },
-                  out);
+    // the keys that reach a value which few more than k do; keys past those that
+    // the lanes hold replace them in turn
+    for (int i0 = kJoinKeys * kWave;; i0 += (kJoinKeys - 1) * kWave) {
+        uint32_t q[kJoinKeys];
+#pragma unroll
+        for (int x = 0; x < kJoinKeys; x++)
+            q[x] = (uint32_t)(key[x] >> 32);
+        const uint32_t lo = reached<kJoinKeys>(q, k, 0, ~0u);
+        int found = 0;
+#pragma unroll
+        for (int x = 0; x < kJoinKeys; x++) {
+            const unsigned long long who = __ballot(key[x] && q[x] >= lo);
+            if (key[x] && q[x] >= lo)
+                cand[found + __popcll(who & ((1ull << lane) - 1))] = key[x];
+            found += __popcll(who);
+        }
+        const bool last = i0 >= all;
+        auto out = [&](int rank, unsigned long long kk) {
+            if (last)
+                write_top(a, row, r, rank, kk);
+            else
+                cand[rank] = kk;
+        };
+        if (found <= kWave)
+            rank_keys<1>(cand, found, k, lane, out);
+        else
+            rank_keys<kJoinKeys>(cand, found, k, lane, out);
+        if (last)
+            return;
+        key[0] = lane < min(found, k) ? cand[lane] : 0;
+#pragma unroll
+        for (int x = 1; x < kJoinKeys; x++) {
+            const int i = i0 + (x - 1) * kWave + lane;
+            key[x] = i < all ? keys[i] : 0;
+        }
+        wave_lds();
+    }
 }
 
-// Slices of a row of n entries, whose first word may begin before it.
-static long score_slices(int n) { return ((long)n + 7 + kSlice - 1) / kSlice; }
+// How a row of n entries is cut: chunks (the first word may begin `before`
+// entries before the row), chunks of a run, runs.  Rows are cut until there are
+// four workgroups a CU; a run has at least a chunk for each wave, and four where
+// the rows alone fill the chip, since joining runs costs a launch of 4 us (333
+// rows of 32003 fp32, half of them masked: 13 us as one run, 17 as three; 1000
+// rows of 128256: 98 and 95).
+static void cut_row(int n, int before, int rows, bool bf16, long *chunks, long *per, long *runs)
+{
+    const long entries = kChunkBytes / (bf16 ? 2 : 4);
+    *chunks = (n + before + entries - 1) / entries;
+    const long least = rows >= 256 ? 4 * kScoreW : kScoreW;
+    *runs = std::min((*chunks + least - 1) / least, (1024 + (long)rows - 1) / rows);
+    *per = (*chunks + *runs - 1) / *runs;
+    *runs = (*chunks + *per - 1) / *per;
+}
 
 }  // namespace be42
 
@@ -428,16 +618,23 @@ extern "C" size_t be42_logprobs_workspace_bytes(int n, int rows, int top_k)
 {
     if (n <= 0 || rows <= 0 || top_k < 0 || top_k > kTopMax || top_k > n)
         return 0;
-    const size_t per = (size_t)rows * score_slices(n);
-    return per * (sizeof(float4) + top_k * sizeof(unsigned long long));
+    size_t most = 0;                        // of either type
+    for (int i = 0; i < 4; i++) {           // and alignment
+        long chunks, per, runs;
+        cut_row(n, i & 1 ? 7 : 0, rows, i >> 1, &chunks, &per, &runs);
+        most = std::max(most, (size_t)rows * runs);
+    }
+    return most * (sizeof(Sums) + top_k * sizeof(unsigned long long));
 }
 
 extern "C" int be42_logprobs(float *logprobs, float *entropy, int *top_ids, float *top_logprobs, const void *logits,
                              int logits_bf16, int row_stride, int n, int rows, float temp, const int *tokens,
                              int n_tokens, int top_k, void *workspace, size_t workspace_bytes, void *stream)
 {
-    BE42_CHECK(n > 0 && n <= 1 << 30 && rows >= 0 && row_stride >= n, "be42_logprobs: %d rows of %d at stride %d", rows, n, row_stride);
-    BE42_CHECK(temp > 0.0f && std::isfinite(temp) && std::isfinite(1.0f / temp), "be42_logprobs: temperature %g",
+    BE42_CHECK(n > 0 && n <= 1 << 30 && rows >= 0 && row_stride >= n, "be42_logprobs: %d rows of %d at stride %d", rows,
+               n, row_stride);
+    const float c = (float)(1.44269504088896340736 / (double)temp);
+    BE42_CHECK(temp > 0.0f && std::isfinite(temp) && std::isfinite(c) && c >= 1e-30f, "be42_logprobs: temperature %g",
                (double)temp);
     if (rows == 0)
         return BE42_OK;
@@ -452,29 +649,33 @@ extern "C" int be42_logprobs(float *logprobs, float *entropy, int *top_ids, floa
     const size_t need = be42_logprobs_workspace_bytes(n, rows, top_k);
     BE42_CHECK(!workspace || (!((uintptr_t)workspace & 15) && workspace_bytes >= need),
                "be42_logprobs: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, need);
-    const long slices = score_slices(n), blocks = slices * rows;
+    long chunks, per, runs;
+    const bool aligned = !((uintptr_t)logits & 15) && row_stride % (logits_bf16 ? 8 : 4) == 0;
+    cut_row(n, aligned ? 0 : 7, rows, logits_bf16 != 0, &chunks, &per, &runs);
+    const long blocks = runs * rows;
     BE42_CHECK(blocks <= 0x7FFFFFFF, "be42_logprobs: %d rows of %d", rows, n);
-    ScoreArgs a = {logits, (size_t)row_stride, logprobs, entropy, top_logprobs, top_ids, tokens, n_tokens, top_k, n,
-                   (int)slices, temp, (float)(1.44269504088896340736 / (double)temp)};
+    ScoreArgs a = {logits, (size_t)row_stride, logprobs, entropy, top_logprobs, top_ids, tokens, n_tokens, top_k, n, c,
+                   (int)chunks, (int)per, (int)runs};
     hipStream_t s = as_stream(stream);
-    if (slices > 1) {
+    if (runs > 1) {
         if (!workspace)
             workspace = be42::workspace(need, s);
         if (!workspace)
             return BE42_ENOMEM;
-        a.stats = (float4 *)workspace;
-        a.keys = (unsigned long long *)(a.stats + blocks);
+        a.sums = (Sums *)workspace;
+        a.keys = (unsigned long long *)(a.sums + blocks);
     }
-    const dim3 g((unsigned)blocks), t(kScoreT);
+    const dim3 g((unsigned)blocks), t(kWave * kScoreW);
     if (logits_bf16)
-        hipLaunchKernelGGL(k_score_slice<true>, g, t, 0, s, a);
+        hipLaunchKernelGGL(k_score_run<true>, g, t, 0, s, a);
     else
-        hipLaunchKernelGGL(k_score_slice<false>, g, t, 0, s, a);
-    if (slices > 1) {
+        hipLaunchKernelGGL(k_score_run<false>, g, t, 0, s, a);
+    if (runs > 1) {
+        const dim3 w(kWave);
         if (logits_bf16)
-            hipLaunchKernelGGL(k_score_join<true>, dim3(rows), t, 0, s, a);
+            hipLaunchKernelGGL(k_score_join<true>, dim3(rows), w, 0, s, a);
         else
-            hipLaunchKernelGGL(k_score_join<false>, dim3(rows), t, 0, s, a);
+            hipLaunchKernelGGL(k_score_join<false>, dim3(rows), w, 0, s, a);
     }
     BE42_LAUNCH_CHECK();
     return BE42_OK;

@@ -13,6 +13,7 @@
 // pages are read once for 16 rows.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "be42_common.h"
 #include "paged_dev.h"
@@ -31,9 +32,10 @@ struct PrefixArgs {
     size_t q_stride;
     int n_queries, n_heads, prefix_slot, prefix_len, max_len;
     float scale;
-    // the cut: parts of the prefix and of the own tokens, tokens of each, and
-    // tiles of 16 rows that a KV head has over the prefix and over one query
-    int parts_p, parts_o, chunk_p, chunk_o, tiles_p, tiles_o;
+    // the cut: parts of the prefix and of the own tokens, tokens of each, tiles of
+    // rows that a KV head has over the prefix and over one query (of 16), and rows
+    // of a prefix tile
+    int parts_p, parts_o, chunk_p, chunk_o, tiles_p, tiles_o, rows_p;
 };
 
 // tokens a slot holds (0 for a slot outside the pool)
@@ -91,6 +93,67 @@ __device__ __forceinline__ v4f mfma16(bf16x8 a, bf16x8 b, v4f c)
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
+__device__ __forceinline__ v16f mfma32(bf16x8 a, bf16x8 b, v16f c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// eight elements of a query row from element `at` on, in NP parts, negated for a
+// negative scale
+template <int NP>
+__device__ __forceinline__ void load_q(const PrefixArgs &a, size_t at, bf16x8 (&Q)[NP])
+{
+    const bool flip = a.scale < 0.0f;
+    if constexpr (NP == 1) {
+        uint32_t w[4];
+        __builtin_memcpy(w, (const uint16_t *)a.q + at, 16);
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            w[j] ^= flip ? 0x80008000u : 0u;
+        Q[0] = __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+    } else {
+        float x[8];
+        __builtin_memcpy(x, (const float *)a.q + at, 32);
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            x[j] = flip ? -x[j] : x[j];
+        split8<NP>(x, Q);
+    }
+}
+
+// The largest of three, NaN if one is.  (fmaxf adds a canonicalizing move for
+// each operand; in inline assembly the wait states after a matrix product would
+// be missing.)
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
+}
+
+// x and the other half's x (lane ^ 32), in either order; with quarters of a wave
+// (lane ^ 16) likewise
+__device__ __forceinline__ void halves(float x, float &a, float &b)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    a = __uint_as_float(r[0]);
+    b = __uint_as_float(r[1]);
+}
+__device__ __forceinline__ void quarters(float x, float &a, float &b)
+{
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    a = __uint_as_float(r[0]);
+    b = __uint_as_float(r[1]);
+}
+
+// A read of LDS that direct-to-LDS loads fill, after the barrier that waited for
+// them.  The argument's promise not to alias keeps the compiler from waiting for
+// every such load in flight before each read (32 us a pass at 32 queries over
+// 8192 tokens, 21 without).
+template <class T>
+__device__ __forceinline__ T ring_read(const void *__restrict__ p)
+{
+    return *(const T *)p;
+}
+
 constexpr int kPartWaves = 4;
 constexpr int kStep = 32;         // tokens of a wave's step: two pages
 
@@ -123,26 +186,9 @@ __device__ __forceinline__ void part16(const be42_kv_pool &P, const PrefixArgs &
     {
         const int ri = min(row0 + c, rows - 1);
         const size_t at = (size_t)(b0 + ri / G) * a.q_stride + (size_t)(kvh * G + ri % G) * HD;
-        const bool flip = a.scale < 0.0f;
 #pragma unroll
-        for (int kb = 0; kb < NK; kb++) {
-            const int d = KV8 ? 64 * (kb / 2) + 16 * g + 8 * (kb % 2) : 32 * kb + 8 * g;
-            if constexpr (NP == 1) {
-                uint32_t w[4];
-                __builtin_memcpy(w, (const uint16_t *)a.q + at + d, 16);
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    w[j] ^= flip ? 0x80008000u : 0u;
-                Q[kb][0] = __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
-            } else {
-                float x[8];
-                __builtin_memcpy(x, (const float *)a.q + at + d, 32);
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-                    x[j] = flip ? -x[j] : x[j];
-                split8<NP>(x, Q[kb]);
-            }
-        }
+        for (int kb = 0; kb < NK; kb++)
+            load_q<NP>(a, at + (KV8 ? 64 * (kb / 2) + 16 * g + 8 * (kb % 2) : 32 * kb + 8 * g), Q[kb]);
     }
     const float sc = fabsf(a.scale) * 1.44269504088896340736f;
 
@@ -242,10 +288,11 @@ __device__ __forceinline__ void part16(const be42_kv_pool &P, const PrefixArgs &
                 if (KV8)
                     vsc[j] = out ? 0.0f : vsc[j];
             }
-        float top = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
-        top = fmaxf(top, __shfl_xor(top, 16, kWave));
-        top = fmaxf(top, __shfl_xor(top, 32, kWave));
-        const float mn = fmaxf(m, top * sc);
+        float top = max3(max3(p[0], p[1], p[2]), max3(p[3], p[4], p[5]), max3(p[6], p[7], p[7])), other;
+        quarters(top, top, other);
+        top = max3(top, other, other);
+        halves(top, top, other);
+        const float mn = fmaxf(m, max3(top, other, other) * sc);
         if (__any(mn > m)) {
             const float f = __builtin_amdgcn_exp2f(m - mn);
             l *= f;
@@ -336,12 +383,293 @@ __device__ __forceinline__ void store_out4(void *out, size_t at, float4 v)
     }
 }
 
+// ---- many rows ------------------------------------------------------------------
+// Rows of the prefix in 32x32 tiles, a wave for 32 of the workgroup's 128 rows;
+// the waves share each step's two pages through a ring in LDS, which
+// direct-to-LDS loads fill kRing - 1 steps ahead.  The products are transposed
+// as in part16: a lane keeps query row c = lane % 32, and with h = lane / 32 its
+// sixteen scores are tokens 8 h .. 8 h + 7 of the first page, then of the second
+// (operand row i is token 8 (i / 4 % 2) + 4 (i / 8 % 2) + i % 4 of page i / 16).
+#ifndef RING
+#define RING 4
+#define WFROM 32
+#define WMIN 4
+#define WWANT 256
+#endif
+constexpr int kRing = RING, kWideFrom = WFROM, kWideMin = WMIN, kWideWant = WWANT;
+constexpr int kWideRows = 32 * kPartWaves;
+
+template <bool KV8, int HD>
+struct WideShared {
+    static constexpr int kPageBytes = kPage * HD * (KV8 ? 1 : 2);
+    struct Stage {
+        alignas(16) char k[2][kPageBytes], v[2][kPageBytes];
+        float scale[KV8 ? 2 : 1][2][kPage];     // of K and V, of each page
+    };
+    Stage ring[kRing];
+};
+
+template <bool KV8, int HD, int NP, int PP>
+__device__ __forceinline__ void part32(const be42_kv_pool &P, const PrefixArgs &a, WideShared<KV8, HD> &S, int slot,
+                                       int lo, int hi, int kvh, int row0, int rows, int part)
+{
+    using Shared = WideShared<KV8, HD>;
+    constexpr int NK = HD / 16, NE = HD / 32, kRowBytes = HD * (KV8 ? 1 : 2), kRowWords = kRowBytes / 16;
+    constexpr int kPageLoads = Shared::kPageBytes / 1024;             // of a wave, 1 KB each
+    constexpr int kLoads = 4 * kPageLoads / kPartWaves + (KV8 ? 1 : 0);    // a wave's loads of a step
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, h = lane >> 5;
+    const int G = a.n_heads / P.n_kv;
+    const int ns = (hi - lo + kStep - 1) / kStep;
+    // physical pages of 32 steps: lane 2 i + e holds page e of step i
+    int pages = 0;
+    auto load_pages = [&](int i0) {
+        const int e = lane & 1, lp = lo / kPage + 2 * i0 + lane;
+        // a last step's second page may lie past the part: its first one stands in (masked)
+        const int at = lp * kPage < hi ? lp : lp - e;
+        pages = at * kPage < hi ? P.page_table[(size_t)slot * P.max_logical + at] : 0;
+        pages = min(max(pages, 0), P.capacity - 1);
+    };
+    if (ns)
+        load_pages(0);
+
+    // the lane's query row: bf16 pages take element 16 kb + 8 h + j in k block
+    // kb, INT8 pages (16 codes a read) 32 (kb / 2) + 16 h + 8 (kb % 2) + j
+    bf16x8 Q[NK][NP];
+    const int ri = row0 + 32 * wave + c, rc = min(ri, rows - 1);
+    const size_t qat = (size_t)(rc / G) * a.q_stride + (size_t)(kvh * G + rc % G) * HD;
+#pragma unroll
+    for (int kb = 0; kb < NK; kb++)
+        load_q<NP>(a, qat + (KV8 ? 32 * (kb / 2) + 16 * h + 8 * (kb % 2) : 16 * kb + 8 * h), Q[kb]);
+    const float sc = fabsf(a.scale) * 1.44269504088896340736f;
+    // K rows of kRowWords 16-byte words: word x of row t lies at x ^ swz(t), so
+    // that the rows of an operand spread over the banks
+    auto swz = [](int t) { return t / (16 / kRowWords) % kRowWords; };
+    auto load = [&](int i) {
+        if (i && (i & 31) == 0)
+            load_pages(i);
+        typename Shared::Stage &st = S.ring[i % kRing];
+        const size_t head[2] = {(size_t)__builtin_amdgcn_readlane(pages, 2 * (i & 31)) * P.n_kv + kvh,
+                                (size_t)__builtin_amdgcn_readlane(pages, 2 * (i & 31) + 1) * P.n_kv + kvh};
+#pragma unroll
+        for (int x = 0; x < 4 * kPageLoads / kPartWaves; x++) {
+            const int y = x * kPartWaves + wave;                      // K pages, then V pages
+            const bool of_k = y < 2 * kPageLoads;
+            const int page = y / kPageLoads % 2, at = y % kPageLoads * 64 + lane, t = at / kRowWords;
+            const char *base = (const char *)(of_k ? P.k : P.v) + (page ? head[1] : head[0]) * Shared::kPageBytes;
+            const int from = of_k ? t * kRowWords + (at % kRowWords ^ swz(t)) : at;
+            __builtin_amdgcn_global_load_lds((const void *)(base + 16 * from),
+                                             (lds_void *)((of_k ? st.k[page] : st.v[page]) + y % kPageLoads * 1024), 16, 0, 0);
+        }
+        if constexpr (KV8) {
+            // (every wave loads all scales, so that all wait for the same number of loads)
+            const float *from = (lane < 32 ? P.k_scale : P.v_scale) + (lane & 16 ? head[1] : head[0]) * kPage + lane % 16;
+            __builtin_amdgcn_global_load_lds((const void *)from, (lds_void *)&st.scale[0][0][0], 4, 0, 0);
+        }
+        // (the counts that are waited for assume that steps are loaded in order)
+        asm volatile("" ::: "memory");
+    };
+    for (int i = 0; i < kRing - 1 && i < ns; i++)
+        load(i);
+
+    v16f O[NE];
+#pragma unroll
+    for (int e = 0; e < NE; e++)
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+            O[e][i] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    const int kpage = c >> 4, ktok = 8 * (c >> 2 & 1) + 4 * (c >> 3 & 1) + (c & 3), kswz = swz(ktok);
+
+    auto step = [&](int i, auto cut) {
+        constexpr bool CUT = decltype(cut)::value;     // the part ends within the step
+        // step i is in LDS, and every wave is done with step i - 1, whose place
+        // the next load takes
+        if (i + kRing - 2 < ns)
+            stage_barrier<(kRing - 2) * kLoads>();
+        else
+            stage_barrier<0>();
+        if (i + kRing - 1 < ns)
+            load(i + kRing - 1);
+        const typename Shared::Stage &st = S.ring[i % kRing];
+        const int left = CUT ? hi - lo - i * kStep : kStep;
+        v16f s;
+#pragma unroll
+        for (int j = 0; j < 16; j++)
+            s[j] = 0.0f;
+        // all of K's operands are asked for before the first product, V's (the
+        // first page's where registers are short) before the softmax: read as
+        // they are needed they cost a wait of 130 cycles every two products
+        constexpr int NR = KV8 ? NK / 2 : NK;
+        const char *krow = st.k[kpage] + ktok * kRowBytes;
+        uint4 kw[NR];
+#pragma unroll
+        for (int x = 0; x < NR; x++)
+            kw[x] = ring_read<uint4>(krow + 16 * ((2 * x + h) ^ kswz));
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int kb = 0; kb < NK; kb++) {
+            bf16x8 k;
+            if constexpr (KV8)
+                k = kb % 2 ? codes8(kw[kb / 2].z, kw[kb / 2].w) : codes8(kw[kb / 2].x, kw[kb / 2].y);
+            else
+                k = __builtin_bit_cast(bf16x8, kw[KV8 ? 0 : kb]);
+#pragma unroll
+            for (int n = NP - 1; n >= 0; n--)
+                s = mfma32(k, Q[kb][n], s);
+        }
+        uint4 vw[2][KV8 ? 1 : NE];
+        uint32_t v8[2][KV8 ? 8 : 1];
+        auto read_v = [&](int pg) {
+            if constexpr (KV8) {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    v8[pg][j] = NE == 4 ? ring_read<uint32_t>(st.v[pg] + (8 * h + j) * HD + NE * c)
+                                        : ring_read<uint16_t>(st.v[pg] + (8 * h + j) * HD + NE * c);
+            } else {
+#pragma unroll
+                for (int e = 0; e < NE; e++)
+                    vw[pg][e] = ring_read<uint4>(st.v[pg] + (32 * e + c) * 32 + 16 * h);
+            }
+        };
+        read_v(0);
+        if (NP == 1)
+            read_v(1);
+        __builtin_amdgcn_sched_barrier(0);
+        float p[16];
+#pragma unroll
+        for (int j = 0; j < 16; j++)
+            p[j] = s[j];
+        if constexpr (KV8)
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) {
+                const float4 x = ring_read<float4>(&st.scale[0][j / 8][8 * h + j % 8]);
+                p[j] *= x.x;
+                p[j + 1] *= x.y;
+                p[j + 2] *= x.z;
+                p[j + 3] *= x.w;
+            }
+        if constexpr (CUT)
+#pragma unroll
+            for (int j = 0; j < 16; j++)
+                p[j] = 16 * (j / 8) + 8 * h + j % 8 >= left ? -INFINITY : p[j];
+        float top = max3(p[0], p[1], p[2]), other;
+#pragma unroll
+        for (int j = 3; j < 15; j += 2)
+            top = max3(top, p[j], p[j + 1]);
+        top = max3(top, p[15], p[15]);
+        halves(top, top, other);
+        const float mn = fmaxf(m, max3(top, other, other) * sc);
+        if (__any(mn > m)) {
+            const float f = __builtin_amdgcn_exp2f(m - mn);
+            l *= f;
+#pragma unroll
+            for (int e = 0; e < NE; e++)
+                O[e] *= f;
+            m = mn;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            p[j] = __builtin_amdgcn_exp2f(__fmaf_rn(p[j], sc, -m));
+            l += p[j];
+        }
+        if constexpr (KV8)
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) {
+                const float4 x = ring_read<float4>(&st.scale[KV8 ? 1 : 0][j / 8][8 * h + j % 8]);
+                const float v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+                    p[j + q] *= CUT && 16 * (j / 8) + 8 * h + j % 8 + q >= left ? 0.0f : v[q];
+            }
+#pragma unroll
+        for (int pg = 0; pg < 2; pg++) {
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                x[j] = p[8 * pg + j];
+            bf16x8 W[PP];
+            split8<PP>(x, W);
+            if (pg == 0 && NP > 1)
+                read_v(1);
+#pragma unroll
+            for (int e = 0; e < NE; e++) {
+                uint4 w;
+                if constexpr (KV8) {
+                    uint32_t x[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const v2f r = {(float)(int8_t)(v8[pg][2 * j] >> (8 * e)), (float)(int8_t)(v8[pg][2 * j + 1] >> (8 * e))};
+                        x[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, bf16x2));
+                    }
+                    w = make_uint4(x[0], x[1], x[2], x[3]);
+                } else {
+                    w = vw[pg][KV8 ? 0 : e];
+                    // V of tokens past the part is whatever the page held: a weight
+                    // of zero times a NaN pattern would be NaN
+                    if constexpr (CUT) {
+                        const int ok = left - 16 * pg - 8 * h;        // of the lane's eight tokens
+                        w.x &= (ok > 0 ? 0xFFFFu : 0u) | (ok > 1 ? 0xFFFF0000u : 0u);
+                        w.y &= (ok > 2 ? 0xFFFFu : 0u) | (ok > 3 ? 0xFFFF0000u : 0u);
+                        w.z &= (ok > 4 ? 0xFFFFu : 0u) | (ok > 5 ? 0xFFFF0000u : 0u);
+                        w.w &= (ok > 6 ? 0xFFFFu : 0u) | (ok > 7 ? 0xFFFF0000u : 0u);
+                    }
+                }
+                const bf16x8 v = __builtin_bit_cast(bf16x8, w);
+#pragma unroll
+                for (int n = PP - 1; n >= 0; n--)
+                    O[e] = mfma32(v, W[n], O[e]);
+            }
+        }
+    };
+    const int whole = (hi - lo) / kStep;
+    for (int i = 0; i < whole; i++)
+        step(i, std::false_type());
+    if (whole < ns)
+        step(whole, std::true_type());
+    l += __shfl_xor(l, 32, kWave);
+    if (ri >= rows)
+        return;
+    const size_t row = (size_t)(ri / G) * a.n_heads + kvh * G + ri % G;
+    const size_t all = (size_t)a.n_queries * a.n_heads;
+    const bool last = a.parts_p + a.parts_o == 1;
+    if (!last && h == 0)
+        *(float2 *)(a.part_ml + 2 * (part * all + row)) = make_float2(m, l);
+    if (!last && l == 0.0f)
+        return;
+    const float f = last ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+    // four dims at a time: 32 e + 8 x + 4 h + 0 .. 3, INT8 pages NE (8 x + 4 h + i) + e
+    auto store = [&](int d, float v0, float v1, float v2, float v3) {
+        const float4 v = make_float4(v0 * f, v1 * f, v2 * f, v3 * f);
+        if (last)
+            store_out4<NP == 1>(a.out, row * HD + d, v);
+        else
+            *(float4 *)(a.part_o + (part * all + row) * HD + d) = v;
+    };
+    if constexpr (KV8) {
+#pragma unroll
+        for (int y = 0; y < 4 * NE; y++) {          // 16 NE dims, four of them at NE (8 x + 4 h) + 4 ..
+            const int x = y / NE, d4 = 4 * (y % NE);
+            auto at = [&](int q) { return O[(d4 + q) % NE][4 * x + (d4 + q) / NE]; };
+            store(NE * (8 * x + 4 * h) + d4, at(0), at(1), at(2), at(3));
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < NE; e++)
+#pragma unroll
+            for (int x = 0; x < 4; x++)
+                store(32 * e + 8 * x + 4 * h, O[e][4 * x], O[e][4 * x + 1], O[e][4 * x + 2], O[e][4 * x + 3]);
+    }
+}
+
 // block: (KV head, row tile, part) of the prefix, then (KV head, row tile,
 // query, part) of the own tokens
 template <bool KV8, int HD, bool QB>
 __global__ __launch_bounds__(64 * kPartWaves, 2) void k_prefix_part(const be42_kv_pool P, const PrefixArgs a)
 {
-    __shared__ PartShared<HD> S;
+    __shared__ union {
+        PartShared<HD> few;
+        WideShared<KV8, HD> many;
+    } S;
     const int G = a.n_heads / P.n_kv;
     const unsigned of_prefix = (unsigned)P.n_kv * a.tiles_p * a.parts_p;
     unsigned id = blockIdx.x;
@@ -363,7 +691,7 @@ __global__ __launch_bounds__(64 * kPartWaves, 2) void k_prefix_part(const be42_k
             n = min(n, a.lens[b0]);
         chunk = a.chunk_o;
     } else {
-        row0 = 16 * (int)(id % (unsigned)a.tiles_p);
+        row0 = a.rows_p * (int)(id % (unsigned)a.tiles_p);
         part = (int)(id / (unsigned)a.tiles_p);
         b0 = 0;
         rows = a.n_queries * G;
@@ -374,19 +702,24 @@ __global__ __launch_bounds__(64 * kPartWaves, 2) void k_prefix_part(const be42_k
     lo = part * chunk;
     part += own ? a.parts_p : 0;
     const int hi = max(lo, min(n, lo + chunk));
-    part16<KV8, HD, QB ? 1 : 3, QB ? 1 : 3>(P, a, S, slot, lo, hi, kvh, b0, row0, rows);
+    constexpr int NP = QB ? 1 : 3;
+    if (!own && a.rows_p == kWideRows) {
+        part32<KV8, HD, NP, NP>(P, a, S.many, slot, lo, hi, kvh, row0, rows, part);
+        return;
+    }
+    part16<KV8, HD, NP, NP>(P, a, S.few, slot, lo, hi, kvh, b0, row0, rows);
 
     const int c = threadIdx.x >> 4, d4 = threadIdx.x & 15, ri = row0 + c;
     if (ri >= rows)
         return;
-    float top = S.m[0][c], w[kPartWaves], l = 0.0f;
+    float top = S.few.m[0][c], w[kPartWaves], l = 0.0f;
 #pragma unroll
     for (int x = 1; x < kPartWaves; x++)
-        top = fmaxf(top, S.m[x][c]);
+        top = fmaxf(top, S.few.m[x][c]);
 #pragma unroll
     for (int x = 0; x < kPartWaves; x++) {
-        w[x] = part_weight(S.m[x][c], S.l[x][c], top);
-        l += w[x] * S.l[x][c];
+        w[x] = part_weight(S.few.m[x][c], S.few.l[x][c], top);
+        l += w[x] * S.few.l[x][c];
     }
     const size_t row = (size_t)(b0 + ri / G) * a.n_heads + kvh * G + ri % G;
     const size_t all = (size_t)a.n_queries * a.n_heads;
@@ -402,7 +735,7 @@ __global__ __launch_bounds__(64 * kPartWaves, 2) void k_prefix_part(const be42_k
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
         for (int y = 0; y < kPartWaves; y++) {
-            const float4 o = *(const float4 *)&S.o[y][c][d];
+            const float4 o = *(const float4 *)&S.few.o[y][c][d];
             v.x = __fmaf_rn(w[y], o.x, v.x);
             v.y = __fmaf_rn(w[y], o.y, v.y);
             v.z = __fmaf_rn(w[y], o.z, v.z);
@@ -460,27 +793,32 @@ __global__ __launch_bounds__(256) void k_prefix_join(const PrefixArgs a, int par
 // Tokens of a slot that a call may name: their sums stay within 32 bits.
 constexpr int kMaxTokens = 1 << 30;
 
-// The cut of the tokens.  A part has at least 128 tokens (a step for each of the
-// workgroup's waves); prefix and own tokens are each cut into as many parts as
-// give them two workgroups a CU.
-static void cut(int tokens, long tiles, int *parts, int *chunk)
+// The cut of the tokens: as many parts as give `want` workgroups, of at least
+// `unit` tokens.
+static void cut(int tokens, long tiles, int unit, long want, int *parts, int *chunk)
 {
     *parts = *chunk = 0;
     if (!tokens)
         return;
-    const int unit = kPartWaves * kStep, units = (int)(((long)tokens + unit - 1) / unit);
-    const int want = (int)std::min<long>(units, std::max<long>(1, (512 + tiles - 1) / tiles));
-    *chunk = (units + want - 1) / want * unit;
+    const long units = ((long)tokens + unit - 1) / unit;
+    const long n = std::min(units, (want + tiles - 1) / tiles);
+    *chunk = (int)((units + n - 1) / n * unit);
     *parts = (int)(((long)tokens + *chunk - 1) / *chunk);
 }
 
 static void plan_prefix(PrefixArgs &a, int n_kv)
 {
     const int G = a.n_heads / n_kv;
-    a.tiles_p = (int)(((long)a.n_queries * G + 15) / 16);
+    const long rows = (long)a.n_queries * G;
+    a.rows_p = rows > kWideFrom ? kWideRows : 16;
+    a.tiles_p = (int)((rows + a.rows_p - 1) / a.rows_p);
     a.tiles_o = (G + 15) / 16;
-    cut(a.prefix_len, (long)a.tiles_p * n_kv, &a.parts_p, &a.chunk_p);
-    cut(a.max_len, (long)a.tiles_o * n_kv * a.n_queries, &a.parts_o, &a.chunk_o);
+    const int unit = kPartWaves * kStep;
+    if (a.rows_p == kWideRows)
+        cut(a.prefix_len, (long)a.tiles_p * n_kv, kStep * kWideMin, kWideWant, &a.parts_p, &a.chunk_p);
+    else
+        cut(a.prefix_len, (long)a.tiles_p * n_kv, unit, 512, &a.parts_p, &a.chunk_p);
+    cut(a.max_len, (long)a.tiles_o * n_kv * a.n_queries, unit, 512, &a.parts_o, &a.chunk_o);
 }
 
 }  // namespace be42

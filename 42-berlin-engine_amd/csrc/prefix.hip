@@ -38,18 +38,29 @@ struct PrefixArgs {
     int parts_p, parts_o, chunk_p, chunk_o, tiles_p, tiles_o, rows_p;
 };
 
-// tokens a slot holds (0 for a slot outside the pool)
-__device__ __forceinline__ int slot_tokens(const be42_kv_pool &P, int slot)
+// The first `want` tokens of a slot, cut at what it holds (0 for a slot outside
+// the pool).  How full the last page is takes two more dependent loads, which
+// only those who look at it wait for.
+__device__ __forceinline__ int slot_tokens(const be42_kv_pool &P, int slot, int want)
 {
-    if (slot < 0 || slot >= P.n_layers)
+    if (slot < 0 || slot >= P.n_layers || want <= 0)
         return 0;
     const int pages = min(P.n_logical[slot], P.max_logical);
-    if (pages <= 0)
-        return 0;
+    if (want <= (pages - 1) * kPage || pages <= 0)
+        return max(min(want, pages * kPage), 0);
     const int last = P.page_table[(size_t)slot * P.max_logical + pages - 1];
     if (last < 0 || last >= P.capacity)
         return 0;
-    return (pages - 1) * kPage + min(P.ntok[last], kPage);
+    return min(want, (pages - 1) * kPage + min(P.ntok[last], kPage));
+}
+
+// Physical page of a slot's logical page.  Asked for before it is known how many
+// pages the slot has: what lies past them is some page of the pool, whose tokens
+// are masked.
+__device__ __forceinline__ int table_page(const be42_kv_pool &P, int slot, int logical)
+{
+    const size_t at = (size_t)min(max(slot, 0), P.n_layers - 1) * P.max_logical + min(logical, P.max_logical - 1);
+    return min(max(P.page_table[at], 0), P.capacity - 1);
 }
 
 // Eight fp32 as N bf16 parts: each part the rest rounded to bf16, so that three
@@ -154,7 +165,13 @@ __device__ __forceinline__ T ring_read(const void *__restrict__ p)
     return *(const T *)p;
 }
 
-constexpr int kPartWaves = 4;
+// What a row's sums count from may lie this much (a factor of 256) below its
+// largest score so far: the sums are rescaled past that only.  With the exact
+// maximum some of a wave's 32 rows has a new one in most steps, and the rescaling
+// was a third of the vector work.
+constexpr float kSlack = 8.0f;
+
+constexpr int kPartWaves = 8;
 constexpr int kStep = 32;         // tokens of a wave's step: two pages
 
 template <int HD>
@@ -205,11 +222,7 @@ __device__ __forceinline__ void part16(const be42_kv_pool &P, const PrefixArgs &
     // physical pages of the wave's next 32 steps: lane 2 i + e holds page e of step i
     int pages = 0;
     auto load_pages = [&](int i0) {
-        const int e = lane & 1, lp = lo / kPage + 2 * (wave + kPartWaves * (i0 + lane / 2)) + e;
-        // a step's second page may lie past the part: its first one stands in (masked)
-        const int at = lp * kPage < hi ? lp : lp - e;
-        pages = at * kPage < hi ? P.page_table[(size_t)slot * P.max_logical + at] : 0;
-        pages = min(max(pages, 0), P.capacity - 1);
+        pages = table_page(P, slot, lo / kPage + 2 * (wave + kPartWaves * (i0 + lane / 2)) + (lane & 1));
     };
     auto head_of = [&](int i, int e) {
         return (size_t)__builtin_amdgcn_readlane(pages, 2 * (i & 31) + e) * P.n_kv + kvh;
@@ -292,14 +305,14 @@ __device__ __forceinline__ void part16(const be42_kv_pool &P, const PrefixArgs &
         quarters(top, top, other);
         top = max3(top, other, other);
         halves(top, top, other);
-        const float mn = fmaxf(m, max3(top, other, other) * sc);
-        if (__any(mn > m)) {
-            const float f = __builtin_amdgcn_exp2f(m - mn);
+        const float mn = max3(top, other, other) * sc;
+        if (__any(mn > m + kSlack)) {
+            const float now = fmaxf(m, mn), f = __builtin_amdgcn_exp2f(m - now);
             l *= f;
 #pragma unroll
             for (int e = 0; e < NE; e++)
                 O[e] *= f;
-            m = mn;
+            m = now;
         }
 #pragma unroll
         for (int j = 0; j < 8; j++) {
@@ -384,93 +397,98 @@ __device__ __forceinline__ void store_out4(void *out, size_t at, float4 v)
 }
 
 // ---- many rows ------------------------------------------------------------------
-// Rows of the prefix in 32x32 tiles, a wave for 32 of the workgroup's 128 rows;
-// the waves share each step's two pages through a ring in LDS, which
-// direct-to-LDS loads fill kRing - 1 steps ahead.  The products are transposed
-// as in part16: a lane keeps query row c = lane % 32, and with h = lane / 32 its
-// sixteen scores are tokens 8 h .. 8 h + 7 of the first page, then of the second
-// (operand row i is token 8 (i / 4 % 2) + 4 (i / 8 % 2) + i % 4 of page i / 16).
-#ifndef RING
-#define RING 4
-#define WFROM 32
-#define WMIN 4
-#define WWANT 256
-#endif
-constexpr int kRing = RING, kWideFrom = WFROM, kWideMin = WMIN, kWideWant = WWANT;
-constexpr int kWideRows = 32 * kPartWaves;
-
-template <bool KV8, int HD>
+// Rows of the prefix in 32x32 tiles: of a workgroup's eight waves, R share the
+// tokens and take 32 rows each, and T = 8 / R share the rows and take each the
+// next two pages, whose sums are joined in LDS at the end.  Pages come through a
+// ring in LDS that direct-to-LDS loads fill NS - 1 stages (of T steps) ahead.
+// The products are transposed as in part16: a lane keeps query row c = lane %
+// 32, and with h = lane / 32 its sixteen scores are tokens 8 h .. 8 h + 7 of the
+// first page, then of the second (operand row i is token 8 (i / 4 % 2) +
+// 4 (i / 8 % 2) + i % 4 of page i / 16).
+template <bool KV8, int HD, int R>
 struct WideShared {
-    static constexpr int kPageBytes = kPage * HD * (KV8 ? 1 : 2);
-    struct Stage {
+    static constexpr int T = kPartWaves / R, kPageBytes = kPage * HD * (KV8 ? 1 : 2);
+    struct Step {
         alignas(16) char k[2][kPageBytes], v[2][kPageBytes];
         float scale[KV8 ? 2 : 1][2][kPage];     // of K and V, of each page
     };
-    Stage ring[kRing];
+    static constexpr int NS = 128 * 1024 / (T * 4 * kPageBytes) < 4 ? 2 : 4;
+    struct Sums {
+        float o[T][32 * R][HD + 4];
+        float m[T][32 * R], l[T][32 * R];
+    };
+    union {
+        Step ring[NS][T];
+        Sums sums;
+    };
 };
 
-template <bool KV8, int HD, int NP, int PP>
-__device__ __forceinline__ void part32(const be42_kv_pool &P, const PrefixArgs &a, WideShared<KV8, HD> &S, int slot,
-                                       int lo, int hi, int kvh, int row0, int rows, int part)
+template <bool KV8, int HD, int NP, int PP, int R>
+__device__ __forceinline__ void part32(const be42_kv_pool &P, const PrefixArgs &a, WideShared<KV8, HD, R> &S, int slot,
+                                       int lo, int hi, int kvh, int row0, int rows)
 {
-    using Shared = WideShared<KV8, HD>;
+    using Shared = WideShared<KV8, HD, R>;
     constexpr int NK = HD / 16, NE = HD / 32, kRowBytes = HD * (KV8 ? 1 : 2), kRowWords = kRowBytes / 16;
+    constexpr int T = Shared::T, NS = Shared::NS, kStage = T * kStep;
     constexpr int kPageLoads = Shared::kPageBytes / 1024;             // of a wave, 1 KB each
-    constexpr int kLoads = 4 * kPageLoads / kPartWaves + (KV8 ? 1 : 0);    // a wave's loads of a step
+    constexpr int kStepLoads = 4 * kPageLoads, kWaveLoads = T * kStepLoads / kPartWaves;
+    // a wave's loads of a stage; scales: a load a step, by one wave of each T
+    constexpr int kLoads = kWaveLoads + (KV8 ? 1 : 0);
+    static_assert(kWaveLoads >= 1 && T <= kPartWaves, "each wave loads");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, h = lane >> 5;
+    const int rg = wave % R, tg = wave / R;
     const int G = a.n_heads / P.n_kv;
-    const int ns = (hi - lo + kStep - 1) / kStep;
-    // physical pages of 32 steps: lane 2 i + e holds page e of step i
-    int pages = 0;
-    auto load_pages = [&](int i0) {
-        const int e = lane & 1, lp = lo / kPage + 2 * i0 + lane;
-        // a last step's second page may lie past the part: its first one stands in (masked)
-        const int at = lp * kPage < hi ? lp : lp - e;
-        pages = at * kPage < hi ? P.page_table[(size_t)slot * P.max_logical + at] : 0;
-        pages = min(max(pages, 0), P.capacity - 1);
-    };
-    if (ns)
-        load_pages(0);
+    const int ns = (hi - lo + kStage - 1) / kStage;
+    // physical pages of the next stages: lane 2 T i + p holds page p of stage i
+    constexpr int kHeld = kWave / (2 * T);
+    int pages = table_page(P, slot, lo / kPage + lane);
 
     // the lane's query row: bf16 pages take element 16 kb + 8 h + j in k block
     // kb, INT8 pages (16 codes a read) 32 (kb / 2) + 16 h + 8 (kb % 2) + j
     bf16x8 Q[NK][NP];
-    const int ri = row0 + 32 * wave + c, rc = min(ri, rows - 1);
+    const int rc = min(row0 + 32 * rg + c, rows - 1);
     const size_t qat = (size_t)(rc / G) * a.q_stride + (size_t)(kvh * G + rc % G) * HD;
 #pragma unroll
     for (int kb = 0; kb < NK; kb++)
         load_q<NP>(a, qat + (KV8 ? 32 * (kb / 2) + 16 * h + 8 * (kb % 2) : 16 * kb + 8 * h), Q[kb]);
     const float sc = fabsf(a.scale) * 1.44269504088896340736f;
+
     // K rows of kRowWords 16-byte words: word x of row t lies at x ^ swz(t), so
     // that the rows of an operand spread over the banks
     auto swz = [](int t) { return t / (16 / kRowWords) % kRowWords; };
     auto load = [&](int i) {
-        if (i && (i & 31) == 0)
-            load_pages(i);
-        typename Shared::Stage &st = S.ring[i % kRing];
-        const size_t head[2] = {(size_t)__builtin_amdgcn_readlane(pages, 2 * (i & 31)) * P.n_kv + kvh,
-                                (size_t)__builtin_amdgcn_readlane(pages, 2 * (i & 31) + 1) * P.n_kv + kvh};
+        if (i && i % kHeld == 0)
+            pages = table_page(P, slot, (lo + i * kStage) / kPage + lane);
 #pragma unroll
-        for (int x = 0; x < 4 * kPageLoads / kPartWaves; x++) {
-            const int y = x * kPartWaves + wave;                      // K pages, then V pages
-            const bool of_k = y < 2 * kPageLoads;
-            const int page = y / kPageLoads % 2, at = y % kPageLoads * 64 + lane, t = at / kRowWords;
-            const char *base = (const char *)(of_k ? P.k : P.v) + (page ? head[1] : head[0]) * Shared::kPageBytes;
+        for (int x = 0; x < kWaveLoads; x++) {
+            const int y = x * kPartWaves + wave, step = y / kStepLoads, z = y % kStepLoads;      // K pages, then V pages
+            const bool of_k = z < 2 * kPageLoads;
+            const int page = z / kPageLoads % 2, at = z % kPageLoads * 64 + lane, t = at / kRowWords;
+            const size_t head = (size_t)__builtin_amdgcn_readlane(pages, 2 * (i % kHeld * T + step) + page) * P.n_kv + kvh;
+            const char *base = (const char *)(of_k ? P.k : P.v) + head * Shared::kPageBytes;
             const int from = of_k ? t * kRowWords + (at % kRowWords ^ swz(t)) : at;
+            typename Shared::Step &st = S.ring[i % NS][step];
             __builtin_amdgcn_global_load_lds((const void *)(base + 16 * from),
-                                             (lds_void *)((of_k ? st.k[page] : st.v[page]) + y % kPageLoads * 1024), 16, 0, 0);
+                                             (lds_void *)((of_k ? st.k[page] : st.v[page]) + z % kPageLoads * 1024), 16, 0, 0);
         }
         if constexpr (KV8) {
-            // (every wave loads all scales, so that all wait for the same number of loads)
-            const float *from = (lane < 32 ? P.k_scale : P.v_scale) + (lane & 16 ? head[1] : head[0]) * kPage + lane % 16;
-            __builtin_amdgcn_global_load_lds((const void *)from, (lds_void *)&st.scale[0][0][0], 4, 0, 0);
+            // (every wave loads the scales of a step, so that all wait for the same number of loads)
+            const int step = wave % T, at = 2 * (i % kHeld * T + step);
+            const size_t h0 = (size_t)__builtin_amdgcn_readlane(pages, at) * P.n_kv + kvh;
+            const size_t h1 = (size_t)__builtin_amdgcn_readlane(pages, at + 1) * P.n_kv + kvh;
+            const float *from = (lane < 32 ? P.k_scale : P.v_scale) + (lane & 16 ? h1 : h0) * kPage + lane % 16;
+            __builtin_amdgcn_global_load_lds((const void *)from, (lds_void *)&S.ring[i % NS][step].scale[0][0][0], 4, 0, 0);
         }
-        // (the counts that are waited for assume that steps are loaded in order)
+        // (the counts that are waited for assume that stages are loaded in order)
         asm volatile("" ::: "memory");
     };
-    for (int i = 0; i < kRing - 1 && i < ns; i++)
+    for (int i = 0; i < NS - 1 && i < ns; i++)
         load(i);
 
+#ifdef PRIO
+    if (wave < kPartWaves / 2)
+        __builtin_amdgcn_s_setprio(1);
+#endif
     v16f O[NE];
 #pragma unroll
     for (int e = 0; e < NE; e++)
@@ -481,17 +499,19 @@ __device__ __forceinline__ void part32(const be42_kv_pool &P, const PrefixArgs &
     const int kpage = c >> 4, ktok = 8 * (c >> 2 & 1) + 4 * (c >> 3 & 1) + (c & 3), kswz = swz(ktok);
 
     auto step = [&](int i, auto cut) {
-        constexpr bool CUT = decltype(cut)::value;     // the part ends within the step
-        // step i is in LDS, and every wave is done with step i - 1, whose place
+        constexpr bool CUT = decltype(cut)::value;     // the part ends within the stage
+        // stage i is in LDS, and every wave is done with stage i - 1, whose place
         // the next load takes
-        if (i + kRing - 2 < ns)
-            stage_barrier<(kRing - 2) * kLoads>();
+        if (i + NS - 2 < ns)
+            stage_barrier<(NS - 2) * kLoads>();
         else
             stage_barrier<0>();
-        if (i + kRing - 1 < ns)
-            load(i + kRing - 1);
-        const typename Shared::Stage &st = S.ring[i % kRing];
-        const int left = CUT ? hi - lo - i * kStep : kStep;
+        if (i + NS - 1 < ns)
+            load(i + NS - 1);
+        const typename Shared::Step &st = S.ring[i % NS][tg];
+        const int left = CUT ? hi - lo - i * kStage - tg * kStep : kStep;
+        if (CUT && left <= 0)
+            return;
         v16f s;
 #pragma unroll
         for (int j = 0; j < 16; j++)
@@ -558,14 +578,14 @@ __device__ __forceinline__ void part32(const be42_kv_pool &P, const PrefixArgs &
             top = max3(top, p[j], p[j + 1]);
         top = max3(top, p[15], p[15]);
         halves(top, top, other);
-        const float mn = fmaxf(m, max3(top, other, other) * sc);
-        if (__any(mn > m)) {
-            const float f = __builtin_amdgcn_exp2f(m - mn);
+        const float mn = max3(top, other, other) * sc;
+        if (__any(mn > m + kSlack)) {
+            const float now = fmaxf(m, mn), f = __builtin_amdgcn_exp2f(m - now);
             l *= f;
 #pragma unroll
             for (int e = 0; e < NE; e++)
                 O[e] *= f;
-            m = mn;
+            m = now;
         }
 #pragma unroll
         for (int j = 0; j < 16; j++) {
@@ -621,107 +641,45 @@ __device__ __forceinline__ void part32(const be42_kv_pool &P, const PrefixArgs &
             }
         }
     };
-    const int whole = (hi - lo) / kStep;
+    const int whole = (hi - lo) / kStage;
     for (int i = 0; i < whole; i++)
         step(i, std::false_type());
     if (whole < ns)
         step(whole, std::true_type());
+
+    // the sums of the T waves of each row; dims of operand row x = 8 (i / 4) +
+    // 4 h + i % 4 of tile e: 32 e + x, INT8 pages NE x + e
     l += __shfl_xor(l, 32, kWave);
-    if (ri >= rows)
-        return;
-    const size_t row = (size_t)(ri / G) * a.n_heads + kvh * G + ri % G;
-    const size_t all = (size_t)a.n_queries * a.n_heads;
-    const bool last = a.parts_p + a.parts_o == 1;
-    if (!last && h == 0)
-        *(float2 *)(a.part_ml + 2 * (part * all + row)) = make_float2(m, l);
-    if (!last && l == 0.0f)
-        return;
-    const float f = last ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
-    // four dims at a time: 32 e + 8 x + 4 h + 0 .. 3, INT8 pages NE (8 x + 4 h + i) + e
-    auto store = [&](int d, float v0, float v1, float v2, float v3) {
-        const float4 v = make_float4(v0 * f, v1 * f, v2 * f, v3 * f);
-        if (last)
-            store_out4<NP == 1>(a.out, row * HD + d, v);
-        else
-            *(float4 *)(a.part_o + (part * all + row) * HD + d) = v;
-    };
-    if constexpr (KV8) {
-#pragma unroll
-        for (int y = 0; y < 4 * NE; y++) {          // 16 NE dims, four of them at NE (8 x + 4 h) + 4 ..
-            const int x = y / NE, d4 = 4 * (y % NE);
-            auto at = [&](int q) { return O[(d4 + q) % NE][4 * x + (d4 + q) / NE]; };
-            store(NE * (8 * x + 4 * h) + d4, at(0), at(1), at(2), at(3));
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < NE; e++)
-#pragma unroll
-            for (int x = 0; x < 4; x++)
-                store(32 * e + 8 * x + 4 * h, O[e][4 * x], O[e][4 * x + 1], O[e][4 * x + 2], O[e][4 * x + 3]);
+    __syncthreads();                       // every wave is done with the ring
+    const int r = 32 * rg + c;
+    if (h == 0) {
+        S.sums.m[tg][r] = m;
+        S.sums.l[tg][r] = l;
     }
+#pragma unroll
+    for (int i = 0; i < 16; i++)
+#pragma unroll
+        for (int e = 0; e < NE; e++) {
+            const int x = 8 * (i / 4) + 4 * h + i % 4;
+            S.sums.o[tg][r][KV8 ? NE * x + e : 32 * e + x] = O[e][i];
+        }
+    __syncthreads();
 }
 
-// block: (KV head, row tile, part) of the prefix, then (KV head, row tile,
-// query, part) of the own tokens
-template <bool KV8, int HD, bool QB>
-__global__ __launch_bounds__(64 * kPartWaves, 2) void k_prefix_part(const be42_kv_pool P, const PrefixArgs a)
+// Writes rows first .. of a part whose NW waves (or groups of them) left their
+// sums in LDS: m, l [NW][], o [NW][][HD + 4]; `lanes` threads a row.
+template <int HD, bool QB, int NW, class S>
+__device__ __forceinline__ void write_part(const PrefixArgs &a, const S &sums, int c, int d4, int lanes, size_t row, int part)
 {
-    __shared__ union {
-        PartShared<HD> few;
-        WideShared<KV8, HD> many;
-    } S;
-    const int G = a.n_heads / P.n_kv;
-    const unsigned of_prefix = (unsigned)P.n_kv * a.tiles_p * a.parts_p;
-    unsigned id = blockIdx.x;
-    int slot, lo, n, chunk, part, b0, row0, rows;
-    const bool own = id >= of_prefix;
-    if (own)
-        id -= of_prefix;
-    const int kvh = (int)(id % (unsigned)P.n_kv);
-    id /= (unsigned)P.n_kv;
-    if (own) {
-        row0 = 16 * (int)(id % (unsigned)a.tiles_o);
-        id /= (unsigned)a.tiles_o;
-        b0 = (int)(id % (unsigned)a.n_queries);
-        part = (int)(id / (unsigned)a.n_queries);
-        rows = G;
-        slot = a.slots ? a.slots[b0] : b0;
-        n = min(slot_tokens(P, slot), a.max_len);
-        if (a.lens)
-            n = min(n, a.lens[b0]);
-        chunk = a.chunk_o;
-    } else {
-        row0 = a.rows_p * (int)(id % (unsigned)a.tiles_p);
-        part = (int)(id / (unsigned)a.tiles_p);
-        b0 = 0;
-        rows = a.n_queries * G;
-        slot = a.prefix_slot;
-        n = min(slot_tokens(P, slot), a.prefix_len);
-        chunk = a.chunk_p;
-    }
-    lo = part * chunk;
-    part += own ? a.parts_p : 0;
-    const int hi = max(lo, min(n, lo + chunk));
-    constexpr int NP = QB ? 1 : 3;
-    if (!own && a.rows_p == kWideRows) {
-        part32<KV8, HD, NP, NP>(P, a, S.many, slot, lo, hi, kvh, row0, rows, part);
-        return;
-    }
-    part16<KV8, HD, NP, NP>(P, a, S.few, slot, lo, hi, kvh, b0, row0, rows);
-
-    const int c = threadIdx.x >> 4, d4 = threadIdx.x & 15, ri = row0 + c;
-    if (ri >= rows)
-        return;
-    float top = S.few.m[0][c], w[kPartWaves], l = 0.0f;
+    float top = sums.m[0][c], w[NW], l = 0.0f;
 #pragma unroll
-    for (int x = 1; x < kPartWaves; x++)
-        top = fmaxf(top, S.few.m[x][c]);
+    for (int x = 1; x < NW; x++)
+        top = fmaxf(top, sums.m[x][c]);
 #pragma unroll
-    for (int x = 0; x < kPartWaves; x++) {
-        w[x] = part_weight(S.few.m[x][c], S.few.l[x][c], top);
-        l += w[x] * S.few.l[x][c];
+    for (int x = 0; x < NW; x++) {
+        w[x] = part_weight(sums.m[x][c], sums.l[x][c], top);
+        l += w[x] * sums.l[x][c];
     }
-    const size_t row = (size_t)(b0 + ri / G) * a.n_heads + kvh * G + ri % G;
     const size_t all = (size_t)a.n_queries * a.n_heads;
     const bool last = a.parts_p + a.parts_o == 1;
     if (!last && d4 == 0)
@@ -729,13 +687,11 @@ __global__ __launch_bounds__(64 * kPartWaves, 2) void k_prefix_part(const be42_k
     if (!last && l == 0.0f)
         return;                    // k_prefix_join reads no values of a part without tokens
     const float inv = last ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
-#pragma unroll
-    for (int x = 0; x < HD / 64; x++) {
-        const int d = 64 * x + 4 * d4;
+    for (int d = 4 * d4; d < HD; d += 4 * lanes) {
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int y = 0; y < kPartWaves; y++) {
-            const float4 o = *(const float4 *)&S.few.o[y][c][d];
+        for (int y = 0; y < NW; y++) {
+            const float4 o = *(const float4 *)&sums.o[y][c][d];
             v.x = __fmaf_rn(w[y], o.x, v.x);
             v.y = __fmaf_rn(w[y], o.y, v.y);
             v.z = __fmaf_rn(w[y], o.z, v.z);
@@ -748,12 +704,69 @@ __global__ __launch_bounds__(64 * kPartWaves, 2) void k_prefix_part(const be42_k
     }
 }
 
-// one wave per row: its parts by weight; lanes of head_dim / 4 words take the
-// parts in turn
+// block: (KV head, row tile, part) of the prefix, then (KV head, row tile,
+// query, part) of the own tokens.  R: waves that share the prefix' tokens (0: its
+// rows go in tiles of 16).
+template <bool KV8, int HD, bool QB, int R>
+__global__ __launch_bounds__(64 * kPartWaves, 2) void k_prefix_part(const be42_kv_pool P, const PrefixArgs a)
+{
+    __shared__ union {
+        PartShared<HD> few;
+        std::conditional_t<R != 0, WideShared<KV8, HD, R ? R : 4>, char> many;
+    } S;
+    constexpr int NP = QB ? 1 : 3, kRows = R ? 32 * R : 16;
+    const int G = a.n_heads / P.n_kv;
+    const unsigned of_prefix = (unsigned)P.n_kv * a.tiles_p * a.parts_p;
+    unsigned id = blockIdx.x;
+    int slot, n, chunk, part, b0, row0, rows;
+    const bool own = id >= of_prefix;
+    if (own)
+        id -= of_prefix;
+    const int kvh = (int)(id % (unsigned)P.n_kv);
+    id /= (unsigned)P.n_kv;
+    if (own) {
+        row0 = 16 * (int)(id % (unsigned)a.tiles_o);
+        id /= (unsigned)a.tiles_o;
+        b0 = (int)(id % (unsigned)a.n_queries);
+        part = (int)(id / (unsigned)a.n_queries);
+        rows = G;
+        slot = a.slots ? a.slots[b0] : b0;
+        n = a.lens ? min(a.lens[b0], a.max_len) : a.max_len;
+        chunk = a.chunk_o;
+    } else {
+        row0 = kRows * (int)(id % (unsigned)a.tiles_p);
+        part = (int)(id / (unsigned)a.tiles_p);
+        b0 = 0;
+        rows = a.n_queries * G;
+        slot = a.prefix_slot;
+        n = a.prefix_len;
+        chunk = a.chunk_p;
+    }
+    const int lo = part * chunk, hi = max(lo, slot_tokens(P, slot, min(n, lo + chunk)));
+    part += own ? a.parts_p : 0;
+    auto row_at = [&](int ri) { return (size_t)(b0 + ri / G) * a.n_heads + kvh * G + ri % G; };
+    if constexpr (R != 0)
+        if (!own) {
+            constexpr int kLanes = HD / 4;
+            part32<KV8, HD, NP, NP, R>(P, a, S.many, slot, lo, hi, kvh, row0, rows);
+            for (int c = threadIdx.x / kLanes; c < kRows && row0 + c < rows; c += 64 * kPartWaves / kLanes)
+                write_part<HD, QB, kPartWaves / R>(a, S.many.sums, c, threadIdx.x % kLanes, kLanes, row_at(row0 + c), part);
+            return;
+        }
+    part16<KV8, HD, NP, NP>(P, a, S.few, slot, lo, hi, kvh, b0, row0, rows);
+    constexpr int kLanes = HD / 4;
+    const int c = threadIdx.x / kLanes;
+    if (c < 16 && row0 + c < rows)
+        write_part<HD, QB, kPartWaves>(a, S.few, c, threadIdx.x % kLanes, kLanes, row_at(row0 + c), part);
+}
+
+// One wave per row: its parts by weight.  Lanes of head_dim / 4 words take the
+// parts in turn, kAhead loads each in flight: one at a time, 32 parts of 1024
+// rows took 11.6 us.
 template <int HD, bool QB>
 __global__ __launch_bounds__(256) void k_prefix_join(const PrefixArgs a, int parts)
 {
-    constexpr int L = HD / 4, PER = kWave / L;
+    constexpr int L = HD / 4, PER = kWave / L, kAhead = 8;
     const size_t all = (size_t)a.n_queries * a.n_heads, row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, sub = lane / L;
     if (row >= all)
@@ -765,17 +778,26 @@ __global__ __launch_bounds__(256) void k_prefix_join(const PrefixArgs a, int par
     top = wave_max(top);
     float l = 0.0f;
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int p = sub; p < parts; p += PER) {
-        const float2 x = ml[p * all + row];
-        if (x.y == 0.0f)
-            continue;
-        const float w = part_weight(x.x, x.y, top);
-        const float4 o = *(const float4 *)(a.part_o + (p * all + row) * HD + 4 * (lane % L));
-        l = __fmaf_rn(w, x.y, l);
-        v.x = __fmaf_rn(w, o.x, v.x);
-        v.y = __fmaf_rn(w, o.y, v.y);
-        v.z = __fmaf_rn(w, o.z, v.z);
-        v.w = __fmaf_rn(w, o.w, v.w);
+    for (int p0 = sub; p0 < parts; p0 += kAhead * PER) {
+        float4 o[kAhead];
+        float2 x[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) {
+            const size_t at = (size_t)min(p0 + i * PER, parts - 1) * all + row;
+            x[i] = ml[at];
+            o[i] = *(const float4 *)(a.part_o + at * HD + 4 * (lane % L));
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) {
+            // (a part without tokens left no values)
+            const bool in = p0 + i * PER < parts && x[i].y != 0.0f;
+            const float w = in ? __builtin_amdgcn_exp2f(x[i].x - top) : 0.0f;
+            l = in ? __fmaf_rn(w, x[i].y, l) : l;
+            v.x = in ? __fmaf_rn(w, o[i].x, v.x) : v.x;
+            v.y = in ? __fmaf_rn(w, o[i].y, v.y) : v.y;
+            v.z = in ? __fmaf_rn(w, o[i].z, v.z) : v.z;
+            v.w = in ? __fmaf_rn(w, o[i].w, v.w) : v.w;
+        }
     }
 #pragma unroll
     for (int o = L; o < kWave; o <<= 1) {
@@ -792,6 +814,12 @@ __global__ __launch_bounds__(256) void k_prefix_join(const PrefixArgs a, int par
 
 // Tokens of a slot that a call may name: their sums stay within 32 bits.
 constexpr int kMaxTokens = 1 << 30;
+
+#ifndef W4
+#define W4 64
+#define W2 32
+#endif
+constexpr int kWide4 = W4, kWide2 = W2;
 
 // The cut of the tokens: as many parts as give `want` workgroups, of at least
 // `unit` tokens.
@@ -810,15 +838,12 @@ static void plan_prefix(PrefixArgs &a, int n_kv)
 {
     const int G = a.n_heads / n_kv;
     const long rows = (long)a.n_queries * G;
-    a.rows_p = rows > kWideFrom ? kWideRows : 16;
+    a.rows_p = rows > kWide4 ? 128 : rows > kWide2 ? 64 : 16;
     a.tiles_p = (int)((rows + a.rows_p - 1) / a.rows_p);
     a.tiles_o = (G + 15) / 16;
     const int unit = kPartWaves * kStep;
-    if (a.rows_p == kWideRows)
-        cut(a.prefix_len, (long)a.tiles_p * n_kv, kStep * kWideMin, kWideWant, &a.parts_p, &a.chunk_p);
-    else
-        cut(a.prefix_len, (long)a.tiles_p * n_kv, unit, 512, &a.parts_p, &a.chunk_p);
-    cut(a.max_len, (long)a.tiles_o * n_kv * a.n_queries, unit, 512, &a.parts_o, &a.chunk_o);
+    cut(a.prefix_len, (long)a.tiles_p * n_kv, unit, 256, &a.parts_p, &a.chunk_p);
+    cut(a.max_len, (long)a.tiles_o * n_kv * a.n_queries, unit, 256, &a.parts_o, &a.chunk_o);
 }
 
 }  // namespace be42
@@ -885,20 +910,24 @@ extern "C" int be42_prefix_attention(const be42_kv_pool *pool, const void *q, in
         a.part_o = (float *)workspace;
         a.part_ml = a.part_o + (size_t)parts * rows * P.head_dim;
     }
-    auto go = [&](auto part, auto join) {
-        if (parts)
-            hipLaunchKernelGGL(part, dim3((unsigned)blocks), dim3(64 * kPartWaves), 0, s, P, a);
+    auto go = [&](auto kv8, auto hd, auto qb) {
+        constexpr bool KV8 = decltype(kv8)::value, QB = decltype(qb)::value;
+        constexpr int HD = decltype(hd)::value;
+        const dim3 g((unsigned)blocks), t(64 * kPartWaves);
+        if (parts && a.rows_p == 128)
+            hipLaunchKernelGGL((k_prefix_part<KV8, HD, QB, 4>), g, t, 0, s, P, a);
+        else if (parts && a.rows_p == 64)
+            hipLaunchKernelGGL((k_prefix_part<KV8, HD, QB, 2>), g, t, 0, s, P, a);
+        else if (parts)
+            hipLaunchKernelGGL((k_prefix_part<KV8, HD, QB, 0>), g, t, 0, s, P, a);
         if (parts != 1)
-            hipLaunchKernelGGL(join, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a, parts);
+            hipLaunchKernelGGL((k_prefix_join<HD, QB>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a, parts);
     };
-    const bool i8 = P.kind == BE42_KV_INT8;
-    if (P.head_dim == 64) {
-        if (q_bf16) i8 ? go(k_prefix_part<true, 64, true>, k_prefix_join<64, true>) : go(k_prefix_part<false, 64, true>, k_prefix_join<64, true>);
-        else i8 ? go(k_prefix_part<true, 64, false>, k_prefix_join<64, false>) : go(k_prefix_part<false, 64, false>, k_prefix_join<64, false>);
-    } else {
-        if (q_bf16) i8 ? go(k_prefix_part<true, 128, true>, k_prefix_join<128, true>) : go(k_prefix_part<false, 128, true>, k_prefix_join<128, true>);
-        else i8 ? go(k_prefix_part<true, 128, false>, k_prefix_join<128, false>) : go(k_prefix_part<false, 128, false>, k_prefix_join<128, false>);
-    }
+    auto of_type = [&](auto kv8, auto hd) { q_bf16 ? go(kv8, hd, std::true_type()) : go(kv8, hd, std::false_type()); };
+    auto of_dim = [&](auto kv8) {
+        P.head_dim == 64 ? of_type(kv8, std::integral_constant<int, 64>()) : of_type(kv8, std::integral_constant<int, 128>());
+    };
+    P.kind == BE42_KV_INT8 ? of_dim(std::true_type()) : of_dim(std::false_type());
     BE42_LAUNCH_CHECK();
     return BE42_OK;
 }

@@ -171,7 +171,7 @@ __device__ __forceinline__ T ring_read(const void *__restrict__ p)
 // was a third of the vector work.
 constexpr float kSlack = 8.0f;
 
-constexpr int kPartWaves = 8;
+constexpr int kPartWaves = 4;
 constexpr int kStep = 32;         // tokens of a wave's step: two pages
 
 template <int HD>
@@ -397,10 +397,10 @@ __device__ __forceinline__ void store_out4(void *out, size_t at, float4 v)
 }
 
 // ---- many rows ------------------------------------------------------------------
-// Rows of the prefix in 32x32 tiles: of a workgroup's eight waves, R share the
-// tokens and take 32 rows each, and T = 8 / R share the rows and take each the
+// Rows of the prefix in 32x32 tiles: of a workgroup's four waves, R share the
+// tokens and take 32 rows each, and T = 4 / R share the rows and take each the
 // next two pages, whose sums are joined in LDS at the end.  Pages come through a
-// ring in LDS that direct-to-LDS loads fill NS - 1 stages (of T steps) ahead.
+// ring in LDS that direct-to-LDS loads fill ahead, a stage of T steps at a time.
 // The products are transposed as in part16: a lane keeps query row c = lane %
 // 32, and with h = lane / 32 its sixteen scores are tokens 8 h .. 8 h + 7 of the
 // first page, then of the second (operand row i is token 8 (i / 4 % 2) +
@@ -412,7 +412,7 @@ struct WideShared {
         alignas(16) char k[2][kPageBytes], v[2][kPageBytes];
         float scale[KV8 ? 2 : 1][2][kPage];     // of K and V, of each page
     };
-    static constexpr int NS = 128 * 1024 / (T * 4 * kPageBytes) < 4 ? 2 : 4;
+    static constexpr int NS = T * 4 * kPageBytes > 16 * 1024 ? 2 : 4;       // 64 KB: two workgroups a CU
     struct Sums {
         float o[T][32 * R][HD + 4];
         float m[T][32 * R], l[T][32 * R];
@@ -435,6 +435,7 @@ __device__ __forceinline__ void part32(const be42_kv_pool &P, const PrefixArgs &
     // a wave's loads of a stage; scales: a load a step, by one wave of each T
     constexpr int kLoads = kWaveLoads + (KV8 ? 1 : 0);
     static_assert(kWaveLoads >= 1 && T <= kPartWaves, "each wave loads");
+    constexpr int D = NS - 1;                  // stages that are loaded ahead
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, h = lane >> 5;
     const int rg = wave % R, tg = wave / R;
     const int G = a.n_heads / P.n_kv;
@@ -482,13 +483,9 @@ __device__ __forceinline__ void part32(const be42_kv_pool &P, const PrefixArgs &
         // (the counts that are waited for assume that stages are loaded in order)
         asm volatile("" ::: "memory");
     };
-    for (int i = 0; i < NS - 1 && i < ns; i++)
+    for (int i = 0; i < D && i < ns; i++)
         load(i);
 
-#ifdef PRIO
-    if (wave < kPartWaves / 2)
-        __builtin_amdgcn_s_setprio(1);
-#endif
     v16f O[NE];
 #pragma unroll
     for (int e = 0; e < NE; e++)
@@ -498,21 +495,18 @@ __device__ __forceinline__ void part32(const be42_kv_pool &P, const PrefixArgs &
     float m = -INFINITY, l = 0.0f;
     const int kpage = c >> 4, ktok = 8 * (c >> 2 & 1) + 4 * (c >> 3 & 1) + (c & 3), kswz = swz(ktok);
 
-    auto step = [&](int i, auto cut) {
-        constexpr bool CUT = decltype(cut)::value;     // the part ends within the stage
-        // stage i is in LDS, and every wave is done with stage i - 1, whose place
-        // the next load takes
-        if (i + NS - 2 < ns)
-            stage_barrier<(NS - 2) * kLoads>();
+    // stage i is in LDS, and every wave is done with the stage whose place the
+    // next load takes
+    auto begin = [&](int i) {
+        if (i + D - 1 < ns)
+            stage_barrier<(D - 1) * kLoads>();
         else
             stage_barrier<0>();
-        if (i + NS - 1 < ns)
-            load(i + NS - 1);
+        if (i + D < ns)
+            load(i + D);
+    };
+    auto scores = [&](int i, v16f &s) {
         const typename Shared::Step &st = S.ring[i % NS][tg];
-        const int left = CUT ? hi - lo - i * kStage - tg * kStep : kStep;
-        if (CUT && left <= 0)
-            return;
-        v16f s;
 #pragma unroll
         for (int j = 0; j < 16; j++)
             s[j] = 0.0f;
@@ -537,6 +531,11 @@ __device__ __forceinline__ void part32(const be42_kv_pool &P, const PrefixArgs &
             for (int n = NP - 1; n >= 0; n--)
                 s = mfma32(k, Q[kb][n], s);
         }
+    };
+    auto values = [&](int i, const v16f &s, auto cut) {
+        constexpr bool CUT = decltype(cut)::value;     // the part ends within the stage
+        const typename Shared::Step &st = S.ring[i % NS][tg];
+        const int left = CUT ? hi - lo - i * kStage - tg * kStep : kStep;
         uint4 vw[2][KV8 ? 1 : NE];
         uint32_t v8[2][KV8 ? 8 : 1];
         auto read_v = [&](int pg) {
@@ -642,10 +641,20 @@ __device__ __forceinline__ void part32(const be42_kv_pool &P, const PrefixArgs &
         }
     };
     const int whole = (hi - lo) / kStage;
-    for (int i = 0; i < whole; i++)
-        step(i, std::false_type());
-    if (whole < ns)
-        step(whole, std::true_type());
+    const bool mine = hi - lo - whole * kStage > tg * kStep;          // of the stage that the part's end cuts
+    v16f s;
+    for (int i = 0; i < whole; i++) {
+        begin(i);
+        scores(i, s);
+        values(i, s, std::false_type());
+    }
+    if (whole < ns) {
+        begin(whole);
+        if (mine) {
+            scores(whole, s);
+            values(whole, s, std::true_type());
+        }
+    }
 
     // the sums of the T waves of each row; dims of operand row x = 8 (i / 4) +
     // 4 h + i % 4 of tile e: 32 e + x, INT8 pages NE x + e
@@ -704,6 +713,11 @@ __device__ __forceinline__ void write_part(const PrefixArgs &a, const S &sums, i
     }
 }
 
+// bf16 queries: weights are rounded to bf16 where the matrix cores are what is
+// waited for (many rows; the result is then 1.4 times as far from 64 bits as its
+// own rounding to bf16 puts it), and kept to 16 bits, which costs nothing, where
+// memory is.  fp32 queries: three parts hold all 24 bits of queries and weights.
+//
 // block: (KV head, row tile, part) of the prefix, then (KV head, row tile,
 // query, part) of the own tokens.  R: waves that share the prefix' tokens (0: its
 // rows go in tiles of 16).
@@ -714,7 +728,7 @@ __global__ __launch_bounds__(64 * kPartWaves, 2) void k_prefix_part(const be42_k
         PartShared<HD> few;
         std::conditional_t<R != 0, WideShared<KV8, HD, R ? R : 4>, char> many;
     } S;
-    constexpr int NP = QB ? 1 : 3, kRows = R ? 32 * R : 16;
+    constexpr int NP = QB ? 1 : 3, kRows = R ? 32 * R : 16, kLanes = HD / 4;
     const int G = a.n_heads / P.n_kv;
     const unsigned of_prefix = (unsigned)P.n_kv * a.tiles_p * a.parts_p;
     unsigned id = blockIdx.x;
@@ -747,16 +761,13 @@ __global__ __launch_bounds__(64 * kPartWaves, 2) void k_prefix_part(const be42_k
     auto row_at = [&](int ri) { return (size_t)(b0 + ri / G) * a.n_heads + kvh * G + ri % G; };
     if constexpr (R != 0)
         if (!own) {
-            constexpr int kLanes = HD / 4;
             part32<KV8, HD, NP, NP, R>(P, a, S.many, slot, lo, hi, kvh, row0, rows);
             for (int c = threadIdx.x / kLanes; c < kRows && row0 + c < rows; c += 64 * kPartWaves / kLanes)
                 write_part<HD, QB, kPartWaves / R>(a, S.many.sums, c, threadIdx.x % kLanes, kLanes, row_at(row0 + c), part);
             return;
         }
-    part16<KV8, HD, NP, NP>(P, a, S.few, slot, lo, hi, kvh, b0, row0, rows);
-    constexpr int kLanes = HD / 4;
-    const int c = threadIdx.x / kLanes;
-    if (c < 16 && row0 + c < rows)
+    part16<KV8, HD, NP, QB ? 2 : 3>(P, a, S.few, slot, lo, hi, kvh, b0, row0, rows);
+    for (int c = threadIdx.x / kLanes; c < 16 && row0 + c < rows; c += 64 * kPartWaves / kLanes)
         write_part<HD, QB, kPartWaves>(a, S.few, c, threadIdx.x % kLanes, kLanes, row_at(row0 + c), part);
 }
 
@@ -815,11 +826,7 @@ __global__ __launch_bounds__(256) void k_prefix_join(const PrefixArgs a, int par
 // Tokens of a slot that a call may name: their sums stay within 32 bits.
 constexpr int kMaxTokens = 1 << 30;
 
-#ifndef W4
-#define W4 64
-#define W2 32
-#endif
-constexpr int kWide4 = W4, kWide2 = W2;
+
 
 // The cut of the tokens: as many parts as give `want` workgroups, of at least
 // `unit` tokens.
@@ -834,16 +841,24 @@ static void cut(int tokens, long tiles, int unit, long want, int *parts, int *ch
     *parts = (int)(((long)tokens + *chunk - 1) / *chunk);
 }
 
+// Rows of a prefix tile: up to 32 rows of a KV head go in tiles of 16 (8192
+// tokens, 32 rows: 16 us, 20 in one of 64), up to 256 in tiles of 64 (128 rows:
+// 30 us, 34 in one of 128), more in tiles of 128 (32768 tokens, 512 rows and own
+// tokens: 150 us, 175 in tiles of 64).  The prefix gets a workgroup a CU, so that
+// own tokens, which wait for memory, run beside it (two: 166 us); where there are
+// few of those and the parts stay long, it gets two (512 rows alone 108 us, 135
+// with one).
 static void plan_prefix(PrefixArgs &a, int n_kv)
 {
-    const int G = a.n_heads / n_kv;
+    const int G = a.n_heads / n_kv, unit = kPartWaves * kStep;
     const long rows = (long)a.n_queries * G;
-    a.rows_p = rows > kWide4 ? 128 : rows > kWide2 ? 64 : 16;
+    a.rows_p = rows > 256 ? 128 : rows > 32 ? 64 : 16;
     a.tiles_p = (int)((rows + a.rows_p - 1) / a.rows_p);
     a.tiles_o = (G + 15) / 16;
-    const int unit = kPartWaves * kStep;
-    cut(a.prefix_len, (long)a.tiles_p * n_kv, unit, 256, &a.parts_p, &a.chunk_p);
-    cut(a.max_len, (long)a.tiles_o * n_kv * a.n_queries, unit, 256, &a.parts_o, &a.chunk_o);
+    const long tiles = (long)a.tiles_p * n_kv, read = (long)a.prefix_len * a.tiles_p;
+    const bool two = a.rows_p == 16 || (a.prefix_len * tiles >= 512 * 1024 && 2L * a.n_queries * a.max_len < read);
+    cut(a.prefix_len, tiles, unit, two ? 512 : 256, &a.parts_p, &a.chunk_p);
+    cut(a.max_len, (long)a.tiles_o * n_kv * a.n_queries, unit, 512, &a.parts_o, &a.chunk_o);
 }
 
 }  // namespace be42

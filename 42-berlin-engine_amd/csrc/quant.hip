@@ -10,6 +10,7 @@
 // a per-binade threshold table measured on the host at init.
 #include <cmath>
 #include <cstring>
+#include <type_traits>
 
 #include "be42_common.h"
 
@@ -265,12 +266,194 @@ __global__ __launch_bounds__(256) void k_norm_quant_rows(uint8_t *q, float *scal
     }
 }
 
+// A row of up to NV words of VE elements a thread (16 bytes of fp32 or of bf16)
+// is held in registers from the sum to the codes, so that x, the residual and w
+// are read once, all in flight together.  TPR threads a row, 256 / TPR rows a
+// block; threads of one wave need no barrier.
+template <int TPR>
+__device__ __forceinline__ double row_sum(double v, double *red)
+{
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+        v += __shfl_xor(v, o, kWave);
+    if constexpr (TPR > kWave) {
+        if ((threadIdx.x & 63) == 0)
+            red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = red[0];
+#pragma unroll
+        for (int w = 1; w < TPR / kWave; w++)
+            v += red[w];
+    }
+    return v;
+}
+template <int TPR>
+__device__ __forceinline__ float row_max(float v, float *red)
+{
+    v = wave_max(v);
+    if constexpr (TPR > kWave) {
+        if ((threadIdx.x & 63) == 0)
+            red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = red[0];
+#pragma unroll
+        for (int w = 1; w < TPR / kWave; w++)
+            v = fmaxf(v, red[w]);
+    }
+    return v;
+}
+
+template <bool BF16>
+struct Word {
+    static constexpr int VE = BF16 ? 8 : 4;
+    float v[VE];
+    __device__ __forceinline__ void load(const void *p, size_t at)
+    {
+        const uint4 w = *(const uint4 *)((const char *)p + at * (BF16 ? 2 : 4));
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < VE; j++)
+            v[j] = __uint_as_float(!BF16 ? u[j % 4] : j & 1 ? u[j / 2] & 0xFFFF0000u : u[j / 2] << 16);
+    }
+    __device__ __forceinline__ void store(void *p, size_t at) const
+    {
+        uint32_t u[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            u[j] = !BF16 ? __float_as_uint(v[j])
+                         : __float_as_uint(v[2 * j % VE]) >> 16 | (__float_as_uint(v[(2 * j + 1) % VE]) & 0xFFFF0000u);
+        *(uint4 *)((char *)p + at * (BF16 ? 2 : 4)) = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+};
+
+template <bool FP8, bool BF16, int TPR, int NV>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_quant_vec(uint8_t *__restrict__ q, float *__restrict__ scales,
+                                                                          void *sum, const void *x, size_t x_stride,
+                                                                          const void *res, size_t res_stride,
+                                                                          const uint16_t *__restrict__ w, int rows, int cols,
+                                                                          float eps)
+{
+    constexpr int VE = Word<BF16>::VE, kRows = TPR < 256 ? 256 / TPR : 1;
+    __shared__ double redd[TPR > kWave ? TPR / kWave : 1];
+    __shared__ float red[TPR > kWave ? TPR / kWave : 1];
+    const int t = threadIdx.x % TPR;
+    const size_t row = (size_t)blockIdx.x * kRows + threadIdx.x / TPR;
+    if (kRows > 1 && row >= (size_t)rows)
+        return;                            // (whole waves, and no barrier follows)
+    Word<BF16> h[NV], r[NV];
+    uint32_t wt[NV][VE / 2];
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        const int i = (t + TPR * j) * VE;
+#pragma unroll
+        for (int e = 0; e < VE; e++)
+            h[j].v[e] = r[j].v[e] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < VE / 2; e++)
+            wt[j][e] = 0;
+        if (i < cols) {
+            h[j].load(x, row * x_stride + i);
+            if (res)
+                r[j].load(res, row * res_stride + i);
+            __builtin_memcpy(wt[j], __builtin_assume_aligned(w + i, 2 * VE), 2 * VE);
+        }
+    }
+    double ss = 0.0;
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        const int i = (t + TPR * j) * VE;
+        if (res)
+#pragma unroll
+            for (int e = 0; e < VE; e++)
+                h[j].v[e] = act_add<BF16>(h[j].v[e], r[j].v[e]);
+        if (sum && i < cols)
+            h[j].store(sum, row * cols + i);
+#pragma unroll
+        for (int e = 0; e < VE; e++)
+            ss = fma((double)h[j].v[e], (double)h[j].v[e], ss);
+    }
+    const double f = 1.0 / sqrt(row_sum<TPR>(ss, redd) / cols + (double)eps);
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+#pragma unroll
+        for (int e = 0; e < VE; e++) {
+            const uint32_t u = wt[j][e / 2];
+            h[j].v[e] = norm_value(h[j].v[e], f, (uint16_t)(e & 1 ? u >> 16 : u));
+            m = fmaxf(m, fabsf(h[j].v[e]));
+        }
+    m = row_max<TPR>(m, red);
+    float scale = 1.0f, inv = 1.0f;
+    if (m > 0.0f) {
+        scale = m / (FP8 ? 224.0f : 127.0f);
+        inv = FP8 ? 1.0f / scale : 127.0f / m;
+    }
+    if (t == 0)
+        scales[row] = scale;
+    auto code = [&](float y) { return FP8 ? (uint32_t)f32_to_fp8(y * inv) : (uint32_t)(uint8_t)f32_to_int8(y, inv); };
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        const int i = (t + TPR * j) * VE;
+        uint32_t c[VE / 4];
+#pragma unroll
+        for (int e = 0; e < VE; e += 4)
+            c[e / 4] = code(h[j].v[e]) | code(h[j].v[e + 1]) << 8 | code(h[j].v[e + 2]) << 16 | code(h[j].v[e + 3]) << 24;
+        if (i < cols)
+            __builtin_memcpy(__builtin_assume_aligned(q + row * cols + i, VE), c, VE);
+    }
+}
+
+// Rows in 16-byte words where every row of x, the residual, w and the outputs
+// begins on one and has whole ones; others an element at a time.  Threads of a
+// row: few for many rows, as many as leave a word each for few.
+template <bool FP8, bool BF16>
+static bool launch_norm_vec(uint8_t *q, float *scales, void *sum, const void *x, size_t x_stride, const void *res,
+                            size_t res_stride, const uint16_t *w, int rows, int cols, float eps, hipStream_t s)
+{
+    constexpr int VE = Word<BF16>::VE;
+    if (cols % VE || x_stride % VE || (res && res_stride % VE) ||
+        (((uintptr_t)x | (uintptr_t)res | (uintptr_t)sum) & 15) || (uintptr_t)w % (2 * VE) || (uintptr_t)q % VE)
+        return false;
+    const int words = cols / VE;
+    auto go = [&](auto tpr, auto nv) {
+        constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
+        constexpr int per = TPR < 256 ? 256 / TPR : 1;
+        hipLaunchKernelGGL((k_norm_quant_vec<FP8, BF16, TPR, NV>), dim3((rows + per - 1) / per), dim3(TPR < 256 ? 256 : TPR), 0,
+                           s, q, scales, sum, x, x_stride, res, res_stride, w, rows, cols, eps);
+        return true;
+    };
+    using std::integral_constant;
+    constexpr integral_constant<int, 1> one;
+    constexpr integral_constant<int, 2> two;
+    constexpr integral_constant<int, 4> four;
+    if (words <= 64)
+        return go(integral_constant<int, 64>(), one);
+    if (words <= 128 && rows >= 1024)
+        return go(integral_constant<int, 64>(), two);
+    if (words <= 256)
+        return go(integral_constant<int, 256>(), one);
+    if (words <= 512 && rows >= 256)
+        return go(integral_constant<int, 256>(), two);
+    if (words <= 1024 && rows >= 256)
+        return go(integral_constant<int, 256>(), four);
+    if (words <= 1024)
+        return go(integral_constant<int, 1024>(), one);
+    if (words <= 2048)
+        return go(integral_constant<int, 1024>(), two);
+    if (words <= 4096)
+        return go(integral_constant<int, 1024>(), four);
+    return false;
+}
+
 template <bool FP8>
 static void launch_norm_quant(uint8_t *q, float *scales, void *sum, const void *x, size_t x_stride, const void *res,
                               size_t res_stride, bool bf16, const uint16_t *w, int rows, int cols, float eps,
                               hipStream_t s)
 {
     const dim3 g(rows), b(256);
+    if (bf16 ? launch_norm_vec<FP8, true>(q, scales, sum, x, x_stride, res, res_stride, w, rows, cols, eps, s)
+             : launch_norm_vec<FP8, false>(q, scales, sum, x, x_stride, res, res_stride, w, rows, cols, eps, s))
+        return;
     if (bf16)
         hipLaunchKernelGGL((k_norm_quant_rows<FP8, true>), g, b, 0, s, q, scales, sum, x, x_stride, res, res_stride,
                            w, cols, eps);

@@ -46,6 +46,25 @@ __device__ __forceinline__ uint8_t f32_to_fp8(float v)
     return (uint8_t)(sign | ((uint32_t)e << 3) | (uint32_t)m);
 }
 
+// f32_to_fp8 of a finite value in half the instructions: the kept mantissa bits
+// are counted up by the next bit unless they are all ones (8 frac + 0.5 is exact
+// in fp32, so its integer part is that).  Compared with it over all fp32 values;
+// the pass over 300 x 14336 fp32 15.3 -> 14.7 us.
+__device__ __forceinline__ uint8_t finite_to_fp8(float v)
+{
+    const float a = fminf(fabsf(v), 448.0f);
+    const uint32_t u = __float_as_uint(a);
+    int ex = (int)(u >> 23) - 127;
+    uint32_t c = (u >> 20) - ((127u - 7u) << 3) + ((u & 0x700000u) != 0x700000u ? u >> 19 & 1u : 0u);
+    if ((u & 0x7FFFFFu) >= 0x7FFFC0u && ex + 1 >= kFp8ThrE0 && ex + 1 < kFp8ThrE0 + kFp8ThrN &&
+        a >= c_fp8_thr[ex + 1 - kFp8ThrE0]) {
+        ex++;                                              // log2f rounded up to an integer
+        c = (uint32_t)(ex + 7) << 3;
+    }
+    if (ex < -6)                                           // multiples of 2^-9
+        c = (uint32_t)min((int)__fmaf_rn(a, 512.0f, 0.5f), 7);
+    return (uint8_t)(a == 0.0f ? 0u : c | (__float_as_uint(v) >> 24 & 0x80u));
+}
 
 // quant_f32_to_int8's code of one element (ops_quant.c:262-267)
 __device__ __forceinline__ int8_t f32_to_int8(float v, float inv)
@@ -178,8 +197,9 @@ static bool launch_quant_vec(uint8_t *q, float *scales, const float *x, int rows
 // ---- residual + RMS norm + codes -----------------------------------------------
 // h = x + residual in the stream's type, y = fp32(h / sqrt(mean h^2 + eps) * w)
 // and the codec's code of y.  The sum of squares and the product are formed in
-// 64 bits and rounded once to fp32, so y, and with it every code, is the same
-// for any split of the row over threads.
+// 64 bits and rounded once to fp32, so y does not depend on how the row is split
+// over threads, but where the product falls within 2^-50 of the middle between
+// two fp32 values.
 
 // element i of a row of the residual stream (fp32 or bf16) as fp32
 template <bool BF16>
@@ -262,7 +282,7 @@ __global__ __launch_bounds__(256) void k_norm_quant_rows(uint8_t *q, float *scal
         scales[row] = scale;
     for (int i = threadIdx.x; i < cols; i += 256) {
         const float y = norm_value(again(i), r, w[i]);
-        q[row * cols + i] = FP8 ? f32_to_fp8(y * inv) : (uint8_t)f32_to_int8(y, inv);
+        q[row * cols + i] = FP8 ? finite_to_fp8(y * inv) : (uint8_t)f32_to_int8(y, inv);
     }
 }
 
@@ -303,45 +323,52 @@ __device__ __forceinline__ float row_max(float v, float *red)
     return v;
 }
 
-template <bool BF16>
+template <bool BF16, int VE>
 struct Word {
-    static constexpr int VE = BF16 ? 8 : 4;
     float v[VE];
     __device__ __forceinline__ void load(const void *p, size_t at)
     {
-        const uint4 w = *(const uint4 *)((const char *)p + at * (BF16 ? 2 : 4));
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+        if constexpr (VE == 1) {
+            v[0] = act_load<BF16>(p, at);
+        } else {
+            const uint4 w = *(const uint4 *)((const char *)p + at * (BF16 ? 2 : 4));
+            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-        for (int j = 0; j < VE; j++)
-            v[j] = __uint_as_float(!BF16 ? u[j % 4] : j & 1 ? u[j / 2] & 0xFFFF0000u : u[j / 2] << 16);
+            for (int j = 0; j < VE; j++)
+                v[j] = __uint_as_float(!BF16 ? u[j % 4] : j & 1 ? u[j / 2] & 0xFFFF0000u : u[j / 2] << 16);
+        }
     }
     __device__ __forceinline__ void store(void *p, size_t at) const
     {
-        uint32_t u[4];
+        if constexpr (VE == 1) {
+            act_store<BF16>(p, at, v[0]);
+        } else {
+            uint32_t u[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            u[j] = !BF16 ? __float_as_uint(v[j])
-                         : __float_as_uint(v[2 * j % VE]) >> 16 | (__float_as_uint(v[(2 * j + 1) % VE]) & 0xFFFF0000u);
-        *(uint4 *)((char *)p + at * (BF16 ? 2 : 4)) = make_uint4(u[0], u[1], u[2], u[3]);
+            for (int j = 0; j < 4; j++)
+                u[j] = !BF16 ? __float_as_uint(v[j])
+                             : __float_as_uint(v[2 * j % VE]) >> 16 | (__float_as_uint(v[(2 * j + 1) % VE]) & 0xFFFF0000u);
+            *(uint4 *)((char *)p + at * (BF16 ? 2 : 4)) = make_uint4(u[0], u[1], u[2], u[3]);
+        }
     }
 };
 
-template <bool FP8, bool BF16, int TPR, int NV>
+template <bool FP8, bool BF16, int VE, int TPR, int NV>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_quant_vec(uint8_t *__restrict__ q, float *__restrict__ scales,
                                                                           void *sum, const void *x, size_t x_stride,
                                                                           const void *res, size_t res_stride,
                                                                           const uint16_t *__restrict__ w, int rows, int cols,
                                                                           float eps)
 {
-    constexpr int VE = Word<BF16>::VE, kRows = TPR < 256 ? 256 / TPR : 1;
+    constexpr int kRows = TPR < 256 ? 256 / TPR : 1;
     __shared__ double redd[TPR > kWave ? TPR / kWave : 1];
     __shared__ float red[TPR > kWave ? TPR / kWave : 1];
     const int t = threadIdx.x % TPR;
     const size_t row = (size_t)blockIdx.x * kRows + threadIdx.x / TPR;
     if (kRows > 1 && row >= (size_t)rows)
         return;                            // (whole waves, and no barrier follows)
-    Word<BF16> h[NV], r[NV];
-    uint32_t wt[NV][VE / 2];
+    Word<BF16, VE> h[NV], r[NV];
+    uint16_t wt[NV][VE];
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         const int i = (t + TPR * j) * VE;
@@ -349,7 +376,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_quant_vec(uint8_
         for (int e = 0; e < VE; e++)
             h[j].v[e] = r[j].v[e] = 0.0f;
 #pragma unroll
-        for (int e = 0; e < VE / 2; e++)
+        for (int e = 0; e < VE; e++)
             wt[j][e] = 0;
         if (i < cols) {
             h[j].load(x, row * x_stride + i);
@@ -378,8 +405,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_quant_vec(uint8_
     for (int j = 0; j < NV; j++)
 #pragma unroll
         for (int e = 0; e < VE; e++) {
-            const uint32_t u = wt[j][e / 2];
-            h[j].v[e] = norm_value(h[j].v[e], f, (uint16_t)(e & 1 ? u >> 16 : u));
+            h[j].v[e] = norm_value(h[j].v[e], f, wt[j][e]);
             m = fmaxf(m, fabsf(h[j].v[e]));
         }
     m = row_max<TPR>(m, red);
@@ -390,59 +416,84 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_quant_vec(uint8_
     }
     if (t == 0)
         scales[row] = scale;
-    auto code = [&](float y) { return FP8 ? (uint32_t)f32_to_fp8(y * inv) : (uint32_t)(uint8_t)f32_to_int8(y, inv); };
+    auto code = [&](float y) { return FP8 ? (uint32_t)finite_to_fp8(y * inv) : (uint32_t)(uint8_t)f32_to_int8(y, inv); };
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         const int i = (t + TPR * j) * VE;
-        uint32_t c[VE / 4];
+        if constexpr (VE == 1) {
+            if (i < cols)
+                q[row * cols + i] = (uint8_t)code(h[j].v[0]);
+        } else {
+            uint32_t c[VE / 4];
 #pragma unroll
-        for (int e = 0; e < VE; e += 4)
-            c[e / 4] = code(h[j].v[e]) | code(h[j].v[e + 1]) << 8 | code(h[j].v[e + 2]) << 16 | code(h[j].v[e + 3]) << 24;
-        if (i < cols)
-            __builtin_memcpy(__builtin_assume_aligned(q + row * cols + i, VE), c, VE);
+            for (int e = 0; e < VE; e += 4)
+                c[e / 4] = code(h[j].v[e]) | code(h[j].v[e + 1]) << 8 | code(h[j].v[e + 2]) << 16 | code(h[j].v[e + 3]) << 24;
+            if (i < cols)
+                __builtin_memcpy(__builtin_assume_aligned(q + row * cols + i, VE), c, VE);
+        }
     }
 }
 
-// Rows in 16-byte words where every row of x, the residual, w and the outputs
-// begins on one and has whole ones; others an element at a time.  Threads of a
-// row: few for many rows, as many as leave a word each for few.
+// Rows of up to 16384 fp32 or 32768 bf16 elements go in 16-byte words where every
+// row of x, the residual, w and the outputs begins on one and has whole ones, and
+// else, up to 8192, an element at a time; longer ones take the three passes above.
+// The fewest threads that hold the row in four words each (a wave two, 512 eight):
+// few large loads a thread and as many rows a CU as fit.  Measured, fp32 with a
+// residual (the bytes of 8192 x 4096 at the rate of a large copy: 84 us):
+//   1 x 4096 3.8 us, 2048 x 4096 18.6 (1024 threads: 3.7 and 22.1), 8192 x 4096 82
+//   30000 x 512 35.9 (256 threads 49.9), 30000 x 256 18.4 (44.1)
+//   2000 x 8192 to E4M3 40.8 (256 threads of eight words 48.8)
+//   2000 x 12288 to E4M3 75.2 (1024 threads 81.2), 300 x 12288 14.1 (15.8)
+//   3000 x 4099, element at a time, 45.6 (the three passes 63.3)
+// A few hundred rows are bound by one row's way through load, sum and maximum
+// (1 x 8192: 4.5 us), very wide ones to E4M3 by the codec's instructions.
 template <bool FP8, bool BF16>
 static bool launch_norm_vec(uint8_t *q, float *scales, void *sum, const void *x, size_t x_stride, const void *res,
                             size_t res_stride, const uint16_t *w, int rows, int cols, float eps, hipStream_t s)
 {
-    constexpr int VE = Word<BF16>::VE;
-    if (cols % VE || x_stride % VE || (res && res_stride % VE) ||
-        (((uintptr_t)x | (uintptr_t)res | (uintptr_t)sum) & 15) || (uintptr_t)w % (2 * VE) || (uintptr_t)q % VE)
-        return false;
-    const int words = cols / VE;
-    auto go = [&](auto tpr, auto nv) {
-        constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
-        constexpr int per = TPR < 256 ? 256 / TPR : 1;
-        hipLaunchKernelGGL((k_norm_quant_vec<FP8, BF16, TPR, NV>), dim3((rows + per - 1) / per), dim3(TPR < 256 ? 256 : TPR), 0,
-                           s, q, scales, sum, x, x_stride, res, res_stride, w, rows, cols, eps);
-        return true;
-    };
+    constexpr int VE = BF16 ? 8 : 4;
     using std::integral_constant;
+    constexpr integral_constant<int, VE> vec;
     constexpr integral_constant<int, 1> one;
     constexpr integral_constant<int, 2> two;
     constexpr integral_constant<int, 4> four;
+    constexpr integral_constant<int, 8> eight;
+    constexpr integral_constant<int, 64> wave;
+    constexpr integral_constant<int, 256> some;
+    constexpr integral_constant<int, 512> more;
+    constexpr integral_constant<int, 1024> most;
+    auto go = [&](auto ve, auto tpr, auto nv) {
+        constexpr int TPR = decltype(tpr)::value;
+        constexpr int per = TPR < 256 ? 256 / TPR : 1;
+        hipLaunchKernelGGL((k_norm_quant_vec<FP8, BF16, decltype(ve)::value, TPR, decltype(nv)::value>),
+                           dim3((rows + per - 1) / per), dim3(TPR < 256 ? 256 : TPR), 0, s, q, scales, sum, x, x_stride, res,
+                           res_stride, w, rows, cols, eps);
+        return true;
+    };
+    if (cols % VE || x_stride % VE || (res && res_stride % VE) ||
+        (((uintptr_t)x | (uintptr_t)res | (uintptr_t)sum) & 15) || (uintptr_t)w % (2 * VE) || (uintptr_t)q % VE) {
+        if (cols <= 64)
+            return go(one, wave, one);
+        if (cols <= 512)
+            return go(one, some, two);
+        if (cols <= 2048)
+            return go(one, some, eight);
+        return cols <= 8192 && go(one, most, eight);
+    }
+    const int words = cols / VE;
     if (words <= 64)
-        return go(integral_constant<int, 64>(), one);
-    if (words <= 128 && rows >= 1024)
-        return go(integral_constant<int, 64>(), two);
+        return go(vec, wave, one);
+    if (words <= 128)
+        return go(vec, wave, two);
     if (words <= 256)
-        return go(integral_constant<int, 256>(), one);
-    if (words <= 512 && rows >= 256)
-        return go(integral_constant<int, 256>(), two);
-    if (words <= 1024 && rows >= 256)
-        return go(integral_constant<int, 256>(), four);
+        return go(vec, some, one);
+    if (words <= 512)
+        return go(vec, some, two);
     if (words <= 1024)
-        return go(integral_constant<int, 1024>(), one);
+        return go(vec, some, four);
     if (words <= 2048)
-        return go(integral_constant<int, 1024>(), two);
-    if (words <= 4096)
-        return go(integral_constant<int, 1024>(), four);
-    return false;
+        return go(vec, most, two);
+    return words <= 4096 && go(vec, more, eight);
 }
 
 template <bool FP8>

@@ -8,6 +8,7 @@ libamdhip64.so.7; the library then binds to the already-loaded copy).
 There is no CPU path here: when the library or a GPU is missing, calls raise.
 """
 import ctypes as C
+import functools
 import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -157,6 +158,8 @@ class Lib:
             fn.restype = res
             fn.argtypes = args
         self._inited = False
+        self._prefix_bytes = functools.lru_cache(4096)(self.lib.be42_prefix_attention_workspace_bytes)
+        self._logprobs_bytes = functools.lru_cache(4096)(self.lib.be42_logprobs_workspace_bytes)
 
     # -- plumbing -------------------------------------------------------------
     def device_available(self):
@@ -217,13 +220,17 @@ class Lib:
             raise Be42Error(f"{name}: {what} is not contiguous")
 
     def _rows(self, name, what, x, dtypes, cols=None, dev=None):
-        """Element stride of the rows of a 2-d tensor whose rows are dense."""
+        """Element stride of the rows of a 2-d tensor whose rows are dense (ctypes
+        would cut one past 32 bits without a word)."""
         if x.dim() != 2 or x.dtype not in dtypes or (cols is not None and x.shape[1] != cols) or \
                 (dev is not None and x.device != dev):
             raise Be42Error(f"{name}: {what} is {x.dtype} {tuple(x.shape)} on {x.device}")
         if x.shape[1] > 1 and x.stride(1) != 1:
             raise Be42Error(f"{name}: {what} has rows that are not dense")
-        return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+        stride = x.stride(0) if x.shape[0] > 1 else x.shape[1]
+        if max(stride, x.shape[0], x.shape[1]) >= 1 << 31:
+            raise Be42Error(f"{name}: {what} has shape {tuple(x.shape)}, rows {stride} apart: past 32 bits")
+        return stride
 
     # -- quant codecs ---------------------------------------------------------
     def quant_rows_int8(self, x):
@@ -260,11 +267,11 @@ class Lib:
             if residual.shape[0] != rows:
                 raise Be42Error(f"{name}: residual has {residual.shape[0]} rows, x {rows}")
             if sum is None:
-                sum = t.empty((rows, cols), dtype=dt, device=dev)
+                sum = t.empty(rows, cols, dtype=dt, device=dev)
         if sum is not None:
             self._want(name, "sum", sum, (dt,), (rows, cols), dev)
         self._want(name, "w", w, (t.bfloat16,), (cols,), dev)
-        q = t.empty((rows, cols), dtype=t.int8 if kind == "int8" else t.uint8, device=dev)
+        q = t.empty(rows, cols, dtype=t.int8 if kind == "int8" else t.uint8, device=dev)
         s = t.empty(rows, dtype=t.float32, device=dev)
         self._device_call(x, name, q.data_ptr(), s.data_ptr(), None if sum is None else sum.data_ptr(), x.data_ptr(), xs,
                           None if residual is None else residual.data_ptr(), rs, dt == t.bfloat16, w.data_ptr(), rows,
@@ -412,7 +419,9 @@ class Lib:
     def logprobs(self, logits, tokens=None, temp=1.0, top_k=0, entropy=False, workspace=None):
         """Of logits [rows][n] (float32 or bfloat16, rows may be strided): a dict
         of "logprobs" [rows][j] for the given tokens [rows][j] (int32), "entropy"
-        [rows], "top_ids" and "top_logprobs" [rows][top_k], as far as asked for."""
+        [rows], "top_ids" and "top_logprobs" [rows][top_k], as far as asked for.
+        workspace: be42_logprobs_workspace_bytes bytes (uint8) to use instead of
+        a new tensor."""
         t, name = self.torch, "be42_logprobs"
         dev = logits.device
         ls = self._rows(name, "logits", logits, (t.float32, t.bfloat16))
@@ -423,20 +432,21 @@ class Lib:
                 raise Be42Error(f"{name}: tokens has shape {tuple(tokens.shape)}")
             given = tokens.shape[1]
             self._want(name, "tokens", tokens, (t.int32,), (rows, given), dev)
-            got["logprobs"] = t.empty((rows, given), dtype=t.float32, device=dev)
+            got["logprobs"] = t.empty(rows, given, dtype=t.float32, device=dev)
         if entropy:
             got["entropy"] = t.empty(rows, dtype=t.float32, device=dev)
         if top_k:
-            got["top_ids"] = t.empty((rows, top_k), dtype=t.int32, device=dev)
-            got["top_logprobs"] = t.empty((rows, top_k), dtype=t.float32, device=dev)
-        ws, wsb = None, 0
-        if workspace is not None:
+            got["top_ids"] = t.empty(rows, top_k, dtype=t.int32, device=dev)
+            got["top_logprobs"] = t.empty(rows, top_k, dtype=t.float32, device=dev)
+        if workspace is None:
+            workspace = t.empty(self._logprobs_bytes(n, rows, top_k), dtype=t.uint8, device=dev)
+        else:
             self._want(name, "workspace", workspace, (t.uint8,), None, dev)
-            ws, wsb = workspace.data_ptr(), workspace.numel()
         at = {k: v.data_ptr() for k, v in got.items()}
         self._device_call(logits, name, at.get("logprobs"), at.get("entropy"), at.get("top_ids"), at.get("top_logprobs"),
                           logits.data_ptr(), logits.dtype == t.bfloat16, ls, n, rows, temp,
-                          None if tokens is None else tokens.data_ptr(), given, top_k, ws, wsb)
+                          None if tokens is None else tokens.data_ptr(), given, top_k,
+                          workspace.data_ptr(), workspace.numel())
         return got
 
     def kv_pool(self, kind, n_layers, n_kv, head_dim, max_logical, hpT=None):
@@ -485,30 +495,37 @@ class Lib:
         queries may be strided) over the first prefix_len tokens of slot
         prefix_slot, read once for all, and the first lens[b] tokens of slot
         slots[b] (None: slot b / all its tokens).  max_len bounds lens (None:
-        what a slot can hold; the closer, the better the work is split)."""
+        what a slot can hold; the closer, the better the work is split).
+        workspace: be42_prefix_attention_workspace_bytes bytes (uint8) to use
+        instead of a new tensor."""
         t, name = self.torch, "be42_prefix_attention"
         if q.dim() != 3 or q.shape[2] != pool.head_dim or q.dtype not in (t.float32, t.bfloat16):
             raise Be42Error(f"{name}: q is {q.dtype} {tuple(q.shape)}")
         B, H, hd = q.shape
+        dev = q.device
+        if q.get_device() != pool.device:
+            raise Be42Error(f"{name}: q on {dev}, the pool on GPU {pool.device}")
         if B and ((hd > 1 and q.stride(2) != 1) or (H > 1 and q.stride(1) != hd)):
             raise Be42Error(f"{name}: q has rows that are not dense")
         qs = q.stride(0) if B > 1 else H * hd
         for what, x in (("slots", slots), ("lens", lens)):
             if x is not None:
-                self._want(name, what, x, (t.int32,), (B,), q.device)
+                self._want(name, what, x, (t.int32,), (B,), dev)
         if out is None:
-            out = t.empty((B, H, hd), dtype=q.dtype, device=q.device)
+            out = t.empty(B, H, hd, dtype=q.dtype, device=dev)
         else:
-            self._want(name, "out", out, (q.dtype,), (B, H, hd), q.device)
+            self._want(name, "out", out, (q.dtype,), (B, H, hd), dev)
         if max_len is None:
             max_len = pool.max_logical * 16
-        ws, wsb = None, 0
-        if workspace is not None:
-            self._want(name, "workspace", workspace, (t.uint8,), None, q.device)
-            ws, wsb = workspace.data_ptr(), workspace.numel()
+        if max(qs, prefix_slot, prefix_len, max_len) >= 1 << 31 or min(prefix_slot, prefix_len, max_len) < 0:
+            raise Be42Error(f"{name}: queries {qs} apart, slot {prefix_slot}, prefix_len {prefix_len}, max_len {max_len}")
+        if workspace is None:
+            workspace = t.empty(self._prefix_bytes(B, H, pool.n_kv, hd, prefix_len, max_len), dtype=t.uint8, device=dev)
+        else:
+            self._want(name, "workspace", workspace, (t.uint8,), None, dev)
         self._device_call(q, name, pool.handle, q.data_ptr(), q.dtype == t.bfloat16, qs, B, H, prefix_slot, prefix_len,
                           None if slots is None else slots.data_ptr(), None if lens is None else lens.data_ptr(), max_len,
-                          scale, out.data_ptr(), ws, wsb)
+                          scale, out.data_ptr(), workspace.data_ptr(), workspace.numel())
         return out
 
     # -- linear KV cache [T][n_kv][head_dim] bf16 (kv_cache.c) ------------------
@@ -569,6 +586,7 @@ class KVPool:
         self.s = C.cast(h, C.POINTER(KVPoolStruct)).contents
         self.kind, self.n_layers, self.n_kv, self.head_dim = kind, n_layers, n_kv, head_dim
         self.max_logical = max_logical
+        self.device = lib.torch.cuda.current_device()
 
     def append(self, layer, k, v, pos0):
         n = k.shape[0]

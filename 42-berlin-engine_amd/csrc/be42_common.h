@@ -18,6 +18,9 @@ int hip_fail(hipError_t e, const char *what, const char *file, int line);
 
 // Grow-only device workspace, one per device, owned by the library.
 void *workspace(size_t bytes, hipStream_t s);
+// Is the stream being captured?  A graph that used the library's workspace would
+// go on using it after a larger call has replaced it.
+bool captured(hipStream_t s);
 
 // FP8 encoder exponent thresholds (see quant.hip): thr[i] is the smallest
 // float a in [2^(i+e0-1), 2^(i+e0)) for which glibc's floorf(log2f(a)) returns
@@ -58,6 +61,7 @@ inline hipStream_t as_stream(void *s) { return reinterpret_cast<hipStream_t>(s);
 namespace be42 {
 
 constexpr int kWave = 64;
+constexpr int kMaxBlocks = (1 << 24) - 1;   // of 256 threads: a launch has less than 2^32 threads
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v8i __attribute__((ext_vector_type(8)));

@@ -910,7 +910,7 @@ extern "C" int be42_prefix_attention(const be42_kv_pool *pool, const void *q, in
     const int parts = a.parts_p + a.parts_o;
     const long blocks = (long)P.n_kv * ((long)a.tiles_p * a.parts_p + (long)a.tiles_o * n_queries * a.parts_o);
     const size_t rows = (size_t)n_queries * n_heads;
-    BE42_CHECK(blocks <= 0x7FFFFFFF && (long)n_queries * (n_heads / P.n_kv) <= 0x7FFFFFFF - 16,
+    BE42_CHECK(blocks <= kMaxBlocks && rows <= 4 * (size_t)kMaxBlocks,
                "be42_prefix_attention: %d queries of %d heads", n_queries, n_heads);
     const size_t need = be42_prefix_attention_workspace_bytes(n_queries, n_heads, P.n_kv, P.head_dim, prefix_len,
                                                               max_len);
@@ -918,6 +918,7 @@ extern "C" int be42_prefix_attention(const be42_kv_pool *pool, const void *q, in
                "be42_prefix_attention: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, need);
     hipStream_t s = as_stream(stream);
     if (parts > 1) {
+        BE42_CHECK(workspace || !captured(s), "be42_prefix_attention: a captured call needs a workspace of the caller's");
         if (!workspace)
             workspace = be42::workspace(need, s);
         if (!workspace)

@@ -8,6 +8,7 @@
 // max reduction, the divisions are IEEE divisions, roundf rounds half away
 // from zero, and the FP8 exponent reproduces glibc's floorf(log2f(a)) through
 // a per-binade threshold table measured on the host at init.
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <type_traits>
@@ -625,13 +626,18 @@ static int norm_quant_rows(const char *name, bool fp8, uint8_t *q, float *scales
         const int rc = ensure_thresholds();
         if (rc)
             return rc;
-        launch_norm_quant<true>(q, scales, sum, x, x_stride, residual, residual_stride, act_bf16 != 0, w, rows, cols,
-                                eps, as_stream(stream));
-    } else {
-        launch_norm_quant<false>(q, scales, sum, x, x_stride, residual, residual_stride, act_bf16 != 0, w, rows, cols,
-                                 eps, as_stream(stream));
     }
-    BE42_LAUNCH_CHECK();
+    // a launch has less than 2^32 threads
+    constexpr int kMost = 1 << 21;
+    const size_t sz = act_bf16 ? 2 : 4;
+    for (size_t r = 0; r < (size_t)rows; r += kMost) {
+        const int some = (int)std::min((size_t)rows - r, (size_t)kMost);
+        auto at = [&](const void *p, size_t stride) { return p ? (const char *)p + r * stride * sz : nullptr; };
+        auto go = fp8 ? launch_norm_quant<true> : launch_norm_quant<false>;
+        go(q + r * cols, scales + r, (void *)at(sum, cols), at(x, x_stride), x_stride, at(residual, residual_stride),
+           residual_stride, act_bf16 != 0, w, some, cols, eps, as_stream(stream));
+        BE42_LAUNCH_CHECK();
+    }
     return BE42_OK;
 }
 

@@ -62,6 +62,12 @@ void *workspace(size_t bytes, hipStream_t s)
     return w.ptr;
 }
 
+bool captured(hipStream_t s)
+{
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    return s && hipStreamIsCapturing(s, &st) == hipSuccess && st != hipStreamCaptureStatusNone;
+}
+
 }  // namespace be42
 
 using namespace be42;

@@ -653,11 +653,12 @@ extern "C" int be42_logprobs(float *logprobs, float *entropy, int *top_ids, floa
     const bool aligned = !((uintptr_t)logits & 15) && row_stride % (logits_bf16 ? 8 : 4) == 0;
     cut_row(n, aligned ? 0 : 7, rows, logits_bf16 != 0, &chunks, &per, &runs);
     const long blocks = runs * rows;
-    BE42_CHECK(blocks <= 0x7FFFFFFF, "be42_logprobs: %d rows of %d", rows, n);
+    BE42_CHECK(blocks <= kMaxBlocks, "be42_logprobs: %d rows of %d (at most %d)", rows, n, kMaxBlocks);
     ScoreArgs a = {logits, (size_t)row_stride, logprobs, entropy, top_logprobs, top_ids, tokens, n_tokens, top_k, n, c,
                    (int)chunks, (int)per, (int)runs};
     hipStream_t s = as_stream(stream);
     if (runs > 1) {
+        BE42_CHECK(workspace || !captured(s), "be42_logprobs: a captured call needs a workspace of the caller's");
         if (!workspace)
             workspace = be42::workspace(need, s);
         if (!workspace)

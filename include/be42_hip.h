@@ -9,8 +9,9 @@
  *
  * One stream at a time per device: the library keeps one grow-only workspace,
  * one split-K partial-sum buffer and the exchange buffers of the split route +
- * attention per process (used by the GEMVs, by be42_paged_attention /
- * be42_lsh_attention without a caller workspace, by be42_lsh_attention and the
+ * attention per process (used by the GEMVs, by be42_paged_attention,
+ * be42_lsh_attention, be42_prefix_attention and be42_logprobs without a caller
+ * workspace, by be42_lsh_attention and the
  * decoder when at most 64 (query, KV head) pairs are split over several
  * workgroups each, and by the decoder's fallback paths), so calls that use
  * them must not run concurrently on two streams.  Calls on one stream are
@@ -64,8 +65,9 @@ int be42_quant_rows_fp8(uint8_t *q, float *scales, const float *x, int rows, int
  * before the norm reads it); row r begins at element r * x_stride / r *
  * residual_stride.  sum (may be NULL) takes h, [rows][cols] in the rows' type;
  * it may be x or residual itself where that one's rows are contiguous, and
- * overlaps neither otherwise.  w: [cols] bf16.  A row whose h holds an infinity
- * or a NaN gets unspecified codes; other rows are not touched by it. */
+ * overlaps neither otherwise.  w: [cols] bf16.  A row whose h or y holds an
+ * infinity or a NaN, or whose largest |y| is above 0 but below 2^-120, gets
+ * unspecified codes; other rows are not touched by it. */
 int be42_norm_quant_rows_int8(int8_t *q, float *scales, void *sum, const void *x, int x_stride,
                               const void *residual, int residual_stride, int act_bf16, const uint16_t *w, int rows,
                               int cols, float eps, void *stream);
@@ -286,8 +288,11 @@ int  be42_lsh_attention_status(void *stream);
  * lens and a slot's pages are cut at the tokens the slot holds, and a slot
  * outside the pool holds none.  The launch depends on prefix_len and max_len
  * alone, so slots and lens may change between replays of a captured graph.
- * workspace NULL: the library's (grow-only), else a device buffer of
- * be42_prefix_attention_workspace_bytes() bytes, 16-byte aligned. */
+ * out overlaps no input.  At most 2^24 - 1 workgroups a launch (n_queries *
+ * n_heads above 2^20 may be refused).
+ * workspace NULL: the library's (grow-only; refused while the stream is
+ * captured), else a device buffer of be42_prefix_attention_workspace_bytes()
+ * bytes, 16-byte aligned, that no call on another stream uses meanwhile. */
 size_t be42_prefix_attention_workspace_bytes(int n_queries, int n_heads, int n_kv, int head_dim, int prefix_len,
                                              int max_len);
 int    be42_prefix_attention(const be42_kv_pool *pool, const void *q, int q_bf16, int q_stride, int n_queries,
@@ -457,9 +462,11 @@ int be42_sample_top_p_dt(int *out, const void *logits, int logits_bf16, int n, i
  * Logits of -infinity are tokens of probability zero.  A row without a
  * distribution (it holds a NaN or +infinity, or nothing but -infinity) gets NaN
  * log probabilities and entropy; its top_ids take a NaN for -infinity.
- * n_tokens and top_k may be 0 (their arrays are then not used).
- * workspace NULL: the library's (grow-only), else a device buffer of
- * be42_logprobs_workspace_bytes() bytes, 16-byte aligned. */
+ * n_tokens and top_k may be 0 (their arrays are then not used).  n <= 2^30 and
+ * rows < 2^24.
+ * workspace NULL: the library's (grow-only; refused while the stream is
+ * captured), else a device buffer of be42_logprobs_workspace_bytes() bytes,
+ * 16-byte aligned, that no call on another stream uses meanwhile. */
 size_t be42_logprobs_workspace_bytes(int n, int rows, int top_k);
 int    be42_logprobs(float *logprobs, float *entropy, int *top_ids, float *top_logprobs, const void *logits,
                      int logits_bf16, int row_stride, int n, int rows, float temp, const int *tokens, int n_tokens,

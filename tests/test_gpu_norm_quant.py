@@ -161,3 +161,16 @@ def test_graph_and_other_stream(be, orc):
         torch.cuda.synchronize()
         check(got, defined(orc, a, b, w.cpu(), EPS, "fp8"))
         assert torch.equal(be.norm_quant_rows(x, w, EPS, "fp8", residual=r)[0], got[0])
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+@pytest.mark.parametrize("cols", [8, 3])
+def test_more_rows_than_one_launch_takes(be, orc, kind, cols):
+    rows = (1 << 21) + 3
+    gen = torch.Generator().manual_seed(13)
+    x, r = (torch.randn(rows, cols, generator=gen).bfloat16() for _ in range(2))
+    w = torch.randn(cols, generator=gen).bfloat16()
+    q, s, h = be.norm_quant_rows(x.cuda(), w.cuda(), EPS, kind, residual=r.cuda())
+    at = [0, 1, rows // 2, (1 << 21) - 1, 1 << 21, rows - 1]
+    check((q[at], s[at], h[at]), defined(orc, x[at], r[at], w, EPS, kind))
+    assert torch.equal(h.cpu(), x + r)

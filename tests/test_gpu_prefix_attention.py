@@ -297,3 +297,59 @@ def test_graph_decodes_on(be):
         torch.cuda.synchronize()
         again = run(be, pool, qc, k, v, 3, 200, [int(p) for p in place], [held[p] for p in place], 12, scale=0.125)
         assert torch.equal(again, got), step
+
+
+def test_two_graphs_and_two_streams(be):
+    """Calls without a workspace share none: two graphs replayed at once, a larger
+    eager call and calls on two streams leave each other's results alone."""
+    pool, _, _ = make_pool(be, "bf16", 9, 2, 64, [30] * 8 + [3000], 40)
+    sizes = ((4, 3000), (8, 1700))
+    qs = [queries(41 + i, b, 8, 64, False).cuda() for i, (b, _) in enumerate(sizes)]
+    call = lambda i: be.prefix_attention(pool, qs[i], 8, sizes[i][1], 0.125, max_len=30)  # noqa: E731
+    want = [call(0), call(1)]
+    many = queries(43, 64, 8, 64, False).cuda()
+    slots = torch.zeros(64, dtype=torch.int32, device="cuda")
+    streams, graphs, got = [torch.cuda.Stream() for _ in qs], [torch.cuda.CUDAGraph() for _ in qs], []
+    torch.cuda.synchronize()
+    for i in range(2):
+        with torch.cuda.graph(graphs[i], stream=streams[i]):
+            got.append(call(i))
+    for _ in range(4):
+        be.prefix_attention(pool, many, 8, 3000, 0.125, slots=slots, max_len=30)
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+            a.zero_()
+        torch.cuda.synchronize()
+    eager = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                eager[i].append(call(i))
+    torch.cuda.synchronize()
+    for runs, b in zip(eager, want):
+        assert all(torch.equal(a, b) for a in runs)
+
+
+def test_calls_that_would_use_anothers_memory_are_refused(be):
+    import be42
+    pool, _, _ = make_pool(be, "bf16", 3, 2, 64, [5, 9, 300], 44)
+    q, out = torch.zeros(2, 4, 64, device="cuda"), torch.zeros(2, 4, 64, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=torch.cuda.Stream()):
+        rc = be.lib.be42_prefix_attention(pool.handle, be.p(q), 0, 256, 2, 4, 2, 300, None, None, 9, 0.1, be.p(out), None, 0,
+                                          be.stream())
+        said = be.last_error()
+        out.add_(1)
+    assert rc == -1 and "captured" in said
+    for kw in (dict(prefix_len=(1 << 32) + 30), dict(max_len=1 << 32), dict(prefix_slot=(1 << 32) + 2)):
+        a = dict(prefix_slot=2, prefix_len=30, scale=0.1, max_len=9)
+        a.update(kw)
+        with pytest.raises(be42.Be42Error):
+            be.prefix_attention(pool, q, **a)
+    pool.device = 1                           # as if it lay on another GPU
+    with pytest.raises(be42.Be42Error, match="pool on GPU 1"):
+        be.prefix_attention(pool, q, 2, 30, 0.1, max_len=9)

@@ -199,3 +199,47 @@ def test_graph_and_other_stream(be):
         be.logprobs(torch.randn(70, 5000, device="cuda"), top_k=3)
         for name, v in eager.items():
             assert torch.equal(v, got[name]), (k, name)
+
+
+def test_two_graphs_and_two_streams(be):
+    """Calls without a workspace share none: two graphs replayed at once, a larger
+    eager call and calls on two streams leave each other's results alone."""
+    shapes = ((3, 128256), (5, 60000))
+    xs = [torch.randn(s, generator=torch.Generator().manual_seed(50 + i)).cuda() for i, s in enumerate(shapes)]
+    want = [be.logprobs(x, top_k=10, entropy=True) for x in xs]
+    big = torch.randn(9, 500000, device="cuda")
+    streams, graphs, got = [torch.cuda.Stream() for _ in xs], [torch.cuda.CUDAGraph() for _ in xs], []
+    torch.cuda.synchronize()
+    for x, s, g in zip(xs, streams, graphs):
+        with torch.cuda.graph(g, stream=s):
+            got.append(be.logprobs(x, top_k=10, entropy=True))
+    for _ in range(4):
+        be.logprobs(big, top_k=64, entropy=True)
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(a[n], b[n]) for n in b)
+            for n in a:
+                a[n].zero_()
+        torch.cuda.synchronize()
+    eager = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                eager[i].append(be.logprobs(xs[i], top_k=10, entropy=True))
+    torch.cuda.synchronize()
+    for runs, b in zip(eager, want):
+        assert all(torch.equal(a[n], b[n]) for a in runs for n in b)
+
+
+def test_capture_with_the_librarys_workspace_is_refused(be):
+    x, ent = torch.randn(2, 128256, device="cuda"), torch.zeros(2, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=torch.cuda.Stream()):
+        rc = be.lib.be42_logprobs(None, be.p(ent), None, None, be.p(x), 0, x.shape[1], x.shape[1], 2, 1.0, None, 0, 0, None, 0,
+                                  be.stream())
+        said = be.last_error()
+        ent.add_(1)
+    assert rc == -1 and "captured" in said

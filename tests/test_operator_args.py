@@ -57,6 +57,7 @@ def score(lib, **kw):
 
 
 @pytest.mark.parametrize("kw,word", [
+    (dict(rows=1 << 24, n=1, row_stride=1, top_k=1), "at most"),
     (dict(logits=None), "null"), (dict(n=0), "rows of"), (dict(rows=-1), "rows of"), (dict(row_stride=99), "stride"),
     (dict(n=(1 << 30) + 1, row_stride=INT_MAX), "rows of"),
     (dict(temp=0.0), "temperature"), (dict(temp=-1.0), "temperature"), (dict(temp=float("inf")), "temperature"),
@@ -107,6 +108,7 @@ def prefix(lib, p=None, **kw):
     (dict(max_len=(1 << 30) + 1), "holds"),
     (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(q=PTR + 2), "unaligned"),
     (dict(out=PTR + 2), "unaligned"), (dict(q=PTR + 1, q_bf16=1), "unaligned"),
+    (dict(n_queries=1 << 25, max_len=0), "queries of"), (dict(n_queries=1 << 24), "queries of"),
     (dict(slots=None, n_queries=5), "slots"), (dict(workspace=PTR + 8, bytes=1 << 30), "workspace"),
     (dict(workspace=PTR, bytes=8), "workspace"),
 ])
@@ -130,3 +132,13 @@ def test_prefix_attention_workspace(lib):
     assert f(1, 4, 2, 64, 0, 0) > 0 and f(128, 32, 8, 128, 32768, 1024) > 0
     # sizes past 32 bits do not wrap
     assert f(1 << 20, 64, 8, 128, 1 << 20, 1 << 20) >= f(1 << 10, 64, 8, 128, 1 << 20, 1 << 20) > 0
+
+
+@pytest.mark.parametrize("shape,stride", [((2, 64), 1 << 31), ((2, 64), (1 << 32) + 64), ((1 << 31, 2), 2),
+                                          ((1, (1 << 32) + 8), 1 << 33)])
+def test_strides_and_shapes_past_32_bits(lib, shape, stride):
+    """ctypes would pass them on cut to 32 bits."""
+    import torch
+    x = torch.empty(0, device="meta", dtype=torch.bfloat16).as_strided(shape, (stride, 1))
+    with pytest.raises(be42.Be42Error, match="32 bits"):
+        lib._rows("f", "x", x, (torch.bfloat16,))

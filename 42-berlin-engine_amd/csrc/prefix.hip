@@ -425,7 +425,7 @@ struct WideShared {
 
 template <bool KV8, int HD, int NP, int PP, int R>
 __device__ __forceinline__ void part32(const be42_kv_pool &P, const PrefixArgs &a, WideShared<KV8, HD, R> &S, int slot,
-                                       int lo, int hi, int kvh, int row0, int rows)
+                                       int lo, int want, int kvh, int row0, int rows)
 {
     using Shared = WideShared<KV8, HD, R>;
     constexpr int NK = HD / 16, NE = HD / 32, kRowBytes = HD * (KV8 ? 1 : 2), kRowWords = kRowBytes / 16;
@@ -439,7 +439,6 @@ __device__ __forceinline__ void part32(const be42_kv_pool &P, const PrefixArgs &
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, h = lane >> 5;
     const int rg = wave % R, tg = wave / R;
     const int G = a.n_heads / P.n_kv;
-    const int ns = (hi - lo + kStage - 1) / kStage;
     // physical pages of the next stages: lane 2 T i + p holds page p of stage i
     constexpr int kHeld = kWave / (2 * T);
     int pages = table_page(P, slot, lo / kPage + lane);
@@ -483,8 +482,10 @@ __device__ __forceinline__ void part32(const be42_kv_pool &P, const PrefixArgs &
         // (the counts that are waited for assume that stages are loaded in order)
         asm volatile("" ::: "memory");
     };
-    for (int i = 0; i < D && i < ns; i++)
+    // the first stages are asked for before it is known how many there are
+    for (int i = 0; i < D; i++)
         load(i);
+    const int hi = max(lo, slot_tokens(P, slot, want)), ns = (hi - lo + kStage - 1) / kStage;
 
     v16f O[NE];
 #pragma unroll
@@ -659,7 +660,7 @@ __device__ __forceinline__ void part32(const be42_kv_pool &P, const PrefixArgs &
     // the sums of the T waves of each row; dims of operand row x = 8 (i / 4) +
     // 4 h + i % 4 of tile e: 32 e + x, INT8 pages NE x + e
     l += __shfl_xor(l, 32, kWave);
-    __syncthreads();                       // every wave is done with the ring
+    stage_barrier<0>();                    // every wave is done with the ring, and its loads are
     const int r = 32 * rg + c;
     if (h == 0) {
         S.sums.m[tg][r] = m;
@@ -675,52 +676,71 @@ __device__ __forceinline__ void part32(const be42_kv_pool &P, const PrefixArgs &
     __syncthreads();
 }
 
-// Writes rows first .. of a part whose NW waves (or groups of them) left their
-// sums in LDS: m, l [NW][], o [NW][][HD + 4]; `lanes` threads a row.
-template <int HD, bool QB, int NW, class S>
-__device__ __forceinline__ void write_part(const PrefixArgs &a, const S &sums, int c, int d4, int lanes, size_t row, int part)
+// Writes the rows of a part, row0 .. rows - 1 of the tile's, whose waves (or groups
+// of them) left their sums in LDS: m, l [NW][ROWS], o [NW][ROWS][HD + 4].  HD / 4
+// threads a row; a thread reads kAt rows at once (one at a time a tile of 64 rows
+// took 2.6 us, LDS's latency four times over for each).
+template <int HD, bool QB, int NW, int ROWS, class S>
+__device__ __forceinline__ void write_part(const PrefixArgs &a, const S &sums, int row0, int rows, int b0, int kvh, int G,
+                                           int part)
 {
-    float top = sums.m[0][c], w[NW], l = 0.0f;
-#pragma unroll
-    for (int x = 1; x < NW; x++)
-        top = fmaxf(top, sums.m[x][c]);
-#pragma unroll
-    for (int x = 0; x < NW; x++) {
-        w[x] = part_weight(sums.m[x][c], sums.l[x][c], top);
-        l += w[x] * sums.l[x][c];
-    }
+    constexpr int L = HD / 4, kApart = 64 * kPartWaves / L, kAt = ROWS / kApart < 4 ? ROWS / kApart : 4;
     const size_t all = (size_t)a.n_queries * a.n_heads;
     const bool last = a.parts_p + a.parts_o == 1;
-    if (!last && d4 == 0)
-        *(float2 *)(a.part_ml + 2 * (part * all + row)) = make_float2(top, l);
-    if (!last && l == 0.0f)
-        return;                    // k_prefix_join reads no values of a part without tokens
-    const float inv = last ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
-    for (int d = 4 * d4; d < HD; d += 4 * lanes) {
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const int d = 4 * (threadIdx.x % L), more_q = kApart / G, more_h = kApart % G;
+    int c = threadIdx.x / L, qi = (row0 + c) / G, hi = (row0 + c) % G;       // query and head of the group of row c
+#pragma unroll 1
+    while (row0 + c < rows && c < ROWS) {
+        float m[kAt][NW], l[kAt][NW];
+        float4 o[kAt][NW];
 #pragma unroll
-        for (int y = 0; y < NW; y++) {
-            const float4 o = *(const float4 *)&sums.o[y][c][d];
-            v.x = __fmaf_rn(w[y], o.x, v.x);
-            v.y = __fmaf_rn(w[y], o.y, v.y);
-            v.z = __fmaf_rn(w[y], o.z, v.z);
-            v.w = __fmaf_rn(w[y], o.w, v.w);
+        for (int i = 0; i < kAt; i++)
+#pragma unroll
+            for (int x = 0; x < NW; x++) {
+                m[i][x] = sums.m[x][c + i * kApart];
+                l[i][x] = sums.l[x][c + i * kApart];
+                o[i][x] = *(const float4 *)&sums.o[x][c + i * kApart][d];
+            }
+#pragma unroll
+        for (int i = 0; i < kAt; i++) {
+            float top = m[i][0], sum = 0.0f;
+#pragma unroll
+            for (int x = 1; x < NW; x++)
+                top = fmaxf(top, m[i][x]);
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int x = 0; x < NW; x++) {
+                const float w = part_weight(m[i][x], l[i][x], top);
+                sum += w * l[i][x];
+                v.x = __fmaf_rn(w, o[i][x].x, v.x);
+                v.y = __fmaf_rn(w, o[i][x].y, v.y);
+                v.z = __fmaf_rn(w, o[i][x].z, v.z);
+                v.w = __fmaf_rn(w, o[i][x].w, v.w);
+            }
+            if (row0 + c < rows) {
+                const size_t row = (size_t)(b0 + qi) * a.n_heads + kvh * G + hi;
+                if (last) {
+                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                    store_out4<QB>(a.out, row * HD + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+                } else {
+                    if (d == 0)
+                        *(float2 *)(a.part_ml + 2 * (part * all + row)) = make_float2(top, sum);
+                    // (k_prefix_join reads no values of a part without tokens)
+                    if (sum != 0.0f)
+                        *(float4 *)(a.part_o + (part * all + row) * HD + d) = v;
+                }
+            }
+            c += kApart;
+            qi += more_q;
+            hi += more_h;
+            if (hi >= G) {
+                hi -= G;
+                qi++;
+            }
         }
-        if (last)
-            store_out4<QB>(a.out, row * HD + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
-        else
-            *(float4 *)(a.part_o + (part * all + row) * HD + d) = v;
     }
 }
 
-// bf16 queries: weights are rounded to bf16 where the matrix cores are what is
-// waited for (many rows; the result is then 1.4 times as far from 64 bits as its
-// own rounding to bf16 puts it), and kept to 16 bits, which costs nothing, where
-// memory is.  fp32 queries: three parts hold all 24 bits of queries and weights.
-//
-// block: (KV head, row tile, part) of the prefix, then (KV head, row tile,
-// query, part) of the own tokens.  R: waves that share the prefix' tokens (0: its
-// rows go in tiles of 16).
 template <bool KV8, int HD, bool QB, int R>
 __global__ __launch_bounds__(64 * kPartWaves, 2) void k_prefix_part(const be42_kv_pool P, const PrefixArgs a)
 {
@@ -728,7 +748,7 @@ __global__ __launch_bounds__(64 * kPartWaves, 2) void k_prefix_part(const be42_k
         PartShared<HD> few;
         std::conditional_t<R != 0, WideShared<KV8, HD, R ? R : 4>, char> many;
     } S;
-    constexpr int NP = QB ? 1 : 3, kRows = R ? 32 * R : 16, kLanes = HD / 4;
+    constexpr int NP = QB ? 1 : 3, kRows = R ? 32 * R : 16;
     const int G = a.n_heads / P.n_kv;
     const unsigned of_prefix = (unsigned)P.n_kv * a.tiles_p * a.parts_p;
     unsigned id = blockIdx.x;
@@ -756,19 +776,17 @@ __global__ __launch_bounds__(64 * kPartWaves, 2) void k_prefix_part(const be42_k
         n = a.prefix_len;
         chunk = a.chunk_p;
     }
-    const int lo = part * chunk, hi = max(lo, slot_tokens(P, slot, min(n, lo + chunk)));
+    const int lo = part * chunk;
+    n = min(n, lo + chunk);
     part += own ? a.parts_p : 0;
-    auto row_at = [&](int ri) { return (size_t)(b0 + ri / G) * a.n_heads + kvh * G + ri % G; };
     if constexpr (R != 0)
         if (!own) {
-            part32<KV8, HD, NP, NP, R>(P, a, S.many, slot, lo, hi, kvh, row0, rows);
-            for (int c = threadIdx.x / kLanes; c < kRows && row0 + c < rows; c += 64 * kPartWaves / kLanes)
-                write_part<HD, QB, kPartWaves / R>(a, S.many.sums, c, threadIdx.x % kLanes, kLanes, row_at(row0 + c), part);
+            part32<KV8, HD, NP, NP, R>(P, a, S.many, slot, lo, n, kvh, row0, rows);
+            write_part<HD, QB, kPartWaves / R, kRows>(a, S.many.sums, row0, rows, b0, kvh, G, part);
             return;
         }
-    part16<KV8, HD, NP, QB ? 2 : 3>(P, a, S.few, slot, lo, hi, kvh, b0, row0, rows);
-    for (int c = threadIdx.x / kLanes; c < 16 && row0 + c < rows; c += 64 * kPartWaves / kLanes)
-        write_part<HD, QB, kPartWaves>(a, S.few, c, threadIdx.x % kLanes, kLanes, row_at(row0 + c), part);
+    part16<KV8, HD, NP, QB ? 2 : 3>(P, a, S.few, slot, lo, max(lo, slot_tokens(P, slot, n)), kvh, b0, row0, rows);
+    write_part<HD, QB, kPartWaves, 16>(a, S.few, row0, rows, b0, kvh, G, part);
 }
 
 // One wave per row: its parts by weight.  Lanes of head_dim / 4 words take the

@@ -225,14 +225,6 @@ __device__ __forceinline__ float act_add(float x, float r)
     return BF16 ? bf16_to_f32(f32_to_bf16(x + r)) : x + r;
 }
 
-__device__ __forceinline__ double wave_sum_d(double v)
-{
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1)
-        v += __shfl_xor(v, o, kWave);
-    return v;
-}
-
 __device__ __forceinline__ float norm_value(float h, double r, uint16_t w)
 {
     return (float)((double)h * r * (double)bf16_to_f32(w));
@@ -269,7 +261,7 @@ __global__ __launch_bounds__(256) void k_norm_quant_rows(uint8_t *q, float *scal
     float m = 0.0f;
     for (int i = threadIdx.x; i < cols; i += 256)
         m = fmaxf(m, fabsf(norm_value(again(i), r, w[i])));
-    m = wave_max(m);
+    m = wave_top(m);
     if ((threadIdx.x & 63) == 0)
         red[threadIdx.x >> 6] = m;
     __syncthreads();
@@ -294,9 +286,7 @@ __global__ __launch_bounds__(256) void k_norm_quant_rows(uint8_t *q, float *scal
 template <int TPR>
 __device__ __forceinline__ double row_sum(double v, double *red)
 {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1)
-        v += __shfl_xor(v, o, kWave);
+    v = wave_sum_d(v);
     if constexpr (TPR > kWave) {
         if ((threadIdx.x & 63) == 0)
             red[threadIdx.x >> 6] = v;
@@ -311,7 +301,7 @@ __device__ __forceinline__ double row_sum(double v, double *red)
 template <int TPR>
 __device__ __forceinline__ float row_max(float v, float *red)
 {
-    v = wave_max(v);
+    v = wave_top(v);
     if constexpr (TPR > kWave) {
         if ((threadIdx.x & 63) == 0)
             red[threadIdx.x >> 6] = v;

@@ -95,12 +95,6 @@ __device__ __forceinline__ float log_prob(const ScoreArgs &a, const RowSums &r, 
     return r.base != r.base ? NAN : (float)(((double)x * (double)a.c - r.base) * 0.69314718055994530942);
 }
 
-// the wave's largest value, in every lane (lane moves)
-__device__ __forceinline__ float wave_top(float v)
-{
-    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wave_prefix_max(v)), 63));
-}
-
 // s and t under the reference `top` >= p.ref
 __device__ __forceinline__ void rebase(const Sums &p, double top, double &s, double &t)
 {
@@ -113,14 +107,10 @@ __device__ __forceinline__ void rebase(const Sums &p, double top, double &s, dou
 // joins the lanes' sums; every lane gets the reference and the sums
 __device__ __forceinline__ void join_lanes(const Sums &mine, double &ref, double &s, double &t)
 {
-    ref = mine.ref;
-    for (int o = 32; o > 0; o >>= 1)
-        ref = fmax(ref, __shfl_xor(ref, o, kWave));
+    ref = wave_max_d(mine.ref);
     rebase(mine, ref, s, t);
-    for (int o = 32; o > 0; o >>= 1) {
-        s += __shfl_xor(s, o, kWave);
-        t += __shfl_xor(t, o, kWave);
-    }
+    s = wave_sum_d(s);
+    t = wave_sum_d(t);
 }
 
 // the logit of given token j of a row (one outside the row: -infinity)

@@ -250,26 +250,39 @@ struct Run {
         const uint32_t part = at == 0 ? v.x : at == 1 ? v.y : at == 2 ? v.z : v.w;
         return __uint_as_float(!BF16 || (raw && (j & 1)) ? part : j & 1 ? part & 0xFFFF0000u : part << 16);
     }
-    // Maxima of a lane's words, and of all of them; raw: an infinity among bf16
-    // entries may be passed over (the bits behind an upper entry do not change
-    // which entry is the largest, but make an infinity a NaN).
-    __device__ __forceinline__ float tops(int chunk, const uint4 (&w)[kScoreU], float (&mg)[kScoreU], bool raw) const
+    // Maxima of a lane's words, and of all of them; a NaN counts as -infinity.
+    // The bits behind a bf16 pair's upper entry do not change which entry is the
+    // largest, but make an infinity a NaN.  So a maximum that keeps NaN is taken
+    // first, and once more with care where it finds one.
+    __device__ __forceinline__ float tops(int chunk, const uint4 (&w)[kScoreU], float (&mg)[kScoreU]) const
     {
         float top = -INFINITY;
-        raw = raw && inside(chunk);
+        bool fine = inside(chunk);
+        if (fine) {
+#pragma unroll
+            for (int u = 0; u < kScoreU; u++) {
+                mg[u] = entry(w[u], 0, true);
+#pragma unroll
+                for (int j = 1; j < VE; j++)
+                    mg[u] = __builtin_elementwise_maximum(mg[u], entry(w[u], j, true));
+                top = __builtin_elementwise_maximum(top, mg[u]);
+            }
+            fine = !__any(top != top);
+        }
+        if (fine) {
+#pragma unroll
+            for (int u = 0; u < (BF16 ? kScoreU : 0); u++)
+                mg[u] = __uint_as_float(__float_as_uint(mg[u]) & 0xFFFF0000u);
+            return BF16 ? __uint_as_float(__float_as_uint(top) & 0xFFFF0000u) : top;
+        }
+        top = -INFINITY;
 #pragma unroll
         for (int u = 0; u < kScoreU; u++) {
             mg[u] = -INFINITY;
-            if (raw) {
 #pragma unroll
-                for (int j = 0; j < VE; j++)
-                    mg[u] = fmaxf(mg[u], entry(w[u], j, true));
-                if (BF16)
-                    mg[u] = __uint_as_float(__float_as_uint(mg[u]) & 0xFFFF0000u);
-            } else {
-#pragma unroll
-                for (int j = 0; j < VE; j++)
-                    mg[u] = fmaxf(mg[u], (unsigned)id(chunk, u, j) < (unsigned)n ? entry(w[u], j) : -INFINITY);
+            for (int j = 0; j < VE; j++) {
+                const float x = entry(w[u], j);
+                mg[u] = x > mg[u] && (unsigned)id(chunk, u, j) < (unsigned)n ? x : mg[u];
             }
             top = fmaxf(top, mg[u]);
         }
@@ -450,7 +463,7 @@ __global__ __launch_bounds__(kWave *kScoreW) void k_score_run(const ScoreArgs a)
     float m = -INFINITY, ref = 0.0f, s = 0.0f, t = 0.0f;
     for (int c = c0 + wave; c < c1; c += kScoreW) {
         run.load(c, w);
-        const float top = run.tops(c, w, mg, true);
+        const float top = run.tops(c, w, mg);
         keep_packed(w);
         if (__any(top > m)) {
             const float r2 = top > m ? top : ref, d = m == -INFINITY ? 0.0f : (ref - r2) * a.c;
@@ -489,16 +502,6 @@ __global__ __launch_bounds__(kWave *kScoreW) void k_score_run(const ScoreArgs a)
             note(T, c, mg, top, k, lane);
             if (T.n_words >= kWave || c + kScoreW >= c1)
                 look<BF16>(T, run, k, lane);
-        }
-    }
-    if (BF16 && k && __any(!(s < INFINITY))) {
-        // the maxima may have passed over +infinity
-        T = {lds[wave], 0, words[wave], &shared, 0, 0};
-        for (int c = c0 + wave; c < c1; c += kScoreW) {
-            run.load(c, w);
-            const float top = run.tops(c, w, mg, false);
-            note(T, c, mg, top, k, lane);
-            look<BF16>(T, run, k, lane);
         }
     }
     const Sums mine = {(double)m * (double)a.c, s, t};

@@ -107,6 +107,44 @@ def test_masked_rows(be, n):
     assert got["logprobs"][1, 0] == 0 and got["logprobs"][1, 1] == -math.inf and got["entropy"][1] == 0
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("rows,n", [(6, 40), (6, 4099), (29, 34245), (6, 128256)])
+@pytest.mark.parametrize("share", [0.02, 0.3, 0.7, 0.99])
+def test_scattered_masks(be, bf16, rows, n, share):
+    """-infinity here and there, in even and odd places alike."""
+    rng = np.random.default_rng(n + int(100 * share))
+    x = torch.from_numpy((rng.standard_normal((rows, n)) * 2.5).astype(np.float32))
+    off = torch.from_numpy(rng.random((rows, n)) < share)
+    off[0] = False
+    off[1, ::2] = True
+    off[2, 1::2] = True
+    off[:, n // 3] = False
+    x[off] = -math.inf
+    x = x.bfloat16() if bf16 else x
+    tokens = torch.from_numpy(rng.integers(0, n, (rows, 2)).astype(np.int32))
+    for temp, k in ((1.0, 1), (1.5, 20), (1.0, 0)):
+        check(be, x, tokens, temp, k)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("n", [64, 4099, 128256])
+def test_top_ids_beside_nan_and_infinity(be, bf16, n):
+    """NaN of both kinds (the signalling one is what a maximum may pass on) and
+    +infinity, beside which the other alternatives are still found."""
+    rng = np.random.default_rng(n + 77)
+    x = torch.from_numpy((rng.standard_normal((4, n)) * 2.5).astype(np.float32))
+    x = x.bfloat16() if bf16 else x
+    bits = x.view(torch.int16 if bf16 else torch.int32)
+    at = torch.from_numpy(rng.permutation(n)[: max(n // 50, 3)])
+    bits[0, at] = 0x7FA0 if bf16 else 0x7FA00000
+    bits[1, at] = 0x7FC0 if bf16 else 0x7FC00000
+    bits[2, at] = -0x0060 if bf16 else -0x00600000           # a signalling NaN with its sign set
+    x[3, at] = math.inf
+    got = be.logprobs(x.cuda(), top_k=20, entropy=True)
+    assert torch.equal(got["top_ids"].cpu(), ids_of(x.float(), 20))
+    assert torch.isnan(got["entropy"]).all() and torch.isnan(got["top_logprobs"]).all()
+
+
 @pytest.mark.parametrize("n", [64, 5000, 128256])
 def test_rows_without_a_distribution(be, n):
     rng = np.random.default_rng(6)

@@ -132,6 +132,13 @@ __device__ __forceinline__ void load_q(const PrefixArgs &a, size_t at, bf16x8 (&
     }
 }
 
+// The scores' factor, log2(e) |scale|, and not 0: times the -infinity of a token
+// past the part that would be NaN.
+__device__ __forceinline__ float log2_scale(const PrefixArgs &a)
+{
+    return fmaxf(fabsf(a.scale) * 1.44269504088896340736f, 1.17549435e-38f);
+}
+
 // The largest of three, NaN if one is.  (fmaxf adds a canonicalizing move for
 // each operand; in inline assembly the wait states after a matrix product would
 // be missing.)
@@ -207,7 +214,7 @@ __device__ __forceinline__ void part16(const be42_kv_pool &P, const PrefixArgs &
         for (int kb = 0; kb < NK; kb++)
             load_q<NP>(a, at + (KV8 ? 64 * (kb / 2) + 16 * g + 8 * (kb % 2) : 32 * kb + 8 * g), Q[kb]);
     }
-    const float sc = fabsf(a.scale) * 1.44269504088896340736f;
+    const float sc = log2_scale(a);
 
     v4f O[NE];
 #pragma unroll
@@ -451,7 +458,7 @@ __device__ __forceinline__ void part32(const be42_kv_pool &P, const PrefixArgs &
 #pragma unroll
     for (int kb = 0; kb < NK; kb++)
         load_q<NP>(a, qat + (KV8 ? 32 * (kb / 2) + 16 * h + 8 * (kb % 2) : 16 * kb + 8 * h), Q[kb]);
-    const float sc = fabsf(a.scale) * 1.44269504088896340736f;
+    const float sc = log2_scale(a);
 
     // K rows of kRowWords 16-byte words: word x of row t lies at x ^ swz(t), so
     // that the rows of an operand spread over the banks
@@ -915,7 +922,7 @@ extern "C" int be42_prefix_attention(const be42_kv_pool *pool, const void *q, in
     const long held = (long)P.max_logical * kPage;
     BE42_CHECK(prefix_len >= 0 && prefix_len <= std::min(held, (long)kMaxTokens) && max_len >= 0 && max_len <= kMaxTokens,
                "be42_prefix_attention: prefix %d, max_len %d (a slot holds %ld tokens)", prefix_len, max_len, held);
-    BE42_CHECK(std::isfinite(scale), "be42_prefix_attention: scale %g", (double)scale);
+    BE42_CHECK(std::fabs(scale) <= 1e30f, "be42_prefix_attention: scale %g", (double)scale);
     BE42_CHECK(!(((uintptr_t)q | (uintptr_t)out) & (q_bf16 ? 1 : 3)), "be42_prefix_attention: unaligned pointer");
     // without slots query b reads slot b
     BE42_CHECK(slots || max_len == 0 || n_queries <= P.n_layers, "be42_prefix_attention: %d queries over %d slots",

@@ -353,3 +353,14 @@ def test_calls_that_would_use_anothers_memory_are_refused(be):
     pool.device = 1                           # as if it lay on another GPU
     with pytest.raises(be42.Be42Error, match="pool on GPU 1"):
         be.prefix_attention(pool, q, 2, 30, 0.1, max_len=9)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("B", [2, 20, 150])
+def test_scale_of_zero_takes_the_mean(be, kind, bf16, B):
+    pool, k, v = make_pool(be, kind, 3, 2, 64, [5, 40, 333], 45)
+    run(be, pool, queries(46, B, 4, 64, bf16), k, v, 2, 333, [i % 2 for i in range(B)], [5 + i % 30 for i in range(B)], 40,
+        scale=0.0)
+    run(be, pool, queries(46, B, 4, 64, bf16), k, v, 2, 333, [i % 2 for i in range(B)], [5 + i % 30 for i in range(B)], 40,
+        scale=1e-42)

@@ -106,7 +106,7 @@ def prefix(lib, p=None, **kw):
     (dict(prefix_slot=4), "slot"), (dict(prefix_slot=-1), "slot"), (dict(prefix_len=129), "holds"),
     (dict(prefix_len=-1), "holds"), (dict(max_len=-1), "holds"),
     (dict(max_len=(1 << 30) + 1), "holds"),
-    (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(q=PTR + 2), "unaligned"),
+    (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(scale=-1e31), "scale"), (dict(q=PTR + 2), "unaligned"),
     (dict(out=PTR + 2), "unaligned"), (dict(q=PTR + 1, q_bf16=1), "unaligned"),
     (dict(n_queries=1 << 25, max_len=0), "queries of"), (dict(n_queries=1 << 24), "queries of"),
     (dict(slots=None, n_queries=5), "slots"), (dict(workspace=PTR + 8, bytes=1 << 30), "workspace"),

@@ -24,6 +24,7 @@ namespace be42 {
 
 constexpr int kTopMax = 64;
 constexpr int kScoreW = 4;                  // waves of a workgroup, each on its own
+constexpr int kScoreWide = 8;               // of one that has a row to itself
 constexpr int kScoreU = 8;                  // words of 16 bytes a lane holds
 constexpr int kChunkBytes = kWave * kScoreU * 16;
 constexpr int kTopCap = 576;                // a wave's candidates: top_k, and the entries of 64 words
@@ -438,15 +439,43 @@ __device__ __forceinline__ void look(TopKeys &T, const Run<BF16> &run, int k, in
     T.n_words = 0;
 }
 
-// block: (row, run)
-template <bool BF16>
-__global__ __launch_bounds__(kWave *kScoreW) void k_score_run(const ScoreArgs a)
+// Calls out(rank, key) for the k largest of the keys that the lanes hold (0: none),
+// all distinct: those that reach a value which few more than k do are ranked.
+// Returns how many there were.
+template <int N, class F>
+__device__ __forceinline__ int select_keys(const unsigned long long (&key)[N], unsigned long long *cand, int k, int lane, F &&out)
 {
-    __shared__ unsigned long long lds[kScoreW][kTopCap + 8];
-    __shared__ int words[kScoreW][(kScoreU + 1) * kWave];
-    __shared__ unsigned long long merged[kScoreW * kTopMax + 8];
-    __shared__ Sums sums[kScoreW];
+    uint32_t q[N];
+#pragma unroll
+    for (int x = 0; x < N; x++)
+        q[x] = (uint32_t)(key[x] >> 32);
+    const uint32_t lo = reached<N>(q, k);
+    int found = 0;
+#pragma unroll
+    for (int x = 0; x < N; x++) {
+        const bool in = key[x] && q[x] >= lo;
+        const unsigned long long who = __ballot(in);
+        if (in)
+            cand[found + __popcll(who & ((1ull << lane) - 1))] = key[x];
+        found += __popcll(who);
+    }
+    if (found <= kWave)
+        rank_keys<1>(cand, found, k, lane, out);
+    else
+        rank_keys<N>(cand, found, k, lane, out);
+    return found;
+}
+
+// block: (row, run)
+template <bool BF16, int W>
+__global__ __launch_bounds__(kWave *W) void k_score_run(const ScoreArgs a)
+{
+    __shared__ unsigned long long lds[W][kTopCap + 8];
+    __shared__ int words[W][(kScoreU + 1) * kWave];
+    __shared__ unsigned long long merged[W * kTopMax + 8];
+    __shared__ Sums sums[W];
     __shared__ uint32_t shared;
+    constexpr bool AHEAD = W > 4;            // few rows: a wave loads the next chunk beside this one
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), k = a.top_k;
     const int row = (int)(blockIdx.x / (unsigned)a.runs), part = (int)(blockIdx.x % (unsigned)a.runs);
     const int c0 = part * a.per, c1 = min(c0 + a.per, a.chunks);
@@ -457,12 +486,22 @@ __global__ __launch_bounds__(kWave *kScoreW) void k_score_run(const ScoreArgs a)
         shared = 0;
     __syncthreads();
     TopKeys T = {lds[wave], 0, words[wave], &shared, 0, 0};
-    uint4 w[kScoreU];
+    uint4 w[kScoreU], next[kScoreU];
     float mg[kScoreU];
     // each lane by itself: its largest entry and its sums, z = (x - m) c
     float m = -INFINITY, ref = 0.0f, s = 0.0f, t = 0.0f;
-    for (int c = c0 + wave; c < c1; c += kScoreW) {
-        run.load(c, w);
+    if (AHEAD && c0 + wave < c1)
+        run.load(c0 + wave, next);
+    for (int c = c0 + wave; c < c1; c += W) {
+        if constexpr (AHEAD) {
+#pragma unroll
+            for (int u = 0; u < kScoreU; u++)
+                w[u] = next[u];
+            if (c + W < c1)
+                run.load(c + W, next);
+        } else {
+            run.load(c, w);
+        }
         const float top = run.tops(c, w, mg);
         keep_packed(w);
         if (__any(top > m)) {
@@ -500,7 +539,7 @@ __global__ __launch_bounds__(kWave *kScoreW) void k_score_run(const ScoreArgs a)
         }
         if (k) {
             note(T, c, mg, top, k, lane);
-            if (T.n_words >= kWave || c + kScoreW >= c1)
+            if (T.n_words >= kWave || c + W >= c1)
                 look<BF16>(T, run, k, lane);
         }
     }
@@ -514,7 +553,7 @@ __global__ __launch_bounds__(kWave *kScoreW) void k_score_run(const ScoreArgs a)
     __syncthreads();
     if (wave)
         return;
-    join_lanes(lane < kScoreW ? sums[lane] : Sums{-INFINITY, 0.0f, 0.0f}, rs, ss, tt);
+    join_lanes(lane < W ? sums[lane] : Sums{-INFINITY, 0.0f, 0.0f}, rs, ss, tt);
     RowSums r = {};
     if (single) {
         r = row_sums(rs, ss, tt);
@@ -532,12 +571,12 @@ __global__ __launch_bounds__(kWave *kScoreW) void k_score_run(const ScoreArgs a)
         else
             a.keys[(size_t)blockIdx.x * k + rank] = key;
     };
-    if (kScoreW * k <= kWave)
-        rank_keys<1>(merged, kScoreW * k, k, lane, out);
-    else if (kScoreW * k <= 2 * kWave)
-        rank_keys<2>(merged, kScoreW * k, k, lane, out);
-    else
-        rank_keys<kScoreW>(merged, kScoreW * k, k, lane, out);
+    unsigned long long key[W];
+#pragma unroll
+    for (int x = 0; x < W; x++)
+        key[x] = x * kWave + lane < W * k ? merged[x * kWave + lane] : 0;
+    wave_lds();
+    select_keys<W>(key, merged, k, lane, out);
 }
 
 // The runs of a row, one wave a row.
@@ -576,19 +615,6 @@ __global__ __launch_bounds__(kWave) void k_score_join(const ScoreArgs a)
     // the keys that reach a value which few more than k do; keys past those that
     // the lanes hold replace them in turn
     for (int i0 = kJoinKeys * kWave;; i0 += (kJoinKeys - 1) * kWave) {
-        uint32_t q[kJoinKeys];
-#pragma unroll
-        for (int x = 0; x < kJoinKeys; x++)
-            q[x] = (uint32_t)(key[x] >> 32);
-        const uint32_t lo = reached<kJoinKeys>(q, k);
-        int found = 0;
-#pragma unroll
-        for (int x = 0; x < kJoinKeys; x++) {
-            const unsigned long long who = __ballot(key[x] && q[x] >= lo);
-            if (key[x] && q[x] >= lo)
-                cand[found + __popcll(who & ((1ull << lane) - 1))] = key[x];
-            found += __popcll(who);
-        }
         const bool last = i0 >= all;
         auto out = [&](int rank, unsigned long long kk) {
             if (last)
@@ -596,10 +622,7 @@ __global__ __launch_bounds__(kWave) void k_score_join(const ScoreArgs a)
             else
                 cand[rank] = kk;
         };
-        if (found <= kWave)
-            rank_keys<1>(cand, found, k, lane, out);
-        else
-            rank_keys<kJoinKeys>(cand, found, k, lane, out);
+        const int found = select_keys<kJoinKeys>(key, cand, k, lane, out);
         if (last)
             return;
         key[0] = lane < min(found, k) ? cand[lane] : 0;
@@ -613,17 +636,23 @@ __global__ __launch_bounds__(kWave) void k_score_join(const ScoreArgs a)
 }
 
 // How a row of n entries is cut: chunks (the first word may begin `before`
-// entries before the row), chunks of a run, runs.  Rows are cut until there are
-// four workgroups a CU; a run has at least a chunk for each wave, and four where
-// the rows alone fill the chip, since joining runs costs a launch of 4 us (333
-// rows of 32003 fp32, half of them masked: 13 us as one run, 17 as three; 1000
-// rows of 128256: 98 and 95).
-static void cut_row(int n, int before, int rows, bool bf16, long *chunks, long *per, long *runs)
+// entries before the row), chunks of a run, runs, and the waves of a workgroup.
+// Up to 256 rows, a workgroup of eight waves takes a whole row where that has up
+// to 24 chunks, or where the rows come near to filling the chip (fp32, top 5, in
+// us: 1 x 32000 8.6, cut 9.6; 1 x 64000 11.4, cut 9.6; 64 x 128256 19.4, cut 16.6;
+// 120 x 128256 19.4, cut 23.5; 200 x 32000 12.7, cut 16.0); rows of up to four
+// chunks do with four waves (200 x 8000 8.3, eight 8.7).  Other rows are cut
+// until there are four workgroups a CU; a run has at least a chunk for each wave,
+// and four where the rows alone fill the chip, since joining runs costs a launch
+// of 4 us (333 x 32003 without alternatives 14.3 uncut).
+static void cut_row(int n, int before, int rows, bool bf16, long *chunks, long *per, long *runs, int *waves)
 {
     const long entries = kChunkBytes / (bf16 ? 2 : 4);
     *chunks = (n + before + entries - 1) / entries;
+    const bool whole = rows <= 256 && *chunks > kScoreW && (*chunks <= 3 * kScoreWide || rows > 96);
+    *waves = whole ? kScoreWide : kScoreW;
     const long least = rows >= 256 ? 4 * kScoreW : kScoreW;
-    *runs = std::min((*chunks + least - 1) / least, (1024 + (long)rows - 1) / rows);
+    *runs = whole ? 1 : std::min((*chunks + least - 1) / least, (1024 + (long)rows - 1) / rows);
     *per = (*chunks + *runs - 1) / *runs;
     *runs = (*chunks + *per - 1) / *per;
 }
@@ -639,7 +668,8 @@ extern "C" size_t be42_logprobs_workspace_bytes(int n, int rows, int top_k)
     size_t most = 0;                        // of either type
     for (int i = 0; i < 4; i++) {           // and alignment
         long chunks, per, runs;
-        cut_row(n, i & 1 ? 7 : 0, rows, i >> 1, &chunks, &per, &runs);
+        int waves;
+        cut_row(n, i & 1 ? 7 : 0, rows, i >> 1, &chunks, &per, &runs, &waves);
         most = std::max(most, (size_t)rows * runs);
     }
     return most * (sizeof(Sums) + top_k * sizeof(unsigned long long));
@@ -668,8 +698,9 @@ extern "C" int be42_logprobs(float *logprobs, float *entropy, int *top_ids, floa
     BE42_CHECK(!workspace || (!((uintptr_t)workspace & 15) && workspace_bytes >= need),
                "be42_logprobs: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, need);
     long chunks, per, runs;
+    int waves;
     const bool aligned = !((uintptr_t)logits & 15) && row_stride % (logits_bf16 ? 8 : 4) == 0;
-    cut_row(n, aligned ? 0 : 7, rows, logits_bf16 != 0, &chunks, &per, &runs);
+    cut_row(n, aligned ? 0 : 7, rows, logits_bf16 != 0, &chunks, &per, &runs, &waves);
     const long blocks = runs * rows;
     BE42_CHECK(blocks <= kMaxBlocks, "be42_logprobs: %d rows of %d (at most %d)", rows, n, kMaxBlocks);
     ScoreArgs a = {logits, (size_t)row_stride, logprobs, entropy, top_logprobs, top_ids, tokens, n_tokens, top_k, n, c,
@@ -684,11 +715,15 @@ extern "C" int be42_logprobs(float *logprobs, float *entropy, int *top_ids, floa
         a.sums = (Sums *)workspace;
         a.keys = (unsigned long long *)(a.sums + blocks);
     }
-    const dim3 g((unsigned)blocks), t(kWave * kScoreW);
-    if (logits_bf16)
-        hipLaunchKernelGGL(k_score_run<true>, g, t, 0, s, a);
-    else
-        hipLaunchKernelGGL(k_score_run<false>, g, t, 0, s, a);
+    const dim3 g((unsigned)blocks), t(kWave * waves);
+    auto run = [&](auto bf16) {
+        constexpr bool BF16 = decltype(bf16)::value;
+        if (waves == kScoreWide)
+            hipLaunchKernelGGL((k_score_run<BF16, kScoreWide>), g, t, 0, s, a);
+        else
+            hipLaunchKernelGGL((k_score_run<BF16, kScoreW>), g, t, 0, s, a);
+    };
+    logits_bf16 ? run(std::true_type()) : run(std::false_type());
     if (runs > 1) {
         const dim3 w(kWave);
         if (logits_bf16)

@@ -14,7 +14,7 @@
 // Instruction bound for bf16 (an entry costs a shift or mask, half a maximum, a
 // difference, a product, the exponential -- four times as long as another
 // instruction --, an add and an fma): 2000 x 128256 with five alternatives 109 us,
-// 4.7 TB/s.  Memory bound for fp32: 1000 x 128256 85 us without alternatives, 6.0
+// 4.7 TB/s.  Memory bound for fp32: 1000 x 128256 98 us without alternatives, 5.2
 // TB/s.  One row of 128256 takes 11.6 us, two launches of which the loads are 2.4.
 #include <algorithm>
 #include <cmath>

@@ -174,3 +174,15 @@ def test_more_rows_than_one_launch_takes(be, orc, kind, cols):
     at = [0, 1, rows // 2, (1 << 21) - 1, 1 << 21, rows - 1]
     check((q[at], s[at], h[at]), defined(orc, x[at], r[at], w, EPS, kind))
     assert torch.equal(h.cpu(), x + r)
+
+
+@pytest.mark.parametrize("cols", [4096, 1001])
+def test_rows_past_32_bits(be, orc, cols):
+    """Three rows 2^31 - 8 elements apart, the last past 2^32."""
+    apart = (1 << 31) - 8
+    x, r, w = inputs(np.random.default_rng(14), 3, cols, True)
+    far = torch.empty(2 * apart + cols, dtype=x.dtype, device="cuda").as_strided((3, cols), (apart, 1))
+    far.copy_(x)
+    check(be.norm_quant_rows(far, w.cuda(), EPS, "int8", residual=r.cuda()), defined(orc, x, r, w, EPS, "int8"))
+    far.copy_(r)
+    check(be.norm_quant_rows(x.cuda(), w.cuda(), EPS, "fp8", residual=far), defined(orc, x, r, w, EPS, "fp8"))

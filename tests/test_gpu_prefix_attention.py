@@ -364,3 +364,29 @@ def test_scale_of_zero_takes_the_mean(be, kind, bf16, B):
         scale=0.0)
     run(be, pool, queries(46, B, 4, 64, bf16), k, v, 2, 333, [i % 2 for i in range(B)], [5 + i % 30 for i in range(B)], 40,
         scale=1e-42)
+
+
+def test_pages_past_32_bits(be):
+    """A pool whose pages lie past 4 GiB of K and of V: a slot of 33 copies of the
+    same tokens attends as one copy does, and a slot behind it as it should."""
+    import be42
+    kvh, hd, n, copies = 64, 128, 8192, 33
+    pool = be.kv_pool(be42.KV_BF16, 2, kvh, hd, copies * n // PAGE + 32)
+    gen = torch.Generator(device="cuda").manual_seed(47)
+    k, v = (torch.randn(n, kvh * hd, generator=gen, device="cuda") for _ in range(2))
+    for i in range(copies):
+        pool.append(0, k, v, i * n)
+    k1, v1 = (torch.randn(333, kvh * hd, generator=gen, device="cuda") for _ in range(2))
+    pool.append(1, k1, v1, 0)
+    assert copies * n * kvh * hd * 2 > 1 << 32
+    for bf16 in (False, True):
+        q = queries(48, 3, kvh, hd, bf16).cuda()
+        one = be.prefix_attention(pool, q, 0, n, 0.09, max_len=0).double()
+        all_ = be.prefix_attention(pool, q, 0, copies * n, 0.09, max_len=0).double()
+        # either is off by the tolerance above: scores below 30, sums of up to 2^18 terms
+        assert (one - all_).abs().max() <= (2.0 ** -7 if bf16 else 2 * (2 * 34 * 2.0 ** -22 + 2.0 ** -20)) * v.abs().max()
+        kk, vv = (x.bfloat16().double().view(333, kvh, hd).cpu().numpy() for x in (k1, v1))
+        got = be.prefix_attention(pool, q, 1, 333, 0.09, max_len=0)
+        want, tol, vmax = reference(q.cpu().double().numpy(), [kk[:0], kk], [vv[:0], vv], kvh, 0.09, 1, 333, [0] * 3, [0] * 3, 0)
+        off = np.abs(got.cpu().double().numpy() - want).max(-1)
+        assert (off <= tol + (2.0 ** -7 * vmax[0] if bf16 else 0.0)).all()

@@ -1,8 +1,9 @@
 """Log probabilities, entropy and top alternatives (be42_logprobs) against
 float64.  Tolerances: a logit's z = (x - max) / T carries at most three fp32
 roundings (2^-24 of |z| each, with T's inverse), its exponential and the sum's
-additions at most 80 more (runs of 64 entries are added up in fp32, the rest in
-64 bits), so log s is off by no more than e = 2^-24 * (3 * sum p |z| + 80) and
+additions at most 80 more (a lane adds its entries, up to 128 at these sizes, in
+fp32, each off by 2^-24 of a sum that grows from nothing: half of 128; lanes and
+runs are added in 64 bits), so log s is off by no more than e = 2^-24 * (3 * sum p |z| + 80) and
 the stored results by half a step more.  The entropy's second sum has the same
 terms weighted with z."""
 import math
@@ -281,3 +282,14 @@ def test_capture_with_the_librarys_workspace_is_refused(be):
         said = be.last_error()
         ent.add_(1)
     assert rc == -1 and "captured" in said
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_rows_past_32_bits(be, bf16):
+    """Three rows 2^31 - 8 entries apart, the last past 2^32."""
+    n, apart = 40000, (1 << 31) - 8
+    x = torch.randn(3, n, generator=torch.Generator().manual_seed(60)) * 2.5
+    x = x.bfloat16() if bf16 else x
+    far = torch.empty(2 * apart + n, dtype=x.dtype, device="cuda").as_strided((3, n), (apart, 1))
+    far.copy_(x)
+    check(be, x, torch.tensor([[0, 7], [n - 1, 5], [n // 2, 1]], dtype=torch.int32), 1.0, 10, dev=far)

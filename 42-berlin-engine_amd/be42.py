@@ -194,16 +194,17 @@ class Lib:
         """Entry point `name` on x's device and that device's current stream,
         which is its last argument.  (Plain integers for pointers and the raw
         stream: made of objects a call takes 4 us longer than its kernel.)"""
-        if not x.is_cuda:
+        dev, cuda = x.get_device(), self.torch._C
+        if dev < 0:
             raise Be42Error(f"{name}: tensors on {x.device}, not on a GPU")
-        self.init()
-        dev, t = x.get_device(), self.torch
-        if dev == t._C._cuda_getDevice():
-            rc = getattr(self.lib, name)(*args, t._C._cuda_getCurrentRawStream(dev))
+        if not self._inited:
+            self.init()
+        if dev == cuda._cuda_getDevice():
+            rc = getattr(self.lib, name)(*args, cuda._cuda_getCurrentRawStream(dev))
         else:
-            with t.cuda.device(dev):
-                rc = getattr(self.lib, name)(*args, t._C._cuda_getCurrentRawStream(dev))
-        if rc != BE42_OK:
+            with self.torch.cuda.device(dev):
+                rc = getattr(self.lib, name)(*args, cuda._cuda_getCurrentRawStream(dev))
+        if rc:
             self.check(rc, name)
 
     @staticmethod
@@ -222,14 +223,18 @@ class Lib:
     def _rows(self, name, what, x, dtypes, cols=None, dev=None):
         """Element stride of the rows of a 2-d tensor whose rows are dense (ctypes
         would cut one past 32 bits without a word)."""
-        if x.dim() != 2 or x.dtype not in dtypes or (cols is not None and x.shape[1] != cols) or \
+        shape, strides = x.shape, x.stride()
+        if len(shape) != 2 or x.dtype not in dtypes or (cols is not None and shape[1] != cols) or \
                 (dev is not None and x.device != dev):
-            raise Be42Error(f"{name}: {what} is {x.dtype} {tuple(x.shape)} on {x.device}")
-        if x.shape[1] > 1 and x.stride(1) != 1:
+            raise Be42Error(f"{name}: {what} is {x.dtype} {tuple(shape)} on {x.device}")
+        rows, n = shape
+        stride, one = strides
+        if one != 1 and n > 1:
             raise Be42Error(f"{name}: {what} has rows that are not dense")
-        stride = x.stride(0) if x.shape[0] > 1 else x.shape[1]
-        if max(stride, x.shape[0], x.shape[1]) >= 1 << 31:
-            raise Be42Error(f"{name}: {what} has shape {tuple(x.shape)}, rows {stride} apart: past 32 bits")
+        if rows <= 1:
+            stride = n
+        if stride >= 1 << 31 or rows >= 1 << 31 or n >= 1 << 31:
+            raise Be42Error(f"{name}: {what} has shape {tuple(shape)}, rows {stride} apart: past 32 bits")
         return stride
 
     # -- quant codecs ---------------------------------------------------------

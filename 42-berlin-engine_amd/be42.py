@@ -524,13 +524,18 @@ class Lib:
             max_len = pool.max_logical * 16
         if max(qs, prefix_slot, prefix_len, max_len) >= 1 << 31 or min(prefix_slot, prefix_len, max_len) < 0:
             raise Be42Error(f"{name}: queries {qs} apart, slot {prefix_slot}, prefix_len {prefix_len}, max_len {max_len}")
+        at = size = 0
         if workspace is None:
-            workspace = t.empty(self._prefix_bytes(B, H, pool.n_kv, hd, prefix_len, max_len), dtype=t.uint8, device=dev)
+            size = self._prefix_bytes(B, H, pool.n_kv, hd, prefix_len, max_len)
+            if size > 16 or t._C._cuda_isCurrentStreamCapturing():       # (16: a call in one launch uses none)
+                workspace = t.empty(size, dtype=t.uint8, device=dev)
         else:
             self._want(name, "workspace", workspace, (t.uint8,), None, dev)
+        if workspace is not None:
+            at, size = workspace.data_ptr(), workspace.numel()
         self._device_call(q, name, pool.handle, q.data_ptr(), q.dtype == t.bfloat16, qs, B, H, prefix_slot, prefix_len,
                           None if slots is None else slots.data_ptr(), None if lens is None else lens.data_ptr(), max_len,
-                          scale, out.data_ptr(), workspace.data_ptr(), workspace.numel())
+                          scale, out.data_ptr(), at or None, size)
         return out
 
     # -- linear KV cache [T][n_kv][head_dim] bf16 (kv_cache.c) ------------------

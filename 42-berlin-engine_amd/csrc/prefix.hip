@@ -46,6 +46,7 @@ struct PrefixArgs {
     // rows that a KV head has over the prefix and over one query (of 16), and rows
     // of a prefix tile
     int parts_p, parts_o, chunk_p, chunk_o, tiles_p, tiles_o, rows_p;
+    bool whole;               // one launch: k_prefix_whole
 };
 
 // The first `want` tokens of a slot, cut at what it holds (0 for a slot outside
@@ -191,10 +192,10 @@ constexpr float kSlack = 8.0f;
 constexpr int kPartWaves = 4;
 constexpr int kStep = 32;         // tokens of a wave's step: two pages
 
-template <int HD>
+template <int HD, int N = kPartWaves>
 struct PartShared {
-    float o[kPartWaves][16][HD + 4];
-    float m[kPartWaves][16], l[kPartWaves][16];
+    float o[N][16][HD + 4];
+    float m[N][16], l[N][16];
 };
 
 // Rows of a part in 16x16 tiles.  Both products are formed transposed, S^T =
@@ -204,25 +205,28 @@ struct PartShared {
 // tokens are tokens 8 g .. 8 g + 7 -- row 4 g + i of score tile t is given to
 // token 8 g + 4 t + i -- which is the operand the second product takes from
 // it.  Weights go from one product to the other in registers.
-template <bool KV8, int HD, int NP, int PP>
-__device__ __forceinline__ void part16(const be42_kv_pool &P, const PrefixArgs &a, PartShared<HD> &S, int slot,
-                                       int lo, int hi, int kvh, int b0, int row0, int rows)
+//
+// `share` waves take the steps in turn, from step `first` on this one; its sums
+// go to rows to .. to + rows - row0 - 1 of place `at` in LDS.
+template <bool KV8, int HD, int NP, int PP, class Shared>
+__device__ __forceinline__ void part16(const be42_kv_pool &P, const PrefixArgs &a, Shared &S, int slot, int lo, int hi, int kvh,
+                                       int b0, int row0, int rows, int first, int share, int at, int to)
 {
     constexpr int NK = HD / 32, NE = HD / 16;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const int G = a.n_heads / P.n_kv;
     const int ns = (hi - lo + kStep - 1) / kStep;
-    const int mine = ns > wave ? (ns - wave + kPartWaves - 1) / kPartWaves : 0;   // steps wave, wave + 4, ..
+    const int mine = ns > first ? (ns - first + share - 1) / share : 0;      // steps first, first + share, ..
 
     // the lane's query row, eight elements a k block: bf16 pages take element
     // 32 kb + 8 g + j there, INT8 pages (16 codes a load) 64 (kb / 2) + 16 g + 8 (kb % 2) + j
     bf16x8 Q[NK][NP];
     {
         const int ri = min(row0 + c, rows - 1);
-        const size_t at = (size_t)(b0 + ri / G) * a.q_stride + (size_t)(kvh * G + ri % G) * HD;
+        const size_t row = (size_t)(b0 + ri / G) * a.q_stride + (size_t)(kvh * G + ri % G) * HD;
 #pragma unroll
         for (int kb = 0; kb < NK; kb++)
-            load_q<NP>(a, at + (KV8 ? 64 * (kb / 2) + 16 * g + 8 * (kb % 2) : 32 * kb + 8 * g), Q[kb]);
+            load_q<NP>(a, row + (KV8 ? 64 * (kb / 2) + 16 * g + 8 * (kb % 2) : 32 * kb + 8 * g), Q[kb]);
     }
     const float sc = log2_scale(a);
 
@@ -239,7 +243,7 @@ __device__ __forceinline__ void part16(const be42_kv_pool &P, const PrefixArgs &
     // physical pages of the wave's next 32 steps: lane 2 i + e holds page e of step i
     int pages = 0;
     auto load_pages = [&](int i0) {
-        pages = table_page(P, slot, lo / kPage + 2 * (wave + kPartWaves * (i0 + lane / 2)) + (lane & 1));
+        pages = table_page(P, slot, lo / kPage + 2 * (first + share * (i0 + lane / 2)) + (lane & 1));
     };
     auto head_of = [&](int i, int e) {
         return (size_t)__builtin_amdgcn_readlane(pages, 2 * (i & 31) + e) * P.n_kv + kvh;
@@ -283,7 +287,7 @@ __device__ __forceinline__ void part16(const be42_kv_pool &P, const PrefixArgs &
         load_v(0);
     }
     for (int i = 0; i < mine; i++) {
-        const int left = hi - lo - (wave + kPartWaves * i) * kStep;      // tokens from this step on
+        const int left = hi - lo - (first + share * i) * kStep;      // tokens from this step on
         v4f s[2] = {v4f{0.0f, 0.0f, 0.0f, 0.0f}, v4f{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
         for (int kb = 0; kb < NK; kb++)
@@ -378,19 +382,19 @@ __device__ __forceinline__ void part16(const be42_kv_pool &P, const PrefixArgs &
             load_v(i + 1);
     }
 
-    // the four waves' sums of the part
     l += __shfl_xor(l, 16, kWave);
     l += __shfl_xor(l, 32, kWave);
+    if (row0 + c >= rows)
+        return;
     if (g == 0) {
-        S.m[wave][c] = m;
-        S.l[wave][c] = l;
+        S.m[at][to + c] = m;
+        S.l[at][to + c] = l;
     }
 #pragma unroll
     for (int e = 0; e < NE; e++)
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            S.o[wave][c][KV8 ? NE * (4 * g + i) + e : 16 * e + 4 * g + i] = O[e][i];
-    __syncthreads();
+            S.o[at][to + c][KV8 ? NE * (4 * g + i) + e : 16 * e + 4 * g + i] = O[e][i];
 }
 
 // Weight of a partial result whose maximum is m against the maximum of all; one
@@ -810,8 +814,33 @@ __global__ __launch_bounds__(64 * kPartWaves, 2) void k_prefix_part(const be42_k
             write_part<HD, QB, kPartWaves / R, kRows>(a, S.many.sums, row0, rows, b0, kvh, G, part);
             return;
         }
-    part16<KV8, HD, NP, QB ? 2 : 3>(P, a, S.few, slot, lo, max(lo, slot_tokens(P, slot, n)), kvh, b0, row0, rows);
+    const int wave = threadIdx.x >> 6;
+    part16<KV8, HD, NP, QB ? 2 : 3>(P, a, S.few, slot, lo, max(lo, slot_tokens(P, slot, n)), kvh, b0, row0, rows, wave, kPartWaves,
+                                    wave, 0);
+    __syncthreads();
     write_part<HD, QB, kPartWaves, 16>(a, S.few, row0, rows, b0, kvh, G, part);
+}
+
+// A call with few tokens in one launch: a workgroup takes as many queries as 16
+// rows hold, the prefix with all its waves, then each wave the own tokens of every
+// fourth query.  (Those keep sums of their own: in the tile of all rows a weight
+// of zero times a NaN in one query's pages would reach the others.)
+template <bool KV8, int HD, bool QB>
+__global__ __launch_bounds__(64 * kPartWaves, 2) void k_prefix_whole(const be42_kv_pool P, const PrefixArgs a)
+{
+    __shared__ PartShared<HD, kPartWaves + 1> S;
+    constexpr int NP = QB ? 1 : 3, PP = QB ? 2 : 3;
+    const int G = a.n_heads / P.n_kv, fit = 16 / G, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kvh = (int)(blockIdx.x % (unsigned)P.n_kv), b0 = (int)(blockIdx.x / (unsigned)P.n_kv) * fit;
+    const int rows = min(fit, a.n_queries - b0) * G;
+    part16<KV8, HD, NP, PP>(P, a, S, a.prefix_slot, 0, slot_tokens(P, a.prefix_slot, a.prefix_len), kvh, b0, 0, rows, wave,
+                            kPartWaves, wave, 0);
+    for (int j = wave; j * G < rows; j += kPartWaves) {
+        const int b = b0 + j, slot = a.slots ? a.slots[b] : b, n = a.lens ? min(a.lens[b], a.max_len) : a.max_len;
+        part16<KV8, HD, NP, PP>(P, a, S, slot, 0, slot_tokens(P, slot, n), kvh, b, 0, G, 0, 1, kPartWaves, j * G);
+    }
+    __syncthreads();
+    write_part<HD, QB, kPartWaves + 1, 16>(a, S, 0, rows, b0, kvh, G, 0);
 }
 
 // One wave per row: its parts by weight.  Lanes of head_dim / 4 words take the
@@ -895,6 +924,19 @@ static void plan_prefix(PrefixArgs &a, int n_kv)
 {
     const int G = a.n_heads / n_kv, unit = kPartWaves * kStep;
     const long rows = (long)a.n_queries * G;
+    // Short prefixes and own tokens go in one launch where a wave's steps of 32
+    // tokens are few, up to 32 rows of a KV head five, more eight: fp32, 32 heads on
+    // 8 KV heads, 40 own tokens, 64 queries over 300 tokens 13.0 us, 17.4 in parts;
+    // over 600 (seven steps) 16.1 and 18.4, over 1200 (twelve) 22.6 and 20.8; one
+    // query over 300 9.6 and 9.4, over 600 12.3 and 9.5, besides a second launch's 3
+    // us of the caller's time.
+    const long turns = G <= 16 ? std::min((long)a.n_queries, 16L / G) : 0, each = (turns + kPartWaves - 1) / kPartWaves;
+    const long steps = (a.prefix_len + unit - 1L) / unit + each * ((a.max_len + kStep - 1L) / kStep);
+    a.whole = G <= 16 && steps <= (rows > 32 ? 8 : 5);
+    if (a.whole) {
+        a.parts_p = 1;
+        return;
+    }
     a.rows_p = rows > 256 ? 128 : rows > 32 ? 64 : 16;
     a.tiles_p = (int)((rows + a.rows_p - 1) / a.rows_p);
     a.tiles_o = (G + 15) / 16;
@@ -920,7 +962,8 @@ extern "C" size_t be42_prefix_attention_workspace_bytes(int n_queries, int n_hea
     a.prefix_len = prefix_len;
     a.max_len = max_len;
     plan_prefix(a, n_kv);
-    return 16 + (size_t)(a.parts_p + a.parts_o) * n_queries * n_heads * (head_dim + 2) * sizeof(float);
+    const int parts = a.parts_p + a.parts_o;
+    return 16 + (parts > 1 ? (size_t)parts * n_queries * n_heads * (head_dim + 2) * sizeof(float) : 0);
 }
 
 extern "C" int be42_prefix_attention(const be42_kv_pool *pool, const void *q, int q_bf16, int q_stride, int n_queries,
@@ -960,8 +1003,9 @@ extern "C" int be42_prefix_attention(const be42_kv_pool *pool, const void *q, in
     BE42_CHECK(!workspace || (!((uintptr_t)workspace & 15) && workspace_bytes >= need),
                "be42_prefix_attention: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, need);
     hipStream_t s = as_stream(stream);
+    // (whether or not these sizes use it)
+    BE42_CHECK(workspace || !captured(s), "be42_prefix_attention: a captured call needs a workspace of the caller's");
     if (parts > 1) {
-        BE42_CHECK(workspace || !captured(s), "be42_prefix_attention: a captured call needs a workspace of the caller's");
         if (!workspace)
             workspace = be42::workspace(need, s);
         if (!workspace)
@@ -969,10 +1013,15 @@ extern "C" int be42_prefix_attention(const be42_kv_pool *pool, const void *q, in
         a.part_o = (float *)workspace;
         a.part_ml = a.part_o + (size_t)parts * rows * P.head_dim;
     }
+    const int fit = a.whole ? 16 * P.n_kv / n_heads : 1;
     auto go = [&](auto kv8, auto hd, auto qb) {
         constexpr bool KV8 = decltype(kv8)::value, QB = decltype(qb)::value;
         constexpr int HD = decltype(hd)::value;
         const dim3 g((unsigned)blocks), t(64 * kPartWaves);
+        if (a.whole) {
+            hipLaunchKernelGGL((k_prefix_whole<KV8, HD, QB>), dim3((unsigned)((n_queries + fit - 1) / fit * P.n_kv)), t, 0, s, P, a);
+            return;
+        }
         if (parts && a.rows_p == 128)
             hipLaunchKernelGGL((k_prefix_part<KV8, HD, QB, 4>), g, t, 0, s, P, a);
         else if (parts && a.rows_p == 64)

@@ -5,8 +5,9 @@
 // over the first prefix_len tokens of slot prefix_slot and the first lens[b]
 // tokens of slot slots[b].
 //
-// Tokens are cut into parts, some of the prefix and some of each query's own
-// tokens; one workgroup forms, for a tile of rows (query, head) of one KV head
+// Where there are few tokens, a workgroup sees a few queries' all
+// (k_prefix_whole).  Else they are cut into parts, some of the prefix and some of
+// each query's own tokens; one workgroup forms, for a tile of rows (query, head) of one KV head
 // and one part, m = max s, l = sum 2^(s - m) and o = sum 2^(s - m) v with
 // s = log2(e) * scale * q.k, and k_prefix_join adds the parts of a row with
 // weights 2^(m - max m).  Rows of the prefix are those of all queries, so its
@@ -20,7 +21,7 @@
 // 2.9 TB/s; own tokens alone 64 us, 4.3 TB/s; 128 fp32 rows over 8190 tokens 30 us,
 // of which 4.5 until the first pages are there, 14 products (three bf16 parts each
 // of q and the weights, 0.45 PFLOP/s of them), 3 results and 4.4 the join; the
-// smallest call 7.6 us, two launches.
+// smallest call 7.9 us in one launch, a chain of loads (page table, pages) and steps.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -925,14 +926,15 @@ static void plan_prefix(PrefixArgs &a, int n_kv)
     const int G = a.n_heads / n_kv, unit = kPartWaves * kStep;
     const long rows = (long)a.n_queries * G;
     // Short prefixes and own tokens go in one launch where a wave's steps of 32
-    // tokens are few, up to 32 rows of a KV head five, more eight: fp32, 32 heads on
-    // 8 KV heads, 40 own tokens, 64 queries over 300 tokens 13.0 us, 17.4 in parts;
-    // over 600 (seven steps) 16.1 and 18.4, over 1200 (twelve) 22.6 and 20.8; one
-    // query over 300 9.6 and 9.4, over 600 12.3 and 9.5, besides a second launch's 3
-    // us of the caller's time.
+    // tokens are few, up to 32 rows of a KV head five, up to 256 eight, more twelve.
+    // fp32, 32 heads on 8 KV heads, 40 own tokens, in us: one query over 300 tokens
+    // 9.6, in parts 9.4, over 600 12.3 and 9.5 (besides a second launch's 3 us of the
+    // caller's time); 64 queries over 300 13.0 and 17.4, over 600 (seven steps) 16.1
+    // and 18.4, over 1200 (twelve) 22.4 and 20.5; 512 over 300 35 and 60, over 1200 69
+    // and 77, over 1600 (fifteen) 84 and 82.
     const long turns = G <= 16 ? std::min((long)a.n_queries, 16L / G) : 0, each = (turns + kPartWaves - 1) / kPartWaves;
     const long steps = (a.prefix_len + unit - 1L) / unit + each * ((a.max_len + kStep - 1L) / kStep);
-    a.whole = G <= 16 && steps <= (rows > 32 ? 8 : 5);
+    a.whole = G <= 16 && steps <= (rows > 256 ? 12 : rows > 32 ? 8 : 5);
     if (a.whole) {
         a.parts_p = 1;
         return;

@@ -237,6 +237,18 @@ class Lib:
             raise Be42Error(f"{name}: {what} has shape {tuple(shape)}, rows {stride} apart: past 32 bits")
         return stride
 
+    def _workspace(self, name, given, dev, need, *sizes):
+        """The caller's workspace, or a new one (of the stream, so that no two
+        streams or graphs share it); none where a call of these sizes is one
+        launch, which uses none, unless it is being captured."""
+        if given is not None:
+            self._want(name, "workspace", given, (self.torch.uint8,), None, dev)
+            return given, given.numel()
+        size = need(*sizes)
+        if size <= 16 and not self.torch._C._cuda_isCurrentStreamCapturing():
+            return None, 0
+        return self.torch.empty(size, dtype=self.torch.uint8, device=dev), size
+
     # -- quant codecs ---------------------------------------------------------
     def quant_rows_int8(self, x):
         t = self.torch
@@ -443,15 +455,12 @@ class Lib:
         if top_k:
             got["top_ids"] = t.empty(rows, top_k, dtype=t.int32, device=dev)
             got["top_logprobs"] = t.empty(rows, top_k, dtype=t.float32, device=dev)
-        if workspace is None:
-            workspace = t.empty(self._logprobs_bytes(n, rows, top_k), dtype=t.uint8, device=dev)
-        else:
-            self._want(name, "workspace", workspace, (t.uint8,), None, dev)
+        ws, size = self._workspace(name, workspace, dev, self._logprobs_bytes, n, rows, top_k)
         at = {k: v.data_ptr() for k, v in got.items()}
         self._device_call(logits, name, at.get("logprobs"), at.get("entropy"), at.get("top_ids"), at.get("top_logprobs"),
                           logits.data_ptr(), logits.dtype == t.bfloat16, ls, n, rows, temp,
                           None if tokens is None else tokens.data_ptr(), given, top_k,
-                          workspace.data_ptr(), workspace.numel())
+                          None if ws is None else ws.data_ptr(), size)
         return got
 
     def kv_pool(self, kind, n_layers, n_kv, head_dim, max_logical, hpT=None):
@@ -524,18 +533,10 @@ class Lib:
             max_len = pool.max_logical * 16
         if max(qs, prefix_slot, prefix_len, max_len) >= 1 << 31 or min(prefix_slot, prefix_len, max_len) < 0:
             raise Be42Error(f"{name}: queries {qs} apart, slot {prefix_slot}, prefix_len {prefix_len}, max_len {max_len}")
-        at = size = 0
-        if workspace is None:
-            size = self._prefix_bytes(B, H, pool.n_kv, hd, prefix_len, max_len)
-            if size > 16 or t._C._cuda_isCurrentStreamCapturing():       # (16: a call in one launch uses none)
-                workspace = t.empty(size, dtype=t.uint8, device=dev)
-        else:
-            self._want(name, "workspace", workspace, (t.uint8,), None, dev)
-        if workspace is not None:
-            at, size = workspace.data_ptr(), workspace.numel()
+        ws, size = self._workspace(name, workspace, dev, self._prefix_bytes, B, H, pool.n_kv, hd, prefix_len, max_len)
         self._device_call(q, name, pool.handle, q.data_ptr(), q.dtype == t.bfloat16, qs, B, H, prefix_slot, prefix_len,
                           None if slots is None else slots.data_ptr(), None if lens is None else lens.data_ptr(), max_len,
-                          scale, out.data_ptr(), at or None, size)
+                          scale, out.data_ptr(), None if ws is None else ws.data_ptr(), size)
         return out
 
     # -- linear KV cache [T][n_kv][head_dim] bf16 (kv_cache.c) ------------------

@@ -672,9 +672,10 @@ extern "C" size_t be42_logprobs_workspace_bytes(int n, int rows, int top_k)
         long chunks, per, runs;
         int waves;
         cut_row(n, i & 1 ? 7 : 0, rows, i >> 1, &chunks, &per, &runs, &waves);
-        most = std::max(most, (size_t)rows * runs);
+        if (runs > 1)
+            most = std::max(most, (size_t)rows * runs);
     }
-    return most * (sizeof(Sums) + top_k * sizeof(unsigned long long));
+    return 16 + most * (sizeof(Sums) + top_k * sizeof(unsigned long long));
 }
 
 extern "C" int be42_logprobs(float *logprobs, float *entropy, int *top_ids, float *top_logprobs, const void *logits,
@@ -708,8 +709,9 @@ extern "C" int be42_logprobs(float *logprobs, float *entropy, int *top_ids, floa
     ScoreArgs a = {logits, (size_t)row_stride, logprobs, entropy, top_logprobs, top_ids, tokens, n_tokens, top_k, n, c,
                    (int)chunks, (int)per, (int)runs};
     hipStream_t s = as_stream(stream);
+    // (whether or not these sizes use it)
+    BE42_CHECK(workspace || !captured(s), "be42_logprobs: a captured call needs a workspace of the caller's");
     if (runs > 1) {
-        BE42_CHECK(workspace || !captured(s), "be42_logprobs: a captured call needs a workspace of the caller's");
         if (!workspace)
             workspace = be42::workspace(need, s);
         if (!workspace)

@@ -293,7 +293,8 @@ int  be42_lsh_attention_status(void *stream);
  * n_heads above 2^20 may be refused).
  * workspace NULL: the library's (grow-only; refused while the stream is
  * captured), else a device buffer of be42_prefix_attention_workspace_bytes()
- * bytes, 16-byte aligned, that no call on another stream uses meanwhile. */
+ * bytes, 16-byte aligned, that no call on another stream uses meanwhile (16
+ * bytes: these sizes take one launch, which uses none). */
 size_t be42_prefix_attention_workspace_bytes(int n_queries, int n_heads, int n_kv, int head_dim, int prefix_len,
                                              int max_len);
 int    be42_prefix_attention(const be42_kv_pool *pool, const void *q, int q_bf16, int q_stride, int n_queries,
@@ -467,7 +468,8 @@ int be42_sample_top_p_dt(int *out, const void *logits, int logits_bf16, int n, i
  * rows < 2^24.
  * workspace NULL: the library's (grow-only; refused while the stream is
  * captured), else a device buffer of be42_logprobs_workspace_bytes() bytes,
- * 16-byte aligned, that no call on another stream uses meanwhile. */
+ * 16-byte aligned, that no call on another stream uses meanwhile (16 bytes:
+ * these sizes take one launch, which uses none). */
 size_t be42_logprobs_workspace_bytes(int n, int rows, int top_k);
 int    be42_logprobs(float *logprobs, float *entropy, int *top_ids, float *top_logprobs, const void *logits,
                      int logits_bf16, int row_stride, int n, int rows, float temp, const int *tokens, int n_tokens,

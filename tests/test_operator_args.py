@@ -80,9 +80,10 @@ def test_logprobs_no_rows(lib):
 def test_logprobs_workspace(lib):
     f = lib.lib.be42_logprobs_workspace_bytes
     assert f(0, 1, 0) == 0 and f(10, 0, 0) == 0 and f(10, 1, 11) == 0 and f(100, 1, 65) == 0 and f(100, 1, -1) == 0
-    assert f(1, 1, 0) > 0 and f(128256, 1, 20) <= f(128256, 5000, 20) and f(128256, 5000, 0) <= f(128256, 5000, 64)
+    assert f(1, 1, 0) == f(128256, 5000, 20) == 16                # in one launch
+    assert 16 < f(128256, 1, 0) < f(128256, 1, 20) < f(128256, 40, 20)
     # sizes past 32 bits do not wrap
-    assert f(INT_MAX, INT_MAX, 64) >= f(INT_MAX, 1 << 20, 64) >= f(128256, 5000, 64)
+    assert f(INT_MAX, 1000, 64) > f(INT_MAX, 40, 64) >= f(128256, 40, 64)
 
 
 def pool(**kw):

@@ -640,9 +640,10 @@ __global__ __launch_bounds__(kWave) void k_score_join(const ScoreArgs a)
 // How a row of n entries is cut: chunks (the first word may begin `before`
 // entries before the row), chunks of a run, runs, and the waves of a workgroup.
 // Up to 256 rows, a workgroup of eight waves takes a whole row where that has up
-// to 24 chunks, or where the rows come near to filling the chip (fp32, top 5, in
-// us: 1 x 32000 8.6, cut 9.6; 1 x 64000 11.4, cut 9.6; 64 x 128256 19.4, cut 16.6;
-// 120 x 128256 19.4, cut 23.5; 200 x 32000 12.7, cut 16.0); rows of up to four
+// to 80 K entries, or where the rows come near to filling the chip (fp32, top 5, in
+// us: 1 x 32000 8.6, cut 9.6; 1 x 64000 11.4, cut 9.6 and a second launch's 4 us of
+// the caller's time; 1 x 128256 17, cut 10.4; 64 x 128256 19.4, cut 16.6; 120 x
+// 128256 19.4, cut 23.5; 200 x 32000 12.7, cut 16.0); rows of up to four
 // chunks do with four waves (200 x 8000 8.3, eight 8.7).  Other rows are cut
 // until there are four workgroups a CU; a run has at least a chunk for each wave,
 // and four where the rows alone fill the chip, since joining runs costs a launch
@@ -651,7 +652,7 @@ static void cut_row(int n, int before, int rows, bool bf16, long *chunks, long *
 {
     const long entries = kChunkBytes / (bf16 ? 2 : 4);
     *chunks = (n + before + entries - 1) / entries;
-    const bool whole = rows <= 256 && *chunks > kScoreW && (*chunks <= 3 * kScoreWide || rows > 96);
+    const bool whole = rows <= 256 && *chunks > kScoreW && (*chunks * entries <= 80 * 1024 || rows > 96);
     *waves = whole ? kScoreWide : kScoreW;
     const long least = rows >= 256 ? 4 * kScoreW : kScoreW;
     *runs = whole ? 1 : std::min((*chunks + least - 1) / least, (1024 + (long)rows - 1) / rows);

@@ -431,7 +431,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_quant_vec(uint8_
 // The fewest threads that hold the row in four words each (a wave two, 512 eight):
 // few large loads a thread and as many rows a CU as fit.  Measured, fp32 with a
 // residual (the bytes of 8192 x 4096 at the rate of a large copy: 84 us):
-//   1 x 4096 3.8 us, 2048 x 4096 18.6 (1024 threads: 3.7 and 22.1), 8192 x 4096 82
+//   1 x 4096 3.5 us, 2048 x 4096 18.6 (1024 threads the same and 22.1), 8192 x 4096 81
 //   30000 x 512 35.9 (256 threads 49.9), 30000 x 256 18.4 (44.1)
 //   2000 x 8192 to E4M3 40.8 (256 threads of eight words 48.8)
 //   2000 x 12288 to E4M3 75.2 (1024 threads 81.2), 300 x 12288 14.1 (15.8)

@@ -390,3 +390,23 @@ def test_pages_past_32_bits(be):
         want, tol, vmax = reference(q.cpu().double().numpy(), [kk[:0], kk], [vv[:0], vv], kvh, 0.09, 1, 333, [0] * 3, [0] * 3, 0)
         off = np.abs(got.cpu().double().numpy() - want).max(-1)
         assert (off <= tol + (2.0 ** -7 * vmax[0] if bf16 else 0.0)).all()
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("heads,kvh,prefix", [(8, 8, 100), (8, 2, 100), (8, 2, 3000)])
+def test_nan_of_one_sequences_pages_stays_there(be, bad, bf16, heads, kvh, prefix):
+    """Queries beside it (in one launch: of the same 16 rows) see numbers only."""
+    held = [20, 33, 7, 40, 0, 12]
+    pool, k, v = make_pool(be, "bf16", 7, kvh, 64, held + [prefix], 50)
+    x = torch.full((1, kvh * 64), bad, device="cuda")
+    pool.append(1, x, x, held[1])
+    slots, lens = [0, 1, 2, 3, 4, 5, 1], [20, 34, 7, 40, 0, 12, 33]
+    q = queries(51, 7, heads, 64, bf16)
+    got = be.prefix_attention(pool, q.cuda(), 6, prefix, 0.125, slots=torch.tensor(slots, dtype=torch.int32, device="cuda"),
+                              lens=torch.tensor(lens, dtype=torch.int32, device="cuda"), max_len=40).cpu().double().numpy()
+    want, tol, vmax = reference(q.double().numpy(), k, v, heads, 0.125, 6, prefix, slots, lens, 40)
+    for b in (0, 2, 3, 4, 5, 6):
+        off = np.abs(got[b] - want[b]).max(-1)
+        assert (off <= tol[b] + (2.0 ** -7 * vmax[0] if bf16 else 0.0)).all(), b
+    assert not np.isfinite(got[1]).all()

@@ -920,8 +920,9 @@ static void cut(int tokens, long tiles, int unit, long want, int *parts, int *ch
 // tokens: 150 us, 175 in tiles of 64).  The prefix gets a workgroup a CU, so that
 // own tokens, which wait for memory, run beside it (two: 166 us); where there are
 // few of those and the parts stay long, it gets two (512 rows alone 108 us, 135
-// with one).
-static void plan_prefix(PrefixArgs &a, int n_kv)
+// with one; 128 fp32 rows over 32000 tokens 65 and 71, over 16000 both 42; heads of
+// 64, half the work a token, 64 rows over 32768 tokens 31.5 and 28.5).
+static void plan_prefix(PrefixArgs &a, int n_kv, int head_dim)
 {
     const int G = a.n_heads / n_kv, unit = kPartWaves * kStep;
     const long rows = (long)a.n_queries * G;
@@ -943,7 +944,7 @@ static void plan_prefix(PrefixArgs &a, int n_kv)
     a.tiles_p = (int)((rows + a.rows_p - 1) / a.rows_p);
     a.tiles_o = (G + 15) / 16;
     const long tiles = (long)a.tiles_p * n_kv, read = (long)a.prefix_len * a.tiles_p;
-    const bool two = a.rows_p == 16 || (a.prefix_len * tiles >= 512 * 1024 && 2L * a.n_queries * a.max_len < read);
+    const bool two = a.rows_p == 16 || ((double)a.prefix_len * tiles * head_dim >= 1L << 25 && 2L * a.n_queries * a.max_len < read);
     cut(a.prefix_len, tiles, unit, two ? 512 : 256, &a.parts_p, &a.chunk_p);
     cut(a.max_len, (long)a.tiles_o * n_kv * a.n_queries, unit, 512, &a.parts_o, &a.chunk_o);
 }
@@ -963,7 +964,7 @@ extern "C" size_t be42_prefix_attention_workspace_bytes(int n_queries, int n_hea
     a.n_heads = n_heads;
     a.prefix_len = prefix_len;
     a.max_len = max_len;
-    plan_prefix(a, n_kv);
+    plan_prefix(a, n_kv, head_dim);
     const int parts = a.parts_p + a.parts_o;
     return 16 + (parts > 1 ? (size_t)parts * n_queries * n_heads * (head_dim + 2) * sizeof(float) : 0);
 }
@@ -994,7 +995,7 @@ extern "C" int be42_prefix_attention(const be42_kv_pool *pool, const void *q, in
         return BE42_OK;
     PrefixArgs a = {q, out, slots, lens, nullptr, nullptr, (size_t)q_stride, n_queries, n_heads, prefix_slot, prefix_len,
                     max_len, scale};
-    plan_prefix(a, P.n_kv);
+    plan_prefix(a, P.n_kv, P.head_dim);
     const int parts = a.parts_p + a.parts_o;
     const long blocks = (long)P.n_kv * ((long)a.tiles_p * a.parts_p + (long)a.tiles_o * n_queries * a.parts_o);
     const size_t rows = (size_t)n_queries * n_heads;

@@ -230,14 +230,15 @@ __device__ __forceinline__ float norm_value(float h, double r, uint16_t w)
     return (float)((double)h * r * (double)bf16_to_f32(w));
 }
 
-// Any row: three passes over it, one element a thread.
+// Any row: three passes over it, one element a thread.  (1024 threads: one row of
+// 70000 fp32 46 us, 2000 rows 629; 256 threads 156 and 752.)
 template <bool FP8, bool BF16>
-__global__ __launch_bounds__(256) void k_norm_quant_rows(uint8_t *q, float *scales, void *sum, const void *x,
-                                                         size_t x_stride, const void *res, size_t res_stride,
-                                                         const uint16_t *w, int cols, float eps)
+__global__ __launch_bounds__(1024) void k_norm_quant_rows(uint8_t *q, float *scales, void *sum, const void *x,
+                                                          size_t x_stride, const void *res, size_t res_stride,
+                                                          const uint16_t *w, int cols, float eps)
 {
-    __shared__ double redd[4];
-    __shared__ float red[4];
+    __shared__ double redd[16];
+    __shared__ float red[16];
     const size_t row = blockIdx.x;
     auto load = [&](int i) {
         const float v = act_load<BF16>(x, row * x_stride + i);
@@ -247,7 +248,7 @@ __global__ __launch_bounds__(256) void k_norm_quant_rows(uint8_t *q, float *scal
     // have replaced x or the residual)
     auto again = [&](int i) { return sum ? act_load<BF16>(sum, row * cols + i) : load(i); };
     double ss = 0.0;
-    for (int i = threadIdx.x; i < cols; i += 256) {
+    for (int i = threadIdx.x; i < cols; i += 1024) {
         const float h = load(i);
         if (sum)
             act_store<BF16>(sum, row * cols + i, h);
@@ -257,15 +258,22 @@ __global__ __launch_bounds__(256) void k_norm_quant_rows(uint8_t *q, float *scal
     if ((threadIdx.x & 63) == 0)
         redd[threadIdx.x >> 6] = ss;
     __syncthreads();
-    const double r = 1.0 / sqrt(((redd[0] + redd[1]) + (redd[2] + redd[3])) / cols + (double)eps);
+    ss = redd[0];
+#pragma unroll
+    for (int x = 1; x < 16; x++)
+        ss += redd[x];
+    const double r = 1.0 / sqrt(ss / cols + (double)eps);
     float m = 0.0f;
-    for (int i = threadIdx.x; i < cols; i += 256)
+    for (int i = threadIdx.x; i < cols; i += 1024)
         m = fmaxf(m, fabsf(norm_value(again(i), r, w[i])));
     m = wave_top(m);
     if ((threadIdx.x & 63) == 0)
         red[threadIdx.x >> 6] = m;
     __syncthreads();
-    const float amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    float amax = red[0];
+#pragma unroll
+    for (int x = 1; x < 16; x++)
+        amax = fmaxf(amax, red[x]);
     float scale = 1.0f, inv = 1.0f;
     if (amax > 0.0f) {
         scale = amax / (FP8 ? 224.0f : 127.0f);
@@ -273,7 +281,7 @@ __global__ __launch_bounds__(256) void k_norm_quant_rows(uint8_t *q, float *scal
     }
     if (threadIdx.x == 0)
         scales[row] = scale;
-    for (int i = threadIdx.x; i < cols; i += 256) {
+    for (int i = threadIdx.x; i < cols; i += 1024) {
         const float y = norm_value(again(i), r, w[i]);
         q[row * cols + i] = FP8 ? finite_to_fp8(y * inv) : (uint8_t)f32_to_int8(y, inv);
     }
@@ -425,9 +433,9 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_quant_vec(uint8_
     }
 }
 
-// Rows of up to 16384 fp32 or 32768 bf16 elements go in 16-byte words where every
-// row of x, the residual, w and the outputs begins on one and has whole ones, and
-// else, up to 8192, an element at a time; longer ones take the three passes above.
+// Rows of up to 32768 elements go in 16-byte words where every row of x, the
+// residual, w and the outputs begins on one and has whole ones, and else, up to
+// 16384, an element at a time; longer ones take the three passes above.
 // The fewest threads that hold the row in four words each (a wave two, 512 eight):
 // few large loads a thread and as many rows a CU as fit.  Measured, fp32 with a
 // residual (the bytes of 8192 x 4096 at the rate of a large copy: 84 us):
@@ -435,7 +443,9 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_quant_vec(uint8_
 //   30000 x 512 35.9 (256 threads 49.9), 30000 x 256 18.4 (44.1)
 //   2000 x 8192 to E4M3 40.8 (256 threads of eight words 48.8)
 //   2000 x 12288 to E4M3 75.2 (1024 threads 81.2), 300 x 12288 14.1 (15.8)
-//   3000 x 4099, element at a time, 45.6 (the three passes 63.3)
+//   2000 x 28672 158 (the three passes 295), one such row 9.2 (65)
+//   3000 x 4099, element at a time, 45.6 (the three passes 63.3), 300 x 12289 18.7
+//   (47.7)
 // A few hundred rows are bound by one row's way through load, sum and maximum
 // (1 x 8192: 4.5 us), very wide ones to E4M3 by the codec's instructions.
 template <bool FP8, bool BF16>
@@ -469,7 +479,9 @@ static bool launch_norm_vec(uint8_t *q, float *scales, void *sum, const void *x,
             return go(one, some, two);
         if (cols <= 2048)
             return go(one, some, eight);
-        return cols <= 8192 && go(one, most, eight);
+        if (cols <= 8192)
+            return go(one, most, eight);
+        return cols <= 16384 && go(one, most, integral_constant<int, 16>());
     }
     const int words = cols / VE;
     if (words <= 64)
@@ -484,7 +496,9 @@ static bool launch_norm_vec(uint8_t *q, float *scales, void *sum, const void *x,
         return go(vec, some, four);
     if (words <= 2048)
         return go(vec, most, two);
-    return words <= 4096 && go(vec, more, eight);
+    if (words <= 4096)
+        return go(vec, more, eight);
+    return !BF16 && words <= 8192 && go(vec, most, eight);
 }
 
 template <bool FP8>
@@ -492,7 +506,7 @@ static void launch_norm_quant(uint8_t *q, float *scales, void *sum, const void *
                               size_t res_stride, bool bf16, const uint16_t *w, int rows, int cols, float eps,
                               hipStream_t s)
 {
-    const dim3 g(rows), b(256);
+    const dim3 g(rows), b(1024);
     if (bf16 ? launch_norm_vec<FP8, true>(q, scales, sum, x, x_stride, res, res_stride, w, rows, cols, eps, s)
              : launch_norm_vec<FP8, false>(q, scales, sum, x, x_stride, res, res_stride, w, rows, cols, eps, s))
         return;

@@ -186,3 +186,14 @@ def test_rows_past_32_bits(be, orc, cols):
     check(be.norm_quant_rows(far, w.cuda(), EPS, "int8", residual=r.cuda()), defined(orc, x, r, w, EPS, "int8"))
     far.copy_(r)
     check(be.norm_quant_rows(x.cuda(), w.cuda(), EPS, "fp8", residual=far), defined(orc, x, r, w, EPS, "fp8"))
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("cols", [8193, 16383, 16384, 18432, 28672, 32764, 32768, 32776, 40001])
+def test_long_rows(be, orc, kind, bf16, cols):
+    """About the lengths at which the form of a row changes."""
+    x, r, w = inputs(np.random.default_rng(cols), 3, cols, bf16)
+    for res in (r, None):
+        got = be.norm_quant_rows(x.cuda(), w.cuda(), EPS, kind, residual=None if res is None else res.cuda())
+        check(got, defined(orc, x, res, w, EPS, kind), res is not None)

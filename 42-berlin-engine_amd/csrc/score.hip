@@ -182,8 +182,9 @@ __device__ __forceinline__ void rank_keys(unsigned long long *cand, int n, int k
     wave_lds();
 }
 
-// A wave's run of a row.  Places past the row's ends are set to -1e30, which
-// adds nothing to the sums, and are left out of the maxima.
+// A wave's run of a row.  Places past the row's ends are set to -infinity, which
+// adds nothing to the sums under any reference and temperature (any number does
+// beside a lane whose own entries lie below it), and are left out of the maxima.
 template <bool BF16>
 struct Run {
     static constexpr int VE = BF16 ? 8 : 4;    // entries of a word
@@ -224,7 +225,7 @@ struct Run {
             if (whole <= n - VE)
                 w[u] = *(const uint4 *)(base + (ptrdiff_t)(is_whole(e0) ? e0 : whole) * (BF16 ? 2 : 4));
         }
-        constexpr uint32_t none = BF16 ? 0xF14AF14Au : 0xF149F2CAu;
+        constexpr uint32_t none = BF16 ? 0xFF80FF80u : 0xFF800000u;
 #pragma unroll
         for (int u = 0; u < kScoreU; u++) {
             const int e0 = id(chunk, u, 0);
@@ -514,21 +515,28 @@ __global__ __launch_bounds__(kWave *W) void k_score_run(const ScoreArgs a)
             ref = r2;
             m = fmaxf(m, top);
         }
-        const float s0 = s, t0 = t;
+        // -infinity (0 * -infinity in t) takes a second, careful pass, with exponents
+        // held where they underflow; a chunk that the row's ends cut, whose filling
+        // is that, goes straight there
+        bool careful = !run.inside(c);
+        if (!careful) {
+            const float s0 = s, t0 = t;
 #pragma unroll
-        for (int u = 0; u < kScoreU; u++)
+            for (int u = 0; u < kScoreU; u++)
 #pragma unroll
-            for (int j = 0; j < Run<BF16>::VE; j++) {
-                const float z = (Run<BF16>::entry(w[u], j) - ref) * a.c, e = __builtin_amdgcn_exp2f(z);
-                s += e;
-                t = __fmaf_rn(e, z, t);
+                for (int j = 0; j < Run<BF16>::VE; j++) {
+                    const float z = (Run<BF16>::entry(w[u], j) - ref) * a.c, e = __builtin_amdgcn_exp2f(z);
+                    s += e;
+                    t = __fmaf_rn(e, z, t);
+                }
+            keep_packed(w);
+            careful = __any(!(fabsf(t) < INFINITY));
+            if (careful) {
+                s = s0;
+                t = t0;
             }
-        keep_packed(w);
-        if (__any(!(fabsf(t) < INFINITY))) {
-            // an entry of -infinity (0 * -infinity), or what has no distribution:
-            // again, exponents held where they underflow
-            s = s0;
-            t = t0;
+        }
+        if (careful) {
 #pragma unroll
             for (int u = 0; u < kScoreU; u++)
 #pragma unroll

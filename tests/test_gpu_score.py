@@ -293,3 +293,48 @@ def test_rows_past_32_bits(be, bf16):
     far = torch.empty(2 * apart + n, dtype=x.dtype, device="cuda").as_strided((3, n), (apart, 1))
     far.copy_(x)
     check(be, x, torch.tensor([[0, 7], [n - 1, 5], [n // 2, 1]], dtype=torch.int32), 1.0, 10, dev=far)
+
+
+def low_rows(n, bf16, mask, seed):
+    """Rows that a finite mask leaves one token, four, the first two thirds, the last token of."""
+    rng = np.random.default_rng(seed)
+    x = torch.from_numpy((rng.standard_normal((4, n)) * 2.5).astype(np.float32))
+    lowest = torch.finfo(torch.bfloat16 if bf16 else torch.float32).min
+    fill = lowest if mask == "lowest" else mask
+    keep = torch.zeros(4, n, dtype=torch.bool)
+    keep[0, n // 2] = True
+    keep[1, torch.from_numpy(rng.integers(0, n, 4))] = True
+    keep[2, : n - n // 3] = True
+    keep[3, n - 1] = True
+    x[~keep] = fill
+    tokens = torch.tensor([[n // 2, n - 1]] * 4, dtype=torch.int32)
+    return x.bfloat16() if bf16 else x, tokens
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("n", [1, 5, 70, 3000, 4096, 5001, 32003, 128256])
+@pytest.mark.parametrize("mask", ["lowest", -1e31])
+def test_finite_masks(be, bf16, n, mask):
+    """Whole words, lanes and chunks at the type's lowest value, or at another far
+    below any logit, in rows that end inside a chunk.  (bf16 rounds -1e31 alike
+    for the call and the reference.)"""
+    x, tokens = low_rows(n, bf16, mask, n)
+    for temp, k in ((1.0, min(n, 20)), (1.5, 0)):
+        check(be, x, tokens, temp, k)
+    for off in (1, 3):                                     # rows that begin off 16 bytes
+        wide = torch.full((4, n + 5 + off), math.nan, dtype=x.dtype, device="cuda")
+        wide[:, off:off + n] = x.cuda()
+        check(be, x, tokens, 1.0, min(n, 5), dev=wide[:, off:off + n])
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("n", [1, 5, 70, 5001, 128256])
+@pytest.mark.parametrize("temp", [1e27, 1e29, 1.4e30])
+def test_high_temperatures(be, bf16, n, temp):
+    """All but uniform: nothing but the row's own entries counts, and a mask of
+    -1e30 is a token like others."""
+    rng = np.random.default_rng(n)
+    x = torch.from_numpy((rng.standard_normal((3, n)) * 2.5).astype(np.float32))
+    x[1, ::3] = -1e30
+    x = x.bfloat16() if bf16 else x
+    check(be, x, torch.tensor([[0, n - 1]] * 3, dtype=torch.int32), float(np.float32(temp)), min(n, 7))

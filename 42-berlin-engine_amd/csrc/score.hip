@@ -87,16 +87,17 @@ __device__ __forceinline__ const void *row_of(const ScoreArgs &a, int row)
 // What a row's sums say: NaN for a row without a distribution (s is NaN or
 // infinite where an entry was NaN or +infinity).
 struct RowSums {
-    double base, H;                         // log p(x) = ln 2 (x c - base)
+    double ref, ls, H;                      // log p(x) = ln 2 (x c - ref - ls)
 };
 __device__ __forceinline__ RowSums row_sums(double ref, double s, double t)
 {
     const double ls = ref > -INFINITY && s < INFINITY ? log2(s) : (double)NAN;
-    return {ref + ls, (ls - t / s) * 0.69314718055994530942};
+    return {ref, ls, (ls - t / s) * 0.69314718055994530942};
 }
+// (the reference first: ls would be lost beside one past 2^53 of it)
 __device__ __forceinline__ float log_prob(const ScoreArgs &a, const RowSums &r, float x)
 {
-    return r.base != r.base ? NAN : (float)(((double)x * (double)a.c - r.base) * 0.69314718055994530942);
+    return r.ls != r.ls ? NAN : (float)((((double)x * (double)a.c - r.ref) - r.ls) * 0.69314718055994530942);
 }
 
 // s and t under the reference `top` >= p.ref

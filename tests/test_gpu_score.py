@@ -338,3 +338,17 @@ def test_high_temperatures(be, bf16, n, temp):
     x[1, ::3] = -1e30
     x = x.bfloat16() if bf16 else x
     check(be, x, torch.tensor([[0, n - 1]] * 3, dtype=torch.int32), float(np.float32(temp)), min(n, 7))
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("n", [1, 5, 3000, 32003, 128256])
+def test_rows_far_from_zero(be, bf16, n):
+    """Rows that hold one value only, however large, are uniform: log s is not lost
+    beside the reference."""
+    t = torch.bfloat16 if bf16 else torch.float32
+    f = torch.finfo(t)
+    x = torch.tensor([f.min, -1e30, -1e18, 1e18, f.max], dtype=t)[:, None].expand(5, n).contiguous()
+    tokens = torch.tensor([[0, n - 1]] * 5, dtype=torch.int32)
+    for temp, k in ((1.0, min(n, 5)), (0.25, 0)):
+        got = check(be, x, tokens, temp, k)
+        assert (got["logprobs"].cpu().double() + math.log(n)).abs().max() <= 81 * U * max(1.0, math.log(n))

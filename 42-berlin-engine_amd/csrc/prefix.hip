@@ -8,10 +8,13 @@
 // Where there are few tokens, a workgroup sees a few queries' all
 // (k_prefix_whole).  Else they are cut into parts, some of the prefix and some of
 // each query's own tokens; one workgroup forms, for a tile of rows (query, head) of one KV head
-// and one part, m = max s, l = sum 2^(s - m) and o = sum 2^(s - m) v with
-// s = log2(e) * scale * q.k, and k_prefix_join adds the parts of a row with
-// weights 2^(m - max m).  Rows of the prefix are those of all queries, so its
-// pages are read once for a tile of up to 128 rows.
+// and one part, with s = q.k and c = log2(e) * scale, m = max s, l = sum
+// 2^((s - m) c) and o = sum 2^((s - m) c) v, and k_prefix_join adds the parts of a
+// row with weights 2^((m - max m) c).  (Differences are taken before they are
+// scaled: s c - m c with a rounded m c is off by that rounding, past a score of
+// 2^30 by more than an exponent holds.  It costs an instruction a score, 1 - 3%
+// where those bound the tile.)  Rows of the prefix are those of all queries, so
+// its pages are read once for a tile of up to 128 rows.
 //
 // What bounds it, of a pass (kernel times; a large copy runs at 5.2 to 5.5 TB/s, a
 // large bf16 product at 1.2 PFLOP/s here): 512 bf16 rows over 32768 tokens 103 us,
@@ -144,8 +147,8 @@ __device__ __forceinline__ void load_q(const PrefixArgs &a, size_t at, bf16x8 (&
     }
 }
 
-// The scores' factor, log2(e) |scale|, and not 0: times the -infinity of a token
-// past the part that would be NaN.
+// The scores' factor c, log2(e) |scale| (load_q has the sign), and not 0: times the
+// -infinity of a token past the part that would be NaN.
 __device__ __forceinline__ float log2_scale(const PrefixArgs &a)
 {
     return fmaxf(fabsf(a.scale) * 1.44269504088896340736f, 1.17549435e-38f);
@@ -184,11 +187,14 @@ __device__ __forceinline__ T ring_read(const void *__restrict__ p)
     return *(const T *)p;
 }
 
-// What a row's sums count from may lie this much (a factor of 256) below its
-// largest score so far: the sums are rescaled past that only.  With the exact
+// What a row's sums count from, m, is a score as the products give it, and may lie
+// this much (a factor of 256) below the largest so far: the sums are rescaled past
+// that only.  With the exact
 // maximum some of a wave's 32 rows has a new one in most steps, and the rescaling
 // was a third of the vector work.
 constexpr float kSlack = 8.0f;
+// the least m of a row that has seen a token (-infinity: none)
+constexpr float kLowest = -3.402823466e38f;
 
 constexpr int kPartWaves = 4;
 constexpr int kStep = 32;         // tokens of a wave's step: two pages
@@ -327,9 +333,9 @@ __device__ __forceinline__ void part16(const be42_kv_pool &P, const PrefixArgs &
         quarters(top, top, other);
         top = max3(top, other, other);
         halves(top, top, other);
-        const float mn = max3(top, other, other) * sc;
-        if (__any(mn > m + kSlack)) {
-            const float now = fmaxf(m, mn), f = __builtin_amdgcn_exp2f(m - now);
+        top = fmaxf(max3(top, other, other), kLowest);
+        if (__any((top - m) * sc > kSlack)) {
+            const float now = fmaxf(m, top), f = __builtin_amdgcn_exp2f((m - now) * sc);
             l *= f;
 #pragma unroll
             for (int e = 0; e < NE; e++)
@@ -338,7 +344,7 @@ __device__ __forceinline__ void part16(const be42_kv_pool &P, const PrefixArgs &
         }
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            p[j] = __builtin_amdgcn_exp2f(__fmaf_rn(p[j], sc, -m));
+            p[j] = __builtin_amdgcn_exp2f((p[j] - m) * sc);
             l += p[j];
             if (KV8)
                 p[j] *= vsc[j];
@@ -398,11 +404,17 @@ __device__ __forceinline__ void part16(const be42_kv_pool &P, const PrefixArgs &
             S.o[at][to + c][KV8 ? NE * (4 * g + i) + e : 16 * e + 4 * g + i] = O[e][i];
 }
 
-// Weight of a partial result whose maximum is m against the maximum of all; one
-// without tokens weighs nothing.
-__device__ __forceinline__ float part_weight(float m, float l, float top)
+// Weight of a partial result that counts from m against one from the largest m of
+// all; one without tokens weighs nothing.
+__device__ __forceinline__ float part_weight(float m, float top, float sc)
 {
-    return l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+    return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - top) * sc);
+}
+
+// 1 / the sum of a row's weights, 0 for a row that saw no token
+__device__ __forceinline__ float row_inverse(float top, float sum)
+{
+    return top == -INFINITY ? 0.0f : 1.0f / sum;
 }
 
 template <bool QB>
@@ -600,9 +612,9 @@ __device__ __forceinline__ void part32(const be42_kv_pool &P, const PrefixArgs &
             top = max3(top, p[j], p[j + 1]);
         top = max3(top, p[15], p[15]);
         halves(top, top, other);
-        const float mn = max3(top, other, other) * sc;
-        if (__any(mn > m + kSlack)) {
-            const float now = fmaxf(m, mn), f = __builtin_amdgcn_exp2f(m - now);
+        top = fmaxf(max3(top, other, other), kLowest);
+        if (__any((top - m) * sc > kSlack)) {
+            const float now = fmaxf(m, top), f = __builtin_amdgcn_exp2f((m - now) * sc);
             l *= f;
 #pragma unroll
             for (int e = 0; e < NE; e++)
@@ -611,7 +623,7 @@ __device__ __forceinline__ void part32(const be42_kv_pool &P, const PrefixArgs &
         }
 #pragma unroll
         for (int j = 0; j < 16; j++) {
-            p[j] = __builtin_amdgcn_exp2f(__fmaf_rn(p[j], sc, -m));
+            p[j] = __builtin_amdgcn_exp2f((p[j] - m) * sc);
             l += p[j];
         }
         if constexpr (KV8)
@@ -709,6 +721,7 @@ __device__ __forceinline__ void write_part(const PrefixArgs &a, const S &sums, i
     constexpr int L = HD / 4, kApart = 64 * kPartWaves / L, kAt = ROWS / kApart < 4 ? ROWS / kApart : 4;
     const size_t all = (size_t)a.n_queries * a.n_heads;
     const bool last = a.parts_p + a.parts_o == 1;
+    const float sc = log2_scale(a);
     const int d = 4 * (threadIdx.x % L), more_q = kApart / G, more_h = kApart % G;
     int c = threadIdx.x / L, qi = (row0 + c) / G, hi = (row0 + c) % G;       // query and head of the group of row c
 #pragma unroll 1
@@ -732,7 +745,7 @@ __device__ __forceinline__ void write_part(const PrefixArgs &a, const S &sums, i
             float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int x = 0; x < NW; x++) {
-                const float w = part_weight(m[i][x], l[i][x], top);
+                const float w = part_weight(m[i][x], top, sc);
                 sum += w * l[i][x];
                 v.x = __fmaf_rn(w, o[i][x].x, v.x);
                 v.y = __fmaf_rn(w, o[i][x].y, v.y);
@@ -742,13 +755,13 @@ __device__ __forceinline__ void write_part(const PrefixArgs &a, const S &sums, i
             if (row0 + c < rows) {
                 const size_t row = (size_t)(b0 + qi) * a.n_heads + kvh * G + hi;
                 if (last) {
-                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                    const float inv = row_inverse(top, sum);
                     store_out4<QB>(a.out, row * HD + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
                 } else {
                     if (d == 0)
                         *(float2 *)(a.part_ml + 2 * (part * all + row)) = make_float2(top, sum);
                     // (k_prefix_join reads no values of a part without tokens)
-                    if (sum != 0.0f)
+                    if (top != -INFINITY)
                         *(float4 *)(a.part_o + (part * all + row) * HD + d) = v;
                 }
             }
@@ -860,6 +873,7 @@ __global__ __launch_bounds__(256) void k_prefix_join(const PrefixArgs a, int par
     for (int p = lane; p < parts; p += kWave)
         top = fmaxf(top, ml[p * all + row].x);
     top = wave_max(top);
+    const float sc = log2_scale(a);
     float l = 0.0f;
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int p0 = sub; p0 < parts; p0 += kAhead * PER) {
@@ -874,8 +888,8 @@ __global__ __launch_bounds__(256) void k_prefix_join(const PrefixArgs a, int par
 #pragma unroll
         for (int i = 0; i < kAhead; i++) {
             // (a part without tokens left no values)
-            const bool in = p0 + i * PER < parts && x[i].y != 0.0f;
-            const float w = in ? __builtin_amdgcn_exp2f(x[i].x - top) : 0.0f;
+            const bool in = p0 + i * PER < parts && x[i].x != -INFINITY;
+            const float w = in ? __builtin_amdgcn_exp2f((x[i].x - top) * sc) : 0.0f;
             l = in ? __fmaf_rn(w, x[i].y, l) : l;
             v.x = in ? __fmaf_rn(w, o[i].x, v.x) : v.x;
             v.y = in ? __fmaf_rn(w, o[i].y, v.y) : v.y;
@@ -891,7 +905,7 @@ __global__ __launch_bounds__(256) void k_prefix_join(const PrefixArgs a, int par
         v.z += __shfl_xor(v.z, o, kWave);
         v.w += __shfl_xor(v.w, o, kWave);
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = row_inverse(top, l);
     if (sub == 0)
         store_out4<QB>(a.out, row * HD + 4 * lane, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
 }

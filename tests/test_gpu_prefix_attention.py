@@ -410,3 +410,95 @@ def test_nan_of_one_sequences_pages_stays_there(be, bad, bf16, heads, kvh, prefi
         off = np.abs(got[b] - want[b]).max(-1)
         assert (off <= tol[b] + (2.0 ** -7 * vmax[0] if bf16 else 0.0)).all(), b
     assert not np.isfinite(got[1]).all()
+
+
+def pool_of(be, kind, ks, vs):
+    """A pool whose slot s holds the tokens ks[s], vs[s] ([n][kvh][hd] fp32)."""
+    import be42
+    _, kvh, hd = ks[0].shape
+    pool = be.kv_pool(be42.KV_BF16 if kind == "bf16" else be42.KV_INT8, len(ks), kvh, hd, max(len(a) for a in ks) // PAGE + 1)
+    for s, (a, b) in enumerate(zip(ks, vs)):
+        if len(a):
+            pool.append(s, torch.from_numpy(a).cuda().reshape(len(a), -1), torch.from_numpy(b).cuda().reshape(len(b), -1), 0)
+    return pool
+
+
+def whole_numbers(rng, n, kvh, hd, top):
+    """Numbers of up to `top` with a largest of 127 in each row: INT8 pages (scale
+    1) and bf16 pages hold them exactly."""
+    a = rng.integers(-top, top + 1, (n, kvh, hd)).astype(np.float32)
+    a[np.arange(n)[:, None], np.arange(kvh)[None], rng.integers(0, hd, (n, kvh))] = 127 * rng.choice([-1.0, 1.0], (n, kvh))
+    return a
+
+
+# calls of each form: one launch, tiles of 16, 64 and 128 rows (B, prefix)
+FORMS = [(3, 200), (2, 3000), (20, 4100), (70, 1700)]
+
+
+def check_form(be, B, heads, kvh, hd, prefix, max_len):
+    """Whether a call of FORMS takes the launches that it is meant to."""
+    parts = be.lib.be42_prefix_attention_workspace_bytes(B, heads, kvh, hd, prefix, max_len) > 16
+    assert parts == (prefix > 1000), (B, prefix)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("B,prefix", FORMS)
+@pytest.mark.parametrize("scale", [0.01, 1.0, 1e4, 1e9, -1e9, 1e20, 1e30])
+def test_scores_of_any_size(be, kind, bf16, B, prefix, scale):
+    """Scores that fp32 sums hold exactly, so that only their differences round:
+    weights of tokens that count are off by 2^-22 of themselves at most (two
+    roundings of an exponent below 24, the exponential's own), the sums by 2^-20
+    as above.  V of whole numbers below 128 and of one element in 127: exact in
+    either page.  At large scales one token, or equal ones in either slot or part,
+    takes it all."""
+    kvh, hd, heads = 2, 128, 8
+    rng = np.random.default_rng(B + prefix)
+    held = [(5 * b) % 23 for b in range(B)] + [prefix]
+    k = [whole_numbers(rng, n, kvh, hd, 4) for n in held]
+    v = [whole_numbers(rng, n, kvh, hd, 100) for n in held]
+    for b in range(0, B, 3):                               # the same key in the slot and in the prefix, at places apart
+        if held[b]:
+            k[b][-1] = k[B][prefix // 2] = k[B][0] = k[B][prefix - 1]
+    pool = pool_of(be, kind, k, v)
+    check_form(be, B, heads, kvh, hd, prefix, 23)
+    q = torch.from_numpy(rng.integers(-3, 4, (B, heads, hd)).astype(np.float32))
+    q = q.bfloat16() if bf16 else q
+    k, v = ([a.astype(np.float64) for a in x] for x in (k, v))
+    lens = torch.tensor(held[:B], dtype=torch.int32, device="cuda")
+    got = be.prefix_attention(pool, q.cuda(), B, prefix, scale, lens=lens, max_len=23).double().cpu().numpy()
+    sc = float(np.float32(scale))
+    want = reference(q.double().numpy(), k, v, heads, sc, B, prefix, range(B), held[:B], 23)[0]
+    tol = 127 * 2.0 ** -19 + (2.0 ** -7 * 127 if bf16 else 0.0)
+    assert np.isfinite(got).all() and (np.abs(got - want) <= tol).all(), np.abs(got - want).max()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("B,prefix", FORMS)
+def test_scores_of_minus_infinity(be, kind, B, prefix):
+    """Scores that overflow downwards weigh nothing, also where they come first
+    (the prefix's first steps, all own tokens of some queries); a query that has
+    no others has seen tokens all the same: no zeros, 0 / 0."""
+    kvh, hd, heads = 2, 64, 8
+    rng = np.random.default_rng(B)
+    held = [(5 * b) % 23 for b in range(B)] + [prefix]
+    k, v = ([rng.standard_normal((n, kvh, hd)).astype(np.float32) * x for n in held] for x in (2.0 ** -100, 1.0))
+    k = [np.abs(a) for a in k]
+    for b in range(0, B, 2):
+        k[b][:] = -(2.0 ** 60)
+    k[B][:150] = -(2.0 ** 60)
+    pool = pool_of(be, kind, k, v)
+    q = torch.full((B, heads, hd), 2.0 ** 100, dtype=torch.bfloat16)
+    lens = torch.tensor(held[:B], dtype=torch.int32, device="cuda")
+    got = be.prefix_attention(pool, q.cuda(), B, prefix, 0.125, lens=lens, max_len=23).double().cpu().numpy()
+    keep = [(a > -1).all((1, 2)) for a in k]
+    stay = [a[i] for a, i in zip(k, keep)]
+    pages = pool_of(be, kind, stay, [a[i] for a, i in zip(v, keep)])
+    fewer = torch.tensor([len(a) for a in stay[:B]], dtype=torch.int32, device="cuda")
+    want = be.prefix_attention(pages, q.cuda(), B, len(stay[B]), 0.125, lens=fewer, max_len=23).double().cpu().numpy()
+    # the same tokens in other steps: two roundings to bf16, weights of 16 bits or of bf16, sums
+    assert np.isfinite(got).all() and (np.abs(got - want) <= 2.0 ** -7 * np.abs(v[B]).max()).all()
+    for max_len in (23, 3000):                             # one launch or two
+        bad = be.prefix_attention(pool, q.cuda(), B, 150, 0.125, lens=lens, max_len=max_len).cpu()
+        others = torch.tensor([b % 2 == 1 and held[b] > 0 for b in range(B)])
+        assert torch.isnan(bad[~others]).all() and torch.isfinite(bad[others]).all()

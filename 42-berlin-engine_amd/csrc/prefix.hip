@@ -779,11 +779,11 @@ __device__ __forceinline__ void write_part(const PrefixArgs &a, const S &sums, i
 // One workgroup a tile of rows and part: of the prefix by part32 (R > 0) or
 // part16, of own tokens by part16.  fp32 queries and their weights enter the
 // products with all 24 bits, in three parts.  For bf16 queries, whose output is
-// rounded to bf16 anyway (2^-9 of it at most), the weights are rounded to 16 bits
-// where memory bounds the tile, and to bf16 in the tiles of many rows, which the
-// matrix products bound: each weight is off by 2^-9 of itself at most, and the
-// output by less than that of the largest value (0.0023 relative to the output over
-// 32768 tokens, 0.0017 with 16 bits, at 184 us instead of 146).
+// rounded to bf16 (2^-8 of it at most), the weights are rounded to 16 bits, in two
+// parts, whatever the batch: over 32768 tokens the output is off by 0.0017 of
+// itself, its rounding alone.  (One part, bf16, made that 0.0023, and 0.0026 from
+// the same query's in a batch of few; 128 queries over 32768 tokens and up to 1024
+// of their own 133 us instead of 158.)
 template <bool KV8, int HD, bool QB, int R>
 __global__ __launch_bounds__(64 * kPartWaves, 2) void k_prefix_part(const be42_kv_pool P, const PrefixArgs a)
 {
@@ -824,7 +824,7 @@ __global__ __launch_bounds__(64 * kPartWaves, 2) void k_prefix_part(const be42_k
     part += own ? a.parts_p : 0;
     if constexpr (R != 0)
         if (!own) {
-            part32<KV8, HD, NP, NP, R>(P, a, S.many, slot, lo, n, kvh, row0, rows);
+            part32<KV8, HD, NP, QB ? 2 : 3, R>(P, a, S.many, slot, lo, n, kvh, row0, rows);
             write_part<HD, QB, kPartWaves / R, kRows>(a, S.many.sums, row0, rows, b0, kvh, G, part);
             return;
         }

@@ -283,8 +283,7 @@ int  be42_lsh_attention_status(void *stream);
  * that sees no token gets zeros.  q and out are fp32, or both bf16 with q_bf16;
  * out is [n_queries][n_heads][head_dim].  K, V (as the pages hold them) and fp32
  * queries and weights enter the products with their full precision; bf16 queries
- * are used as they are, and their weights rounded to 16 bits, or to bf16 at worst
- * where a KV head has more than 32 rows (n_queries * n_heads / n_kv).
+ * are used as they are, and their weights rounded to 16 bits.
  * max_len bounds lens: own tokens from max_len on are not seen.  prefix_len,
  * lens and a slot's pages are cut at the tokens the slot holds, and a slot
  * outside the pool holds none.  The launch depends on prefix_len and max_len

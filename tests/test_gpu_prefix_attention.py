@@ -502,3 +502,24 @@ def test_scores_of_minus_infinity(be, kind, B, prefix):
         bad = be.prefix_attention(pool, q.cuda(), B, 150, 0.125, lens=lens, max_len=max_len).cpu()
         others = torch.tensor([b % 2 == 1 and held[b] > 0 for b in range(B)])
         assert torch.isnan(bad[~others]).all() and torch.isfinite(bad[others]).all()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("B,prefix", FORMS)
+def test_weights_of_bf16_queries(be, kind, hd, B, prefix):
+    """bf16 queries lose no more than the rounding of the output, 2^-8 of itself,
+    whatever the batch: a weight enters the products as two bf16 parts, off by 2^-16
+    of itself at most; scores and sums are off as for fp32 queries."""
+    kvh, heads = 2, 8
+    held = [(5 * b) % 23 for b in range(B)] + [prefix]
+    pool, k, v = make_pool(be, kind, B + 1, kvh, hd, held, B)
+    q = queries(B, B, heads, hd, True)
+    lens = torch.tensor(held[:B], dtype=torch.int32, device="cuda")
+    got = be.prefix_attention(pool, q.cuda(), B, prefix, 1 / math.sqrt(hd), lens=lens, max_len=23).double().cpu().numpy()
+    qd = q.double().numpy()
+    want, tol, _ = reference(qd, k, v, heads, 1 / math.sqrt(hd), B, prefix, range(B), held[:B], 23)
+    sizes = reference(qd, k, [np.abs(a) for a in v], heads, 1 / math.sqrt(hd), B, prefix, range(B), held[:B], 23)[0]
+    off = np.abs(got - want)
+    bound = 2.0 ** -8 * np.abs(want) + 2.0 ** -16 * sizes + tol[..., None]
+    assert (off <= bound).all(), (off / bound).max()

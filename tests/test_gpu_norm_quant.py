@@ -197,3 +197,25 @@ def test_long_rows(be, orc, kind, bf16, cols):
     for res in (r, None):
         got = be.norm_quant_rows(x.cuda(), w.cuda(), EPS, kind, residual=None if res is None else res.cuda())
         check(got, defined(orc, x, res, w, EPS, kind), res is not None)
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+def test_the_longest_row(be, orc, kind):
+    """A row of 2^31 - 1: a thread's place in it passes 32 bits with a sign.  61
+    distinct values whose squares add up without rounding."""
+    cols, period = 2 ** 31 - 1, 61
+    base = ((torch.arange(period) - 30) / 8.0).bfloat16()
+    d = base.double()
+    full, rest = divmod(cols, period)
+    mean = (full * (d * d).sum() + (d[:rest] * d[:rest]).sum()) / cols
+    y = (d / torch.sqrt(mean + float(np.float32(EPS)))).float().numpy()
+    codes, scale = (orc.quant_int8 if kind == "int8" else orc.quant_fp8)(y)
+    some = 1 << 15                                         # periods that are repeated at once
+
+    def row(v):
+        v = v.cuda().repeat(some)
+        return v.repeat(-(-cols // v.numel()))[:cols]
+
+    q, s, h = be.norm_quant_rows(row(base)[None], torch.ones(cols, dtype=torch.bfloat16, device="cuda"), EPS, kind)
+    assert h is None and s.cpu().numpy()[0] == np.float32(scale)
+    assert torch.equal(q[0], row(torch.from_numpy(codes)))

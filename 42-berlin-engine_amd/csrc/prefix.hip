@@ -993,7 +993,7 @@ extern "C" int be42_prefix_attention(const be42_kv_pool *pool, const void *q, in
     BE42_CHECK(n_heads > 0 && n_heads % P.n_kv == 0, "be42_prefix_attention: %d heads over %d kv heads", n_heads,
                P.n_kv);
     BE42_CHECK(P.head_dim == 64 || P.head_dim == 128, "be42_prefix_attention: head_dim %d (64 or 128)", P.head_dim);
-    BE42_CHECK(n_queries >= 0 && q_stride >= n_heads * P.head_dim, "be42_prefix_attention: %d queries at stride %d",
+    BE42_CHECK(n_queries >= 0 && q_stride >= (long)n_heads * P.head_dim, "be42_prefix_attention: %d queries at stride %d",
                n_queries, q_stride);
     BE42_CHECK(prefix_slot >= 0 && prefix_slot < P.n_layers, "be42_prefix_attention: prefix slot %d of %d", prefix_slot,
                P.n_layers);

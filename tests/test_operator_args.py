@@ -143,3 +143,10 @@ def test_strides_and_shapes_past_32_bits(lib, shape, stride):
     x = torch.empty(0, device="meta", dtype=torch.bfloat16).as_strided(shape, (stride, 1))
     with pytest.raises(be42.Be42Error, match="32 bits"):
         lib._rows("f", "x", x, (torch.bfloat16,))
+
+
+@pytest.mark.parametrize("n_heads,hd", [(1 << 25, 64), (1 << 24, 128), (1 << 25, 128)])
+def test_prefix_attention_heads_past_32_bits(lib, n_heads, hd):
+    """The elements of a query's heads, counted in 32 bits, would be below any stride."""
+    for n in (1, 2):
+        refused(lib, prefix(lib, pool(head_dim=hd), n_heads=n_heads, n_queries=n, max_len=0), "stride")

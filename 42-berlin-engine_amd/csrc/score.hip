@@ -660,7 +660,7 @@ __global__ __launch_bounds__(kWave) void k_score_join(const ScoreArgs a)
 static void cut_row(int n, int before, int rows, bool bf16, long *chunks, long *per, long *runs, int *waves)
 {
     const long entries = kChunkBytes / (bf16 ? 2 : 4);
-    *chunks = (n + before + entries - 1) / entries;
+    *chunks = ((long)n + before + entries - 1) / entries;
     const bool whole = rows <= 256 && *chunks > kScoreW && (*chunks * entries <= 80 * 1024 || rows > 96);
     *waves = whole ? kScoreWide : kScoreW;
     const long least = rows >= 256 ? 4 * kScoreW : kScoreW;

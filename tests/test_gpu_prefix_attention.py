@@ -523,3 +523,31 @@ def test_weights_of_bf16_queries(be, kind, hd, B, prefix):
     off = np.abs(got - want)
     bound = 2.0 ** -8 * np.abs(want) + 2.0 ** -16 * sizes + tol[..., None]
     assert (off <= bound).all(), (off / bound).max()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("B,heads,kvh,prefix,max_len", [
+    (65, 5, 1, 1537, 17), (65, 5, 1, 5003, 17), (129, 4, 2, 2049, 17), (129, 4, 2, 1800, 0), (257, 1, 1, 2048, 5),
+    (14, 20, 1, 100, 17), (14, 20, 1, 100, 0), (8, 66, 2, 333, 40)])
+def test_tiles_of_128_rows(be, kind, bf16, hd, B, heads, kvh, prefix, max_len):
+    """More than 256 rows of a KV head, in tiles of 128 whose last is cut, over
+    prefixes whose parts end inside a stage and a page; the tolerance of bf16
+    queries as for their weights above."""
+    G = heads // kvh
+    assert B * G > 256
+    whole = be.lib.be42_prefix_attention_workspace_bytes(B, heads, kvh, hd, prefix, max_len) == 16
+    assert whole == (prefix == 100 and max_len == 0)       # (in one part; groups above 16 have no one-launch form)
+    held = [(5 * b) % (max_len + 1) for b in range(B)] + [prefix]
+    pool, k, v = make_pool(be, kind, B + 1, kvh, hd, held, B + prefix)
+    q = queries(B, B, heads, hd, bf16)
+    lens = torch.tensor(held[:B], dtype=torch.int32, device="cuda")
+    args = heads, 1 / math.sqrt(hd), B, prefix, range(B), held[:B], max_len
+    got = be.prefix_attention(pool, q.cuda(), B, prefix, args[1], lens=lens, max_len=max_len).double().cpu().numpy()
+    qd = q.double().numpy()
+    want, tol, _ = reference(qd, k, v, *args)
+    bound = np.broadcast_to(tol[..., None], want.shape)
+    if bf16:
+        bound = bound + 2.0 ** -8 * np.abs(want) + 2.0 ** -16 * reference(qd, k, [np.abs(a) for a in v], *args)[0]
+    assert (np.abs(got - want) <= bound).all(), (np.abs(got - want) / bound).max()

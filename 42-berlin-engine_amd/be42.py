@@ -6,6 +6,7 @@ the process holds exactly one HIP runtime (torch ships its own
 libamdhip64.so.7; the library then binds to the already-loaded copy).
 
 There is no CPU path here: when the library or a GPU is missing, calls raise.
+Nor is there autograd: results carry no gradient, whatever their inputs require.
 """
 import ctypes as C
 import functools
@@ -510,8 +511,9 @@ class Lib:
         prefix_slot, read once for all, and the first lens[b] tokens of slot
         slots[b] (None: slot b / all its tokens).  max_len bounds lens (None:
         what a slot can hold; the closer, the better the work is split).
-        workspace: be42_prefix_attention_workspace_bytes bytes (uint8) to use
-        instead of a new tensor."""
+        out: where the result goes, overlapping no input.  workspace:
+        be42_prefix_attention_workspace_bytes bytes (uint8) to use instead of a
+        new tensor."""
         t, name = self.torch, "be42_prefix_attention"
         if q.dim() != 3 or q.shape[2] != pool.head_dim or q.dtype not in (t.float32, t.bfloat16):
             raise Be42Error(f"{name}: q is {q.dtype} {tuple(q.shape)}")

@@ -17,13 +17,14 @@
 // its pages are read once for a tile of up to 128 rows.
 //
 // What bounds it, of a pass (kernel times; a large copy runs at 5.2 to 5.5 TB/s, a
-// large bf16 product at 1.2 PFLOP/s here): 512 bf16 rows over 32768 tokens 103 us,
-// 0.67 PFLOP/s, matrix and vector instructions of a SIMD's two waves hardly
-// overlapping (forming the next step's scores beside this one's weights changed
-// nothing); 128 sequences of up to 1024 own tokens behind the same prefix 143 us,
-// 2.9 TB/s; own tokens alone 64 us, 4.3 TB/s; 128 fp32 rows over 8190 tokens 30 us,
-// of which 4.5 until the first pages are there, 14 products (three bf16 parts each
-// of q and the weights, 0.45 PFLOP/s of them), 3 results and 4.4 the join; the
+// large bf16 product at 1.2 PFLOP/s here): 512 bf16 rows over 32768 tokens 121 us,
+// 0.85 PFLOP/s with the weights' second part; matrix units are busy for 41% of a
+// SIMD's cycles, vector units for 45%, both at once for 15% (forming the next
+// step's scores beside this one's weights changed nothing); 128 sequences of up to
+// 1024 own tokens behind the same prefix 156 us, 2.6 TB/s, each byte read once; own
+// tokens alone 64 us, 4.3 TB/s; 128 fp32 rows over 8190 tokens 30 us, of which 4.5
+// until the first pages are there, 14 products (three bf16 parts each of q and the
+// weights, 0.45 PFLOP/s of them; one wave a SIMD), 3 results and 4.4 the join; the
 // smallest call 7.9 us in one launch, a chain of loads (page table, pages) and steps.
 #include <algorithm>
 #include <cmath>
@@ -446,7 +447,7 @@ struct WideShared {
         alignas(16) char k[2][kPageBytes], v[2][kPageBytes];
         float scale[KV8 ? 2 : 1][2][kPage];     // of K and V, of each page
     };
-    static constexpr int NS = T * 4 * kPageBytes > 16 * 1024 ? 2 : 4;       // 64 KB: two workgroups a CU
+    static constexpr int NS = T * 4 * kPageBytes > 16 * 1024 ? 2 : 4;       // a ring of 64 KB at most, where two workgroups a CU fit
     struct Sums {
         float o[T][32 * R][HD + 4];
         float m[T][32 * R], l[T][32 * R];
@@ -913,8 +914,6 @@ __global__ __launch_bounds__(256) void k_prefix_join(const PrefixArgs a, int par
 // Tokens of a slot that a call may name: their sums stay within 32 bits.
 constexpr int kMaxTokens = 1 << 30;
 
-
-
 // The cut of the tokens: as many parts as give `want` workgroups, of at least
 // `unit` tokens.
 static void cut(int tokens, long tiles, int unit, long want, int *parts, int *chunk)
@@ -928,14 +927,17 @@ static void cut(int tokens, long tiles, int unit, long want, int *parts, int *ch
     *parts = (int)(((long)tokens + *chunk - 1) / *chunk);
 }
 
-// Rows of a prefix tile: up to 32 rows of a KV head go in tiles of 16 (8192
-// tokens, 32 rows: 16 us, 20 in one of 64), up to 256 in tiles of 64 (128 rows:
-// 30 us, 34 in one of 128), more in tiles of 128 (32768 tokens, 512 rows and own
-// tokens: 150 us, 175 in tiles of 64).  The prefix gets a workgroup a CU, so that
-// own tokens, which wait for memory, run beside it (two: 166 us); where there are
-// few of those and the parts stay long, it gets two (512 rows alone 108 us, 135
-// with one; 128 fp32 rows over 32000 tokens 65 and 71, over 16000 both 42; heads of
-// 64, half the work a token, 64 rows over 32768 tokens 31.5 and 28.5).
+// Rows of a prefix tile: up to 32 rows of a KV head go in tiles of 16 (fp32, 32
+// rows over 2000 tokens 12.1 us, 14.1 in one of 64; over 32000 39.8 and 40.5; over
+// 8192 20.9 and 19.4; four rows 9.6 and 12.1, 34.0 and 38.9, 18.5 and 18.4), up to
+// 256 in tiles of 64 (128 rows over 8192: 27.9 us, 31.0 in one of 128), more in
+// tiles of 128 (32768 tokens, 512 bf16 rows and own tokens: 157 us, 178 in tiles of
+// 64).  The prefix gets a workgroup a CU, so that own tokens, which wait for memory,
+// run beside it (two: 162 us; 128 fp32 rows over 8190 tokens and up to 256 own
+// tokens 30.0, two 35.7); where there are few of those and the parts stay long, it
+// gets two (512 rows alone 121 us, 142 with one; 128 fp32 rows over 32000 tokens 64
+// and 68, over 16000 41.5 and 40.5; heads of 64, half the work a token, 64 rows over
+// 32768 tokens 31.4 and 27.9).
 static void plan_prefix(PrefixArgs &a, int n_kv, int head_dim)
 {
     const int G = a.n_heads / n_kv, unit = kPartWaves * kStep;

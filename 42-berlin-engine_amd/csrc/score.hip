@@ -15,7 +15,7 @@
 // difference, a product, the exponential -- four times as long as another
 // instruction --, an add and an fma): 2000 x 128256 with five alternatives 109 us,
 // 4.7 TB/s.  Memory bound for fp32: 1000 x 128256 98 us without alternatives, 5.2
-// TB/s.  One row of 128256 takes 11.6 us, two launches of which the loads are 2.4.
+// TB/s.  One row of 128256 takes 11.2 us, two launches of which the loads are 2.4.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -652,7 +652,9 @@ __global__ __launch_bounds__(kWave) void k_score_join(const ScoreArgs a)
 // to 80 K entries, or where the rows come near to filling the chip (fp32, top 5, in
 // us: 1 x 32000 8.6, cut 9.6; 1 x 64000 11.4, cut 9.6 and a second launch's 4 us of
 // the caller's time; 1 x 128256 17, cut 10.4; 64 x 128256 19.4, cut 16.6; 120 x
-// 128256 19.4, cut 23.5; 200 x 32000 12.7, cut 16.0); rows of up to four
+// 128256 19.4, cut 23.5; 200 x 32000 12.7, cut 16.0; in a captured graph, where a
+// launch costs no caller's time, 1 x 32000 9.6, cut 10.5, 64 x 32000 10.4 and 12.0, 64
+// x 64000 13.7 and 14.0, but 1 x 64000 12.2 and 10.1); rows of up to four
 // chunks do with four waves (200 x 8000 8.3, eight 8.7).  Other rows are cut
 // until there are four workgroups a CU; a run has at least a chunk for each wave,
 // and four where the rows alone fill the chip, since joining runs costs a launch

@@ -284,10 +284,12 @@ int  be42_lsh_attention_status(void *stream);
  * out is [n_queries][n_heads][head_dim].  K, V (as the pages hold them) and fp32
  * queries and weights enter the products with their full precision; bf16 queries
  * are used as they are, and their weights rounded to 16 bits.
- * max_len bounds lens: own tokens from max_len on are not seen.  prefix_len,
- * lens and a slot's pages are cut at the tokens the slot holds, and a slot
- * outside the pool holds none.  The launch depends on prefix_len and max_len
- * alone, so slots and lens may change between replays of a captured graph.
+ * Scores may be of any size that fp32 holds, |scale| up to 1e30.
+ * max_len bounds lens: own tokens from max_len on are not seen.  prefix_len (at
+ * most the 16 * max_logical tokens that a slot has pages for) and lens are cut at
+ * the tokens the slot holds, and a slot outside the pool holds none.  The launch
+ * depends on prefix_len and max_len alone, so slots and lens may change between
+ * replays of a captured graph.
  * out overlaps no input.  At most 2^24 - 1 workgroups a launch (n_queries *
  * n_heads above 2^20 may be refused).
  * workspace NULL: the library's (grow-only; refused while the stream is
@@ -460,7 +462,9 @@ int be42_sample_top_p_dt(int *out, const void *logits, int logits_bf16, int n, i
  *   top_ids / top_logprobs [r][0 .. top_k): the top_k <= 64 (and <= n) largest
  *     logits in descending order, equal ones (and +0, -0) in ascending id order,
  *     and their log probabilities.
- * Logits of -infinity are tokens of probability zero.  A row without a
+ * Logits of -infinity are tokens of probability zero; any other is a number like
+ * the rest (a row all at the type's lowest value is uniform), and a log
+ * probability below fp32's range is -infinity.  A row without a
  * distribution (it holds a NaN or +infinity, or nothing but -infinity) gets NaN
  * log probabilities and entropy; its top_ids take a NaN for -infinity.
  * n_tokens and top_k may be 0 (their arrays are then not used).  n <= 2^30 and

@@ -911,8 +911,12 @@ __global__ __launch_bounds__(256) void k_prefix_join(const PrefixArgs a, int par
         store_out4<QB>(a.out, row * HD + 4 * lane, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
 }
 
-// Tokens of a slot that a call may name: their sums stay within 32 bits.
+// Tokens of a slot that a call may name: their sums stay within 32 bits.  Rows
+// (queries x heads) that it may have: the join's launch, a wave each, has less than
+// 2^32 threads.  (The workspace's size is given up to twice as many: the plan's
+// numbers of tiles fit an int.)
 constexpr int kMaxTokens = 1 << 30;
+constexpr size_t kMaxRows = 4 * (size_t)kMaxBlocks;
 
 // The cut of the tokens: as many parts as give `want` workgroups, of at least
 // `unit` tokens.
@@ -973,7 +977,8 @@ extern "C" size_t be42_prefix_attention_workspace_bytes(int n_queries, int n_hea
                                                         int prefix_len, int max_len)
 {
     if (n_queries <= 0 || n_heads <= 0 || n_kv <= 0 || n_heads % n_kv || (head_dim != 64 && head_dim != 128) ||
-        prefix_len < 0 || prefix_len > kMaxTokens || max_len < 0 || max_len > kMaxTokens)
+        prefix_len < 0 || prefix_len > kMaxTokens || max_len < 0 || max_len > kMaxTokens ||
+        (size_t)n_queries * n_heads > 2 * kMaxRows)
         return 0;
     PrefixArgs a = {};
     a.n_queries = n_queries;
@@ -1009,14 +1014,14 @@ extern "C" int be42_prefix_attention(const be42_kv_pool *pool, const void *q, in
                n_queries, P.n_layers);
     if (n_queries == 0)
         return BE42_OK;
+    const size_t rows = (size_t)n_queries * n_heads;
+    BE42_CHECK(rows <= kMaxRows, "be42_prefix_attention: %d queries of %d heads", n_queries, n_heads);
     PrefixArgs a = {q, out, slots, lens, nullptr, nullptr, (size_t)q_stride, n_queries, n_heads, prefix_slot, prefix_len,
                     max_len, scale};
     plan_prefix(a, P.n_kv, P.head_dim);
     const int parts = a.parts_p + a.parts_o;
     const long blocks = (long)P.n_kv * ((long)a.tiles_p * a.parts_p + (long)a.tiles_o * n_queries * a.parts_o);
-    const size_t rows = (size_t)n_queries * n_heads;
-    BE42_CHECK(blocks <= kMaxBlocks && rows <= 4 * (size_t)kMaxBlocks,
-               "be42_prefix_attention: %d queries of %d heads", n_queries, n_heads);
+    BE42_CHECK(blocks <= kMaxBlocks, "be42_prefix_attention: %d queries of %d heads", n_queries, n_heads);
     const size_t need = be42_prefix_attention_workspace_bytes(n_queries, n_heads, P.n_kv, P.head_dim, prefix_len,
                                                               max_len);
     BE42_CHECK(!workspace || (!((uintptr_t)workspace & 15) && workspace_bytes >= need),

@@ -150,3 +150,12 @@ def test_prefix_attention_heads_past_32_bits(lib, n_heads, hd):
     """The elements of a query's heads, counted in 32 bits, would be below any stride."""
     for n in (1, 2):
         refused(lib, prefix(lib, pool(head_dim=hd), n_heads=n_heads, n_queries=n, max_len=0), "stride")
+
+
+@pytest.mark.parametrize("n_queries,n_heads", [(INT_MAX, 1 << 20), (1 << 29, 1 << 15), (INT_MAX, 1 << 24)])
+def test_prefix_attention_rows_past_32_bits(lib, n_queries, n_heads):
+    """Their tiles of 128, counted in 32 bits, would be none, or fewer than none."""
+    assert lib.lib.be42_prefix_attention_workspace_bytes(n_queries, n_heads, 1, 64, 1000, 0) == 0
+    assert lib.lib.be42_prefix_attention_workspace_bytes(n_queries, n_heads, 1, 64, 1000, 30) == 0
+    p = pool(n_kv=1, max_logical=100)
+    refused(lib, prefix(lib, p, n_queries=n_queries, n_heads=n_heads, q_stride=INT_MAX, prefix_len=1000, max_len=0), "queries of")

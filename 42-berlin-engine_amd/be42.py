@@ -449,11 +449,15 @@ class Lib:
             if tokens.dim() != 2:
                 raise Be42Error(f"{name}: tokens has shape {tuple(tokens.shape)}")
             given = tokens.shape[1]
+            if given >= 1 << 31:
+                raise Be42Error(f"{name}: {given} tokens a row: past 32 bits")
             self._want(name, "tokens", tokens, (t.int32,), (rows, given), dev)
             got["logprobs"] = t.empty(rows, given, dtype=t.float32, device=dev)
         if entropy:
             got["entropy"] = t.empty(rows, dtype=t.float32, device=dev)
         if top_k:
+            if not 0 < top_k < 1 << 31:
+                raise Be42Error(f"{name}: top {top_k}")
             got["top_ids"] = t.empty(rows, top_k, dtype=t.int32, device=dev)
             got["top_logprobs"] = t.empty(rows, top_k, dtype=t.float32, device=dev)
         ws, size = self._workspace(name, workspace, dev, self._logprobs_bytes, n, rows, top_k)

@@ -702,8 +702,8 @@ extern "C" int be42_logprobs(float *logprobs, float *entropy, int *top_ids, floa
     if (rows == 0)
         return BE42_OK;
     BE42_CHECK(logits, "be42_logprobs: null pointer");
-    BE42_CHECK(n_tokens >= 0 && (n_tokens == 0 || (tokens && logprobs)), "be42_logprobs: %d tokens a row, %s", n_tokens,
-               tokens ? "no logprobs" : "no ids");
+    BE42_CHECK(n_tokens >= 0 && n_tokens <= 1 << 30 && (n_tokens == 0 || (tokens && logprobs)),
+               "be42_logprobs: %d tokens a row, %s", n_tokens, tokens ? "no logprobs" : "no ids");
     BE42_CHECK(top_k >= 0 && top_k <= kTopMax && top_k <= n, "be42_logprobs: top %d of %d (at most %d)", top_k, n,
                kTopMax);
     BE42_CHECK(top_k == 0 || (top_ids && top_logprobs), "be42_logprobs: top %d without arrays", top_k);

@@ -467,8 +467,8 @@ int be42_sample_top_p_dt(int *out, const void *logits, int logits_bf16, int n, i
  * probability below fp32's range is -infinity.  A row without a
  * distribution (it holds a NaN or +infinity, or nothing but -infinity) gets NaN
  * log probabilities and entropy; its top_ids take a NaN for -infinity.
- * n_tokens and top_k may be 0 (their arrays are then not used).  n <= 2^30 and
- * rows < 2^24.
+ * n_tokens and top_k may be 0 (their arrays are then not used).  n and n_tokens
+ * are at most 2^30, rows less than 2^24.
  * workspace NULL: the library's (grow-only; refused while the stream is
  * captured), else a device buffer of be42_logprobs_workspace_bytes() bytes,
  * 16-byte aligned, that no call on another stream uses meanwhile (16 bytes:

@@ -159,3 +159,15 @@ def test_prefix_attention_rows_past_32_bits(lib, n_queries, n_heads):
     assert lib.lib.be42_prefix_attention_workspace_bytes(n_queries, n_heads, 1, 64, 1000, 30) == 0
     p = pool(n_kv=1, max_logical=100)
     refused(lib, prefix(lib, p, n_queries=n_queries, n_heads=n_heads, q_stride=INT_MAX, prefix_len=1000, max_len=0), "queries of")
+
+
+def test_logprobs_of_many_tokens(lib):
+    """A wave's place among them is an int; ctypes would pass longer lists on cut to 32 bits."""
+    for n_tokens in ((1 << 30) + 1, INT_MAX):
+        refused(lib, score(lib, n_tokens=n_tokens), "tokens")
+    import torch
+    x = torch.empty(1, 64, device="meta")
+    for kw, word in ((dict(tokens=torch.empty(1, (1 << 32) + 3, device="meta", dtype=torch.int32)), "32 bits"),
+                     (dict(top_k=(1 << 32) + 3), "top"), (dict(top_k=-1), "top")):
+        with pytest.raises(be42.Be42Error, match=word):
+            lib.logprobs(x, **kw)

@@ -299,8 +299,9 @@ def prepare(case, seed):
         if op == "append":
             s["runs"] = np.stack([p["slot"], p["pos0"], p["count"]], 1).astype(np.int32)
         else:
-            s["runs"] = np.stack([p["src"], p["slot"], p["pos0"], p["count"]], 1).astype(np.int32)
-            s["index"] = p["index"].astype(np.int32)
+            # of the first layer; the others' slots follow
+            s["runs"] = np.stack([p["src"], p["slot"], p["pos0"], p["count"]], 1).astype(np.int32)[:case["batch"]]
+            s["index"] = p["index"].astype(np.int32)[:len(p["index"]) // case["layers"]]
     else:
         slot = np.repeat(p["slot"], p["count"])
         pos = np.concatenate([a + np.arange(n) for a, n in zip(p["pos0"], p["count"])])
@@ -336,7 +337,7 @@ def run(s):
                                 q_norm=s["q_norm"], k_norm=s["k_norm"], eps=EPS)
             return dict(s["pages"], q=q)
         if op == "accept":
-            lib.kv_accept(s["pool"], s["runs"], s["index"])
+            lib.kv_accept(s["pool"], s["runs"], s["index"], layers=s["layers"], from_step=1, to_step=s["batch"])
             return s["pages"]
         if op == "tree":
             return lib.tree_attention(s["pool"], s["q"], s["starts"], s["parents"], s["trees"], s["scale"], s["drafts"],

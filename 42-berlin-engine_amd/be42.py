@@ -39,6 +39,14 @@ SIGNATURES = {
     "be42_norm_quant_rows_fp8": (i32, [vp, vp, vp, vp, i32, vp, i32, i32, vp, i32, i32, f32, vp]),
     "be42_prefix_attention_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32]),
     "be42_prefix_attention": (i32, [vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, i32, f32, vp, vp, sz, vp]),
+    "be42_quant_blocks_fp8": (i32, [vp, vp, vp, i32, i32, i32, i32, vp]),
+    "be42_gemm_fp8_block": (i32, [vp, i32, vp, vp, vp, vp, i32, i32, i32, vp]),
+    "be42_linear_fp8_block_workspace_bytes": (sz, [i32, i32, i32]),
+    "be42_linear_fp8_block": (i32, [vp, i32, vp, i32, i32, vp, vp, i32, i32, i32, vp, sz, vp]),
+    "be42_rope_append": (i32, [vp, vp, i32, vp, i32, i32, vp, i32, vp, i32, i32, vp, vp, f32, vp, vp, vp, i32, vp]),
+    "be42_kv_accept": (i32, [vp, vp, i32, vp, i32, i32, i32, vp]),
+    "be42_tree_attention_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32, i32]),
+    "be42_tree_attention": (i32, [vp, vp, i32, i32, i32, i32, vp, i32, i32, vp, i32, vp, vp, i32, f32, vp, vp, sz, vp]),
     "be42_logprobs_workspace_bytes": (sz, [i32, i32, i32]),
     "be42_logprobs": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, i32, f32, vp, i32, i32, vp, sz, vp]),
     "be42_gemv_q8": (i32, [vp, vp, vp, vp, i32, i32, i32, vp]),
@@ -107,6 +115,11 @@ class GemvSeg(C.Structure):
     _fields_ = [("w", C.c_void_p), ("w_scale", C.c_void_p), ("y", C.c_void_p), ("n", C.c_int)]
 
 
+class RopeStruct(C.Structure):
+    """Layout of be42_rope (include/be42_hip.h)."""
+    _fields_ = [("cos", C.c_void_p), ("sin", C.c_void_p), ("len", C.c_int), ("dim", C.c_int), ("interleaved", C.c_int)]
+
+
 class DecoderConfig(C.Structure):
     """Layout of be42_decoder_config (include/be42_hip.h)."""
     _fields_ = [(n, C.c_int) for n in ("n_layers", "dim", "n_heads", "n_kv_heads", "head_dim", "hidden_dim", "vocab",
@@ -160,6 +173,8 @@ class Lib:
             fn.argtypes = args
         self._inited = False
         self._prefix_bytes = functools.lru_cache(4096)(self.lib.be42_prefix_attention_workspace_bytes)
+        self._tree_bytes = functools.lru_cache(4096)(self.lib.be42_tree_attention_workspace_bytes)
+        self._linear_bytes = functools.lru_cache(4096)(self.lib.be42_linear_fp8_block_workspace_bytes)
         self._logprobs_bytes = functools.lru_cache(4096)(self.lib.be42_logprobs_workspace_bytes)
 
     # -- plumbing -------------------------------------------------------------
@@ -296,6 +311,18 @@ class Lib:
                           cols, eps)
         return q, s, sum
 
+    def quant_blocks_fp8(self, x):
+        """E4M3 codes (uint8) of x [rows][cols] (float32 or bfloat16, rows may be
+        strided) with a scale for 128 elements of a row: (codes [rows][cols],
+        scales [rows][ceil(cols / 128)])."""
+        t, name = self.torch, "be42_quant_blocks_fp8"
+        xs = self._rows(name, "x", x, (t.float32, t.bfloat16))
+        rows, cols = x.shape
+        q = t.empty(rows, cols, dtype=t.uint8, device=x.device)
+        s = t.empty(rows, -(-cols // 128), dtype=t.float32, device=x.device)
+        self._device_call(x, name, q.data_ptr(), s.data_ptr(), x.data_ptr(), x.dtype == t.bfloat16, xs, rows, cols)
+        return q, s
+
     def dequant_rows_int8(self, q, s):
         t = self.torch
         rows, cols = q.shape
@@ -392,6 +419,54 @@ class Lib:
         self._call("be42_gemm_prepared_multi", C.addressof(arr), len(segs), self.p(buf), k, m, fp8,
                    self.stream(stream))
         return outs
+
+    def _block_operands(self, name, m, k, wq, sw, dtype, out, dev):
+        """What the products with block scales share: n, the output and its dtype."""
+        t = self.torch
+        if wq.dim() != 2 or wq.shape[1] != k:
+            raise Be42Error(f"{name}: weights have shape {tuple(wq.shape)}, rows of activations {k}")
+        n = wq.shape[0]
+        self._want(name, "weights", wq, (t.uint8,), None, dev)
+        self._want(name, "weight scales", sw, (t.float32,), (-(-n // 128), -(-k // 128)), dev)
+        if max(m, n, k) >= 1 << 31:
+            raise Be42Error(f"{name}: {m} rows, {n} x {k} weights: past 32 bits")
+        dtype = dtype or (t.float32 if out is None else out.dtype)
+        if dtype not in (t.float32, t.bfloat16):
+            raise Be42Error(f"{name}: output in {dtype}")
+        if out is None:
+            out = t.empty(m, n, dtype=dtype, device=dev)
+        else:
+            self._want(name, "out", out, (dtype,), (m, n), dev)
+        return n, out, dtype == t.bfloat16
+
+    def gemm_fp8_block(self, xq, sx, wq, sw, dtype=None, out=None):
+        """Y [m][n] (float32 or bfloat16) = codes xq [m][k] with scales sx
+        [m][k / 128] x codes wq [n][k] with scales sw [n / 128][k / 128], the
+        last blocks short where 128 does not divide (quant_blocks_fp8)."""
+        t, name = self.torch, "be42_gemm_fp8_block"
+        if xq.dim() != 2:
+            raise Be42Error(f"{name}: codes have shape {tuple(xq.shape)}")
+        m, k = xq.shape
+        self._want(name, "codes", xq, (t.uint8,))
+        self._want(name, "scales", sx, (t.float32,), (m, -(-k // 128)), xq.device)
+        n, out, yb = self._block_operands(name, m, k, wq, sw, dtype, out, xq.device)
+        self._device_call(xq, name, out.data_ptr(), yb, xq.data_ptr(), sx.data_ptr(), wq.data_ptr(), sw.data_ptr(), m, n, k)
+        return out
+
+    def linear_fp8_block(self, x, wq, sw, dtype=None, out=None, workspace=None):
+        """gemm_fp8_block of x [m][k] (float32 or bfloat16, rows may be strided),
+        whose codes are those of quant_blocks_fp8.  workspace:
+        be42_linear_fp8_block_workspace_bytes bytes (uint8) to use instead of a
+        new tensor."""
+        t, name = self.torch, "be42_linear_fp8_block"
+        xs = self._rows(name, "x", x, (t.float32, t.bfloat16))
+        m, k = x.shape
+        dev = x.device
+        n, out, yb = self._block_operands(name, m, k, wq, sw, dtype, out, dev)
+        ws, size = self._workspace(name, workspace, dev, self._linear_bytes, m, n, k)
+        self._device_call(x, name, out.data_ptr(), yb, x.data_ptr(), x.dtype == t.bfloat16, xs, wq.data_ptr(), sw.data_ptr(),
+                          m, n, k, None if ws is None else ws.data_ptr(), size)
+        return out
 
     # -- LSH / paged KV / attention --------------------------------------------
     def lsh_projection(self, dim, seed):
@@ -545,6 +620,141 @@ class Lib:
                           scale, out.data_ptr(), None if ws is None else ws.data_ptr(), size)
         return out
 
+    @staticmethod
+    def _host_ints(name, what, x, cols=None):
+        """A dense int32 array of host integers, [n] or [n][cols]."""
+        import numpy as np
+        a = np.ascontiguousarray(x, np.int64) if not (isinstance(x, np.ndarray) and x.dtype == np.int32) else x
+        if a.dtype != np.int32:
+            if a.size and (a.min() < -(1 << 31) or a.max() >= 1 << 31):
+                raise Be42Error(f"{name}: {what} past 32 bits")
+            a = a.astype(np.int32)
+        if not a.flags.c_contiguous:
+            a = np.ascontiguousarray(a)
+        if cols is not None and not a.size:
+            a = a.reshape(0, cols)
+        if a.ndim != (1 if cols is None else 2) or (cols is not None and a.shape[1] != cols):
+            raise Be42Error(f"{name}: {what} has shape {a.shape}")
+        return a
+
+    def _heads(self, name, what, x, dt, rows, hd, dev):
+        """Element stride of the rows of x [rows][heads][hd], whose heads lie one
+        after the other."""
+        if x.dim() != 3 or x.shape[0] != rows or x.shape[2] != hd or x.dtype != dt or x.device != dev:
+            raise Be42Error(f"{name}: {what} is {x.dtype} {tuple(x.shape)} on {x.device}")
+        H = x.shape[1]
+        if rows and ((hd > 1 and x.stride(2) != 1) or (H > 1 and x.stride(1) != hd)):
+            raise Be42Error(f"{name}: {what} has rows that are not dense")
+        stride = x.stride(0) if rows > 1 else H * hd
+        if not 0 <= stride < 1 << 31:
+            raise Be42Error(f"{name}: {what} has rows {stride} apart")
+        return stride
+
+    def rope_append(self, pool, runs, k, v, q=None, rope=None, positions=None, q_norm=None, k_norm=None, eps=1e-5,
+                    out=None):
+        """Tokens of a q/k/v product -> rotated queries, and K and V in the pages:
+        q [n][n_heads][head_dim], k and v [n][n_kv][head_dim] (float32 or
+        bfloat16, rows may be strided: views of one product).  runs (host): rows
+        (slot, pos0, count), whose tokens follow one another, n in all.  q_norm,
+        k_norm [head_dim] bfloat16: weights of a norm of each head before the
+        rotation.  rope: a Rope (None: no rotation); positions [n] int32 (device)
+        where a token's angle is not that of its place.  Returns the rotated
+        queries, in a new tensor or in out (q itself: in place)."""
+        t, name = self.torch, "be42_rope_append"
+        dev, dt, hd = k.device, k.dtype, pool.head_dim
+        if dt not in (t.float32, t.bfloat16) or k.get_device() != pool.device:
+            raise Be42Error(f"{name}: k is {dt} on {dev}, the pool on GPU {pool.device}")
+        runs = self._host_ints(name, "runs", runs, 3)
+        n = k.shape[0]
+        if int(runs[:, 2].sum(dtype="int64")) != n or (n and runs[:, 2].min() < 0):
+            raise Be42Error(f"{name}: {n} tokens, the runs have {runs[:, 2].tolist()}")
+        ks, vs = (self._heads(name, what, x, dt, n, hd, dev) for what, x in (("k", k), ("v", v)))
+        if k.shape[1] != pool.n_kv or v.shape[1] != pool.n_kv:
+            raise Be42Error(f"{name}: k {tuple(k.shape)}, v {tuple(v.shape)}: the pool has {pool.n_kv} heads")
+        H, qs, os_ = 0, 0, 0
+        if q is not None:
+            H, qs = q.shape[1] if q.dim() == 3 else 0, self._heads(name, "q", q, dt, n, hd, dev)
+            if out is None:
+                out = t.empty(n, H, hd, dtype=dt, device=dev)
+                os_ = H * hd
+            else:
+                os_ = self._heads(name, "out", out, dt, n, hd, dev)
+                if out.shape[1] != H:
+                    raise Be42Error(f"{name}: out has shape {tuple(out.shape)}")
+        elif out is not None:
+            raise Be42Error(f"{name}: out without q")
+        for what, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+            if w is not None:
+                self._want(name, what, w, (t.bfloat16,), (hd,), dev)
+        if rope is not None and rope.cos.device != dev:
+            raise Be42Error(f"{name}: rope on {rope.cos.device}, not on {dev}")
+        if positions is not None:
+            self._want(name, "positions", positions, (t.int32,), (n,), dev)
+        at = [None if x is None else x.data_ptr() for x in (q, q_norm, k_norm, positions, out)]
+        self._device_call(k, name, pool.handle, runs.ctypes.data, len(runs), at[0], qs, H, k.data_ptr(), ks, v.data_ptr(), vs,
+                          dt == t.bfloat16, at[1], at[2], eps, None if rope is None else rope.at, at[3], at[4], os_)
+        return out
+
+    def kv_accept(self, pool, runs, index, layers=1, from_step=0, to_step=0):
+        """Tokens that one slot holds, behind what others hold.  runs (host): rows
+        (from, to, pos0, count): `count` tokens at positions pos0 .. of slot `to`,
+        taken from slot `from` at the places that index (host), run after run,
+        names.  The same for each of `layers` layers, whose slots lie from_step
+        and to_step apart."""
+        name = "be42_kv_accept"
+        runs, index = self._host_ints(name, "runs", runs, 4), self._host_ints(name, "index", index)
+        if int(runs[:, 3].sum(dtype="int64")) != len(index):
+            raise Be42Error(f"{name}: {len(index)} tokens, the runs have {runs[:, 3].tolist()}")
+        self._pool_call(pool, name, runs.ctypes.data, len(runs), index.ctypes.data, layers, from_step, to_step)
+
+    def _pool_call(self, pool, name, *args):
+        """Entry point `name` of a pool, on its device's current stream."""
+        t = self.torch
+        with t.cuda.device(pool.device):
+            self._call(name, pool.handle, *args, self.stream())
+
+    def tree_attention(self, pool, q, starts, parents, draft_slot, scale, max_tree, slots=None, lens=None, max_len=None,
+                       out=None, workspace=None):
+        """Attention of drafted tokens: q [n][n_heads][head_dim] (float32 or
+        bfloat16, rows may be strided), tree b the tokens starts[b] .. starts[b +
+        1] - 1 (int32 [n_trees + 1]), at most max_tree <= 256 of them, over the
+        first lens[b] tokens of slot slots[b] (None: slot b / all its tokens) and,
+        in slot draft_slot, where token i has its K and V, over itself and the
+        drafts above it (parents int32 [n], counted within the tree, -1 none; None:
+        each follows the one before).  max_len bounds lens (None: what a slot can
+        hold; the closer, the better the work is split).  out: where the result
+        goes; rows of tokens in no tree are left as they were (a new tensor's:
+        undefined).  workspace: be42_tree_attention_workspace_bytes bytes (uint8) to
+        use instead of a new tensor."""
+        t, name = self.torch, "be42_tree_attention"
+        if q.dim() != 3 or q.dtype not in (t.float32, t.bfloat16):
+            raise Be42Error(f"{name}: q is {q.dtype} {tuple(q.shape)}")
+        n, H, hd = q.shape
+        dev = q.device
+        if q.get_device() != pool.device:
+            raise Be42Error(f"{name}: q on {dev}, the pool on GPU {pool.device}")
+        qs = self._heads(name, "q", q, q.dtype, n, pool.head_dim, dev)
+        trees = starts.numel() - 1
+        if trees < 0:
+            raise Be42Error(f"{name}: starts is empty")
+        for what, x, size in (("starts", starts, trees + 1), ("parents", parents, n), ("slots", slots, trees), ("lens", lens, trees)):
+            if x is not None:
+                self._want(name, what, x, (t.int32,), (size,), dev)
+        if out is None:
+            out = t.empty(n, H, hd, dtype=q.dtype, device=dev)
+        else:
+            self._want(name, "out", out, (q.dtype,), (n, H, hd), dev)
+        if max_len is None:
+            max_len = pool.max_logical * 16
+        if max(max_tree, draft_slot, max_len) >= 1 << 31 or min(draft_slot, max_len) < 0:
+            raise Be42Error(f"{name}: max_tree {max_tree}, draft slot {draft_slot}, max_len {max_len}")
+        ws, size = self._workspace(name, workspace, dev, self._tree_bytes, n, trees, H, pool.n_kv, hd, max_tree, max_len)
+        self._device_call(q, name, pool.handle, q.data_ptr(), q.dtype == t.bfloat16, qs, n, H, starts.data_ptr(), trees, max_tree,
+                          None if parents is None else parents.data_ptr(), draft_slot,
+                          None if slots is None else slots.data_ptr(), None if lens is None else lens.data_ptr(), max_len,
+                          scale, out.data_ptr(), None if ws is None else ws.data_ptr(), size)
+        return out
+
     # -- linear KV cache [T][n_kv][head_dim] bf16 (kv_cache.c) ------------------
     def kv_linear_append(self, k_cache, v_cache, pos, k, v, stream=None):
         """Row `pos` of the bf16 caches from fp32 k, v [n_kv * head_dim]."""
@@ -582,6 +792,29 @@ class Lib:
         self._call("be42_kv_linear_evict", self.p(k_cache), self.p(v_cache), n, heads, dim, self.p(q), self.p(w),
                    keep_k, C.byref(new_len), self.stream(stream))
         return new_len.value
+
+
+class Rope:
+    """Tables of a rotation: cos and sin [len][dim / 2] float32 on the GPU, for the
+    pairs (i, i + dim / 2), or (2 i, 2 i + 1) if interleaved, of a head's first dim
+    elements.  Positions from len on are not rotated."""
+
+    def __init__(self, cos, sin, interleaved=False):
+        for what, x in (("cos", cos), ("sin", sin)):
+            if x.dim() != 2 or x.shape != cos.shape or str(x.dtype) != "torch.float32" or not x.is_contiguous() or \
+                    x.device != cos.device or max(x.shape) >= 1 << 30:
+                raise Be42Error(f"Rope: {what} is {x.dtype} {tuple(x.shape)} on {x.device}")
+        self.cos, self.sin = cos, sin
+        self.struct = RopeStruct(cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1], bool(interleaved))
+        self.at = C.addressof(self.struct)
+
+
+class PoolArray:
+    """Memory of a pool's array for torch.as_tensor; it keeps the pool."""
+
+    def __init__(self, pool, ptr, shape, typestr):
+        self.pool = pool
+        self.__cuda_array_interface__ = dict(shape=shape, typestr=typestr, data=(ptr, False), version=2, strides=None)
 
 
 class KVPool:
@@ -637,6 +870,23 @@ class KVPool:
         out = np.zeros(self.max_logical, np.int32)
         n = self.lib.lib.be42_kv_layer_pages(self.handle, layer, out.ctypes.data, self.max_logical)
         return out[:n].copy()
+
+    def tensors(self):
+        """The pool's pages as tensors on its memory (not copies; they keep the pool
+        until it is closed): k, v [page][n_kv][16][head_dim] int8 with k_scale,
+        v_scale [page][n_kv][16], or bfloat16, whose v is [page][n_kv][head_dim][16];
+        centroid [page][head_dim]."""
+        t, s, int8 = self.lib.torch, self.s, self.kind == KV_INT8
+        cap, kvh, hd = s.capacity, self.n_kv, self.head_dim
+        kind = "|i1" if int8 else "<i2"
+        shapes = dict(k=((cap, kvh, 16, hd), kind), v=((cap, kvh, 16, hd) if int8 else (cap, kvh, hd, 16), kind),
+                      centroid=((cap, hd), "<f4"))
+        if int8:
+            shapes.update(k_scale=((cap, kvh, 16), "<f4"), v_scale=((cap, kvh, 16), "<f4"))
+        with t.cuda.device(self.device):
+            got = {name: t.as_tensor(PoolArray(self, getattr(s, name), shape, kind), device=f"cuda:{self.device}")
+                   for name, (shape, kind) in shapes.items()}
+        return {name: x.view(t.bfloat16) if x.dtype == t.int16 else x for name, x in got.items()}
 
     def fetch(self, field, count, dtype):
         """Copy `count` elements of a device array of the pool to the host."""

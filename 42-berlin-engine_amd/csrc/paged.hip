@@ -55,6 +55,8 @@ struct PoolImpl {
     std::vector<int> logical_len;  // [n_layers]
     std::vector<int> registered;   // [cap]
     std::vector<int> n_indexed;    // [n_layers]
+    std::vector<unsigned> mark;    // [n_layers] the last plan_runs call that filled a slot
+    unsigned marks = 0;
     // page lists of a bulk append (device copy, and the host array it is
     // copied from, which stays untouched until the next bulk append has
     // waited for the stream)
@@ -279,6 +281,9 @@ extern "C" int be42_kv_create(be42_kv_pool **out, int kind, int n_layers, int n_
     alloc((void **)&P.hpT, head_dim * 16 * sizeof(float));
     if (e == hipSuccess) e = hipMemset(P.k, 0, kvbytes);
     if (e == hipSuccess) e = hipMemset(P.v, 0, kvbytes);
+    // (pages as tensors show zeros, not what the memory held)
+    if (e == hipSuccess && P.k_scale) e = hipMemset(P.k_scale, 0, cap * n_kv * kPage * sizeof(float));
+    if (e == hipSuccess && P.v_scale) e = hipMemset(P.v_scale, 0, cap * n_kv * kPage * sizeof(float));
     if (e == hipSuccess) e = hipMemset(P.ntok, 0, cap * sizeof(int));
     if (e == hipSuccess) e = hipMemset(P.centroid, 0, cap * head_dim * sizeof(float));
     if (e == hipSuccess) e = hipMemset(P.page_table, 0xFF, cap * sizeof(int));
@@ -619,6 +624,71 @@ extern "C" int be42_kv_export(const be42_kv_pool *pool, int *page_table, int *fr
 }
 
 namespace be42 {
+
+int slot_pages(const be42_kv_pool *pool, int slot)
+{
+    return reinterpret_cast<const PoolImpl *>(pool)->logical_len[slot];
+}
+
+int plan_runs(be42_kv_pool *pool, const char *who, const be42_kv_run *runs, int n_runs, const int *from,
+              std::vector<int> &pages)
+{
+    PoolImpl *p = impl(pool);
+    be42_kv_pool &P = p->pub;
+    if (p->mark.empty())
+        p->mark.assign(P.n_layers, 0);
+    if (++p->marks == 0) {
+        std::fill(p->mark.begin(), p->mark.end(), 0);
+        p->marks = 1;
+    }
+    long need = 0, touched = 0;
+    for (int r = 0; r < n_runs; r++) {
+        const be42_kv_run &u = runs[r];
+        BE42_CHECK(u.slot >= 0 && u.slot < P.n_layers, "%s: slot %d out of range", who, u.slot);
+        BE42_CHECK(u.pos0 >= 0 && u.count >= 0 && ((long)u.pos0 + u.count + kPage - 1) / kPage <= P.max_logical,
+                   "%s: positions %d .. of %d tokens (a slot has %d pages)", who, u.pos0, u.count, P.max_logical);
+        BE42_CHECK(p->mark[u.slot] != p->marks, "%s: slot %d given twice", who, u.slot);
+        p->mark[u.slot] = p->marks;
+        if (!u.count)
+            continue;
+        const int first = u.pos0 / kPage, end = (u.pos0 + u.count - 1) / kPage + 1, have = p->logical_len[u.slot];
+        // pages are appended in order: a gap would leave unmapped pages
+        BE42_CHECK(first <= have, "%s: position %d skips page %d", who, u.pos0, have);
+        need += std::max(0, end - have);
+        touched += end - first;
+    }
+    for (int r = 0; from && r < n_runs; r++) {
+        BE42_CHECK(from[r] >= 0 && from[r] < P.n_layers, "%s: slot %d out of range", who, from[r]);
+        BE42_CHECK(p->mark[from[r]] != p->marks, "%s: slot %d is read and filled", who, from[r]);
+    }
+    if (need > p->free_top + 1) {
+        set_error("%s: page pool exhausted: %ld pages, %d are free", who, need, p->free_top + 1);
+        return BE42_ENOMEM;
+    }
+    pages.clear();
+    pages.reserve(touched);
+    for (int r = 0; r < n_runs; r++) {
+        const be42_kv_run &u = runs[r];
+        if (!u.count)
+            continue;
+        const int end = (u.pos0 + u.count - 1) / kPage + 1, full = (u.pos0 + u.count) / kPage;
+        const size_t base = (size_t)u.slot * P.max_logical;
+        for (int blk = u.pos0 / kPage; blk < end; blk++) {
+            int fresh = 0;
+            if (blk >= p->logical_len[u.slot]) {
+                p->page_table[base + blk] = pool_alloc(p);
+                p->logical_len[u.slot] = blk + 1;
+                fresh = kNewPage;
+            }
+            const int phys = p->page_table[base + blk];
+            if (blk < full)
+                p->registered[phys] = 1;
+            pages.push_back(phys | fresh);
+        }
+        p->n_indexed[u.slot] = std::max(p->n_indexed[u.slot], full > u.pos0 / kPage ? full : 0);
+    }
+    return BE42_OK;
+}
 
 // Host bookkeeping of one decode token for each of n distinct layer slots
 // (paged.c:195-272 per slot): page allocation, page table, seal list.

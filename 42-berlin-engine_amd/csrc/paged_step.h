@@ -61,6 +61,17 @@ int plan_append_run(be42_kv_pool *pool, int layer, int pos0, int n, int *L, Appe
 int launch_append_run(const be42_kv_pool &P, const AppendRun &r, const int *d_lists, const float *k, const float *v,
                       hipStream_t s);
 
+// host: bookkeeping of runs of consecutive positions of distinct slots.  Checked as
+// a whole before anything is changed; pages[] gets the physical page of every
+// logical page that a run touches, run after run, with kNewPage where it is new (its
+// page table entry is to be published).  from (may be NULL): slots that are read
+// meanwhile, which must lie in the pool and not among the runs'.
+constexpr int kNewPage = 1 << 30;
+int plan_runs(be42_kv_pool *pool, const char *who, const be42_kv_run *runs, int n_runs, const int *from,
+              std::vector<int> &pages);
+// host: logical pages that a slot has
+int slot_pages(const be42_kv_pool *pool, int slot);
+
 // device: the router (k_route, lsh.hip) of n_queries queries; lim (device,
 // optional) as in lsh_attention_prefix; cand / ncand / qhash optional
 int launch_route(const be42_kv_pool &P, const float *q, const int *slots, const int *lim, int n_queries, int H,

@@ -195,6 +195,37 @@ static bool launch_quant_vec(uint8_t *q, float *scales, const float *x, int rows
     return true;
 }
 
+// E4M3 codes with a scale for 128 elements of a row (a group of 32 lanes each, four
+// elements a lane): f32_to_fp8 of x / scale, scale = amax / 224, as k_quant_rows_fp8
+// forms them of a row of 128.
+template <bool BF16>
+__global__ __launch_bounds__(256) void k_quant_blocks(uint8_t *q, float *scales, const void *x, size_t x_stride, int rows,
+                                                      int cols, int blocks)
+{
+    const size_t at = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (at >= (size_t)rows * blocks)
+        return;
+    const size_t row = at / blocks;
+    const int b = (int)(at % blocks), c0 = b * 128 + 4 * (threadIdx.x & 31);
+    float v[4], m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const size_t i = row * x_stride + c0 + j;
+        v[j] = c0 + j >= cols ? 0.0f : BF16 ? bf16_to_f32(((const uint16_t *)x)[i]) : ((const float *)x)[i];
+        m = fmaxf(m, fabsf(v[j]));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        m = fmaxf(m, __shfl_xor(m, o, 32));
+    const float scale = m > 0.0f ? m / 224.0f : 1.0f, inv = m > 0.0f ? 1.0f / scale : 1.0f;
+    if ((threadIdx.x & 31) == 0)
+        scales[at] = scale;
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (c0 + j < cols)
+            q[row * cols + c0 + j] = f32_to_fp8(v[j] * inv);
+}
+
 // ---- residual + RMS norm + codes -----------------------------------------------
 // h = x + residual in the stream's type, y = fp32(h / sqrt(mean h^2 + eps) * w)
 // and the codec's code of y.  The sum of squares and the product are formed in
@@ -688,6 +719,26 @@ extern "C" int be42_fp8_decode(float *out, const uint8_t *q, size_t n, void *str
     if (blocks > 8192)
         blocks = 8192;
     hipLaunchKernelGGL(k_fp8_decode, dim3(blocks), dim3(256), 0, as_stream(stream), out, q, n);
+    BE42_LAUNCH_CHECK();
+    return BE42_OK;
+}
+
+extern "C" int be42_quant_blocks_fp8(uint8_t *q, float *scales, const void *x, int x_bf16, int x_stride, int rows,
+                                     int cols, void *stream)
+{
+    BE42_CHECK(rows == 0 || (q && scales && x), "be42_quant_blocks_fp8: null pointer");
+    BE42_CHECK(rows >= 0 && cols > 0, "be42_quant_blocks_fp8: bad shape (%d, %d)", rows, cols);
+    BE42_CHECK(x_stride >= cols, "be42_quant_blocks_fp8: rows of %d at stride %d", cols, x_stride);
+    BE42_CHECK(!((uintptr_t)x & (x_bf16 ? 1 : 3)) && !((uintptr_t)scales & 3), "be42_quant_blocks_fp8: unaligned pointer");
+    if (rows == 0)
+        return BE42_OK;
+    const long blocks = ((long)cols + 127) / 128, groups = (rows * blocks + 7) / 8;
+    BE42_CHECK(groups <= kMaxBlocks, "be42_quant_blocks_fp8: %d rows of %d", rows, cols);
+    const dim3 g((unsigned)groups), b(256);
+    if (x_bf16)
+        hipLaunchKernelGGL(k_quant_blocks<true>, g, b, 0, as_stream(stream), q, scales, x, (size_t)x_stride, rows, cols, (int)blocks);
+    else
+        hipLaunchKernelGGL(k_quant_blocks<false>, g, b, 0, as_stream(stream), q, scales, x, (size_t)x_stride, rows, cols, (int)blocks);
     BE42_LAUNCH_CHECK();
     return BE42_OK;
 }

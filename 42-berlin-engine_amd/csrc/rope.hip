@@ -1,0 +1,425 @@
+// rope.hip -- tokens into the pages of several slots at once: norms of queries and
+// keys, rotation and append in one pass (be42_rope_append), and drafted tokens that
+// were right behind their sequences (be42_kv_accept).
+//
+// A workgroup takes the tokens of a call that go into one page, for one KV head: the
+// query heads of its group, its K and its V row.  Pages are planned on the host and
+// go with the launch by value, so nothing is copied to the device beforehand; the
+// workgroup of KV head 0 seals the page where its last position is written.
+#include <algorithm>
+#include <new>
+#include <type_traits>
+
+#include "be42_common.h"
+#include "paged_dev.h"
+#include "paged_step.h"
+
+namespace be42 {
+
+// What a launch takes: pieces of runs, and the physical page of every page that they
+// touch.  (Arguments of a kernel are at most 4 KB.)
+constexpr int kPieces = 64, kPiecePages = 640;
+struct Piece {
+    int slot, pos0, n, tok0, page0;    // page0: its first page's place in pages
+};
+struct RopeArgs {
+    int n, n_pages;
+    Piece piece[kPieces];
+    int pages[kPiecePages];
+};
+
+struct RopeIn {
+    const void *q, *k, *v;
+    void *q_out;
+    const uint16_t *q_norm, *k_norm;
+    const float *cos_t, *sin_t;
+    const int *positions;
+    size_t q_stride, k_stride, v_stride, q_out_stride;
+    int n_heads, rope_len, rope_dim, interleaved;
+    float eps;
+};
+
+// The piece that page `at` of a launch belongs to: lanes compare, one each.
+template <class A>
+__device__ __forceinline__ int piece_of(const A &a, int at)
+{
+    if (a.n == 1)
+        return 0;
+    const int lane = threadIdx.x & 63;
+    return __popcll(__ballot(lane < a.n && a.piece[min(lane, kPieces - 1)].page0 <= at)) - 1;
+}
+
+// The page table's and the page's words, by the workgroup of KV head 0.
+__device__ __forceinline__ void publish(const be42_kv_pool &P, int slot, int pos0, int n, int blk, int phys, bool fresh)
+{
+    const int end = pos0 + n;
+    if (fresh) {
+        P.page_table[(size_t)slot * P.max_logical + blk] = phys;
+        if (end <= (blk + 1) * kPage)
+            P.n_logical[slot] = blk + 1;
+    }
+    P.ntok[phys] = min(end - blk * kPage, kPage);
+    // the last page that the piece fills
+    if (end >= (blk + 1) * kPage && end < (blk + 2) * kPage && blk + 1 > P.n_indexed[slot])
+        P.n_indexed[slot] = blk + 1;
+}
+
+template <bool BF16>
+__device__ __forceinline__ float act_at(const void *p, size_t i)
+{
+    return BF16 ? bf16_to_f32(((const uint16_t *)p)[i]) : ((const float *)p)[i];
+}
+
+// One wave a row, a lane a pair of elements (two pairs where head_dim is past 128):
+// the pairs of the rotation, then neighbours behind them.
+template <bool KV8, bool BF16, int NP>
+__global__ __launch_bounds__(256) void k_rope_append(const be42_kv_pool P, const RopeArgs a, const RopeIn x)
+{
+    __shared__ float c[256];
+    const int h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const Piece &u = a.piece[piece_of(a, blockIdx.x)];
+    const int blk = u.pos0 / kPage + ((int)blockIdx.x - u.page0);
+    const int entry = a.pages[blockIdx.x], phys = entry & ~kNewPage;
+    const int lo = max(u.pos0, blk * kPage), T = min(u.pos0 + u.n, (blk + 1) * kPage) - lo;
+    const int tok0 = u.tok0 + lo - u.pos0, off0 = lo - blk * kPage;
+    const int hd = P.head_dim, G = x.n_heads / P.n_kv, half = x.rope_dim / 2;
+    if (h == 0 && threadIdx.x == 0)
+        publish(P, u.slot, u.pos0, u.n, blk, phys, entry & kNewPage);
+    for (int r = wave; r < T * (G + 2); r += 4) {
+        const int kind = r / T, i = r % T, tok = tok0 + i;     // query heads, then K, then V
+        const bool is_v = kind == G + 1, is_k = kind == G;
+        const size_t at = is_v ? tok * x.v_stride + (size_t)h * hd
+                        : is_k ? tok * x.k_stride + (size_t)h * hd
+                               : tok * x.q_stride + (size_t)(h * G + kind) * hd;
+        const void *from = is_v ? x.v : is_k ? x.k : x.q;
+        const uint16_t *w = is_v ? nullptr : is_k ? x.k_norm : x.q_norm;
+        int e0[NP], e1[NP];
+        float y0[NP], y1[NP];
+        bool in[NP];
+#pragma unroll
+        for (int j = 0; j < NP; j++) {
+            const int p = lane + 64 * j;
+            in[j] = p < hd / 2;
+            const bool apart = p < half && !x.interleaved;
+            e0[j] = apart ? p : 2 * p;
+            e1[j] = apart ? p + half : 2 * p + 1;
+            y0[j] = in[j] ? act_at<BF16>(from, at + e0[j]) : 0.0f;
+            y1[j] = in[j] ? act_at<BF16>(from, at + e1[j]) : 0.0f;
+        }
+        if (w) {
+            double ss = 0.0;
+#pragma unroll
+            for (int j = 0; j < NP; j++)
+                ss = fma((double)y1[j], (double)y1[j], fma((double)y0[j], (double)y0[j], ss));
+            const double s = 1.0 / sqrt(wave_sum_d(ss) / hd + (double)x.eps);
+#pragma unroll
+            for (int j = 0; j < NP; j++)
+                if (in[j]) {
+                    y0[j] = (float)((double)y0[j] * s * (double)bf16_to_f32(w[e0[j]]));
+                    y1[j] = (float)((double)y1[j] * s * (double)bf16_to_f32(w[e1[j]]));
+                }
+        }
+        const int pos = x.positions ? x.positions[tok] : lo + i;
+        if (!is_v && pos >= 0 && pos < x.rope_len)
+#pragma unroll
+            for (int j = 0; j < NP; j++) {
+                const int p = lane + 64 * j;
+                if (p < half) {
+                    const float cs = x.cos_t[(size_t)pos * half + p], sn = x.sin_t[(size_t)pos * half + p];
+                    const float z0 = __fmaf_rn(y0[j], cs, -(y1[j] * sn)), z1 = __fmaf_rn(y0[j], sn, y1[j] * cs);
+                    y0[j] = z0;
+                    y1[j] = z1;
+                }
+            }
+        if (!is_v && !is_k) {
+            const size_t to = tok * x.q_out_stride + (size_t)(h * G + kind) * hd;
+#pragma unroll
+            for (int j = 0; j < NP; j++)
+                if (in[j]) {
+                    if (BF16) {
+                        ((uint16_t *)x.q_out)[to + e0[j]] = f32_to_bf16(y0[j]);
+                        ((uint16_t *)x.q_out)[to + e1[j]] = f32_to_bf16(y1[j]);
+                    } else {
+                        ((float *)x.q_out)[to + e0[j]] = y0[j];
+                        ((float *)x.q_out)[to + e1[j]] = y1[j];
+                    }
+                }
+            continue;
+        }
+        const size_t head = (size_t)phys * P.n_kv + h;
+        const int off = off0 + i;
+        if constexpr (KV8) {
+            float m = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NP; j++)
+                m = fmaxf(m, fmaxf(fabsf(y0[j]), fabsf(y1[j])));
+            m = wave_top(m);
+            const float sc = m > 0.0f ? m / 127.0f : 1.0f, inv = m > 0.0f ? 127.0f / m : 1.0f;
+            int8_t *to = (int8_t *)(is_k ? P.k : P.v) + (head * kPage + off) * hd;
+#pragma unroll
+            for (int j = 0; j < NP; j++)
+                if (in[j]) {
+                    const int c0 = (int)roundf(y0[j] * inv), c1 = (int)roundf(y1[j] * inv);
+                    to[e0[j]] = (int8_t)max(min(c0, 127), -127);
+                    to[e1[j]] = (int8_t)max(min(c1, 127), -127);
+                }
+            if (lane == 0)
+                (is_k ? P.k_scale : P.v_scale)[head * kPage + off] = sc;
+        } else {
+            // (V pages are [dim][16 tokens])
+            uint16_t *to = is_k ? (uint16_t *)P.k + (head * kPage + off) * hd : (uint16_t *)P.v + head * kPage * hd + off;
+            const int step = is_k ? 1 : kPage;
+#pragma unroll
+            for (int j = 0; j < NP; j++)
+                if (in[j]) {
+                    to[e0[j] * step] = f32_to_bf16(y0[j]);
+                    to[e1[j] * step] = f32_to_bf16(y1[j]);
+                }
+        }
+    }
+    if (h == 0 && off0 + T == kPage) {
+        __syncthreads();                   // the page's rows are in memory
+        seal_page<!KV8>(P.k, P.k_scale, P.centroid, P.page_hash + (size_t)u.slot * P.max_logical + blk, phys, P.hpT, P.n_kv, hd, c);
+    }
+}
+
+// Pieces of a launch of be42_kv_accept, the same for each of its layers; tokens to
+// take, and the physical page of every page touched, layer after layer.
+constexpr int kTakes = 64, kTaken = 256, kTakePages = 352;
+struct TakeArgs {
+    int n, n_pages, layer0, from_step, to_step;
+    struct {
+        int from, slot, pos0, n, tok0, page0;
+    } piece[kTakes];
+    int index[kTaken];
+    int pages[kTakePages];
+};
+
+template <bool KV8>
+__global__ __launch_bounds__(256) void k_kv_accept(const be42_kv_pool P, const TakeArgs a)
+{
+    __shared__ float c[256];
+    const int h = blockIdx.y, layer = blockIdx.z, hd = P.head_dim;
+    const auto &u = a.piece[piece_of(a, blockIdx.x)];
+    const int from = u.from + (a.layer0 + layer) * a.from_step, slot = u.slot + (a.layer0 + layer) * a.to_step;
+    const int blk = u.pos0 / kPage + ((int)blockIdx.x - u.page0);
+    const int entry = a.pages[layer * a.n_pages + blockIdx.x], phys = entry & ~kNewPage;
+    const int lo = max(u.pos0, blk * kPage), T = min(u.pos0 + u.n, (blk + 1) * kPage) - lo;
+    const int off0 = lo - blk * kPage;
+    if (h == 0 && threadIdx.x == 0)
+        publish(P, slot, u.pos0, u.n, blk, phys, entry & kNewPage);
+    const size_t head = (size_t)phys * P.n_kv + h;
+    for (int i = 0; i < T; i++) {
+        const int src = a.index[u.tok0 + lo - u.pos0 + i], off = off0 + i;
+        const int page = min(max(P.page_table[(size_t)from * P.max_logical + src / kPage], 0), P.capacity - 1);
+        const size_t sh = (size_t)page * P.n_kv + h;
+        const int so = src % kPage;
+        for (int d = threadIdx.x; d < hd; d += 256) {
+            if constexpr (KV8) {
+                ((int8_t *)P.k)[(head * kPage + off) * hd + d] = ((const int8_t *)P.k)[(sh * kPage + so) * hd + d];
+                ((int8_t *)P.v)[(head * kPage + off) * hd + d] = ((const int8_t *)P.v)[(sh * kPage + so) * hd + d];
+            } else {
+                ((uint16_t *)P.k)[(head * kPage + off) * hd + d] = ((const uint16_t *)P.k)[(sh * kPage + so) * hd + d];
+                ((uint16_t *)P.v)[(head * hd + d) * kPage + off] = ((const uint16_t *)P.v)[(sh * hd + d) * kPage + so];
+            }
+        }
+        if (KV8 && threadIdx.x == 0) {
+            P.k_scale[head * kPage + off] = P.k_scale[sh * kPage + so];
+            P.v_scale[head * kPage + off] = P.v_scale[sh * kPage + so];
+        }
+    }
+    if (h == 0 && off0 + T == kPage) {
+        __syncthreads();                   // the page's rows are in memory
+        seal_page<!KV8>(P.k, P.k_scale, P.centroid, P.page_hash + (size_t)slot * P.max_logical + blk, phys, P.hpT, P.n_kv, hd, c);
+    }
+}
+
+static int rope_append(be42_kv_pool *pool, const be42_kv_run *runs, int n_runs, const RopeIn &x, bool bf16, hipStream_t s)
+{
+    be42_kv_pool &P = *pool;
+    std::vector<int> pages;
+    const int rc = plan_runs(pool, "be42_rope_append", runs, n_runs, nullptr, pages);
+    if (rc)
+        return rc;
+    RopeArgs a;
+    a.n = a.n_pages = 0;
+    auto launch = [&]() {
+        auto go = [&](auto kv8, auto act, auto np) {
+            hipLaunchKernelGGL((k_rope_append<decltype(kv8)::value, decltype(act)::value, decltype(np)::value>),
+                               dim3(a.n_pages, P.n_kv), dim3(256), 0, s, P, a, x);
+        };
+        auto of_dim = [&](auto kv8, auto act) {
+            P.head_dim > 128 ? go(kv8, act, std::integral_constant<int, 2>()) : go(kv8, act, std::integral_constant<int, 1>());
+        };
+        auto of_kind = [&](auto act) { P.kind == BE42_KV_INT8 ? of_dim(std::true_type(), act) : of_dim(std::false_type(), act); };
+        bf16 ? of_kind(std::true_type()) : of_kind(std::false_type());
+        a.n = a.n_pages = 0;
+    };
+    size_t at = 0;
+    int tok = 0;
+    for (int r = 0; r < n_runs; r++) {
+        int pos = runs[r].pos0, left = runs[r].count;
+        while (left) {
+            // as many of its pages as the launch has room for
+            const int want = (pos + left - 1) / kPage - pos / kPage + 1, take = std::min(want, kPiecePages - a.n_pages);
+            if (a.n == kPieces || !take) {
+                launch();
+                continue;
+            }
+            const int n = std::min(left, (pos / kPage + take) * kPage - pos);
+            a.piece[a.n++] = {runs[r].slot, pos, n, tok, a.n_pages};
+            std::copy_n(pages.begin() + at, take, a.pages + a.n_pages);
+            a.n_pages += take;
+            at += take;
+            pos += n;
+            tok += n;
+            left -= n;
+        }
+    }
+    if (a.n)
+        launch();
+    BE42_LAUNCH_CHECK();
+    return BE42_OK;
+}
+
+static int kv_accept(be42_kv_pool *pool, const be42_kv_take *runs, int n_runs, const int *index, int n_layers,
+                     int from_step, int to_step, hipStream_t s)
+{
+    be42_kv_pool &P = *pool;
+    std::vector<be42_kv_run> all;
+    std::vector<int> from, pages;
+    for (int l = 0; l < n_layers; l++)
+        for (int r = 0; r < n_runs; r++) {
+            const long a = runs[r].from + (long)l * from_step, b = runs[r].to + (long)l * to_step;
+            BE42_CHECK(a >= 0 && a < P.n_layers && b >= 0 && b < P.n_layers, "be42_kv_accept: slot %ld or %ld out of range", a, b);
+            from.push_back((int)a);
+            all.push_back({(int)b, runs[r].pos0, runs[r].count});
+            BE42_CHECK(runs[r].count >= 0, "be42_kv_accept: positions %d .. of %d tokens", runs[r].pos0, runs[r].count);
+        }
+    size_t at = 0;
+    for (int r = 0; r < n_runs; r++)
+        for (int i = 0; i < runs[r].count; i++, at++)
+            for (int l = 0; l < n_layers; l++)
+                BE42_CHECK(index[at] >= 0 && index[at] / kPage < slot_pages(pool, from[l * n_runs + r]),
+                           "be42_kv_accept: token %d of slot %d, which has %d pages", index[at], from[l * n_runs + r],
+                           slot_pages(pool, from[l * n_runs + r]));
+    const int rc = plan_runs(pool, "be42_kv_accept", all.data(), (int)all.size(), from.data(), pages);
+    if (rc)
+        return rc;
+    const size_t per_layer = pages.size() / n_layers;        // positions are every layer's
+    TakeArgs a;
+    a.from_step = from_step;
+    a.to_step = to_step;
+    a.n = a.n_pages = 0;
+    size_t first = 0;                                        // of the pages of a layer
+    int toks = 0;
+    auto launch = [&]() {
+        const int most = kTakePages / a.n_pages;
+        for (int l = 0; l < n_layers; l += most) {
+            const int n = std::min(most, n_layers - l);
+            a.layer0 = l;
+            for (int i = 0; i < n; i++)
+                std::copy_n(pages.begin() + (l + i) * per_layer + first, a.n_pages, a.pages + i * a.n_pages);
+            const dim3 g(a.n_pages, P.n_kv, n);
+            if (P.kind == BE42_KV_INT8)
+                hipLaunchKernelGGL(k_kv_accept<true>, g, dim3(256), 0, s, P, a);
+            else
+                hipLaunchKernelGGL(k_kv_accept<false>, g, dim3(256), 0, s, P, a);
+        }
+        first += a.n_pages;
+        a.n = a.n_pages = toks = 0;
+    };
+    at = 0;
+    for (int r = 0; r < n_runs; r++) {
+        int pos = runs[r].pos0, left = runs[r].count;
+        while (left) {
+            if (a.n == kTakes || toks == kTaken || a.n_pages == kTakePages) {
+                launch();
+                continue;
+            }
+            // as many tokens and pages as the launch has room for
+            int n = std::min(left, kTaken - toks);
+            n = std::min(n, (pos / kPage + kTakePages - a.n_pages) * kPage - pos);
+            // a piece ends with a page or with its run
+            const int np = (pos + n - 1) / kPage - pos / kPage + 1;
+            if (n < left)
+                n = np > 1 || (pos + n) % kPage == 0 ? (pos + n) / kPage * kPage - pos : 0;
+            if (!n) {
+                launch();
+                continue;
+            }
+            a.piece[a.n++] = {runs[r].from, runs[r].to, pos, n, toks, a.n_pages};
+            std::copy_n(index + at, n, a.index + toks);
+            a.n_pages += (pos + n - 1) / kPage - pos / kPage + 1;
+            toks += n;
+            at += n;
+            pos += n;
+            left -= n;
+        }
+    }
+    if (a.n)
+        launch();
+    BE42_LAUNCH_CHECK();
+    return BE42_OK;
+}
+
+}  // namespace be42
+
+using namespace be42;
+
+extern "C" int be42_rope_append(be42_kv_pool *pool, const be42_kv_run *runs, int n_runs, const void *q, int q_stride,
+                                int n_heads, const void *k, int k_stride, const void *v, int v_stride, int act_bf16,
+                                const uint16_t *q_norm, const uint16_t *k_norm, float eps, const be42_rope *rope,
+                                const int *positions, void *q_out, int q_out_stride, void *stream)
+{
+    BE42_CHECK(pool && (n_runs == 0 || runs), "be42_rope_append: null pointer");
+    const be42_kv_pool &P = *pool;
+    BE42_CHECK(n_runs >= 0, "be42_rope_append: %d runs", n_runs);
+    long tokens = 0;
+    for (int r = 0; r < n_runs; r++)
+        tokens += std::max(runs[r].count, 0);
+    BE42_CHECK(tokens == 0 || (k && v), "be42_rope_append: null pointer");
+    BE42_CHECK(tokens < 1L << 31, "be42_rope_append: %ld tokens", tokens);
+    BE42_CHECK(n_heads >= 0 && n_heads % P.n_kv == 0 && (!tokens || (n_heads == 0) == (q == nullptr)),
+               "be42_rope_append: %d query heads over %d kv heads", n_heads, P.n_kv);
+    BE42_CHECK(!q || q_out, "be42_rope_append: null q_out");
+    const long row = (long)P.n_kv * P.head_dim, qrow = (long)n_heads * P.head_dim;
+    BE42_CHECK(k_stride >= row && v_stride >= row && (!q || (q_stride >= qrow && q_out_stride >= qrow)),
+               "be42_rope_append: strides %d, %d, %d, %d of rows of %ld and %ld", q_stride, k_stride, v_stride,
+               q_out_stride, qrow, row);
+    BE42_CHECK(!q || q != q_out || q_stride == q_out_stride, "be42_rope_append: q in place at strides %d and %d",
+               q_stride, q_out_stride);
+    BE42_CHECK((!q_norm && !k_norm) || (eps >= 0.0f && eps < INFINITY), "be42_rope_append: eps %g", (double)eps);
+    BE42_CHECK(!rope || (rope->len >= 0 && rope->dim >= 0 && rope->dim % 2 == 0 && rope->dim <= P.head_dim),
+               "be42_rope_append: a rope of %d positions, %d elements (head_dim %d)", rope->len, rope->dim, P.head_dim);
+    BE42_CHECK(!rope || !rope->len || !rope->dim || (rope->cos && rope->sin), "be42_rope_append: null table");
+    BE42_CHECK(!(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out) & (act_bf16 ? 1 : 3)) &&
+                   !(((uintptr_t)q_norm | (uintptr_t)k_norm) & 1) && !((uintptr_t)positions & 3) &&
+                   (!rope || !(((uintptr_t)rope->cos | (uintptr_t)rope->sin) & 3)),
+               "be42_rope_append: unaligned pointer");
+    const RopeIn x = {q, k, v, q_out, q_norm, k_norm, rope ? rope->cos : nullptr, rope ? rope->sin : nullptr, positions,
+                      (size_t)q_stride, (size_t)k_stride, (size_t)v_stride, (size_t)q_out_stride, n_heads,
+                      rope ? rope->len : 0, rope ? rope->dim : 0, rope ? rope->interleaved : 0, eps};
+    try {
+        return rope_append(pool, runs, n_runs, x, act_bf16, as_stream(stream));
+    } catch (const std::bad_alloc &) {
+        set_error("be42_rope_append: out of host memory");
+        return BE42_ENOMEM;
+    }
+}
+
+extern "C" int be42_kv_accept(be42_kv_pool *pool, const be42_kv_take *runs, int n_runs, const int *index, int n_layers,
+                              int from_step, int to_step, void *stream)
+{
+    BE42_CHECK(pool && (n_runs == 0 || (runs && index)), "be42_kv_accept: null pointer");
+    BE42_CHECK(n_runs >= 0 && n_layers >= 0 && (long)n_runs * n_layers <= pool->n_layers,
+               "be42_kv_accept: %d runs of %d layers over %d slots", n_runs, n_layers, pool->n_layers);
+    if (!n_runs || !n_layers)
+        return BE42_OK;
+    try {
+        return kv_accept(pool, runs, n_runs, index, n_layers, from_step, to_step, as_stream(stream));
+    } catch (const std::bad_alloc &) {
+        set_error("be42_kv_accept: out of host memory");
+        return BE42_ENOMEM;
+    }
+}

@@ -10,8 +10,8 @@
  * One stream at a time per device: the library keeps one grow-only workspace,
  * one split-K partial-sum buffer and the exchange buffers of the split route +
  * attention per process (used by the GEMVs, by be42_paged_attention,
- * be42_lsh_attention, be42_prefix_attention and be42_logprobs without a caller
- * workspace, by be42_lsh_attention and the
+ * be42_lsh_attention, be42_prefix_attention, be42_tree_attention,
+ * be42_linear_fp8_block and be42_logprobs without a caller workspace, by be42_lsh_attention and the
  * decoder when at most 64 (query, KV head) pairs are split over several
  * workgroups each, and by the decoder's fallback paths), so calls that use
  * them must not run concurrently on two streams.  Calls on one stream are
@@ -74,6 +74,13 @@ int be42_norm_quant_rows_int8(int8_t *q, float *scales, void *sum, const void *x
 int be42_norm_quant_rows_fp8(uint8_t *q, float *scales, void *sum, const void *x, int x_stride,
                              const void *residual, int residual_stride, int act_bf16, const uint16_t *w, int rows,
                              int cols, float eps, void *stream);
+/* E4M3 codes with one scale for 128 elements of a row, the last of a row for what is
+ * left: codes [rows][cols] and scales [rows][blocks], blocks = ceil(cols / 128), as
+ * be42_quant_rows_fp8 gives them for each group, bit for bit.  x is fp32 or (x_bf16)
+ * bf16, row r from element r * x_stride on.  A group that holds an infinity or a NaN
+ * gets unspecified codes and scale. */
+int be42_quant_blocks_fp8(uint8_t *q, float *scales, const void *x, int x_bf16, int x_stride, int rows, int cols,
+                          void *stream);
 /* (float)q * scale[row], dequant_int8_to_f32_avx2 (ops_quant.c:275-305) row-wise */
 int be42_dequant_rows_int8(float *out, const int8_t *q, const float *scales, int rows, int cols,
                            void *stream);
@@ -160,6 +167,29 @@ int    be42_gemm_fp8_prepared(float *y, const uint8_t *w, const float *w_scale, 
 int    be42_gemm_prepared_multi(const be42_gemv_seg *segs, int nseg, const void *xdig, int k, int m, int fp8,
                                 void *stream);
 
+/* E4M3 products with block scales: activations in codes xq [m][k] with scales sx
+ * [m][blocks], one for 128 elements of a row (be42_quant_blocks_fp8), weights wq
+ * [n][k] with scales sw [ceil(n / 128)][blocks], one for 128 x 128, blocks =
+ * ceil(k / 128); the last block of either may be short.
+ *   y[m][n] = sum_b sx[m][b] * sw[n / 128][b] * sum_{k in block b} xq[m][k] * wq[n][k]
+ * y [m][n] is fp32, or bf16 with y_bf16.  Sums are fp32; for fp32 outputs the codes
+ * go through the bf16 matrix cores (exact), for bf16 ones through the 8-bit ones,
+ * whose sums keep about 16 bits.  Codes are E4M3 (bias 7); 0x7F and 0xFF, which the
+ * codecs never give, are NaN.  k % 16 == 0; xq, wq and y 16-byte aligned.  A NaN or
+ * an infinity among the scales reaches the outputs of its rows only. */
+int    be42_gemm_fp8_block(void *y, int y_bf16, const uint8_t *xq, const float *sx, const uint8_t *wq, const float *sw,
+                           int m, int n, int k, void *stream);
+/* The same for activations x [m][k], fp32 or (x_bf16) bf16, row r from element r *
+ * x_stride on: their codes and scales are those of be42_quant_blocks_fp8.  y
+ * overlaps no input.  workspace NULL: the library's (grow-only; refused while the
+ * stream is captured), else a device buffer of
+ * be42_linear_fp8_block_workspace_bytes() bytes, 16-byte aligned, that no call on
+ * another stream uses meanwhile. */
+size_t be42_linear_fp8_block_workspace_bytes(int m, int n, int k);
+int    be42_linear_fp8_block(void *y, int y_bf16, const void *x, int x_bf16, int x_stride, const uint8_t *wq,
+                             const float *sw, int m, int n, int k, void *workspace, size_t workspace_bytes,
+                             void *stream);
+
 /* ---- paged KV cache in HBM ------------------------------------------------------
  * Mirrors t_block_manager / t_paged_kv_cache (src/memory/paged.h:53-99): pages
  * of 16 tokens, [n_kv][16][head_dim] per page, INT8 codes with a per-(token,
@@ -212,6 +242,48 @@ int  be42_kv_layer_pages(const be42_kv_pool *pool, int layer, int *phys_out, int
  * [n][n_kv * head_dim]: the per-step append of a decode batch in one launch. */
 int  be42_kv_append_step(be42_kv_pool *pool, const int *slots, const int *pos, int n, const float *k,
                          const float *v, void *stream);
+/* Tokens of a q/k/v product -> rotated queries, and K and V in the pages, in one
+ * pass.  The tokens are those of n_runs runs, one after the other: run r is
+ * runs[r].count tokens at positions runs[r].pos0 .. of slot runs[r].slot (host
+ * array; a slot at most once a call; positions as be42_kv_append takes them).  Row
+ * t of q, k and v begins at element t * its stride and holds n_heads, n_kv, n_kv
+ * heads of head_dim, fp32 or (act_bf16) bf16.  For each head of q and k:
+ *   x = row; with a weight q_norm / k_norm [head_dim] bf16 (NULL: none)
+ *     x = fp32(x / sqrt(mean(x^2) + eps) * w), formed in 64 bits and rounded once;
+ *   with a rope and position p = positions[t] (device, NULL: the token's own)
+ *     in [0, len): the pairs (i, i + dim / 2), or (2 i, 2 i + 1) if interleaved, of
+ *     the first dim elements become x0 c - x1 s, x0 s + x1 c, c = cos[p][i], s =
+ *     sin[p][i], in fp32 as the decode step rotates; other positions' rows stay.
+ * q goes to q_out (rows q_out_stride apart, in q's type; it may be q itself at its
+ * stride, and overlaps no input otherwise); k and v into the pages as
+ * be42_kv_append stores fp32 rows.  A page whose last position is written gets its
+ * centroid and hash, also where it had some.  q NULL: no queries (n_heads 0).  A
+ * token whose row holds an infinity or NaN gets unspecified q and page rows; others
+ * are not touched by it.  On an error nothing was appended. */
+typedef struct be42_kv_run {
+    int slot, pos0, count;
+} be42_kv_run;
+typedef struct be42_rope {
+    const float *cos, *sin;    /* device [len][dim / 2] */
+    int len, dim, interleaved; /* dim: even, at most head_dim */
+} be42_rope;
+int  be42_rope_append(be42_kv_pool *pool, const be42_kv_run *runs, int n_runs, const void *q, int q_stride,
+                      int n_heads, const void *k, int k_stride, const void *v, int v_stride, int act_bf16,
+                      const uint16_t *q_norm, const uint16_t *k_norm, float eps, const be42_rope *rope,
+                      const int *positions, void *q_out, int q_out_stride, void *stream);
+/* Tokens that one slot holds, behind what another holds: the drafts of a tree that
+ * were right, from the drafts' slot to their sequence's.  Run r puts runs[r].count
+ * tokens at positions runs[r].pos0 .. of slot runs[r].to: tokens index[..] of slot
+ * runs[r].from (host array, the runs' one after the other), as the pages hold them,
+ * bit for bit.  The same for each of n_layers layers: layer l takes slots from + l *
+ * from_step and to + l * to_step.  A slot is filled at most once a call, and none
+ * that is read from.  Pages that fill get their centroid and hash.  On an error
+ * nothing was copied. */
+typedef struct be42_kv_take {
+    int from, to, pos0, count;
+} be42_kv_take;
+int  be42_kv_accept(be42_kv_pool *pool, const be42_kv_take *runs, int n_runs, const int *index, int n_layers,
+                    int from_step, int to_step, void *stream);
 int  be42_kv_page_alloc(be42_kv_pool *pool);
 int  be42_kv_page_free(be42_kv_pool *pool, int phys);
 int  be42_kv_export(const be42_kv_pool *pool, int *page_table, int *free_stack, int *free_top,
@@ -302,6 +374,31 @@ int    be42_prefix_attention(const be42_kv_pool *pool, const void *q, int q_bf16
                              int n_heads, int prefix_slot, int prefix_len, const int *slots, const int *lens,
                              int max_len, float scale, void *out, void *workspace, size_t workspace_bytes,
                              void *stream);
+
+/* Attention of trees of drafted tokens: n_trees trees, tree b the tokens starts[b] ..
+ * starts[b + 1] - 1 (device [n_trees + 1], ascending), at most max_tree <= 256 of
+ * them.  Token i is row i of q [n_heads][head_dim] (at element i * q_stride) and
+ * token i of slot draft_slot, where its K and V are.  It sees the first lens[b]
+ * tokens of slot slots[b] (NULL: slot b / all that the slot holds), itself, and what
+ * lies above it: parents[i] (device, counted within the tree; -1: none) is the draft
+ * it follows, always an earlier one (else it counts as none).  parents NULL: each
+ * follows the one before it.
+ *   out[i][h] = sum_t softmax_t(scale * q[i][h] . k_t) v_t
+ * as be42_prefix_attention forms it: its types, head dims, page kinds, group sizes
+ * and scales, its precision, zeros for a row that sees nothing.  An infinity or NaN in
+ * a draft's K or V reaches only the drafts that see it.
+ * max_len bounds lens: a context's tokens from max_len on are not seen.  Slots are
+ * read up to what they hold.  out rows of tokens that are in no tree, or past
+ * max_tree in theirs, are left as they were.  The launch depends on n_tokens,
+ * n_trees, max_tree and max_len alone, so trees, slots and lens may change between
+ * replays of a captured graph.  out overlaps no input.
+ * workspace as for be42_prefix_attention. */
+size_t be42_tree_attention_workspace_bytes(int n_tokens, int n_trees, int n_heads, int n_kv, int head_dim, int max_tree,
+                                           int max_len);
+int    be42_tree_attention(const be42_kv_pool *pool, const void *q, int q_bf16, int q_stride, int n_tokens, int n_heads,
+                           const int *starts, int n_trees, int max_tree, const int *parents, int draft_slot,
+                           const int *slots, const int *lens, int max_len, float scale, void *out, void *workspace,
+                           size_t workspace_bytes, void *stream);
 
 /* ---- linear (non-paged) bf16 KV cache -----------------------------------------------
  * The cache layout of kv_cache.h:19-27: rows [T][n_kv][head_dim] bf16.

@@ -40,8 +40,9 @@ SIGNATURES = {
     "be42_prefix_attention_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32]),
     "be42_prefix_attention": (i32, [vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, i32, f32, vp, vp, sz, vp]),
     "be42_quant_blocks_fp8": (i32, [vp, vp, vp, i32, i32, i32, i32, vp]),
-    "be42_gemm_fp8_block": (i32, [vp, i32, vp, vp, vp, vp, i32, i32, i32, vp]),
-    "be42_linear_fp8_block_workspace_bytes": (sz, [i32, i32, i32]),
+    "be42_gemm_fp8_block_workspace_bytes": (sz, [i32, i32, i32, i32]),
+    "be42_gemm_fp8_block": (i32, [vp, i32, vp, vp, vp, vp, i32, i32, i32, vp, sz, vp]),
+    "be42_linear_fp8_block_workspace_bytes": (sz, [i32, i32, i32, i32]),
     "be42_linear_fp8_block": (i32, [vp, i32, vp, i32, i32, vp, vp, i32, i32, i32, vp, sz, vp]),
     "be42_rope_append": (i32, [vp, vp, i32, vp, i32, i32, vp, i32, vp, i32, i32, vp, vp, f32, vp, vp, vp, i32, vp]),
     "be42_kv_accept": (i32, [vp, vp, i32, vp, i32, i32, i32, vp]),
@@ -174,6 +175,7 @@ class Lib:
         self._inited = False
         self._prefix_bytes = functools.lru_cache(4096)(self.lib.be42_prefix_attention_workspace_bytes)
         self._tree_bytes = functools.lru_cache(4096)(self.lib.be42_tree_attention_workspace_bytes)
+        self._block_bytes = functools.lru_cache(4096)(self.lib.be42_gemm_fp8_block_workspace_bytes)
         self._linear_bytes = functools.lru_cache(4096)(self.lib.be42_linear_fp8_block_workspace_bytes)
         self._logprobs_bytes = functools.lru_cache(4096)(self.lib.be42_logprobs_workspace_bytes)
 
@@ -439,10 +441,12 @@ class Lib:
             self._want(name, "out", out, (dtype,), (m, n), dev)
         return n, out, dtype == t.bfloat16
 
-    def gemm_fp8_block(self, xq, sx, wq, sw, dtype=None, out=None):
+    def gemm_fp8_block(self, xq, sx, wq, sw, dtype=None, out=None, workspace=None):
         """Y [m][n] (float32 or bfloat16) = codes xq [m][k] with scales sx
         [m][k / 128] x codes wq [n][k] with scales sw [n / 128][k / 128], the
-        last blocks short where 128 does not divide (quant_blocks_fp8)."""
+        last blocks short where 128 does not divide (quant_blocks_fp8).
+        workspace: be42_gemm_fp8_block_workspace_bytes bytes (uint8) to use
+        instead of a new tensor."""
         t, name = self.torch, "be42_gemm_fp8_block"
         if xq.dim() != 2:
             raise Be42Error(f"{name}: codes have shape {tuple(xq.shape)}")
@@ -450,7 +454,9 @@ class Lib:
         self._want(name, "codes", xq, (t.uint8,))
         self._want(name, "scales", sx, (t.float32,), (m, -(-k // 128)), xq.device)
         n, out, yb = self._block_operands(name, m, k, wq, sw, dtype, out, xq.device)
-        self._device_call(xq, name, out.data_ptr(), yb, xq.data_ptr(), sx.data_ptr(), wq.data_ptr(), sw.data_ptr(), m, n, k)
+        ws, size = self._workspace(name, workspace, xq.device, self._block_bytes, m, n, k, yb)
+        self._device_call(xq, name, out.data_ptr(), yb, xq.data_ptr(), sx.data_ptr(), wq.data_ptr(), sw.data_ptr(), m, n, k,
+                          None if ws is None else ws.data_ptr(), size)
         return out
 
     def linear_fp8_block(self, x, wq, sw, dtype=None, out=None, workspace=None):
@@ -463,7 +469,7 @@ class Lib:
         m, k = x.shape
         dev = x.device
         n, out, yb = self._block_operands(name, m, k, wq, sw, dtype, out, dev)
-        ws, size = self._workspace(name, workspace, dev, self._linear_bytes, m, n, k)
+        ws, size = self._workspace(name, workspace, dev, self._linear_bytes, m, n, k, yb)
         self._device_call(x, name, out.data_ptr(), yb, x.data_ptr(), x.dtype == t.bfloat16, xs, wq.data_ptr(), sw.data_ptr(),
                           m, n, k, None if ws is None else ws.data_ptr(), size)
         return out

@@ -1,0 +1,60 @@
+// fp8_codec.h -- the reference's E4M3 encoder, for the kernels of quant.hip and
+// block.hip.
+#pragma once
+
+#include "be42_common.h"
+
+namespace be42 {
+
+// Thresholds of its exponent (quant.hip uploads each source file's copy).
+static __constant__ float c_fp8_thr[kFp8ThrN];
+
+// Reference E4M3 encoder (ops_quant.c:68-98) on the device.
+__device__ __forceinline__ uint8_t f32_to_fp8(float v)
+{
+    if (v == 0.0f)
+        return 0;
+    const uint32_t sign = v < 0.0f ? 0x80u : 0u;
+    float a = fabsf(v);
+    if (a > 448.0f)
+        a = 448.0f;
+    int ex = (int)((__float_as_uint(a) >> 23) & 0xFF) - 127;   // floor(log2 a), a normal
+    if ((__float_as_uint(a) >> 23) == 0)
+        ex = -127;                                            // subnormal: far below e = 0
+    const int up = ex + 1;
+    // a threshold lies at most 64 ulps below its power of two
+    // (host_fp8_thresholds), so the table is read for such values only
+    if ((__float_as_uint(a) & 0x7FFFFFu) >= 0x7FFFC0u && up >= kFp8ThrE0 && up < kFp8ThrE0 + kFp8ThrN &&
+        a >= c_fp8_thr[up - kFp8ThrE0])
+        ex = up;                                              // log2f rounded up to an integer
+    int e = ex + 7;
+    e = e < 0 ? 0 : (e > 15 ? 15 : e);
+    const float frac = (e == 0) ? a * 64.0f
+                                : a * __uint_as_float((uint32_t)(127 + 7 - e) << 23) - 1.0f;
+    int m = (int)__fmaf_rn(frac, 8.0f, 0.5f);
+    if (m > 7)
+        m = 7;
+    return (uint8_t)(sign | ((uint32_t)e << 3) | (uint32_t)m);
+}
+
+// f32_to_fp8 of a finite value in half the instructions: the kept mantissa bits
+// are counted up by the next bit unless they are all ones (8 frac + 0.5 is exact
+// in fp32, so its integer part is that).  Compared with it over all fp32 values;
+// the pass over 300 x 14336 fp32 15.3 -> 14.7 us.
+__device__ __forceinline__ uint8_t finite_to_fp8(float v)
+{
+    const float a = fminf(fabsf(v), 448.0f);
+    const uint32_t u = __float_as_uint(a);
+    int ex = (int)(u >> 23) - 127;
+    uint32_t c = (u >> 20) - ((127u - 7u) << 3) + ((u & 0x700000u) != 0x700000u ? u >> 19 & 1u : 0u);
+    if ((u & 0x7FFFFFu) >= 0x7FFFC0u && ex + 1 >= kFp8ThrE0 && ex + 1 < kFp8ThrE0 + kFp8ThrN &&
+        a >= c_fp8_thr[ex + 1 - kFp8ThrE0]) {
+        ex++;                                              // log2f rounded up to an integer
+        c = (uint32_t)(ex + 7) << 3;
+    }
+    if (ex < -6)                                           // multiples of 2^-9
+        c = (uint32_t)min((int)__fmaf_rn(a, 512.0f, 0.5f), 7);
+    return (uint8_t)(a == 0.0f ? 0u : c | (__float_as_uint(v) >> 24 & 0x80u));
+}
+
+}  // namespace be42

@@ -14,58 +14,9 @@
 #include <type_traits>
 
 #include "be42_common.h"
+#include "fp8_codec.h"
 
 namespace be42 {
-
-__constant__ float c_fp8_thr[kFp8ThrN];
-
-// Reference E4M3 encoder (ops_quant.c:68-98) on the device.
-__device__ __forceinline__ uint8_t f32_to_fp8(float v)
-{
-    if (v == 0.0f)
-        return 0;
-    const uint32_t sign = v < 0.0f ? 0x80u : 0u;
-    float a = fabsf(v);
-    if (a > 448.0f)
-        a = 448.0f;
-    int ex = (int)((__float_as_uint(a) >> 23) & 0xFF) - 127;   // floor(log2 a), a normal
-    if ((__float_as_uint(a) >> 23) == 0)
-        ex = -127;                                            // subnormal: far below e = 0
-    const int up = ex + 1;
-    // a threshold lies at most 64 ulps below its power of two
-    // (host_fp8_thresholds), so the table is read for such values only
-    if ((__float_as_uint(a) & 0x7FFFFFu) >= 0x7FFFC0u && up >= kFp8ThrE0 && up < kFp8ThrE0 + kFp8ThrN &&
-        a >= c_fp8_thr[up - kFp8ThrE0])
-        ex = up;                                              // log2f rounded up to an integer
-    int e = ex + 7;
-    e = e < 0 ? 0 : (e > 15 ? 15 : e);
-    const float frac = (e == 0) ? a * 64.0f
-                                : a * __uint_as_float((uint32_t)(127 + 7 - e) << 23) - 1.0f;
-    int m = (int)__fmaf_rn(frac, 8.0f, 0.5f);
-    if (m > 7)
-        m = 7;
-    return (uint8_t)(sign | ((uint32_t)e << 3) | (uint32_t)m);
-}
-
-// f32_to_fp8 of a finite value in half the instructions: the kept mantissa bits
-// are counted up by the next bit unless they are all ones (8 frac + 0.5 is exact
-// in fp32, so its integer part is that).  Compared with it over all fp32 values;
-// the pass over 300 x 14336 fp32 15.3 -> 14.7 us.
-__device__ __forceinline__ uint8_t finite_to_fp8(float v)
-{
-    const float a = fminf(fabsf(v), 448.0f);
-    const uint32_t u = __float_as_uint(a);
-    int ex = (int)(u >> 23) - 127;
-    uint32_t c = (u >> 20) - ((127u - 7u) << 3) + ((u & 0x700000u) != 0x700000u ? u >> 19 & 1u : 0u);
-    if ((u & 0x7FFFFFu) >= 0x7FFFC0u && ex + 1 >= kFp8ThrE0 && ex + 1 < kFp8ThrE0 + kFp8ThrN &&
-        a >= c_fp8_thr[ex + 1 - kFp8ThrE0]) {
-        ex++;                                              // log2f rounded up to an integer
-        c = (uint32_t)(ex + 7) << 3;
-    }
-    if (ex < -6)                                           // multiples of 2^-9
-        c = (uint32_t)min((int)__fmaf_rn(a, 512.0f, 0.5f), 7);
-    return (uint8_t)(a == 0.0f ? 0u : c | (__float_as_uint(v) >> 24 & 0x80u));
-}
 
 // quant_f32_to_int8's code of one element (ops_quant.c:262-267)
 __device__ __forceinline__ int8_t f32_to_int8(float v, float inv)
@@ -195,35 +146,62 @@ static bool launch_quant_vec(uint8_t *q, float *scales, const float *x, int rows
     return true;
 }
 
-// E4M3 codes with a scale for 128 elements of a row (a group of 32 lanes each, four
-// elements a lane): f32_to_fp8 of x / scale, scale = amax / 224, as k_quant_rows_fp8
-// forms them of a row of 128.
-template <bool BF16>
-__global__ __launch_bounds__(256) void k_quant_blocks(uint8_t *q, float *scales, const void *x, size_t x_stride, int rows,
-                                                      int cols, int blocks)
+// E4M3 codes with a scale for 128 elements of a row, a group of lanes each: f32_to_fp8 of
+// x / scale, scale = amax / 224, as k_quant_rows_fp8 forms them of a row of 128.
+// Rows on words of 16 bytes (VE elements) take 128 / VE lanes a block, others an
+// element a load.  Bound by HBM and by the codec's instructions alike: 4096 x 4096
+// bf16 18 us, 2.8 TB/s.
+template <bool BF16, bool WORDS>
+__global__ __launch_bounds__(256) void k_quant_blocks(uint8_t *__restrict__ q, float *__restrict__ scales, const void *__restrict__ x,
+                                                      size_t x_stride, int rows, int cols, int blocks)
 {
-    const size_t at = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    constexpr int VE = WORDS && BF16 ? 8 : 4, L = 128 / VE, PER = 256 / L;
+    const size_t at = (size_t)blockIdx.x * PER + threadIdx.x / L;
     if (at >= (size_t)rows * blocks)
         return;
-    const size_t row = at / blocks;
-    const int b = (int)(at % blocks), c0 = b * 128 + 4 * (threadIdx.x & 31);
-    float v[4], m = 0.0f;
+    const size_t row = at / (unsigned)blocks;
+    const int b = (int)(at - row * blocks), c0 = b * 128 + VE * (threadIdx.x % L);
+    const size_t from = row * x_stride + c0;
+    float v[VE], m = 0.0f;
+    if constexpr (WORDS) {
+        // (the row is a whole number of words: one is in it or behind it)
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (c0 < cols)
+            w = *(const uint4 *)((const char *)x + from * (BF16 ? 2 : 4));
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const size_t i = row * x_stride + c0 + j;
-        v[j] = c0 + j >= cols ? 0.0f : BF16 ? bf16_to_f32(((const uint16_t *)x)[i]) : ((const float *)x)[i];
-        m = fmaxf(m, fabsf(v[j]));
+        for (int j = 0; j < VE; j++)
+            v[j] = BF16 ? __uint_as_float(j & 1 ? u[j / 2] & 0xFFFF0000u : u[j / 2] << 16) : __uint_as_float(u[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < VE; j++)
+            v[j] = c0 + j >= cols ? 0.0f : BF16 ? bf16_to_f32(((const uint16_t *)x)[from + j]) : ((const float *)x)[from + j];
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        m = fmaxf(m, __shfl_xor(m, o, 32));
-    const float scale = m > 0.0f ? m / 224.0f : 1.0f, inv = m > 0.0f ? 1.0f / scale : 1.0f;
-    if ((threadIdx.x & 31) == 0)
-        scales[at] = scale;
+    for (int j = 0; j < VE; j++)
+        m = fmaxf(m, fabsf(v[j]));
 #pragma unroll
-    for (int j = 0; j < 4; j++)
-        if (c0 + j < cols)
-            q[row * cols + c0 + j] = f32_to_fp8(v[j] * inv);
+    for (int o = L / 2; o > 0; o >>= 1)
+        m = fmaxf(m, __shfl_xor(m, o, L));
+    const float scale = m > 0.0f ? m / 224.0f : 1.0f, inv = m > 0.0f ? 1.0f / scale : 1.0f;
+    if (threadIdx.x % L == 0)
+        scales[at] = scale;
+    uint32_t code[VE / 4] = {};
+#pragma unroll
+    for (int j = 0; j < VE; j++)
+        code[j / 4] |= (uint32_t)finite_to_fp8(v[j] * inv) << (8 * (j % 4));
+    uint8_t *to = q + row * cols + c0;
+    if constexpr (WORDS) {
+        if (c0 < cols)
+#pragma unroll
+            for (int j = 0; j < VE / 4; j++)
+                ((uint32_t *)to)[j] = code[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < VE; j++)
+            if (c0 + j < cols)
+                to[j] = (uint8_t)(code[j / 4] >> (8 * (j % 4)));
+    }
 }
 
 // ---- residual + RMS norm + codes -----------------------------------------------
@@ -584,6 +562,8 @@ static void host_fp8_thresholds(float *thr)
 
 static int g_thr_ready[64];
 
+int upload_block_thresholds(const float *thr);     // block.hip
+
 int upload_fp8_thresholds(int device)
 {
     if (device < 0 || device >= 64)
@@ -593,6 +573,8 @@ int upload_fp8_thresholds(int device)
     float thr[kFp8ThrN];
     host_fp8_thresholds(thr);
     BE42_HIP(hipMemcpyToSymbol(HIP_SYMBOL(c_fp8_thr), thr, sizeof thr));
+    if (const int rc = upload_block_thresholds(thr))
+        return rc;
     g_thr_ready[device] = 1;
     return BE42_OK;
 }
@@ -732,13 +714,19 @@ extern "C" int be42_quant_blocks_fp8(uint8_t *q, float *scales, const void *x, i
     BE42_CHECK(!((uintptr_t)x & (x_bf16 ? 1 : 3)) && !((uintptr_t)scales & 3), "be42_quant_blocks_fp8: unaligned pointer");
     if (rows == 0)
         return BE42_OK;
-    const long blocks = ((long)cols + 127) / 128, groups = (rows * blocks + 7) / 8;
+    const int ve = x_bf16 ? 8 : 4;
+    const bool words = cols % ve == 0 && x_stride % ve == 0 && !((uintptr_t)x & 15) && !((uintptr_t)q & 3);
+    const long blocks = ((long)cols + 127) / 128, per = words ? 2 * ve : 8, groups = (rows * blocks + per - 1) / per;
     BE42_CHECK(groups <= kMaxBlocks, "be42_quant_blocks_fp8: %d rows of %d", rows, cols);
-    const dim3 g((unsigned)groups), b(256);
-    if (x_bf16)
-        hipLaunchKernelGGL(k_quant_blocks<true>, g, b, 0, as_stream(stream), q, scales, x, (size_t)x_stride, rows, cols, (int)blocks);
-    else
-        hipLaunchKernelGGL(k_quant_blocks<false>, g, b, 0, as_stream(stream), q, scales, x, (size_t)x_stride, rows, cols, (int)blocks);
+    if (const int rc = ensure_thresholds())
+        return rc;
+    const dim3 g((unsigned)groups), t(256);
+    auto go = [&](auto bf16, auto w) {
+        hipLaunchKernelGGL((k_quant_blocks<decltype(bf16)::value, decltype(w)::value>), g, t, 0, as_stream(stream), q, scales, x,
+                           (size_t)x_stride, rows, cols, (int)blocks);
+    };
+    auto of_type = [&](auto bf16) { words ? go(bf16, std::true_type()) : go(bf16, std::false_type()); };
+    x_bf16 ? of_type(std::true_type()) : of_type(std::false_type());
     BE42_LAUNCH_CHECK();
     return BE42_OK;
 }

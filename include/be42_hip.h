@@ -11,7 +11,8 @@
  * one split-K partial-sum buffer and the exchange buffers of the split route +
  * attention per process (used by the GEMVs, by be42_paged_attention,
  * be42_lsh_attention, be42_prefix_attention, be42_tree_attention,
- * be42_linear_fp8_block and be42_logprobs without a caller workspace, by be42_lsh_attention and the
+ * be42_gemm_fp8_block, be42_linear_fp8_block and be42_logprobs without a caller
+ * workspace, by be42_lsh_attention and the
  * decoder when at most 64 (query, KV head) pairs are split over several
  * workgroups each, and by the decoder's fallback paths), so calls that use
  * them must not run concurrently on two streams.  Calls on one stream are
@@ -175,17 +176,20 @@ int    be42_gemm_prepared_multi(const be42_gemv_seg *segs, int nseg, const void 
  * y [m][n] is fp32, or bf16 with y_bf16.  Sums are fp32; for fp32 outputs the codes
  * go through the bf16 matrix cores (exact), for bf16 ones through the 8-bit ones,
  * whose sums keep about 16 bits.  Codes are E4M3 (bias 7); 0x7F and 0xFF, which the
- * codecs never give, are NaN.  k % 16 == 0; xq, wq and y 16-byte aligned.  A NaN or
- * an infinity among the scales reaches the outputs of its rows only. */
+ * codecs never give, are NaN.  k % 16 == 0, at most 2^22; xq, wq and y 16-byte aligned.
+ * A NaN or an infinity among the scales reaches the outputs of its rows (or features)
+ * only.  workspace NULL: the library's (grow-only; refused while the stream is
+ * captured), else a device buffer of be42_gemm_fp8_block_workspace_bytes() bytes,
+ * 16-byte aligned, that no call on another stream uses meanwhile (16 bytes: these sizes
+ * use none). */
+size_t be42_gemm_fp8_block_workspace_bytes(int m, int n, int k, int y_bf16);
 int    be42_gemm_fp8_block(void *y, int y_bf16, const uint8_t *xq, const float *sx, const uint8_t *wq, const float *sw,
-                           int m, int n, int k, void *stream);
+                           int m, int n, int k, void *workspace, size_t workspace_bytes, void *stream);
 /* The same for activations x [m][k], fp32 or (x_bf16) bf16, row r from element r *
  * x_stride on: their codes and scales are those of be42_quant_blocks_fp8.  y
- * overlaps no input.  workspace NULL: the library's (grow-only; refused while the
- * stream is captured), else a device buffer of
- * be42_linear_fp8_block_workspace_bytes() bytes, 16-byte aligned, that no call on
- * another stream uses meanwhile. */
-size_t be42_linear_fp8_block_workspace_bytes(int m, int n, int k);
+ * overlaps no input.  workspace as for be42_gemm_fp8_block, of
+ * be42_linear_fp8_block_workspace_bytes() bytes. */
+size_t be42_linear_fp8_block_workspace_bytes(int m, int n, int k, int y_bf16);
 int    be42_linear_fp8_block(void *y, int y_bf16, const void *x, int x_bf16, int x_stride, const uint8_t *wq,
                              const float *sw, int m, int n, int k, void *workspace, size_t workspace_bytes,
                              void *stream);

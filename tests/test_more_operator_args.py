@@ -12,7 +12,7 @@ from test_operator_args import INT_MAX, PTR, lib, pool, refused  # noqa: F401
 
 
 def block_gemm(lib, **kw):
-    a = dict(y=PTR, y_bf16=0, xq=PTR, sx=PTR, wq=PTR, sw=PTR, m=3, n=100, k=144)
+    a = dict(y=PTR, y_bf16=0, xq=PTR, sx=PTR, wq=PTR, sw=PTR, m=3, n=100, k=144, workspace=None, bytes=0)
     assert set(kw) <= set(a)
     a.update(kw)
     return lib.lib.be42_gemm_fp8_block(*a.values(), None)
@@ -25,19 +25,19 @@ def linear(lib, **kw):
     return lib.lib.be42_linear_fp8_block(*a.values(), None)
 
 
-SHAPES = [(dict(m=-1), "m -1"), (dict(n=0), "n 0"), (dict(k=0), "k 0"), (dict(k=136), "multiple"),
+SHAPES = [(dict(m=-1), "m -1"), (dict(n=0), "n 0"), (dict(k=0), "k 0"), (dict(k=136), "multiple"), (dict(k=(1 << 22) + 16), "at most"),
           (dict(m=INT_MAX, n=INT_MAX), "m 2147483647")]
 
 
 @pytest.mark.parametrize("kw,word", SHAPES + [
     (dict(y=None), "null"), (dict(xq=None), "null"), (dict(sx=None), "null"), (dict(wq=None), "null"), (dict(sw=None), "null"),
     (dict(xq=PTR + 8), "unaligned"), (dict(wq=PTR + 8), "unaligned"), (dict(y=PTR + 4), "unaligned"), (dict(sx=PTR + 2), "unaligned"),
-    (dict(sw=PTR + 2), "unaligned")])
+    (dict(sw=PTR + 2), "unaligned"), (dict(workspace=PTR + 8, bytes=1 << 30), "workspace"), (dict(workspace=PTR, bytes=8), "workspace")])
 def test_block_gemm_refusals(lib, kw, word):  # noqa: F811
     refused(lib, block_gemm(lib, **kw), word)
 
 
-@pytest.mark.parametrize("kw,word", SHAPES[:4] + [
+@pytest.mark.parametrize("kw,word", SHAPES[:5] + [
     (dict(m=INT_MAX, n=INT_MAX), "m 2147483647"), (dict(y=None), "null"), (dict(x=None), "null"), (dict(wq=None), "null"),
     (dict(sw=None), "null"), (dict(x_stride=143), "stride"), (dict(x=PTR + 2), "unaligned"), (dict(x=PTR + 1, x_bf16=1), "unaligned"),
     (dict(wq=PTR + 8), "unaligned"), (dict(workspace=PTR + 8, bytes=1 << 30), "workspace"), (dict(workspace=PTR, bytes=8), "workspace")])
@@ -61,10 +61,17 @@ def test_quant_blocks_refusals(lib, kw, word):  # noqa: F811
     refused(lib, lib.lib.be42_quant_blocks_fp8(*a.values(), None), word)
 
 
-def test_linear_workspace(lib):  # noqa: F811
+def test_product_workspaces(lib):  # noqa: F811
+    for f in (lib.lib.be42_gemm_fp8_block_workspace_bytes, lib.lib.be42_linear_fp8_block_workspace_bytes):
+        for bad in ((0, 1, 16), (1, 0, 16), (1, 1, 0), (1, 1, 24), (1, 1, (1 << 22) + 16)):
+            assert f(*bad, 0) == f(*bad, 1) == 0
+        assert f(1, 4096, 4096, 0) == f(2, 4096, 4096, 1) == 16          # in one launch
     f = lib.lib.be42_linear_fp8_block_workspace_bytes
-    assert f(0, 1, 16) == 0 and f(1, 0, 16) == 0 and f(1, 1, 0) == 0 and f(1, 1, 24) == 0
-    assert f(1 << 20, 64, 1 << 16) > 1 << 36       # sizes past 32 bits do not wrap
+    assert f(1 << 20, 64, 1 << 16, 0) > 1 << 36       # sizes past 32 bits do not wrap
+    for m, n, k in ((5, 64, 4096), (40, 4096, 4096), (261, 2064, 14352), (4096, 14336, 4096)):
+        for yb in (0, 1):
+            assert f(m, n, k, yb) >= lib.lib.be42_gemm_fp8_block_workspace_bytes(m, n, k, yb) + m * k + m * (-(-k // 128)) * 4
+    assert lib.lib.be42_gemm_fp8_block_workspace_bytes(261, 2064, 14352, 0) > 16       # few tiles: in parts
 
 
 def tree(lib, p=None, **kw):  # noqa: F811

@@ -44,8 +44,8 @@ SIGNATURES = {
     "be42_gemm_fp8_block": (i32, [vp, i32, vp, vp, vp, vp, i32, i32, i32, vp, sz, vp]),
     "be42_linear_fp8_block_workspace_bytes": (sz, [i32, i32, i32, i32]),
     "be42_linear_fp8_block": (i32, [vp, i32, vp, i32, i32, vp, vp, i32, i32, i32, vp, sz, vp]),
-    "be42_rope_append": (i32, [vp, vp, i32, vp, i32, i32, vp, i32, vp, i32, i32, vp, vp, f32, vp, vp, vp, i32, vp]),
-    "be42_kv_accept": (i32, [vp, vp, i32, vp, i32, i32, i32, vp]),
+    "be42_rope_append": (i32, [vp, vp, i32, i32, vp, i32, i32, vp, i32, vp, i32, i32, vp, vp, f32, vp, vp, vp, i32, vp]),
+    "be42_kv_accept": (i32, [vp, vp, i32, vp, i32, i32, i32, i32, vp]),
     "be42_tree_attention_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32, i32]),
     "be42_tree_attention": (i32, [vp, vp, i32, i32, i32, i32, vp, i32, i32, vp, i32, vp, vp, i32, f32, vp, vp, sz, vp]),
     "be42_logprobs_workspace_bytes": (sz, [i32, i32, i32]),
@@ -212,9 +212,13 @@ class Lib:
         """Entry point `name` on x's device and that device's current stream,
         which is its last argument.  (Plain integers for pointers and the raw
         stream: made of objects a call takes 4 us longer than its kernel.)"""
-        dev, cuda = x.get_device(), self.torch._C
+        dev = x.get_device()
         if dev < 0:
             raise Be42Error(f"{name}: tensors on {x.device}, not on a GPU")
+        self._on(dev, name, *args)
+
+    def _on(self, dev, name, *args):
+        cuda = self.torch._C
         if not self._inited:
             self.init()
         if dev == cuda._cuda_getDevice():
@@ -628,33 +632,33 @@ class Lib:
 
     @staticmethod
     def _host_ints(name, what, x, cols=None):
-        """A dense int32 array of host integers, [n] or [n][cols]."""
+        """A dense int32 array of host integers, [n] or [n][cols], and its address."""
         import numpy as np
-        a = np.ascontiguousarray(x, np.int64) if not (isinstance(x, np.ndarray) and x.dtype == np.int32) else x
-        if a.dtype != np.int32:
+        if not (isinstance(x, np.ndarray) and x.dtype == np.int32 and x.flags.c_contiguous):
+            a = np.asarray(x, np.int64)
             if a.size and (a.min() < -(1 << 31) or a.max() >= 1 << 31):
                 raise Be42Error(f"{name}: {what} past 32 bits")
-            a = a.astype(np.int32)
-        if not a.flags.c_contiguous:
-            a = np.ascontiguousarray(a)
-        if cols is not None and not a.size:
-            a = a.reshape(0, cols)
-        if a.ndim != (1 if cols is None else 2) or (cols is not None and a.shape[1] != cols):
-            raise Be42Error(f"{name}: {what} has shape {a.shape}")
-        return a
+            x = np.ascontiguousarray(a, np.int32)
+        if cols is not None and not x.size:
+            x = x.reshape(0, cols)
+        if x.ndim != (1 if cols is None else 2) or (cols is not None and x.shape[1] != cols):
+            raise Be42Error(f"{name}: {what} has shape {x.shape}")
+        return x, x.__array_interface__["data"][0]
 
     def _heads(self, name, what, x, dt, rows, hd, dev):
-        """Element stride of the rows of x [rows][heads][hd], whose heads lie one
-        after the other."""
-        if x.dim() != 3 or x.shape[0] != rows or x.shape[2] != hd or x.dtype != dt or x.device != dev:
-            raise Be42Error(f"{name}: {what} is {x.dtype} {tuple(x.shape)} on {x.device}")
-        H = x.shape[1]
-        if rows and ((hd > 1 and x.stride(2) != 1) or (H > 1 and x.stride(1) != hd)):
+        """Element stride of the rows of x [rows][heads][hd] on GPU dev, whose heads
+        lie one after the other, and their number."""
+        shape = x.shape
+        if len(shape) != 3 or shape[0] != rows or shape[2] != hd or x.dtype != dt or x.get_device() != dev:
+            raise Be42Error(f"{name}: {what} is {x.dtype} {tuple(shape)} on {x.device}")
+        H, (stride, apart, one) = shape[1], x.stride()
+        if rows and ((hd > 1 and one != 1) or (H > 1 and apart != hd)):
             raise Be42Error(f"{name}: {what} has rows that are not dense")
-        stride = x.stride(0) if rows > 1 else H * hd
+        if rows <= 1:
+            stride = H * hd
         if not 0 <= stride < 1 << 31:
             raise Be42Error(f"{name}: {what} has rows {stride} apart")
-        return stride
+        return stride, H
 
     def rope_append(self, pool, runs, k, v, q=None, rope=None, positions=None, q_norm=None, k_norm=None, eps=1e-5,
                     out=None):
@@ -667,38 +671,38 @@ class Lib:
         where a token's angle is not that of its place.  Returns the rotated
         queries, in a new tensor or in out (q itself: in place)."""
         t, name = self.torch, "be42_rope_append"
-        dev, dt, hd = k.device, k.dtype, pool.head_dim
-        if dt not in (t.float32, t.bfloat16) or k.get_device() != pool.device:
-            raise Be42Error(f"{name}: k is {dt} on {dev}, the pool on GPU {pool.device}")
-        runs = self._host_ints(name, "runs", runs, 3)
+        gpu, dt, hd = pool.device, k.dtype, pool.head_dim
+        if dt != t.float32 and dt != t.bfloat16:
+            raise Be42Error(f"{name}: k is {dt}")
+        runs, at_runs = self._host_ints(name, "runs", runs, 3)
         n = k.shape[0]
-        if int(runs[:, 2].sum(dtype="int64")) != n or (n and runs[:, 2].min() < 0):
-            raise Be42Error(f"{name}: {n} tokens, the runs have {runs[:, 2].tolist()}")
-        ks, vs = (self._heads(name, what, x, dt, n, hd, dev) for what, x in (("k", k), ("v", v)))
-        if k.shape[1] != pool.n_kv or v.shape[1] != pool.n_kv:
+        if n >= 1 << 31:
+            raise Be42Error(f"{name}: {n} tokens")
+        (ks, kh), (vs, vh) = self._heads(name, "k", k, dt, n, hd, gpu), self._heads(name, "v", v, dt, n, hd, gpu)
+        if kh != pool.n_kv or vh != pool.n_kv:
             raise Be42Error(f"{name}: k {tuple(k.shape)}, v {tuple(v.shape)}: the pool has {pool.n_kv} heads")
-        H, qs, os_ = 0, 0, 0
+        H, qs, os_, at_q, at_out = 0, 0, 0, None, None
         if q is not None:
-            H, qs = q.shape[1] if q.dim() == 3 else 0, self._heads(name, "q", q, dt, n, hd, dev)
+            qs, H = self._heads(name, "q", q, dt, n, hd, gpu)
             if out is None:
-                out = t.empty(n, H, hd, dtype=dt, device=dev)
-                os_ = H * hd
+                out, os_ = t.empty(n, H, hd, dtype=dt, device=q.device), H * hd
             else:
-                os_ = self._heads(name, "out", out, dt, n, hd, dev)
-                if out.shape[1] != H:
+                os_, oh = self._heads(name, "out", out, dt, n, hd, gpu)
+                if oh != H:
                     raise Be42Error(f"{name}: out has shape {tuple(out.shape)}")
+            at_q, at_out = q.data_ptr(), out.data_ptr()
         elif out is not None:
             raise Be42Error(f"{name}: out without q")
         for what, w in (("q_norm", q_norm), ("k_norm", k_norm)):
             if w is not None:
-                self._want(name, what, w, (t.bfloat16,), (hd,), dev)
-        if rope is not None and rope.cos.device != dev:
-            raise Be42Error(f"{name}: rope on {rope.cos.device}, not on {dev}")
+                self._want(name, what, w, (t.bfloat16,), (hd,), k.device)
+        if rope is not None and rope.device != gpu:
+            raise Be42Error(f"{name}: rope on GPU {rope.device}, not on {gpu}")
         if positions is not None:
-            self._want(name, "positions", positions, (t.int32,), (n,), dev)
-        at = [None if x is None else x.data_ptr() for x in (q, q_norm, k_norm, positions, out)]
-        self._device_call(k, name, pool.handle, runs.ctypes.data, len(runs), at[0], qs, H, k.data_ptr(), ks, v.data_ptr(), vs,
-                          dt == t.bfloat16, at[1], at[2], eps, None if rope is None else rope.at, at[3], at[4], os_)
+            self._want(name, "positions", positions, (t.int32,), (n,), k.device)
+        self._on(gpu, name, pool.handle, at_runs, len(runs), n, at_q, qs, H, k.data_ptr(), ks, v.data_ptr(), vs,
+                 dt == t.bfloat16, None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(),
+                 eps, None if rope is None else rope.at, None if positions is None else positions.data_ptr(), at_out, os_)
         return out
 
     def kv_accept(self, pool, runs, index, layers=1, from_step=0, to_step=0):
@@ -708,16 +712,11 @@ class Lib:
         names.  The same for each of `layers` layers, whose slots lie from_step
         and to_step apart."""
         name = "be42_kv_accept"
-        runs, index = self._host_ints(name, "runs", runs, 4), self._host_ints(name, "index", index)
-        if int(runs[:, 3].sum(dtype="int64")) != len(index):
-            raise Be42Error(f"{name}: {len(index)} tokens, the runs have {runs[:, 3].tolist()}")
-        self._pool_call(pool, name, runs.ctypes.data, len(runs), index.ctypes.data, layers, from_step, to_step)
-
-    def _pool_call(self, pool, name, *args):
-        """Entry point `name` of a pool, on its device's current stream."""
-        t = self.torch
-        with t.cuda.device(pool.device):
-            self._call(name, pool.handle, *args, self.stream())
+        runs, at = self._host_ints(name, "runs", runs, 4)
+        index, at_index = self._host_ints(name, "index", index)
+        if max(len(runs), len(index), abs(layers), abs(from_step), abs(to_step)) >= 1 << 31:
+            raise Be42Error(f"{name}: {len(runs)} runs, {len(index)} tokens, {layers} layers: past 32 bits")
+        self._on(pool.device, name, pool.handle, at, len(runs), at_index, len(index), layers, from_step, to_step)
 
     def tree_attention(self, pool, q, starts, parents, draft_slot, scale, max_tree, slots=None, lens=None, max_len=None,
                        out=None, workspace=None):
@@ -735,11 +734,8 @@ class Lib:
         t, name = self.torch, "be42_tree_attention"
         if q.dim() != 3 or q.dtype not in (t.float32, t.bfloat16):
             raise Be42Error(f"{name}: q is {q.dtype} {tuple(q.shape)}")
-        n, H, hd = q.shape
-        dev = q.device
-        if q.get_device() != pool.device:
-            raise Be42Error(f"{name}: q on {dev}, the pool on GPU {pool.device}")
-        qs = self._heads(name, "q", q, q.dtype, n, pool.head_dim, dev)
+        n, hd, dev = q.shape[0], pool.head_dim, q.device
+        qs, H = self._heads(name, "q", q, q.dtype, n, hd, pool.device)
         trees = starts.numel() - 1
         if trees < 0:
             raise Be42Error(f"{name}: starts is empty")
@@ -810,7 +806,7 @@ class Rope:
             if x.dim() != 2 or x.shape != cos.shape or str(x.dtype) != "torch.float32" or not x.is_contiguous() or \
                     x.device != cos.device or max(x.shape) >= 1 << 30:
                 raise Be42Error(f"Rope: {what} is {x.dtype} {tuple(x.shape)} on {x.device}")
-        self.cos, self.sin = cos, sin
+        self.cos, self.sin, self.device = cos, sin, cos.get_device()
         self.struct = RopeStruct(cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1], bool(interleaved))
         self.at = C.addressof(self.struct)
 

@@ -70,7 +70,185 @@ __device__ __forceinline__ float act_at(const void *p, size_t i)
     return BF16 ? bf16_to_f32(((const uint16_t *)p)[i]) : ((const float *)p)[i];
 }
 
-// One wave a row, a lane a pair of elements (two pairs where head_dim is past 128):
+// op over the lanes of a group of L (8, 16 or 32), in every one, by lane moves.
+template <int L, class T, class F>
+__device__ __forceinline__ T group_all(T v, F &&op)
+{
+    v = op(v, dpp_mov<0xB1>(v, v));            // neighbours, pairs, halves of 8, of 16
+    v = op(v, dpp_mov<0x4E>(v, v));
+    v = op(v, dpp_mov<0x141>(v, v));
+    if constexpr (L >= 16)
+        v = op(v, dpp_mov<0x140>(v, v));
+    if constexpr (L >= 32)
+        v = op(v, __shfl_xor(v, 16, kWave));
+    return v;
+}
+
+// Four elements from `at` on (any alignment).
+template <bool BF16>
+__device__ __forceinline__ void load4(const void *p, size_t at, float *v)
+{
+    if constexpr (BF16) {
+        uint32_t u[2];
+        __builtin_memcpy(u, (const uint16_t *)p + at, 8);
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            v[j] = __uint_as_float(j & 1 ? u[j / 2] & 0xFFFF0000u : u[j / 2] << 16);
+    } else {
+        __builtin_memcpy(v, (const float *)p + at, 16);
+    }
+}
+__device__ __forceinline__ uint2 bf16_4(const float *v)
+{
+    return make_uint2(f32_to_bf16(v[0]) | (uint32_t)f32_to_bf16(v[1]) << 16, f32_to_bf16(v[2]) | (uint32_t)f32_to_bf16(v[3]) << 16);
+}
+
+// Heads of 64, 128 or 256, a rotation of a multiple of 8 elements.  A group of HD / 8
+// lanes takes a row: lane u the pairs 4 u .. 4 u + 3 of the rotation in two words of
+// four, or eight elements of what is not rotated.  A workgroup takes two heads' rows of
+// the tokens of a page, K and V or two query heads (blockIdx.z), all its loads in
+// flight together and one pair of table words for both heads; rows of V go through LDS
+// where the whole page is written, so that they leave as its lines.  Bound by HBM: 11834 bf16
+// tokens with norms, 32 query heads on 8 KV heads of 128, 86 us in two launches, 3.4
+// TB/s (243 us in the form below); 261 INT8 tokens 6.9 us (25).
+template <bool KV8, bool BF16, int HD>
+__global__ __launch_bounds__(256) void k_rope_append_words(const be42_kv_pool P, const RopeArgs a, const RopeIn x)
+{
+    constexpr int L = HD / 8, PER = 256 / L, TOKENS = PER < kPage ? PER : kPage, VS = kPage + 8;
+    __shared__ float c[256];
+    __shared__ __align__(16) uint16_t vt[KV8 ? 1 : HD][VS];
+    const int h = blockIdx.y, z = blockIdx.z, grp = threadIdx.x / L, l = threadIdx.x % L;
+    const Piece &p = a.piece[piece_of(a, blockIdx.x)];
+    const int blk = p.pos0 / kPage + ((int)blockIdx.x - p.page0);
+    const int entry = a.pages[blockIdx.x], phys = entry & ~kNewPage;
+    const int lo = max(p.pos0, blk * kPage), T = min(p.pos0 + p.n, (blk + 1) * kPage) - lo;
+    const int tok0 = p.tok0 + lo - p.pos0, off0 = lo - blk * kPage;
+    const int G = x.n_heads / P.n_kv, half = x.rope_dim / 2;
+    const bool kv = z == 0, two = kv || 2 * z <= G;
+    const int head = h * G + 2 * (z - 1);
+    if (kv && h == 0 && threadIdx.x == 0)
+        publish(P, p.slot, p.pos0, p.n, blk, phys, entry & kNewPage);
+    // the lane's two words
+    const bool turns = 8 * l < x.rope_dim;
+    const int c0 = turns && !x.interleaved ? 4 * l : 8 * l, c1 = turns && !x.interleaved ? half + 4 * l : 8 * l + 4;
+    const uint16_t *w = kv ? x.k_norm : x.q_norm;
+    for (int i = grp; i < T && grp < TOKENS; i += TOKENS) {
+        const int tok = tok0 + i;
+        float y[2][8], cs[4], sn[4], wt[8];
+        const size_t at0 = kv ? tok * x.k_stride + (size_t)h * HD : tok * x.q_stride + (size_t)head * HD;
+        const size_t at1 = kv ? tok * x.v_stride + (size_t)h * HD : at0 + HD;
+        const void *from0 = kv ? x.k : x.q, *from1 = kv ? x.v : x.q;
+        load4<BF16>(from0, at0 + c0, y[0]);
+        load4<BF16>(from0, at0 + c1, y[0] + 4);
+        if (two) {
+            load4<BF16>(from1, at1 + c0, y[1]);
+            load4<BF16>(from1, at1 + c1, y[1] + 4);
+        }
+        const int pos = x.positions ? x.positions[tok] : lo + i;
+        const bool turn = turns && pos >= 0 && pos < x.rope_len;
+        if (turn) {
+            load4<false>(x.cos_t, (size_t)pos * half + 4 * l, cs);
+            load4<false>(x.sin_t, (size_t)pos * half + 4 * l, sn);
+        }
+        if (w) {
+            load4<true>(w, c0, wt);
+            load4<true>(w, c1, wt + 4);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            if (j && (!two || kv))
+                break;
+            if (w) {
+                double ss = 0.0;
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    ss = fma((double)y[j][e], (double)y[j][e], ss);
+                ss = group_all<L>(ss, [](double a, double b) { return a + b; });
+                const double s = 1.0 / sqrt(ss / HD + (double)x.eps);
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    y[j][e] = (float)((double)y[j][e] * s * (double)wt[e]);
+            }
+            if (turn)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float &u = x.interleaved ? y[j][2 * e] : y[j][e], &v = x.interleaved ? y[j][2 * e + 1] : y[j][4 + e];
+                    const float u0 = u, v0 = v;
+                    u = __fmaf_rn(u0, cs[e], -(v0 * sn[e]));
+                    v = __fmaf_rn(u0, sn[e], v0 * cs[e]);
+                }
+        }
+        if (!kv) {
+            const size_t to = tok * x.q_out_stride + (size_t)head * HD;
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+                if (j == 0 || two)
+#pragma unroll
+                    for (int e = 0; e < 8; e += 4) {
+                        const size_t at = to + j * HD + (e ? c1 : c0);
+                        if constexpr (BF16) {
+                            const uint2 b = bf16_4(y[j] + e);
+                            __builtin_memcpy((uint16_t *)x.q_out + at, &b, 8);
+                        } else {
+                            __builtin_memcpy((float *)x.q_out + at, y[j] + e, 16);
+                        }
+                    }
+            continue;
+        }
+        const int off = off0 + i;
+        const size_t row = ((size_t)phys * P.n_kv + h) * kPage + off;
+        if constexpr (KV8) {
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                float m = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    m = fmaxf(m, fabsf(y[j][e]));
+                m = group_all<L>(m, [](float a, float b) { return fmaxf(a, b); });
+                const float sc = m > 0.0f ? m / 127.0f : 1.0f, inv = m > 0.0f ? 127.0f / m : 1.0f;
+                int8_t *to = (int8_t *)(j ? P.v : P.k) + row * HD;
+#pragma unroll
+                for (int e = 0; e < 8; e += 4) {
+                    uint32_t code = 0;
+#pragma unroll
+                    for (int d = 0; d < 4; d++)
+                        code |= (uint32_t)(uint8_t)max(min((int)roundf(y[j][e + d] * inv), 127), -127) << (8 * d);
+                    *(uint32_t *)(to + (e ? c1 : c0)) = code;
+                }
+                if (l == 0)
+                    (j ? P.v_scale : P.k_scale)[row] = sc;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e += 4)
+                *(uint2 *)((uint16_t *)P.k + row * HD + (e ? c1 : c0)) = bf16_4(y[0] + e);
+            uint16_t *to = (uint16_t *)P.v + (row / kPage) * HD * kPage + off;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int d = (e < 4 ? c0 : c1 - 4) + e;
+                if (T == kPage)
+                    vt[d][i] = f32_to_bf16(y[1][e]);
+                else
+                    to[(size_t)d * kPage] = f32_to_bf16(y[1][e]);
+            }
+        }
+    }
+    if (!kv)
+        return;
+    if constexpr (!KV8)
+        if (T == kPage) {
+            __syncthreads();
+            uint16_t *to = (uint16_t *)P.v + ((size_t)phys * P.n_kv + h) * HD * kPage;
+            for (int i = threadIdx.x; i < 2 * HD; i += 256)
+                *(uint4 *)(to + 8 * i) = *(const uint4 *)&vt[i / 2][8 * (i % 2)];
+        }
+    if (h == 0 && off0 + T == kPage) {
+        __syncthreads();                   // the page's rows are in memory
+        seal_page<!KV8>(P.k, P.k_scale, P.centroid, P.page_hash + (size_t)p.slot * P.max_logical + blk, phys, P.hpT, P.n_kv, HD, c);
+    }
+}
+
+// Any other head, or rotation: one wave a row, a lane a pair of elements (two pairs where head_dim is past 128):
 // the pairs of the rotation, then neighbours behind them.
 template <bool KV8, bool BF16, int NP>
 __global__ __launch_bounds__(256) void k_rope_append(const be42_kv_pool P, const RopeArgs a, const RopeIn x)
@@ -208,24 +386,32 @@ __global__ __launch_bounds__(256) void k_kv_accept(const be42_kv_pool P, const T
     const int off0 = lo - blk * kPage;
     if (h == 0 && threadIdx.x == 0)
         publish(P, slot, u.pos0, u.n, blk, phys, entry & kNewPage);
+    // eight elements of a token's row a thread, all tokens beside each other: one chain of
+    // loads (page table, row), whatever the page takes
     const size_t head = (size_t)phys * P.n_kv + h;
-    for (int i = 0; i < T; i++) {
-        const int src = a.index[u.tok0 + lo - u.pos0 + i], off = off0 + i;
+    const int nw = hd / 8;
+    for (int i = threadIdx.x; i < T * nw; i += 256) {
+        const int t = i / nw, d = 8 * (i % nw), src = a.index[u.tok0 + lo - u.pos0 + t], off = off0 + t, so = src % kPage;
         const int page = min(max(P.page_table[(size_t)from * P.max_logical + src / kPage], 0), P.capacity - 1);
-        const size_t sh = (size_t)page * P.n_kv + h;
-        const int so = src % kPage;
-        for (int d = threadIdx.x; d < hd; d += 256) {
-            if constexpr (KV8) {
-                ((int8_t *)P.k)[(head * kPage + off) * hd + d] = ((const int8_t *)P.k)[(sh * kPage + so) * hd + d];
-                ((int8_t *)P.v)[(head * kPage + off) * hd + d] = ((const int8_t *)P.v)[(sh * kPage + so) * hd + d];
-            } else {
-                ((uint16_t *)P.k)[(head * kPage + off) * hd + d] = ((const uint16_t *)P.k)[(sh * kPage + so) * hd + d];
-                ((uint16_t *)P.v)[(head * hd + d) * kPage + off] = ((const uint16_t *)P.v)[(sh * hd + d) * kPage + so];
+        const size_t sh = (size_t)page * P.n_kv + h, sr = (sh * kPage + so) * hd + d, dr = (head * kPage + off) * hd + d;
+        if constexpr (KV8) {
+            const uint2 k = *(const uint2 *)((const int8_t *)P.k + sr), v = *(const uint2 *)((const int8_t *)P.v + sr);
+            if (d == 0) {
+                P.k_scale[head * kPage + off] = P.k_scale[sh * kPage + so];
+                P.v_scale[head * kPage + off] = P.v_scale[sh * kPage + so];
             }
-        }
-        if (KV8 && threadIdx.x == 0) {
-            P.k_scale[head * kPage + off] = P.k_scale[sh * kPage + so];
-            P.v_scale[head * kPage + off] = P.v_scale[sh * kPage + so];
+            *(uint2 *)((int8_t *)P.k + dr) = k;
+            *(uint2 *)((int8_t *)P.v + dr) = v;
+        } else {
+            const uint4 k = *(const uint4 *)((const uint16_t *)P.k + sr);
+            uint16_t v[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                v[e] = ((const uint16_t *)P.v)[(sh * hd + d + e) * kPage + so];
+            *(uint4 *)((uint16_t *)P.k + dr) = k;
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                ((uint16_t *)P.v)[(head * hd + d + e) * kPage + off] = v[e];
         }
     }
     if (h == 0 && off0 + T == kPage) {
@@ -244,12 +430,26 @@ static int rope_append(be42_kv_pool *pool, const be42_kv_run *runs, int n_runs, 
     RopeArgs a;
     a.n = a.n_pages = 0;
     auto launch = [&]() {
-        auto go = [&](auto kv8, auto act, auto np) {
+        const int z = 1 + (x.n_heads / P.n_kv + 1) / 2;
+        auto words = [&](auto kv8, auto act, auto hd) {
+            hipLaunchKernelGGL((k_rope_append_words<decltype(kv8)::value, decltype(act)::value, decltype(hd)::value>),
+                               dim3(a.n_pages, P.n_kv, z), dim3(256), 0, s, P, a, x);
+        };
+        auto pairs = [&](auto kv8, auto act, auto np) {
             hipLaunchKernelGGL((k_rope_append<decltype(kv8)::value, decltype(act)::value, decltype(np)::value>),
                                dim3(a.n_pages, P.n_kv), dim3(256), 0, s, P, a, x);
         };
         auto of_dim = [&](auto kv8, auto act) {
-            P.head_dim > 128 ? go(kv8, act, std::integral_constant<int, 2>()) : go(kv8, act, std::integral_constant<int, 1>());
+            if (x.rope_dim % 8 == 0 && P.head_dim == 64)
+                words(kv8, act, std::integral_constant<int, 64>());
+            else if (x.rope_dim % 8 == 0 && P.head_dim == 128)
+                words(kv8, act, std::integral_constant<int, 128>());
+            else if (x.rope_dim % 8 == 0 && P.head_dim == 256)
+                words(kv8, act, std::integral_constant<int, 256>());
+            else if (P.head_dim > 128)
+                pairs(kv8, act, std::integral_constant<int, 2>());
+            else
+                pairs(kv8, act, std::integral_constant<int, 1>());
         };
         auto of_kind = [&](auto act) { P.kind == BE42_KV_INT8 ? of_dim(std::true_type(), act) : of_dim(std::false_type(), act); };
         bf16 ? of_kind(std::true_type()) : of_kind(std::false_type());
@@ -282,27 +482,32 @@ static int rope_append(be42_kv_pool *pool, const be42_kv_run *runs, int n_runs, 
     return BE42_OK;
 }
 
-static int kv_accept(be42_kv_pool *pool, const be42_kv_take *runs, int n_runs, const int *index, int n_layers,
+static int kv_accept(be42_kv_pool *pool, const be42_kv_take *runs, int n_runs, const int *index, size_t n_index, int n_layers,
                      int from_step, int to_step, hipStream_t s)
 {
     be42_kv_pool &P = *pool;
     std::vector<be42_kv_run> all;
-    std::vector<int> from, pages;
+    std::vector<int> from, pages, last(n_runs, -1);          // last: the largest token that a run names
+    all.reserve((size_t)n_runs * n_layers);
+    from.reserve((size_t)n_runs * n_layers);
+    size_t at = 0;
+    for (int r = 0; r < n_runs; r++) {
+        BE42_CHECK(runs[r].count >= 0 && (size_t)runs[r].count <= n_index - at, "be42_kv_accept: %zu tokens, the runs have more", n_index);
+        for (int i = 0; i < runs[r].count; i++, at++) {
+            BE42_CHECK(index[at] >= 0, "be42_kv_accept: token %d", index[at]);
+            last[r] = std::max(last[r], index[at]);
+        }
+    }
+    BE42_CHECK(at == n_index, "be42_kv_accept: %zu tokens, the runs have %zu", n_index, at);
     for (int l = 0; l < n_layers; l++)
         for (int r = 0; r < n_runs; r++) {
             const long a = runs[r].from + (long)l * from_step, b = runs[r].to + (long)l * to_step;
             BE42_CHECK(a >= 0 && a < P.n_layers && b >= 0 && b < P.n_layers, "be42_kv_accept: slot %ld or %ld out of range", a, b);
+            BE42_CHECK(last[r] < 0 || last[r] / kPage < slot_pages(pool, (int)a), "be42_kv_accept: token %d of slot %ld, which has %d pages",
+                       last[r], a, slot_pages(pool, (int)a));
             from.push_back((int)a);
             all.push_back({(int)b, runs[r].pos0, runs[r].count});
-            BE42_CHECK(runs[r].count >= 0, "be42_kv_accept: positions %d .. of %d tokens", runs[r].pos0, runs[r].count);
         }
-    size_t at = 0;
-    for (int r = 0; r < n_runs; r++)
-        for (int i = 0; i < runs[r].count; i++, at++)
-            for (int l = 0; l < n_layers; l++)
-                BE42_CHECK(index[at] >= 0 && index[at] / kPage < slot_pages(pool, from[l * n_runs + r]),
-                           "be42_kv_accept: token %d of slot %d, which has %d pages", index[at], from[l * n_runs + r],
-                           slot_pages(pool, from[l * n_runs + r]));
     const int rc = plan_runs(pool, "be42_kv_accept", all.data(), (int)all.size(), from.data(), pages);
     if (rc)
         return rc;
@@ -367,19 +572,19 @@ static int kv_accept(be42_kv_pool *pool, const be42_kv_take *runs, int n_runs, c
 
 using namespace be42;
 
-extern "C" int be42_rope_append(be42_kv_pool *pool, const be42_kv_run *runs, int n_runs, const void *q, int q_stride,
-                                int n_heads, const void *k, int k_stride, const void *v, int v_stride, int act_bf16,
+extern "C" int be42_rope_append(be42_kv_pool *pool, const be42_kv_run *runs, int n_runs, int n_tokens, const void *q,
+                                int q_stride, int n_heads, const void *k, int k_stride, const void *v, int v_stride, int act_bf16,
                                 const uint16_t *q_norm, const uint16_t *k_norm, float eps, const be42_rope *rope,
                                 const int *positions, void *q_out, int q_out_stride, void *stream)
 {
     BE42_CHECK(pool && (n_runs == 0 || runs), "be42_rope_append: null pointer");
     const be42_kv_pool &P = *pool;
-    BE42_CHECK(n_runs >= 0, "be42_rope_append: %d runs", n_runs);
+    BE42_CHECK(n_runs >= 0 && n_tokens >= 0, "be42_rope_append: %d runs, %d tokens", n_runs, n_tokens);
     long tokens = 0;
     for (int r = 0; r < n_runs; r++)
         tokens += std::max(runs[r].count, 0);
+    BE42_CHECK(tokens == n_tokens, "be42_rope_append: %d tokens, the runs have %ld", n_tokens, tokens);
     BE42_CHECK(tokens == 0 || (k && v), "be42_rope_append: null pointer");
-    BE42_CHECK(tokens < 1L << 31, "be42_rope_append: %ld tokens", tokens);
     BE42_CHECK(n_heads >= 0 && n_heads % P.n_kv == 0 && (!tokens || (n_heads == 0) == (q == nullptr)),
                "be42_rope_append: %d query heads over %d kv heads", n_heads, P.n_kv);
     BE42_CHECK(!q || q_out, "be42_rope_append: null q_out");
@@ -408,16 +613,17 @@ extern "C" int be42_rope_append(be42_kv_pool *pool, const be42_kv_run *runs, int
     }
 }
 
-extern "C" int be42_kv_accept(be42_kv_pool *pool, const be42_kv_take *runs, int n_runs, const int *index, int n_layers,
-                              int from_step, int to_step, void *stream)
+extern "C" int be42_kv_accept(be42_kv_pool *pool, const be42_kv_take *runs, int n_runs, const int *index, int n_index,
+                              int n_layers, int from_step, int to_step, void *stream)
 {
-    BE42_CHECK(pool && (n_runs == 0 || (runs && index)), "be42_kv_accept: null pointer");
-    BE42_CHECK(n_runs >= 0 && n_layers >= 0 && (long)n_runs * n_layers <= pool->n_layers,
+    BE42_CHECK(pool && (n_runs == 0 || runs) && (n_index == 0 || index), "be42_kv_accept: null pointer");
+    BE42_CHECK(n_runs >= 0 && n_index >= 0 && n_layers >= 0 && (long)n_runs * n_layers <= pool->n_layers,
                "be42_kv_accept: %d runs of %d layers over %d slots", n_runs, n_layers, pool->n_layers);
+    BE42_CHECK(n_runs || !n_index, "be42_kv_accept: %d tokens without a run", n_index);
     if (!n_runs || !n_layers)
         return BE42_OK;
     try {
-        return kv_accept(pool, runs, n_runs, index, n_layers, from_step, to_step, as_stream(stream));
+        return kv_accept(pool, runs, n_runs, index, (size_t)n_index, n_layers, from_step, to_step, as_stream(stream));
     } catch (const std::bad_alloc &) {
         set_error("be42_kv_accept: out of host memory");
         return BE42_ENOMEM;

@@ -247,7 +247,7 @@ int  be42_kv_layer_pages(const be42_kv_pool *pool, int layer, int *phys_out, int
 int  be42_kv_append_step(be42_kv_pool *pool, const int *slots, const int *pos, int n, const float *k,
                          const float *v, void *stream);
 /* Tokens of a q/k/v product -> rotated queries, and K and V in the pages, in one
- * pass.  The tokens are those of n_runs runs, one after the other: run r is
+ * pass.  The n_tokens tokens are those of n_runs runs, one after the other: run r is
  * runs[r].count tokens at positions runs[r].pos0 .. of slot runs[r].slot (host
  * array; a slot at most once a call; positions as be42_kv_append takes them).  Row
  * t of q, k and v begins at element t * its stride and holds n_heads, n_kv, n_kv
@@ -271,14 +271,14 @@ typedef struct be42_rope {
     const float *cos, *sin;    /* device [len][dim / 2] */
     int len, dim, interleaved; /* dim: even, at most head_dim */
 } be42_rope;
-int  be42_rope_append(be42_kv_pool *pool, const be42_kv_run *runs, int n_runs, const void *q, int q_stride,
+int  be42_rope_append(be42_kv_pool *pool, const be42_kv_run *runs, int n_runs, int n_tokens, const void *q, int q_stride,
                       int n_heads, const void *k, int k_stride, const void *v, int v_stride, int act_bf16,
                       const uint16_t *q_norm, const uint16_t *k_norm, float eps, const be42_rope *rope,
                       const int *positions, void *q_out, int q_out_stride, void *stream);
 /* Tokens that one slot holds, behind what another holds: the drafts of a tree that
  * were right, from the drafts' slot to their sequence's.  Run r puts runs[r].count
  * tokens at positions runs[r].pos0 .. of slot runs[r].to: tokens index[..] of slot
- * runs[r].from (host array, the runs' one after the other), as the pages hold them,
+ * runs[r].from (host array of n_index, the runs' one after the other), as the pages hold them,
  * bit for bit.  The same for each of n_layers layers: layer l takes slots from + l *
  * from_step and to + l * to_step.  A slot is filled at most once a call, and none
  * that is read from.  Pages that fill get their centroid and hash.  On an error
@@ -286,8 +286,8 @@ int  be42_rope_append(be42_kv_pool *pool, const be42_kv_run *runs, int n_runs, c
 typedef struct be42_kv_take {
     int from, to, pos0, count;
 } be42_kv_take;
-int  be42_kv_accept(be42_kv_pool *pool, const be42_kv_take *runs, int n_runs, const int *index, int n_layers,
-                    int from_step, int to_step, void *stream);
+int  be42_kv_accept(be42_kv_pool *pool, const be42_kv_take *runs, int n_runs, const int *index, int n_index,
+                    int n_layers, int from_step, int to_step, void *stream);
 int  be42_kv_page_alloc(be42_kv_pool *pool);
 int  be42_kv_page_free(be42_kv_pool *pool, int phys);
 int  be42_kv_export(const be42_kv_pool *pool, int *page_table, int *free_stack, int *free_top,

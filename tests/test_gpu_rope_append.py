@@ -397,7 +397,7 @@ def test_accept_refusals_change_nothing(be):
             ([(4, 0, 20, 1)], [0], {}, "out of range"), ([(2, -1, 20, 1)], [0], {}, "out of range"),
             ([(2, 0, 20, 1)], [0], dict(layers=2, from_step=2, to_step=1), "out of range"),
             ([(2, 0, 20, 1)], [0], dict(layers=2, from_step=0, to_step=2 ** 31 - 1), "out of range"),
-            ([(2, 0, 20, 1)], [0, 1], {}, "2 tokens"), ([(2, 0, 20, 2), (2, 1, 5, -1)], [0], {}, "positions")):
+            ([(2, 0, 20, 1)], [0, 1], {}, "2 tokens"), ([(2, 0, 20, 2), (2, 1, 5, -1)], [0], {}, "more")):
         with pytest.raises(be42.Be42Error, match=word):
             be.kv_accept(pool, runs, index, **kw)
         same(state(pool), before)

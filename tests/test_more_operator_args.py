@@ -120,7 +120,7 @@ def append(lib, p=None, r=None, rope=None, **kw):  # noqa: F811
     r = runs((0, 0, 3)) if r is None else r
     rope = rope or dict(cos=PTR, sin=PTR, len=100, dim=64, interleaved=0)
     st = be42.RopeStruct(**rope)
-    a = dict(pool=C.addressof(p), runs=r.ctypes.data, n_runs=len(r), q=PTR, q_stride=256, n_heads=4, k=PTR, k_stride=128, v=PTR,
+    a = dict(pool=C.addressof(p), runs=r.ctypes.data, n_runs=len(r), n_tokens=3, q=PTR, q_stride=256, n_heads=4, k=PTR, k_stride=128, v=PTR,
              v_stride=128, bf16=0, q_norm=PTR, k_norm=PTR, eps=1e-5, rope=C.addressof(st), positions=None, q_out=PTR, q_out_stride=256)
     assert set(kw) <= set(a)
     a.update(kw)
@@ -136,17 +136,18 @@ def append(lib, p=None, r=None, rope=None, **kw):  # noqa: F811
     (dict(k=PTR + 1, bf16=1), "unaligned"), (dict(q_norm=PTR + 1), "unaligned"), (dict(positions=PTR + 2), "unaligned"),
     (dict(rope=dict(cos=None, sin=PTR, len=100, dim=64)), "table"), (dict(rope=dict(cos=PTR, sin=PTR, len=100, dim=66)), "rope"),
     (dict(rope=dict(cos=PTR, sin=PTR, len=100, dim=7)), "rope"), (dict(rope=dict(cos=PTR, sin=PTR, len=-1, dim=8)), "rope"),
-    (dict(rope=dict(cos=PTR, sin=PTR + 1, len=9, dim=8)), "unaligned"), (dict(r=runs((0, 0, INT_MAX), (1, 0, INT_MAX))), "tokens")])
+    (dict(rope=dict(cos=PTR, sin=PTR + 1, len=9, dim=8)), "unaligned"), (dict(r=runs((0, 0, INT_MAX), (1, 0, INT_MAX))), "tokens"), (dict(n_tokens=4), "tokens"),
+    (dict(n_tokens=-1), "tokens"), (dict(r=runs((0, 0, 4), (1, 0, -1))), "tokens")])
 def test_rope_append_refusals(lib, kw, word):  # noqa: F811
     refused(lib, append(lib, **kw), word)
 
 
 @pytest.mark.parametrize("kw,word", [
-    (dict(pool=None), "null"), (dict(runs=None), "null"), (dict(index=None), "null"), (dict(n_runs=-1), "runs"),
-    (dict(layers=-1), "layers"), (dict(layers=5), "slots"), (dict(layers=INT_MAX, n_runs=INT_MAX), "slots")])
+    (dict(pool=None), "null"), (dict(runs=None), "null"), (dict(index=None), "null"), (dict(n_runs=-1), "runs"), (dict(n_index=-1), "runs"),
+    (dict(n_runs=0), "without a run"), (dict(layers=-1), "layers"), (dict(layers=5), "slots"), (dict(layers=INT_MAX, n_runs=INT_MAX), "slots")])
 def test_kv_accept_refusals(lib, kw, word):  # noqa: F811
     p, r, i = pool(), runs((3, 0, 0, 1)), np.zeros(1, np.int32)
-    a = dict(pool=C.addressof(p), runs=r.ctypes.data, n_runs=1, index=i.ctypes.data, layers=1, from_step=0, to_step=0)
+    a = dict(pool=C.addressof(p), runs=r.ctypes.data, n_runs=1, index=i.ctypes.data, n_index=1, layers=1, from_step=0, to_step=0)
     a.update(kw)
     refused(lib, lib.lib.be42_kv_accept(*a.values(), None), word)
 

@@ -720,10 +720,13 @@ __device__ __forceinline__ void part32(const be42_kv_pool &P, const PrefixArgs &
         }
     };
     const int whole = (hi - lo) / kStage;
-    const bool mine = hi - lo - whole * kStage > tg * kStep;          // of the stage that the part's end cuts
+    const bool any = row0 + 32 * rg < rows;                           // else the wave only loads
+    const bool mine = any && hi - lo - whole * kStage > tg * kStep;   // of the stage that the part's end cuts
     v16f s;
     for (int i = 0; i < whole; i++) {
         begin(i);
+        if (!any)
+            continue;
         scores(i, s);
         values(i, s, std::false_type());
     }

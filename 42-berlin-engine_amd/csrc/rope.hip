@@ -108,9 +108,9 @@ __device__ __forceinline__ uint2 bf16_4(const float *v)
 // four, or eight elements of what is not rotated.  A workgroup takes two heads' rows of
 // the tokens of a page, K and V or two query heads (blockIdx.z), all its loads in
 // flight together and one pair of table words for both heads; rows of V go through LDS
-// where the whole page is written, so that they leave as its lines.  Bound by HBM: 11834 bf16
+// where the whole page is written, so that they leave as its lines.  Bound by HBM: 11801 bf16
 // tokens with norms, 32 query heads on 8 KV heads of 128, 86 us in two launches, 3.4
-// TB/s (243 us in the form below); 261 INT8 tokens 6.9 us (25).
+// TB/s (243 us in the form below); 218 INT8 tokens 6.9 us (25).
 template <bool KV8, bool BF16, int HD>
 __global__ __launch_bounds__(256) void k_rope_append_words(const be42_kv_pool P, const RopeArgs a, const RopeIn x)
 {

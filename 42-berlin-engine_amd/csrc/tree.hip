@@ -73,11 +73,12 @@ __global__ __launch_bounds__(64 * kPartWaves, 2) void k_tree_part(const be42_kv_
     } S;
     constexpr int NP = QB ? 1 : 3, PP = QB ? 2 : 3, kRows = R ? 32 * R : 16;
     const int G = a.n_heads / P.n_kv, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const unsigned of_drafts = (unsigned)P.n_kv * a.tiles_o * a.n_trees;
+    // (the drafts last: they are short, and end beside the last contexts)
+    const unsigned of_contexts = (unsigned)P.n_kv * a.tiles_p * a.n_trees * a.parts_p;
     unsigned id = blockIdx.x;
-    const bool drafts = id < of_drafts;
-    if (!drafts)
-        id -= of_drafts;
+    const bool drafts = id >= of_contexts;
+    if (drafts)
+        id -= of_contexts;
     const int kvh = (int)(id % (unsigned)P.n_kv);
     id /= (unsigned)P.n_kv;
     const unsigned tiles = drafts ? a.tiles_o : a.tiles_p;
@@ -135,25 +136,71 @@ __global__ __launch_bounds__(64 * kPartWaves, 2) void k_tree_whole(const be42_kv
     write_part<HD, QB, 2 * kPartWaves, 16>(a, S, row0, rows, first, kvh, G, 0);
 }
 
-// The parts of every row that a tree has; the others' are left as they are.
-template <int HD, bool QB>
-__global__ __launch_bounds__(256) void k_tree_join(const TreeArgs a, int parts)
+// The parts of the rows that trees have (the others' are left as they are), a workgroup a
+// few rows of a tree's.  MANY parts: a wave a row (join_row).  Few: HD / 4 lanes a row,
+// all its loads in flight together.  (With four rows for the same lanes, one after the
+// other, 6168 rows took 9 us.)
+constexpr int kFewParts = 8;
+template <int HD>
+constexpr int kJoinRows = 256 / (HD / 4);
+template <int HD, bool QB, bool MANY>
+__global__ __launch_bounds__(256) void k_tree_join(const TreeArgs a, int parts, int chunks)
 {
-    const size_t row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= (size_t)a.n_queries * a.n_heads)
-        return;
-    const int tok = (int)(row / a.n_heads), lane = threadIdx.x & 63;
-    bool in = false;
-    for (int b = 0; b < a.n_trees; b += kWave)
-        if (b + lane < a.n_trees) {
-            int first;
-            const int n = tree_tokens(a, b + lane, first);
-            in |= tok >= first && tok < first + n;
-        }
-    if (__any(in))
-        join_row<HD, QB>(a, parts, row);
+    constexpr int L = HD / 4, ROWS = MANY ? 4 : kJoinRows<HD>;
+    const int b = (int)(blockIdx.x / (unsigned)chunks), c0 = (int)(blockIdx.x % (unsigned)chunks) * ROWS;
+    int first;
+    const int rows = tree_tokens(a, b, first) * a.n_heads, d = 4 * (threadIdx.x % L);
+    const size_t all = (size_t)a.n_queries * a.n_heads, row0 = (size_t)first * a.n_heads;
+    if constexpr (MANY) {
+        const int r = c0 + (threadIdx.x >> 6);
+        if (r < rows)
+            join_row<HD, QB>(a, parts, row0 + r);
+    } else {
+        const int r = c0 + threadIdx.x / L;
+        if (r >= rows)
+            return;
+        const float2 *ml = (const float2 *)a.part_ml;
+        const float sc = log2_scale(a);
+        const size_t row = row0 + r;
+        float2 x[kFewParts];
+        float4 o[kFewParts];
+#pragma unroll
+        for (int j = 0; j < kFewParts; j++)
+            if (j < parts) {
+                const size_t at = j * all + row;
+                x[j] = ml[at];
+                o[j] = *(const float4 *)(a.part_o + at * HD + d);
+            }
+        float top = -INFINITY, l = 0.0f;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int j = 0; j < kFewParts; j++)
+            if (j < parts)
+                top = fmaxf(top, x[j].x);
+#pragma unroll
+        for (int j = 0; j < kFewParts; j++)
+            // (a part without tokens left no values)
+            if (j < parts && x[j].x != -INFINITY) {
+                const float w = __builtin_amdgcn_exp2f((x[j].x - top) * sc);
+                l = __fmaf_rn(w, x[j].y, l);
+                v.x = __fmaf_rn(w, o[j].x, v.x);
+                v.y = __fmaf_rn(w, o[j].y, v.y);
+                v.z = __fmaf_rn(w, o[j].z, v.z);
+                v.w = __fmaf_rn(w, o[j].w, v.w);
+            }
+        const float inv = row_inverse(top, l);
+        store_out4<QB>(a.out, row * HD + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+    }
 }
 
+// Rows of a context's tile: 16 where all of a tree fit (64 trees of 4 INT8 drafts, four
+// heads a KV head, over up to 2048 tokens 38 us, 57 in tiles of 64), up to 192 in tiles
+// of 64 (32 bf16 rows over 8 x 8192 tokens fp32 42 us, 16: 49, 128: 56; 183 INT8 rows 60,
+// 128: 67), more in tiles of 128 (256 rows over 32768 tokens 459, 64: 483).  Two
+// workgroups a CU (four of tiles of 16), of no less than 512 tokens (128), since each
+// takes 5 us before and after its tokens (one tree of 128 rows over 8192 tokens 23 us, in
+// parts of 256 28), and of no more than 4096: lengths differ, and the longest is the last
+// (32768 tokens in parts of 16384 650 us).
 static void plan_tree(TreeArgs &a, int n_kv)
 {
     const int G = a.n_heads / n_kv, unit = kPartWaves * kStep;
@@ -165,10 +212,11 @@ static void plan_tree(TreeArgs &a, int n_kv)
         a.parts_p = 1;
         return;
     }
-    a.rows_p = rows > 64 ? 128 : rows > 16 ? 64 : 16;
+    a.rows_p = rows > 192 ? 128 : rows > 16 ? 64 : 16;
     a.tiles_p = (int)((rows + a.rows_p - 1) / a.rows_p);
     a.parts_o = 1;
-    cut(a.max_len, (long)a.tiles_p * n_kv * a.n_trees, unit, 512, &a.parts_p, &a.chunk_p);
+    const long tiles = (long)a.tiles_p * n_kv * a.n_trees;
+    cut(a.max_len, tiles, a.rows_p == 16 ? unit : 4 * unit, std::max(a.rows_p == 16 ? 1024L : 512L, tiles * ((a.max_len + 4095L) / 4096)), &a.parts_p, &a.chunk_p);
 }
 
 }  // namespace be42
@@ -250,6 +298,7 @@ extern "C" int be42_tree_attention(const be42_kv_pool *pool, const void *q, int 
         a.part_o = (float *)workspace;
         a.part_ml = a.part_o + (size_t)parts * rows * P.head_dim;
     }
+    const int join_rows = parts > kFewParts ? 4 : P.head_dim == 64 ? kJoinRows<64> : kJoinRows<128>, chunks = (max_tree * n_heads + join_rows - 1) / join_rows;
     auto go = [&](auto kv8, auto hd, auto qb) {
         constexpr bool KV8 = decltype(kv8)::value, QB = decltype(qb)::value;
         constexpr int HD = decltype(hd)::value;
@@ -264,8 +313,12 @@ extern "C" int be42_tree_attention(const be42_kv_pool *pool, const void *q, int 
             hipLaunchKernelGGL((k_tree_part<KV8, HD, QB, 2>), g, t, 0, s, P, a);
         else
             hipLaunchKernelGGL((k_tree_part<KV8, HD, QB, 0>), g, t, 0, s, P, a);
-        if (parts > 1)
-            hipLaunchKernelGGL((k_tree_join<HD, QB>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a, parts);
+        if (parts > 1) {
+            if (parts > kFewParts)
+                hipLaunchKernelGGL((k_tree_join<HD, QB, true>), dim3((unsigned)(n_trees * chunks)), dim3(256), 0, s, a, parts, chunks);
+            else
+                hipLaunchKernelGGL((k_tree_join<HD, QB, false>), dim3((unsigned)(n_trees * chunks)), dim3(256), 0, s, a, parts, chunks);
+        }
     };
     auto of_type = [&](auto kv8, auto hd) { q_bf16 ? go(kv8, hd, std::true_type()) : go(kv8, hd, std::false_type()); };
     auto of_dim = [&](auto kv8) {

@@ -64,6 +64,62 @@ __device__ __forceinline__ void publish(const be42_kv_pool &P, int slot, int pos
         P.n_indexed[slot] = blk + 1;
 }
 
+// seal_page of a page whose rows the workgroup has just written, the same sums in the
+// same order; the projection was brought to LDS while the rows were on their way (by
+// load_projection: the chain of the hash's products waits for a load of it every few
+// terms otherwise, and a seal takes 5 us; accepted drafts of 28 layers 6.6
+// us with it, 4.6 without).
+template <int HD = 256>
+struct SealShared {
+    float hp[HD * 16], c[HD];
+};
+template <class S_>
+__device__ __forceinline__ void load_projection(const be42_kv_pool &P, S_ &S)
+{
+    for (int i = threadIdx.x; i < P.head_dim * 4; i += 256)
+        *(float4 *)&S.hp[4 * i] = *(const float4 *)(P.hpT + 4 * i);
+}
+template <bool BF16, class S_>
+__device__ __forceinline__ void seal_written(const be42_kv_pool &P, S_ &S, int slot, int blk, int phys)
+{
+    const int d = threadIdx.x, hd = P.head_dim;
+    __syncthreads();                       // the page's rows are in memory
+    const size_t head0 = (size_t)phys * P.n_kv * kPage;
+    if (d < hd) {
+        float x[kPage], acc = 0.0f;
+#pragma unroll
+        for (int t = 0; t < kPage; t++)
+            x[t] = BF16 ? bf16_to_f32(((const uint16_t *)P.k)[(head0 + t) * hd + d])
+                        : (float)((const int8_t *)P.k)[(head0 + t) * hd + d] * P.k_scale[head0 + t];
+#pragma unroll
+        for (int t = 0; t < kPage; t++)
+            acc = acc + x[t];
+        acc = acc * (1.0f / (float)kPage);
+        S.c[d] = acc;
+        P.centroid[(size_t)phys * hd + d] = acc;
+    }
+    __syncthreads();
+    if (d >= kWave)
+        return;
+    // (head_dim is a multiple of 8)
+    float s = 0.0f;
+    if (d < 16)
+        for (int i = 0; i < hd; i += 8) {
+            float c[8], h[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                c[j] = S.c[i + j];
+                h[j] = S.hp[(i + j) * 16 + d];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                s = __fmaf_rn(c[j], h[j], s);
+        }
+    const unsigned long long m = __ballot(d < 16 && s > 0.0f);
+    if (d == 0)
+        P.page_hash[(size_t)slot * P.max_logical + blk] = (uint16_t)(m & 0xFFFFu);
+}
+
 template <bool BF16>
 __device__ __forceinline__ float act_at(const void *p, size_t i)
 {
@@ -115,7 +171,7 @@ template <bool KV8, bool BF16, int HD>
 __global__ __launch_bounds__(256) void k_rope_append_words(const be42_kv_pool P, const RopeArgs a, const RopeIn x)
 {
     constexpr int L = HD / 8, PER = 256 / L, TOKENS = PER < kPage ? PER : kPage, VS = kPage + 8;
-    __shared__ float c[256];
+    __shared__ __align__(16) SealShared<HD> seal;
     __shared__ __align__(16) uint16_t vt[KV8 ? 1 : HD][VS];
     const int h = blockIdx.y, z = blockIdx.z, grp = threadIdx.x / L, l = threadIdx.x % L;
     const Piece &p = a.piece[piece_of(a, blockIdx.x)];
@@ -126,6 +182,9 @@ __global__ __launch_bounds__(256) void k_rope_append_words(const be42_kv_pool P,
     const int G = x.n_heads / P.n_kv, half = x.rope_dim / 2;
     const bool kv = z == 0, two = kv || 2 * z <= G;
     const int head = h * G + 2 * (z - 1);
+    const bool seals = kv && h == 0 && off0 + T == kPage;
+    if (seals)
+        load_projection(P, seal);
     if (kv && h == 0 && threadIdx.x == 0)
         publish(P, p.slot, p.pos0, p.n, blk, phys, entry & kNewPage);
     // the lane's two words
@@ -242,10 +301,8 @@ __global__ __launch_bounds__(256) void k_rope_append_words(const be42_kv_pool P,
             for (int i = threadIdx.x; i < 2 * HD; i += 256)
                 *(uint4 *)(to + 8 * i) = *(const uint4 *)&vt[i / 2][8 * (i % 2)];
         }
-    if (h == 0 && off0 + T == kPage) {
-        __syncthreads();                   // the page's rows are in memory
-        seal_page<!KV8>(P.k, P.k_scale, P.centroid, P.page_hash + (size_t)p.slot * P.max_logical + blk, phys, P.hpT, P.n_kv, HD, c);
-    }
+    if (seals)
+        seal_written<!KV8>(P, seal, p.slot, blk, phys);
 }
 
 // Any other head, or rotation: one wave a row, a lane a pair of elements (two pairs where head_dim is past 128):
@@ -253,7 +310,7 @@ __global__ __launch_bounds__(256) void k_rope_append_words(const be42_kv_pool P,
 template <bool KV8, bool BF16, int NP>
 __global__ __launch_bounds__(256) void k_rope_append(const be42_kv_pool P, const RopeArgs a, const RopeIn x)
 {
-    __shared__ float c[256];
+    __shared__ __align__(16) SealShared<> seal;
     const int h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Piece &u = a.piece[piece_of(a, blockIdx.x)];
     const int blk = u.pos0 / kPage + ((int)blockIdx.x - u.page0);
@@ -261,6 +318,9 @@ __global__ __launch_bounds__(256) void k_rope_append(const be42_kv_pool P, const
     const int lo = max(u.pos0, blk * kPage), T = min(u.pos0 + u.n, (blk + 1) * kPage) - lo;
     const int tok0 = u.tok0 + lo - u.pos0, off0 = lo - blk * kPage;
     const int hd = P.head_dim, G = x.n_heads / P.n_kv, half = x.rope_dim / 2;
+    const bool seals = h == 0 && off0 + T == kPage;
+    if (seals)
+        load_projection(P, seal);
     if (h == 0 && threadIdx.x == 0)
         publish(P, u.slot, u.pos0, u.n, blk, phys, entry & kNewPage);
     for (int r = wave; r < T * (G + 2); r += 4) {
@@ -355,19 +415,21 @@ __global__ __launch_bounds__(256) void k_rope_append(const be42_kv_pool P, const
                 }
         }
     }
-    if (h == 0 && off0 + T == kPage) {
-        __syncthreads();                   // the page's rows are in memory
-        seal_page<!KV8>(P.k, P.k_scale, P.centroid, P.page_hash + (size_t)u.slot * P.max_logical + blk, phys, P.hpT, P.n_kv, hd, c);
-    }
+    if (seals)
+        seal_written<!KV8>(P, seal, u.slot, blk, phys);
 }
 
-// Pieces of a launch of be42_kv_accept, the same for each of its layers; tokens to
-// take, and the physical page of every page touched, layer after layer.
+// Pieces of a launch of be42_kv_accept, the same for each of its layers, and the tokens
+// to take.  Pages that are old in every layer are looked up in the page tables; the
+// others are listed, layer after layer (a page for every one of 28 layers x 25 pages
+// would take two launches).
 constexpr int kTakes = 64, kTaken = 256, kTakePages = 352;
 struct TakeArgs {
-    int n, n_pages, layer0, from_step, to_step;
+    int n, n_pages, n_listed, layer0, from_step, to_step;
     struct {
-        int from, slot, pos0, n, tok0, page0;
+        int from, slot, pos0;
+        short n, tok0, page0, list0;   // list0: its first listed page's place in a layer's
+        uint32_t listed;               // which of its pages (at most 17)
     } piece[kTakes];
     int index[kTaken];
     int pages[kTakePages];
@@ -376,14 +438,20 @@ struct TakeArgs {
 template <bool KV8>
 __global__ __launch_bounds__(256) void k_kv_accept(const be42_kv_pool P, const TakeArgs a)
 {
-    __shared__ float c[256];
+    __shared__ __align__(16) SealShared<> seal;
     const int h = blockIdx.y, layer = blockIdx.z, hd = P.head_dim;
     const auto &u = a.piece[piece_of(a, blockIdx.x)];
     const int from = u.from + (a.layer0 + layer) * a.from_step, slot = u.slot + (a.layer0 + layer) * a.to_step;
     const int blk = u.pos0 / kPage + ((int)blockIdx.x - u.page0);
-    const int entry = a.pages[layer * a.n_pages + blockIdx.x], phys = entry & ~kNewPage;
+    const int j = (int)blockIdx.x - u.page0;
+    const int entry = u.listed >> j & 1 ? a.pages[layer * a.n_listed + u.list0 + __popc(u.listed & ((1u << j) - 1))]
+                                        : P.page_table[(size_t)slot * P.max_logical + blk];
+    const int phys = entry & ~kNewPage;
     const int lo = max(u.pos0, blk * kPage), T = min(u.pos0 + u.n, (blk + 1) * kPage) - lo;
     const int off0 = lo - blk * kPage;
+    const bool seals = h == 0 && off0 + T == kPage;
+    if (seals)
+        load_projection(P, seal);
     if (h == 0 && threadIdx.x == 0)
         publish(P, slot, u.pos0, u.n, blk, phys, entry & kNewPage);
     // eight elements of a token's row a thread, all tokens beside each other: one chain of
@@ -414,10 +482,8 @@ __global__ __launch_bounds__(256) void k_kv_accept(const be42_kv_pool P, const T
                 ((uint16_t *)P.v)[(head * hd + d + e) * kPage + off] = v[e];
         }
     }
-    if (h == 0 && off0 + T == kPage) {
-        __syncthreads();                   // the page's rows are in memory
-        seal_page<!KV8>(P.k, P.k_scale, P.centroid, P.page_hash + (size_t)slot * P.max_logical + blk, phys, P.hpT, P.n_kv, hd, c);
-    }
+    if (seals)
+        seal_written<!KV8>(P, seal, slot, blk, phys);
 }
 
 static int rope_append(be42_kv_pool *pool, const be42_kv_run *runs, int n_runs, const RopeIn &x, bool bf16, hipStream_t s)
@@ -519,12 +585,31 @@ static int kv_accept(be42_kv_pool *pool, const be42_kv_take *runs, int n_runs, c
     size_t first = 0;                                        // of the pages of a layer
     int toks = 0;
     auto launch = [&]() {
-        const int most = kTakePages / a.n_pages;
+        // the pages that are new somewhere
+        a.n_listed = 0;
+        for (int i = 0; i < a.n; i++) {
+            auto &u = a.piece[i];
+            const int np = (i + 1 < a.n ? a.piece[i + 1].page0 : a.n_pages) - u.page0;
+            u.list0 = (short)a.n_listed;
+            u.listed = 0;
+            for (int j = 0; j < np; j++)
+                for (int l = 0; l < n_layers; l++)
+                    if (pages[l * per_layer + first + u.page0 + j] & kNewPage) {
+                        u.listed |= 1u << j;
+                        a.n_listed++;
+                        break;
+                    }
+        }
+        const int most = a.n_listed ? kTakePages / a.n_listed : n_layers;
         for (int l = 0; l < n_layers; l += most) {
             const int n = std::min(most, n_layers - l);
             a.layer0 = l;
-            for (int i = 0; i < n; i++)
-                std::copy_n(pages.begin() + (l + i) * per_layer + first, a.n_pages, a.pages + i * a.n_pages);
+            int at = 0;
+            for (int k = 0; a.n_listed && k < n; k++)
+                for (int i = 0; i < a.n; i++)
+                    for (int j = 0; a.piece[i].listed >> j; j++)
+                        if (a.piece[i].listed >> j & 1)
+                            a.pages[at++] = pages[(l + k) * per_layer + first + a.piece[i].page0 + j];
             const dim3 g(a.n_pages, P.n_kv, n);
             if (P.kind == BE42_KV_INT8)
                 hipLaunchKernelGGL(k_kv_accept<true>, g, dim3(256), 0, s, P, a);
@@ -538,24 +623,19 @@ static int kv_accept(be42_kv_pool *pool, const be42_kv_take *runs, int n_runs, c
     for (int r = 0; r < n_runs; r++) {
         int pos = runs[r].pos0, left = runs[r].count;
         while (left) {
-            if (a.n == kTakes || toks == kTaken || a.n_pages == kTakePages) {
-                launch();
-                continue;
-            }
-            // as many tokens and pages as the launch has room for
+            // as many tokens as the launch has room for; a piece ends with a page or
+            // with its run
             int n = std::min(left, kTaken - toks);
-            n = std::min(n, (pos / kPage + kTakePages - a.n_pages) * kPage - pos);
-            // a piece ends with a page or with its run
-            const int np = (pos + n - 1) / kPage - pos / kPage + 1;
             if (n < left)
-                n = np > 1 || (pos + n) % kPage == 0 ? (pos + n) / kPage * kPage - pos : 0;
-            if (!n) {
+                n = std::max((pos + n) / kPage * kPage - pos, 0);
+            const int np = (pos + n - 1) / kPage - pos / kPage + 1;
+            if (a.n == kTakes || n <= 0 || a.n_pages + np > kTakePages) {
                 launch();
                 continue;
             }
-            a.piece[a.n++] = {runs[r].from, runs[r].to, pos, n, toks, a.n_pages};
+            a.piece[a.n++] = {runs[r].from, runs[r].to, pos, (short)n, (short)toks, (short)a.n_pages, 0, 0};
             std::copy_n(index + at, n, a.index + toks);
-            a.n_pages += (pos + n - 1) / kPage - pos / kPage + 1;
+            a.n_pages += np;
             toks += n;
             at += n;
             pos += n;

@@ -446,7 +446,8 @@ __global__ __launch_bounds__(256) void k_kv_accept(const be42_kv_pool P, const T
     const int j = (int)blockIdx.x - u.page0;
     const int entry = u.listed >> j & 1 ? a.pages[layer * a.n_listed + u.list0 + __popc(u.listed & ((1u << j) - 1))]
                                         : P.page_table[(size_t)slot * P.max_logical + blk];
-    const int phys = entry & ~kNewPage;
+    // (inside the pool also where the tables are not those that the host knows)
+    const int phys = min(max(entry, 0) & ~kNewPage, P.capacity - 1);
     const int lo = max(u.pos0, blk * kPage), T = min(u.pos0 + u.n, (blk + 1) * kPage) - lo;
     const int off0 = lo - blk * kPage;
     const bool seals = h == 0 && off0 + T == kPage;

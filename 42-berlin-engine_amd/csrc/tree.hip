@@ -33,42 +33,76 @@ __device__ __forceinline__ int tree_tokens(const TreeArgs &a, int b, int &first)
     return min(min(max(a.starts[b + 1], first), a.n_queries) - first, a.max_tree);
 }
 
-struct TreeMask {
-    int parents[kMaxTree];
+struct TreePaths {
+    static constexpr int kWords = kMaxTree / 32;
+    int up[kMaxTree];
+    uint32_t above[kMaxTree][kWords + 1];         // (rows on distinct banks)
+};
+template <int HD, int N>
+struct TreeShared {
+    union {
+        PartShared<HD, N> sums;
+        TreePaths paths;                          // done with before there are sums
+    };
     uint32_t bits[16][SeesPath::kWords];
 };
+static_assert(SeesPath::kWords == TreePaths::kWords + 1 && kMaxTree == 64 * kPartWaves, "a tree from anywhere in a page on; a draft a thread");
 
 // The paths of a tile's rows, from row `row0` of the tree on; bit 0 is token `lo` of
-// the drafts' slot.  A parent that is no earlier draft ends the path, as -1 does.
-__device__ __forceinline__ SeesPath tree_mask(const TreeArgs &a, TreeMask &M, int first, int n, int lo, int hi, int row0, int rows, int G)
+// the drafts' slot.  A parent that is no earlier draft ends the path, as -1 does.  A
+// thread has a draft and what is known of its path, and doubles it each time: the path
+// of the draft where its own ends so far.  (With a thread a row that walks up draft by
+// draft, calls of four chains of 256 took 40 us, with this 16.)
+template <class S>
+__device__ __forceinline__ SeesPath tree_mask(const TreeArgs &a, S &shared, int first, int n, int lo, int hi, int row0, int rows, int G)
 {
-    for (int i = threadIdx.x; i < n; i += blockDim.x)
-        M.parents[i] = a.parents ? a.parents[first + i] : i - 1;
-    for (int i = threadIdx.x; i < 16 * SeesPath::kWords; i += blockDim.x)
-        (&M.bits[0][0])[i] = 0;
-    __syncthreads();
-    if (threadIdx.x < 16) {
-        int at = min(row0 + (int)threadIdx.x, rows - 1) / G;
-        while (at >= 0) {
-            const int bit = first + at - lo;
-            if (first + at < hi)
-                M.bits[threadIdx.x][bit >> 5] |= 1u << (bit & 31);
-            const int up = M.parents[at];
-            at = up < at ? up : -1;
+    constexpr int W = TreePaths::kWords;
+    TreePaths &M = shared.paths;
+    const int i = threadIdx.x, last = min(row0 + 15, rows - 1) / G;
+    uint32_t path[W];
+#pragma unroll
+    for (int w = 0; w < W; w++)
+        path[w] = i >> 5 == w ? 1u << (i & 31) : 0u;
+    int up = -1;
+    if (i <= last) {
+        up = a.parents ? a.parents[first + i] : i - 1;
+        up = up < i ? max(up, -1) : -1;
+    }
+    while (true) {
+        M.up[i] = up;
+#pragma unroll
+        for (int w = 0; w < W; w++)
+            M.above[i][w] = path[w];
+        if (!__syncthreads_or(up >= 0))
+            break;
+        int next = -1;
+        if (up >= 0) {
+            next = M.up[up];
+#pragma unroll
+            for (int w = 0; w < W; w++)
+                path[w] |= M.above[up][w];
         }
+        up = next;
+        __syncthreads();
+    }
+    // from the tree's first draft to the page's first token, and no further than the slot
+    for (int x = threadIdx.x; x < 16 * SeesPath::kWords; x += blockDim.x) {
+        const int r = x / SeesPath::kWords, w = x % SeesPath::kWords, at = min(row0 + r, rows - 1) / G, shift = first - lo;
+        auto held = [&](int v) {
+            const int left = hi - first - 32 * v;
+            return v < 0 || v >= W || left <= 0 ? 0u : M.above[at][v] & (left < 32 ? (1u << left) - 1 : ~0u);
+        };
+        shared.bits[r][w] = held(w) << shift | (uint32_t)((uint64_t)held(w - 1) << shift >> 32);
     }
     __syncthreads();
-    return {&M.bits[0][0], first - lo, hi - lo};
+    return {&shared.bits[0][0], first - lo, hi - lo};
 }
 
 template <bool KV8, int HD, bool QB, int R>
 __global__ __launch_bounds__(64 * kPartWaves, 2) void k_tree_part(const be42_kv_pool P, const TreeArgs a)
 {
     __shared__ union {
-        struct {
-            PartShared<HD> few;
-            TreeMask mask;
-        };
+        TreeShared<HD, kPartWaves> few;
         std::conditional_t<R != 0, WideShared<KV8, HD, R ? R : 4>, char> many;
     } S;
     constexpr int NP = QB ? 1 : 3, PP = QB ? 2 : 3, kRows = R ? 32 * R : 16;
@@ -91,10 +125,10 @@ __global__ __launch_bounds__(64 * kPartWaves, 2) void k_tree_part(const be42_kv_
         return;
     if (drafts) {
         const int lo = first / kPage * kPage, hi = max(first, slot_tokens(P, a.draft_slot, first + n));
-        const SeesPath seen = tree_mask(a, S.mask, first, n, lo, hi, row0, rows, G);
-        part16<KV8, HD, NP, PP>(P, a, S.few, a.draft_slot, lo, hi, kvh, first, row0, rows, wave, kPartWaves, wave, 0, seen);
+        const SeesPath seen = tree_mask(a, S.few, first, n, lo, hi, row0, rows, G);
+        part16<KV8, HD, NP, PP>(P, a, S.few.sums, a.draft_slot, lo, hi, kvh, first, row0, rows, wave, kPartWaves, wave, 0, seen);
         __syncthreads();
-        write_part<HD, QB, kPartWaves, 16>(a, S.few, row0, rows, first, kvh, G, a.parts_p);
+        write_part<HD, QB, kPartWaves, 16>(a, S.few.sums, row0, rows, first, kvh, G, a.parts_p);
         return;
     }
     const int slot = a.slots ? a.slots[b] : b, lo = part * a.chunk_p;
@@ -103,10 +137,10 @@ __global__ __launch_bounds__(64 * kPartWaves, 2) void k_tree_part(const be42_kv_
         part32<KV8, HD, NP, PP, R>(P, a, S.many, slot, lo, want, kvh, first, row0, rows);
         write_part<HD, QB, kPartWaves / R, kRows>(a, S.many.sums, row0, rows, first, kvh, G, part);
     } else {
-        part16<KV8, HD, NP, PP>(P, a, S.few, slot, lo, max(lo, slot_tokens(P, slot, want)), kvh, first, row0, rows, wave, kPartWaves,
+        part16<KV8, HD, NP, PP>(P, a, S.few.sums, slot, lo, max(lo, slot_tokens(P, slot, want)), kvh, first, row0, rows, wave, kPartWaves,
                                 wave, 0);
         __syncthreads();
-        write_part<HD, QB, kPartWaves, 16>(a, S.few, row0, rows, first, kvh, G, part);
+        write_part<HD, QB, kPartWaves, 16>(a, S.few.sums, row0, rows, first, kvh, G, part);
     }
 }
 
@@ -114,8 +148,7 @@ __global__ __launch_bounds__(64 * kPartWaves, 2) void k_tree_part(const be42_kv_
 template <bool KV8, int HD, bool QB>
 __global__ __launch_bounds__(64 * kPartWaves, 2) void k_tree_whole(const be42_kv_pool P, const TreeArgs a)
 {
-    __shared__ PartShared<HD, 2 * kPartWaves> S;
-    __shared__ TreeMask M;
+    __shared__ TreeShared<HD, 2 * kPartWaves> S;
     constexpr int NP = QB ? 1 : 3, PP = QB ? 2 : 3;
     const int G = a.n_heads / P.n_kv, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     unsigned id = blockIdx.x;
@@ -126,14 +159,14 @@ __global__ __launch_bounds__(64 * kPartWaves, 2) void k_tree_whole(const be42_kv
     const int n = tree_tokens(a, b, first), rows = n * G;
     if (row0 >= rows)
         return;
+    const int lo = first / kPage * kPage, hi = max(first, slot_tokens(P, a.draft_slot, first + n));
+    const SeesPath seen = tree_mask(a, S, first, n, lo, hi, row0, rows, G);
     const int slot = a.slots ? a.slots[b] : b;
     const int want = a.lens ? min(a.lens[b], a.max_len) : a.max_len;
-    part16<KV8, HD, NP, PP>(P, a, S, slot, 0, slot_tokens(P, slot, want), kvh, first, row0, rows, wave, kPartWaves, wave, 0);
-    const int lo = first / kPage * kPage, hi = max(first, slot_tokens(P, a.draft_slot, first + n));
-    const SeesPath seen = tree_mask(a, M, first, n, lo, hi, row0, rows, G);
-    part16<KV8, HD, NP, PP>(P, a, S, a.draft_slot, lo, hi, kvh, first, row0, rows, wave, kPartWaves, kPartWaves + wave, 0, seen);
+    part16<KV8, HD, NP, PP>(P, a, S.sums, slot, 0, slot_tokens(P, slot, want), kvh, first, row0, rows, wave, kPartWaves, wave, 0);
+    part16<KV8, HD, NP, PP>(P, a, S.sums, a.draft_slot, lo, hi, kvh, first, row0, rows, wave, kPartWaves, kPartWaves + wave, 0, seen);
     __syncthreads();
-    write_part<HD, QB, 2 * kPartWaves, 16>(a, S, row0, rows, first, kvh, G, 0);
+    write_part<HD, QB, 2 * kPartWaves, 16>(a, S.sums, row0, rows, first, kvh, G, 0);
 }
 
 // The parts of the rows that trees have (the others' are left as they are), a workgroup a
@@ -284,6 +317,9 @@ extern "C" int be42_tree_attention(const be42_kv_pool *pool, const void *q, int 
     const int parts = a.parts_p + a.parts_o;
     const double blocks = (double)P.n_kv * n_trees * (a.whole ? a.tiles_o : (double)a.tiles_p * a.parts_p + a.tiles_o);
     BE42_CHECK(blocks <= kMaxBlocks, "be42_tree_attention: %d trees of up to %d drafts of %d heads", n_trees, max_tree, n_heads);
+    const int join_rows = parts > kFewParts ? 4 : P.head_dim == 64 ? kJoinRows<64> : kJoinRows<128>;
+    const long chunks = ((long)max_tree * n_heads + join_rows - 1) / join_rows;
+    BE42_CHECK(chunks * n_trees <= kMaxBlocks, "be42_tree_attention: %d trees of up to %d drafts of %d heads", n_trees, max_tree, n_heads);
     const size_t need = be42_tree_attention_workspace_bytes(n_tokens, n_trees, n_heads, P.n_kv, P.head_dim, max_tree, max_len);
     BE42_CHECK(!workspace || (!((uintptr_t)workspace & 15) && workspace_bytes >= need),
                "be42_tree_attention: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, need);
@@ -298,7 +334,6 @@ extern "C" int be42_tree_attention(const be42_kv_pool *pool, const void *q, int 
         a.part_o = (float *)workspace;
         a.part_ml = a.part_o + (size_t)parts * rows * P.head_dim;
     }
-    const int join_rows = parts > kFewParts ? 4 : P.head_dim == 64 ? kJoinRows<64> : kJoinRows<128>, chunks = (max_tree * n_heads + join_rows - 1) / join_rows;
     auto go = [&](auto kv8, auto hd, auto qb) {
         constexpr bool KV8 = decltype(kv8)::value, QB = decltype(qb)::value;
         constexpr int HD = decltype(hd)::value;
@@ -315,9 +350,9 @@ extern "C" int be42_tree_attention(const be42_kv_pool *pool, const void *q, int 
             hipLaunchKernelGGL((k_tree_part<KV8, HD, QB, 0>), g, t, 0, s, P, a);
         if (parts > 1) {
             if (parts > kFewParts)
-                hipLaunchKernelGGL((k_tree_join<HD, QB, true>), dim3((unsigned)(n_trees * chunks)), dim3(256), 0, s, a, parts, chunks);
+                hipLaunchKernelGGL((k_tree_join<HD, QB, true>), dim3((unsigned)(n_trees * chunks)), dim3(256), 0, s, a, parts, (int)chunks);
             else
-                hipLaunchKernelGGL((k_tree_join<HD, QB, false>), dim3((unsigned)(n_trees * chunks)), dim3(256), 0, s, a, parts, chunks);
+                hipLaunchKernelGGL((k_tree_join<HD, QB, false>), dim3((unsigned)(n_trees * chunks)), dim3(256), 0, s, a, parts, (int)chunks);
         }
     };
     auto of_type = [&](auto kv8, auto hd) { q_bf16 ? go(kv8, hd, std::true_type()) : go(kv8, hd, std::false_type()); };

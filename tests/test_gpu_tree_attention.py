@@ -236,6 +236,36 @@ def test_bad_drafts_reach_who_sees_them(be, kind, bf16, bad, where, ctx):
                 assert (got[i].double() - clean[i].double()).abs().max() <= (2.0 ** -7 if bf16 else 2.0 ** -19) * 5, i
 
 
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("where", ["k", "v"])
+@pytest.mark.parametrize("H,ctx", [(4, 50), (4, 1603), (32, 1603), (60, 1603)])
+def test_what_lies_behind_the_lengths(be, kind, bf16, where, H, ctx):
+    """NaN in tokens of a slot from its length on, and in drafts behind the last tree."""
+    sizes, kvh, hd = [9, 8], 2, 128
+    pool, k, v = make_pool(be, kind, 3, kvh, hd, [ctx + 40, 45, 30], 28)
+    t, lens = pool.tensors(), [ctx, 13]
+    for slot, at, held in ((0, ctx, ctx + 40), (1, 13, 45), (2, 17, 30)):
+        for i in range(at, held):
+            page, off = int(pool.layer_pages(slot)[i // PAGE]), i % PAGE
+            if kind == "int8":
+                t[where + "_scale"][page, :, off] = math.nan
+            elif where == "k":
+                t["k"][page, :, off] = math.nan
+            else:
+                t["v"][page, :, :, off] = math.nan
+    run(be, pool, k, v, queries(29, 17, H, hd, bf16), H, starts_of(sizes), trees_of(np.random.default_rng(3), sizes), 2, [0, 1], lens, ctx)
+
+
+@pytest.mark.parametrize("n", [256, 255, 129, 33])
+@pytest.mark.parametrize("shape", ["chain", "one"])
+def test_the_deepest_and_the_widest(be, n, shape):
+    """A chain of all drafts behind drafts of another tree, and one root with all others below it."""
+    parents = np.concatenate([trees_of(None, [21], "chain"), np.arange(n) - 1 if shape == "chain" else np.minimum(np.arange(n), 1) - 1])
+    pool, k, v = make_pool(be, "bf16", 3, 1, 64, [700, 5, 21 + n], 30)
+    run(be, pool, k, v, queries(31, 21 + n, 3, 64, False), 3, [0, 21, 21 + n], parents, 2, [0, 1], [700, 5], 700, max_tree=256)
+
+
 def test_infinite_values_give_infinities(be):
     """Of a token that weighs something: with its sign."""
     pool, k, v = make_pool(be, "bf16", 2, 1, 64, [20, 6], 21)

@@ -802,7 +802,8 @@ static int take_workspace(const char *who, void *&workspace, size_t bytes, size_
 static int check_shape(const char *who, long m, long n, long k)
 {
     BE42_CHECK(m >= 0 && n > 0 && k > 0 && k % 16 == 0 && k <= kMaxK, "%s: m %ld, n %ld, k %ld (k a multiple of 16, at most 2^22)", who, m, n, k);
-    BE42_CHECK(((m + 31) / 32) * ((n + 15) / 16) <= kMaxBlocks, "%s: m %ld, n %ld", who, m, n);
+    // (workgroups of up to 512 threads)
+    BE42_CHECK(((m + 31) / 32) * ((n + 15) / 16) <= kMaxBlocks / 2, "%s: m %ld, n %ld", who, m, n);
     return BE42_OK;
 }
 

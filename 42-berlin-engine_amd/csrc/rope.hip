@@ -19,6 +19,7 @@ namespace be42 {
 // What a launch takes: pieces of runs, and the physical page of every page that they
 // touch.  (Arguments of a kernel are at most 4 KB.)
 constexpr int kPieces = 64, kPiecePages = 640;
+constexpr int kMaxGridYZ = 65535;
 struct Piece {
     int slot, pos0, n, tok0, page0;    // page0: its first page's place in pages
 };
@@ -55,8 +56,9 @@ __device__ __forceinline__ void publish(const be42_kv_pool &P, int slot, int pos
     const int end = pos0 + n;
     if (fresh) {
         P.page_table[(size_t)slot * P.max_logical + blk] = phys;
+        // (a replay may come after appends behind the captured ones)
         if (end <= (blk + 1) * kPage)
-            P.n_logical[slot] = blk + 1;
+            P.n_logical[slot] = max(P.n_logical[slot], blk + 1);
     }
     P.ntok[phys] = min(end - blk * kPage, kPage);
     // the last page that the piece fills
@@ -446,8 +448,10 @@ __global__ __launch_bounds__(256) void k_kv_accept(const be42_kv_pool P, const T
     const int j = (int)blockIdx.x - u.page0;
     const int entry = u.listed >> j & 1 ? a.pages[layer * a.n_listed + u.list0 + __popc(u.listed & ((1u << j) - 1))]
                                         : P.page_table[(size_t)slot * P.max_logical + blk];
-    // (inside the pool also where the tables are not those that the host knows)
-    const int phys = min(max(entry, 0) & ~kNewPage, P.capacity - 1);
+    const int phys = entry & ~kNewPage;
+    // a replay after the slot was reset: it has no such page
+    if (entry < 0 || phys >= P.capacity)
+        return;
     const int lo = max(u.pos0, blk * kPage), T = min(u.pos0 + u.n, (blk + 1) * kPage) - lo;
     const int off0 = lo - blk * kPage;
     const bool seals = h == 0 && off0 + T == kPage;
@@ -601,7 +605,7 @@ static int kv_accept(be42_kv_pool *pool, const be42_kv_take *runs, int n_runs, c
                         break;
                     }
         }
-        const int most = a.n_listed ? kTakePages / a.n_listed : n_layers;
+        const int most = std::min(a.n_listed ? kTakePages / a.n_listed : n_layers, kMaxGridYZ);
         for (int l = 0; l < n_layers; l += most) {
             const int n = std::min(most, n_layers - l);
             a.layer0 = l;
@@ -669,6 +673,7 @@ extern "C" int be42_rope_append(be42_kv_pool *pool, const be42_kv_run *runs, int
     BE42_CHECK(n_heads >= 0 && n_heads % P.n_kv == 0 && (!tokens || (n_heads == 0) == (q == nullptr)),
                "be42_rope_append: %d query heads over %d kv heads", n_heads, P.n_kv);
     BE42_CHECK(!q || q_out, "be42_rope_append: null q_out");
+    BE42_CHECK(P.n_kv <= kMaxGridYZ && n_heads / P.n_kv <= kMaxGridYZ, "be42_rope_append: %d query heads, %d kv heads", n_heads, P.n_kv);
     const long row = (long)P.n_kv * P.head_dim, qrow = (long)n_heads * P.head_dim;
     BE42_CHECK(k_stride >= row && v_stride >= row && (!q || (q_stride >= qrow && q_out_stride >= qrow)),
                "be42_rope_append: strides %d, %d, %d, %d of rows of %ld and %ld", q_stride, k_stride, v_stride,
@@ -701,6 +706,7 @@ extern "C" int be42_kv_accept(be42_kv_pool *pool, const be42_kv_take *runs, int 
     BE42_CHECK(n_runs >= 0 && n_index >= 0 && n_layers >= 0 && (long)n_runs * n_layers <= pool->n_layers,
                "be42_kv_accept: %d runs of %d layers over %d slots", n_runs, n_layers, pool->n_layers);
     BE42_CHECK(n_runs || !n_index, "be42_kv_accept: %d tokens without a run", n_index);
+    BE42_CHECK(pool->n_kv <= kMaxGridYZ, "be42_kv_accept: %d kv heads", pool->n_kv);
     if (!n_runs || !n_layers)
         return BE42_OK;
     try {

@@ -263,7 +263,9 @@ int  be42_kv_append_step(be42_kv_pool *pool, const int *slots, const int *pos, i
  * be42_kv_append stores fp32 rows.  A page whose last position is written gets its
  * centroid and hash, also where it had some.  q NULL: no queries (n_heads 0).  A
  * token whose row holds an infinity or NaN gets unspecified q and page rows; others
- * are not touched by it.  On an error nothing was appended. */
+ * are not touched by it.  Captured, it writes the pages that it found or took at the
+ * capture, which its slots keep: none of them is reset between replays.  On an error
+ * nothing was appended. */
 typedef struct be42_kv_run {
     int slot, pos0, count;
 } be42_kv_run;
@@ -281,8 +283,8 @@ int  be42_rope_append(be42_kv_pool *pool, const be42_kv_run *runs, int n_runs, i
  * runs[r].from (host array of n_index, the runs' one after the other), as the pages hold them,
  * bit for bit.  The same for each of n_layers layers: layer l takes slots from + l *
  * from_step and to + l * to_step.  A slot is filled at most once a call, and none
- * that is read from.  Pages that fill get their centroid and hash.  On an error
- * nothing was copied. */
+ * that is read from.  Pages that fill get their centroid and hash.  Captured as
+ * be42_rope_append.  On an error nothing was copied. */
 typedef struct be42_kv_take {
     int from, to, pos0, count;
 } be42_kv_take;

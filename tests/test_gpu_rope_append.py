@@ -386,6 +386,51 @@ def test_accepted_drafts(be, kind, kvh, hd, batch, layers, drafts):
             assert (after["centroid"][after["page_table"].reshape(-1, pages)[b][j]] == o["centroid"][o["page_table"][j]]).all()
 
 
+def test_replays_among_other_appends(be):
+    """A captured append and accept whose pages were new: replayed behind appends that
+    went on, which stay."""
+    pool = filled(be, "bf16", 1, 64, 4, 4, [20, 10, 0, 0], 5)
+    k = torch.randn(40, 1, 64, device="cuda")
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        be.rope_append(pool, [(2, 0, 20)], k[:20], k[:20])
+        be.kv_accept(pool, [(0, 1, 10, 10)], range(10))
+    for _ in range(3):
+        g.replay()
+    rows = held_rows(pool, 0, 10)["k"]
+    for slot, n in ((1, 20), (2, 20)):
+        be.rope_append(pool, [(slot, n, 20)], k[20:], k[20:])
+    torch.cuda.synchronize()
+    before = state(pool)
+    assert list(before["n_logical"]) == [2, 3, 3, 0]
+    k[:20] *= 2
+    g.replay()
+    torch.cuda.synchronize()
+    after = state(pool)
+    same(after, before, ("k", "v", "ntok", "centroid", "page_hash"))
+    for slot, first in ((1, rows), (2, None)):
+        got = held_rows(pool, slot, 40)["k"]
+        assert (got[20:] == k[20:].bfloat16()).all()
+        assert (got[10:20] == first).all() if slot == 1 else (got[:20] == k[:20].bfloat16()).all()
+
+
+def test_a_replayed_accept_after_a_reset_writes_nothing(be):
+    """The slot's page, an old one at the capture, is another's or nobody's by then."""
+    pool = filled(be, "int8", 2, 64, 3, 4, [20, 10, 17], 6)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        be.kv_accept(pool, [(0, 1, 10, 6)], range(6))
+    pool.reset(1)
+    torch.cuda.synchronize()
+    before = state(pool)
+    for _ in range(2):
+        g.replay()
+        torch.cuda.synchronize()
+        same(state(pool), before)
+
+
 def test_accept_refusals_change_nothing(be):
     import be42
     pool = filled(be, "int8", 1, 64, 4, 4, [20, 5, 40, 0], 3)

@@ -152,6 +152,17 @@ def test_kv_accept_refusals(lib, kw, word):  # noqa: F811
     refused(lib, lib.lib.be42_kv_accept(*a.values(), None), word)
 
 
+def test_launches_past_what_a_grid_holds_are_refused(lib):  # noqa: F811
+    """Whose first launch would fit, or whose pages would have been planned."""
+    refused(lib, block_gemm(lib, m=1, n=1 << 28), "n 268435456")
+    refused(lib, linear(lib, m=1, n=1 << 28), "n 268435456")
+    refused(lib, tree(lib, n_heads=2, q_stride=128, n_trees=200000, max_tree=256, max_len=36000), "trees of")
+    refused(lib, append(lib, n_heads=1 << 17, q_stride=1 << 23, q_out_stride=1 << 23), "heads")
+    p, r, i = pool(), runs((3, 0, 0, 1)), np.zeros(1, np.int32)
+    p.n_kv = 65536
+    refused(lib, lib.lib.be42_kv_accept(C.addressof(p), r.ctypes.data, 1, i.ctypes.data, 1, 1, 0, 0, None), "kv heads")
+
+
 def test_rope_layout_matches_the_header():
     assert [n for n, _ in be42.RopeStruct._fields_] == ["cos", "sin", "len", "dim", "interleaved"]
     assert C.sizeof(be42.RopeStruct) == 32

@@ -185,7 +185,7 @@ template <bool F8, bool YB, int WF, int WT, int TF, int TT, int NS, bool CUT, bo
 __global__ __launch_bounds__(WF *WT * 64, WF *WT == 4 ? 2 : 1) void k_block_dma(void *__restrict__ Y, const uint8_t *__restrict__ X,
                                                            const float *__restrict__ sx, const uint8_t *__restrict__ W,
                                                            const float *__restrict__ sw, int M, int N, int K, int tiles_m,
-                                                           int tiles_n)
+                                                           int tiles_n, int tile0)
 {
     constexpr int NW = WF * WT, BF = WF * TF * 16, BT = WT * TT * 16, ROWS = BF + BT;
     constexpr int kLoads = Loader<BT, BF, NW, NS, CUT>::kLoads, SBYTES = Loader<BT, BF, NW, NS, CUT>::SBYTES;
@@ -194,7 +194,7 @@ __global__ __launch_bounds__(WF *WT * 64, WF *WT == 4 ? 2 : 1) void k_block_dma(
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
     int tm, tn;
     tile_of(tiles_m, tiles_n, tm, tn);
-    const int m0 = tm * BT, n0 = tn * BF;
+    const int m0 = tm * BT, n0 = (tile0 + tn) * BF;             // tile0: the first of the features' tiles
     const int wf = wave / WT, wt = wave % WT, blocks = (K + kBlock - 1) / kBlock;
     // this workgroup's blocks: all, or with parts an equal share
     const int first = (int)((long)blocks * blockIdx.y / gridDim.y), kb = (int)((long)blocks * (blockIdx.y + 1) / gridDim.y) - first;
@@ -637,7 +637,7 @@ struct BlockArgs {
     const float *sw;
     int m, n, k;
     float *part;              // [parts][m][n] where there are several
-    int parts;
+    int parts, n0;            // n0: the first feature of the launch
     hipStream_t s;
 };
 
@@ -647,11 +647,11 @@ static void launch_dma(const BlockArgs &a)
     constexpr int BF = WF * TF * 16, BT = WT * TT * 16;
     constexpr int lds = NS * Loader<BT, BF, WF * WT, NS, false>::SBYTES;
     static_assert(lds <= 160 * 1024, "LDS budget");
-    const int tm = (a.m + BT - 1) / BT, tn = (a.n + BF - 1) / BF;
+    const int tm = (a.m + BT - 1) / BT, tn = (a.n - a.n0 + BF - 1) / BF;
     auto go = [&](auto *fn) {
         (void)hipFuncSetAttribute((const void *)fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         hipLaunchKernelGGL(fn, dim3((unsigned)tm * tn, a.parts), dim3(WF * WT * 64), lds, a.s, a.parts > 1 ? a.part : a.y, a.xq, a.sx, a.wq,
-                           a.sw, a.m, a.n, a.k, tm, tn);
+                           a.sw, a.m, a.n, a.k, tm, tn, a.n0 / BF);
     };
     auto of_k = [&](auto part) {
         constexpr bool PART = decltype(part)::value;
@@ -665,10 +665,11 @@ static void launch_dma(const BlockArgs &a)
 }
 
 template <bool YB>
-static void launch_big(void *y, const uint8_t *xq, const float *sx, const uint8_t *wq, const float *sw, int m, int n, int k, hipStream_t s)
+static void launch_big(void *y, const uint8_t *xq, const float *sx, const uint8_t *wq, const float *sw, int m, int n, int k, int tn,
+                       hipStream_t s)
 {
     constexpr int lds = 2 * Loader<256, 256, 8, 2, false>::SBYTES;
-    const int tm = (m + 255) / 256, tn = (n + 255) / 256;
+    const int tm = (m + 255) / 256;
     auto go = [&](auto *fn) {
         (void)hipFuncSetAttribute((const void *)fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         hipLaunchKernelGGL(fn, dim3((unsigned)tm * tn), dim3(512), lds, s, y, xq, sx, wq, sw, m, n, k, tm, tn);
@@ -694,6 +695,7 @@ constexpr TileTime kTileTime[kTiles] = {
 struct Plan {
     Tile tile;
     int parts;                // of the blocks, joined by a launch of their own
+    int front;                // tiles of 256 features that a launch of 256 x 256 takes before
 };
 
 // The tile, and the parts that the blocks are cut into where there are few tiles, that
@@ -702,11 +704,12 @@ struct Plan {
 // 10.7, in one 13.2; 261 x 2064 x 14352 30.9 in 3 parts of 64 x 128, 52.6 in one of 64 x
 // 64, 67.5 in 2 of 128 x 128; 512 x 4096 x 4096 19.4, 26.4 in 128 x 128; 1024 30.0 in
 // deep 128 x 128, 34.9 in 64 x 128; 2048 x 14336 x 4096 141 in 256 x 256, 168 in 128 x
-// 128; 8192^3 532, 648.)
+// 128; 8192^3 532, 648; 4096 x 14336 x 4096 282, with the codes, in three rounds of 256 x
+// 256 and 2048 features in 128 x 128, all in 256 x 256 293.)
 static Plan plan_block(long m, long n, long k, bool yb)
 {
     const long blocks = (k + kBlock - 1) / kBlock;
-    Plan best = {kTile64, 1};
+    Plan best = {kTile64, 1, 0};
     double least = 1e30;
     for (int t = 0; t < kTiles; t++) {
         const TileTime &x = kTileTime[t];
@@ -727,7 +730,27 @@ static Plan plan_block(long m, long n, long k, bool yb)
                 us += 3.0 + 8.0 * parts * m * n / 5e6;
             if (us < least) {
                 least = us;
-                best = {(Tile)t, parts};
+                best = {(Tile)t, parts, 0};
+            }
+        }
+    }
+    if (best.tile != kTile256)
+        return best;
+    // whole rounds of the 256 CUs, and what is left of the features in smaller tiles
+    const long tm = (m + 255) / 256, tn = (n + 255) / 256, rounds = (tm * tn + 255) / 256;
+    for (long r = rounds - 1; r > 0 && r > rounds - 3; r--) {
+        const long front = std::min<long>(256 * r / tm, tn - 1);
+        if (front <= 0)
+            break;
+        const double before = 3.0 + (double)((tm * front + 255) / 256) * blocks * kTileTime[kTile256].one[yb];
+        for (int t = 0; t < kTile256; t++) {
+            const TileTime &x = kTileTime[t];
+            const long wgs = ((m + x.bt - 1) / x.bt) * ((n - 256 * front + x.bf - 1) / x.bf);
+            const bool two = wgs > 256 && x.two[yb] > 0.0f;
+            const double us = before + 3.0 + (double)((wgs + (two ? 511 : 255)) / (two ? 512 : 256)) * blocks * (two ? x.two : x.one)[yb];
+            if (us < least) {
+                least = us;
+                best = {(Tile)t, 1, (int)front};
             }
         }
     }
@@ -761,21 +784,23 @@ static void block_gemm_of(BlockArgs a, void *workspace)
     Plan p = plan_block(a.m, a.n, a.k, YB);
     a.parts = p.parts;
     a.part = (float *)workspace;
+    a.n0 = 256 * p.front;
+    if constexpr (YB)
+        if (p.front || p.tile == kTile256)
+            launch_big<true>(a.y, a.xq, a.sx, a.wq, a.sw, a.m, a.n, a.k, p.front ? p.front : (a.n + 255) / 256, a.s);
     switch (p.tile) {
     case kTile64: launch_dma<F8, YB, 2, 2, 2, 2, 4>(a); break;
     case kTile64x128: launch_dma<F8, YB, 2, 2, 4, 2, 3>(a); break;
     case kTile128: launch_dma<F8, YB, 2, 2, 4, 4, 2>(a); break;
     case kTile128Deep: launch_dma<F8, YB, 2, 2, 4, 4, 4>(a); break;
-    default:
-        if constexpr (YB)
-            launch_big<true>(a.y, a.xq, a.sx, a.wq, a.sw, a.m, a.n, a.k, a.s);
+    default: break;
     }
 }
 
 static void block_gemm(void *y, bool yb, const uint8_t *xq, const float *sx, const uint8_t *wq, const float *sw, int m, int n,
                        int k, void *workspace, hipStream_t s)
 {
-    const BlockArgs a = {y, xq, sx, wq, sw, m, n, k, nullptr, 1, s};
+    const BlockArgs a = {y, xq, sx, wq, sw, m, n, k, nullptr, 1, 0, s};
     yb ? block_gemm_of<true>(a, workspace) : block_gemm_of<false>(a, workspace);
 }
 
@@ -864,7 +889,7 @@ extern "C" int be42_linear_fp8_block(void *y, int y_bf16, const void *x, int x_b
         BE42_HIP(hipGetDevice(&dev));
         if (const int rc = upload_fp8_thresholds(dev))
             return rc;
-        const BlockArgs a = {y, nullptr, nullptr, wq, sw, m, n, k, nullptr, 1, s};
+        const BlockArgs a = {y, nullptr, nullptr, wq, sw, m, n, k, nullptr, 1, 0, s};
         if (y_bf16)
             x_bf16 ? launch_few<true, 2>(a, x, x_stride) : launch_few<true, 1>(a, x, x_stride);
         else

@@ -143,6 +143,19 @@ def test_linear_is_codes_and_product(be, m, n, k, xb, yb):
         assert (got == want).all()
 
 
+@pytest.mark.parametrize("m,n,k", [(4096, 14336, 2048), (4000, 14352, 2064), (3900, 14290, 2048)])
+def test_more_tiles_than_whole_rounds(be, m, n, k):
+    """Features that go in two launches of different tiles: the same bits as alone."""
+    xq, sx, wq, sw = operands(m + n, m, n, k)
+    y = torch.full((m, n), 7.0, dtype=torch.bfloat16, device="cuda")
+    be.gemm_fp8_block(xq, sx, wq, sw, out=y)
+    for a in (0, 12160, n // 128 * 128 - 256):
+        part = y[:, a:a + 1000 if a == 0 else n].contiguous()
+        w = wq[a:a + part.shape[1]]
+        check(part, xq, sx, w, sw[a // 128:a // 128 + -(-w.shape[0] // 128)])
+        assert (be.gemm_fp8_block(xq, sx, w.contiguous(), sw[a // 128:a // 128 + -(-w.shape[0] // 128)].contiguous(), dtype=torch.bfloat16) == part).all()
+
+
 def test_rows_do_not_change_with_the_batch_in_bits_that_count(be):
     """A row's output alone and among others: the same within its tolerance."""
     xq, sx, wq, sw = operands(1, 700, 384, 1040)

@@ -16,15 +16,16 @@
 
 namespace be42 {
 
-// What a launch takes: pieces of runs, and the physical page of every page that they
-// touch.  (Arguments of a kernel are at most 4 KB.)
-constexpr int kPieces = 64, kPiecePages = 640;
+// What a launch takes: pieces of runs, whose physical pages follow one another (new ones
+// mostly do: no list, and prompts of any length in one launch) or are listed.
+constexpr int kPieces = 64, kPiecePages = 480;
 constexpr int kMaxGridYZ = 65535;
 struct Piece {
-    int slot, pos0, n, tok0, page0;    // page0: its first page's place in pages
+    int slot, pos0, n, tok0, page0;    // page0: its first page's workgroup
+    int entry0, step;                  // page j is entry0 + step * j, with step 0 pages[entry0 + j]
 };
 struct RopeArgs {
-    int n, n_pages;
+    int n, n_pages, n_listed;
     Piece piece[kPieces];
     int pages[kPiecePages];
 };
@@ -39,6 +40,14 @@ struct RopeIn {
     int n_heads, rope_len, rope_dim, interleaved;
     float eps;
 };
+// (arguments of a kernel are at most 4 KB)
+static_assert(sizeof(be42_kv_pool) + sizeof(RopeArgs) + sizeof(RopeIn) <= 4096 - 16, "arguments of a launch");
+
+// The entry of page j of a piece: its physical page, and kNewPage.
+__device__ __forceinline__ int page_entry(const RopeArgs &a, const Piece &p, int j)
+{
+    return p.step ? p.entry0 + p.step * j : a.pages[p.entry0 + j];
+}
 
 // The piece that page `at` of a launch belongs to: lanes compare, one each.
 template <class A>
@@ -167,8 +176,8 @@ __device__ __forceinline__ uint2 bf16_4(const float *v)
 // the tokens of a page, K and V or two query heads (blockIdx.z), all its loads in
 // flight together and one pair of table words for both heads; rows of V go through LDS
 // where the whole page is written, so that they leave as its lines.  Bound by HBM: 11801 bf16
-// tokens with norms, 32 query heads on 8 KV heads of 128, 86 us in two launches, 3.4
-// TB/s (243 us in the form below); 218 INT8 tokens 6.9 us (25).
+// tokens with norms, 32 query heads on 8 KV heads of 128, 79 us, 3.7 TB/s (243 us in the
+// form below; with all 740 pages listed, in two launches, 85); 218 INT8 tokens 6.9 us (25).
 template <bool KV8, bool BF16, int HD>
 __global__ __launch_bounds__(256) void k_rope_append_words(const be42_kv_pool P, const RopeArgs a, const RopeIn x)
 {
@@ -178,7 +187,7 @@ __global__ __launch_bounds__(256) void k_rope_append_words(const be42_kv_pool P,
     const int h = blockIdx.y, z = blockIdx.z, grp = threadIdx.x / L, l = threadIdx.x % L;
     const Piece &p = a.piece[piece_of(a, blockIdx.x)];
     const int blk = p.pos0 / kPage + ((int)blockIdx.x - p.page0);
-    const int entry = a.pages[blockIdx.x], phys = entry & ~kNewPage;
+    const int entry = page_entry(a, p, (int)blockIdx.x - p.page0), phys = entry & ~kNewPage;
     const int lo = max(p.pos0, blk * kPage), T = min(p.pos0 + p.n, (blk + 1) * kPage) - lo;
     const int tok0 = p.tok0 + lo - p.pos0, off0 = lo - blk * kPage;
     const int G = x.n_heads / P.n_kv, half = x.rope_dim / 2;
@@ -316,7 +325,7 @@ __global__ __launch_bounds__(256) void k_rope_append(const be42_kv_pool P, const
     const int h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Piece &u = a.piece[piece_of(a, blockIdx.x)];
     const int blk = u.pos0 / kPage + ((int)blockIdx.x - u.page0);
-    const int entry = a.pages[blockIdx.x], phys = entry & ~kNewPage;
+    const int entry = page_entry(a, u, (int)blockIdx.x - u.page0), phys = entry & ~kNewPage;
     const int lo = max(u.pos0, blk * kPage), T = min(u.pos0 + u.n, (blk + 1) * kPage) - lo;
     const int tok0 = u.tok0 + lo - u.pos0, off0 = lo - blk * kPage;
     const int hd = P.head_dim, G = x.n_heads / P.n_kv, half = x.rope_dim / 2;
@@ -499,7 +508,7 @@ static int rope_append(be42_kv_pool *pool, const be42_kv_run *runs, int n_runs, 
     if (rc)
         return rc;
     RopeArgs a;
-    a.n = a.n_pages = 0;
+    a.n = a.n_pages = a.n_listed = 0;
     auto launch = [&]() {
         const int z = 1 + (x.n_heads / P.n_kv + 1) / 2;
         auto words = [&](auto kv8, auto act, auto hd) {
@@ -524,22 +533,48 @@ static int rope_append(be42_kv_pool *pool, const be42_kv_run *runs, int n_runs, 
         };
         auto of_kind = [&](auto act) { P.kind == BE42_KV_INT8 ? of_dim(std::true_type(), act) : of_dim(std::false_type(), act); };
         bf16 ? of_kind(std::true_type()) : of_kind(std::false_type());
-        a.n = a.n_pages = 0;
+        a.n = a.n_pages = a.n_listed = 0;
     };
+    // of `want` pages from `at` on, how many follow one another (and how)
+    auto in_order = [&](size_t at, int want, int &step) {
+        step = want > 1 ? pages[at + 1] - pages[at] : 0;
+        int n = 1;
+        if (step == 1 || step == -1)
+            while (n < want && pages[at + n] - pages[at + n - 1] == step)
+                n++;
+        return n;
+    };
+    constexpr int kInOrder = 16;               // fewer are listed
     size_t at = 0;
     int tok = 0;
     for (int r = 0; r < n_runs; r++) {
         int pos = runs[r].pos0, left = runs[r].count;
         while (left) {
-            // as many of its pages as the launch has room for
-            const int want = (pos + left - 1) / kPage - pos / kPage + 1, take = std::min(want, kPiecePages - a.n_pages);
-            if (a.n == kPieces || !take) {
+            const int want = (pos + left - 1) / kPage - pos / kPage + 1;
+            int step, take = std::min(in_order(at, want, step), kMaxBlocks - a.n_pages);
+            const bool listed = take < kInOrder;
+            if (listed) {
+                // up to where some follow one another, as many as the launch has room for
+                const int room = std::min(want, kPiecePages - a.n_listed);
+                for (step = 0; take < room;) {
+                    int by;
+                    const int n = in_order(at + take, want - take, by);
+                    if (n >= kInOrder)
+                        break;
+                    take += n;
+                }
+                take = std::min(take, room);
+            }
+            if (a.n == kPieces || take <= 0) {
                 launch();
                 continue;
             }
             const int n = std::min(left, (pos / kPage + take) * kPage - pos);
-            a.piece[a.n++] = {runs[r].slot, pos, n, tok, a.n_pages};
-            std::copy_n(pages.begin() + at, take, a.pages + a.n_pages);
+            a.piece[a.n++] = {runs[r].slot, pos, n, tok, a.n_pages, listed ? a.n_listed : pages[at], step};
+            if (listed) {
+                std::copy_n(pages.begin() + at, take, a.pages + a.n_listed);
+                a.n_listed += take;
+            }
             a.n_pages += take;
             at += take;
             pos += n;

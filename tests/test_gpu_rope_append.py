@@ -202,6 +202,41 @@ def test_many_runs_and_pages(be, kind, lens):
     same(state(pool), state(by_hand))
 
 
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("mix", [False, True])
+def test_pages_apart_and_in_a_row(be, kind, mix):
+    """600 pages of which no two follow one another, past what one launch lists; or
+    stretches of such and of others, up and down."""
+    rng = np.random.default_rng(9)
+    kvh, hd, per = 1, 64, 600
+    pool = make(be, kind, 4, kvh, hd, per)
+    row = torch.zeros(2 * per * PAGE, kvh, hd, device="cuda")
+    stretch = [1] * per if not mix else [1, 2, 15, 16, 17, 40, 1, 1, 300, 3, 1, 20, 16]
+    at = 0
+    for n in stretch:
+        c = min(n, per - at) * PAGE
+        if c:
+            be.rope_append(pool, [(0, at * PAGE, c), (1, at * PAGE, c)], row[:2 * c], row[:2 * c])
+            at += c // PAGE
+    pool.reset(0)
+    n = at * PAGE - 5
+    k, v = (rows_of(rng, n + 30, kvh, hd, False).cuda() for _ in range(2))
+    be.rope_append(pool, [(2, 0, 30), (0, 0, n)], k, v)
+    steps = np.diff(pool.layer_pages(0))
+    assert ((np.abs(steps) == 1).sum() > 4) == mix
+    other = make(be, kind, 2, kvh, hd, per)
+    other.append(0, k[30:].reshape(n, -1), v[30:].reshape(n, -1), 0)
+    other.append(1, k[:30].reshape(30, -1), v[:30].reshape(30, -1), 0)
+    for a, b, m in ((0, 0, n), (2, 1, 30)):
+        x, y = held_rows(pool, a, m), held_rows(other, b, m)
+        for name in x:
+            assert (x[name] == y[name]).all(), name
+    x, y = state(pool), state(other)
+    assert (x["page_table"].reshape(4, per) == x["host_table"].reshape(4, per)).all()
+    assert (x["page_hash"].reshape(4, per)[0][:n // PAGE] == y["page_hash"].reshape(2, per)[0][:n // PAGE]).all()
+    assert (x["ntok"][pool.layer_pages(0)] == y["ntok"][other.layer_pages(0)]).all()
+
+
 def test_views_positions_and_in_place(be):
     """q, k and v as views of one product, queries in place and into another view, and
     angles that are not the places', far and negative ones (no rotation) among them."""

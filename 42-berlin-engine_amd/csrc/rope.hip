@@ -59,7 +59,9 @@ __device__ __forceinline__ int piece_of(const A &a, int at)
     return __popcll(__ballot(lane < a.n && a.piece[min(lane, kPieces - 1)].page0 <= at)) - 1;
 }
 
-// The page table's and the page's words, by the workgroup of KV head 0.
+// The page table's and the page's words, by the workgroup of KV head 0.  A launch may hold
+// several pieces of one run, whose ends are not the run's, and their workgroups are here
+// at once: the slot's counts grow by atomic maxima, which leave the run's in any order.
 __device__ __forceinline__ void publish(const be42_kv_pool &P, int slot, int pos0, int n, int blk, int phys, bool fresh)
 {
     const int end = pos0 + n;
@@ -67,12 +69,12 @@ __device__ __forceinline__ void publish(const be42_kv_pool &P, int slot, int pos
         P.page_table[(size_t)slot * P.max_logical + blk] = phys;
         // (a replay may come after appends behind the captured ones)
         if (end <= (blk + 1) * kPage)
-            P.n_logical[slot] = max(P.n_logical[slot], blk + 1);
+            atomicMax(&P.n_logical[slot], blk + 1);
     }
     P.ntok[phys] = min(end - blk * kPage, kPage);
     // the last page that the piece fills
-    if (end >= (blk + 1) * kPage && end < (blk + 2) * kPage && blk + 1 > P.n_indexed[slot])
-        P.n_indexed[slot] = blk + 1;
+    if (end >= (blk + 1) * kPage && end < (blk + 2) * kPage)
+        atomicMax(&P.n_indexed[slot], blk + 1);
 }
 
 // seal_page of a page whose rows the workgroup has just written, the same sums in the

@@ -1,0 +1,82 @@
+"""What an append leaves of its slots' counts (pages in use, pages with a hash, tokens
+of a page) where a launch holds a run in several pieces: pages that follow one another
+by the first, the others listed."""
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_rope_append import PAGE, held_rows, make, rows_of, same, state
+
+pytestmark = pytest.mark.gpu
+
+
+def append_both(be, rng, pool, by_hand, runs):
+    """The same tokens by one call, and by be42_kv_append of each run."""
+    n, kvh, hd = sum(r[2] for r in runs), pool.n_kv, pool.head_dim
+    k, v = (rows_of(rng, n, kvh, hd, False).cuda() for _ in range(2))
+    be.rope_append(pool, runs, k, v)
+    at = 0
+    for slot, p0, c in runs:
+        by_hand.append(slot, k[at:at + c].reshape(c, -1), v[at:at + c].reshape(c, -1), p0)
+        at += c
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("hd", [64, 40])
+@pytest.mark.parametrize("first,then", [(5, 16 * 40), (500, 3000), (17, 16 * 16 + 3), (31, 1 + 16 * 20)])
+def test_runs_that_go_on_from_inside_a_page(be, kind, hd, first, then):
+    """An old page and 16 or more new ones: everything that the pool holds is what
+    be42_kv_append leaves."""
+    rng = np.random.default_rng(first)
+    pool, by_hand = (make(be, kind, 6, 2, hd, -(-(first + then) // PAGE)) for _ in range(2))
+    append_both(be, rng, pool, by_hand, [(s, 0, first) for s in range(6)])
+    same(state(pool), state(by_hand))
+    append_both(be, rng, pool, by_hand, [(s, first, then) for s in (3, 0, 5, 1)])
+    a = state(pool)
+    assert list(a["n_logical"]) == list(a["length"])
+    assert list(a["n_indexed"]) == [(first + then) // PAGE if s in (3, 0, 5, 1) else first // PAGE for s in range(6)]
+    same(a, state(by_hand))
+
+
+def apart(be, kind, hd, per, stretch):
+    """A pool of which the pages that it gives out next lie in such stretches (slot 0
+    had them), the ones between held by slot 1."""
+    pool = make(be, kind, 4, 1, hd, per)
+    row = torch.zeros(2 * per * PAGE, 1, hd, device="cuda")
+    at = 0
+    for n in stretch:
+        c = min(n, per - at) * PAGE
+        if c:
+            be.rope_append(pool, [(0, at * PAGE, c), (1, at * PAGE, c)], row[:2 * c], row[:2 * c])
+            at += c // PAGE
+    pool.reset(0)
+    return pool, at
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("stretch", [[1] * 560, [3, 40, 1], [1, 2, 15, 16, 17, 40, 1, 1, 300, 3, 1, 20, 16], [20, 1, 1, 30, 1, 16, 2, 16]])
+@pytest.mark.parametrize("first", [0, 5])
+def test_pages_of_all_orders(be, kind, stretch, first):
+    """Runs from a page's begin and from inside one, over pages apart (more than a
+    launch lists) and in a row."""
+    rng = np.random.default_rng(len(stretch) + first)
+    hd, per = 64, sum(stretch) + 8
+    pool, pages = apart(be, kind, hd, per, stretch)
+    n = pages * PAGE - 11
+    other = make(be, kind, 4, 1, hd, per)
+    if first:
+        append_both(be, rng, pool, other, [(0, 0, first), (2, 0, 3)])
+    append_both(be, rng, pool, other, [(2, 3 if first else 0, 30), (0, first, n - first)])
+    a, b = state(pool), state(other)
+    assert (a["page_table"] == a["host_table"]).all()
+    lens = [n, pages * PAGE, 33 if first else 30, 0]
+    assert list(a["n_logical"]) == list(a["length"]) == [-(-m // PAGE) for m in lens]
+    assert list(a["n_indexed"]) == [m // PAGE for m in lens]
+    for slot in (0, 2):
+        m, at, bt = lens[slot], pool.layer_pages(slot), other.layer_pages(slot)
+        assert (a["ntok"][at] == b["ntok"][bt]).all()
+        assert (a["page_hash"].reshape(4, per)[slot][:m // PAGE] == b["page_hash"].reshape(4, per)[slot][:m // PAGE]).all()
+        assert (a["centroid"][at[:m // PAGE]] == b["centroid"][bt[:m // PAGE]]).all()
+        x, y = held_rows(pool, slot, m), held_rows(other, slot, m)
+        for name in x:
+            assert (x[name] == y[name]).all(), name

@@ -67,10 +67,12 @@ __device__ __forceinline__ void publish(const be42_kv_pool &P, int slot, int pos
     const int end = pos0 + n;
     if (fresh) {
         P.page_table[(size_t)slot * P.max_logical + blk] = phys;
-        // (a replay may come after appends behind the captured ones)
+        // (a replay may come after appends behind the captured ones, whose pages stay)
         if (end <= (blk + 1) * kPage)
             atomicMax(&P.n_logical[slot], blk + 1);
     }
+    // the page ends with what was written last, as be42_kv_append leaves it: a call at
+    // earlier positions, and a replay like it, takes the page's later tokens off
     P.ntok[phys] = min(end - blk * kPage, kPage);
     // the last page that the piece fills
     if (end >= (blk + 1) * kPage && end < (blk + 2) * kPage)

@@ -263,8 +263,11 @@ int  be42_kv_append_step(be42_kv_pool *pool, const int *slots, const int *pos, i
  * be42_kv_append stores fp32 rows.  A page whose last position is written gets its
  * centroid and hash, also where it had some.  q NULL: no queries (n_heads 0).  A
  * token whose row holds an infinity or NaN gets unspecified q and page rows; others
- * are not touched by it.  Captured, it writes the pages that it found or took at the
- * capture, which its slots keep: none of them is reset between replays.  On an error
+ * are not touched by it.  The page of a run's last token ends with it, as be42_kv_append
+ * leaves it: a call at positions before others of its page takes those off (append them
+ * again); the slot's pages behind it stay.  Captured, it writes the pages that it found
+ * or took at the capture, which its slots keep: none of them is reset between replays.
+ * A replay leaves what a call at the captured positions would leave then.  On an error
  * nothing was appended. */
 typedef struct be42_kv_run {
     int slot, pos0, count;

@@ -80,3 +80,42 @@ def test_pages_of_all_orders(be, kind, stretch, first):
         x, y = held_rows(pool, slot, m), held_rows(other, slot, m)
         for name in x:
             assert (x[name] == y[name]).all(), name
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("later", [3, 12, 20, 60])
+def test_a_replay_leaves_what_the_call_leaves(be, kind, later):
+    """Behind later appends: pages past the captured positions stay, the page of the last
+    captured token ends with it, in a replay as in a call."""
+    rng = np.random.default_rng(later)
+    k, more = (rows_of(rng, n, 1, 64, False).cuda() for n in (40, later))
+    pools = [make(be, kind, 4, 1, 64, 8) for _ in range(2)]
+    for pool in pools:
+        be.rope_append(pool, [(0, 0, 20), (1, 0, 10)], k[:30], k[:30])
+
+    def step(pool):
+        be.rope_append(pool, [(2, 0, 20), (0, 20, 5)], k[:25], k[:25])
+        be.kv_accept(pool, [(0, 1, 10, 10)], range(10))
+
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step(pools[0])
+    for i in range(3):
+        if i == 1:
+            for pool in pools:
+                for slot, n in ((0, 25), (1, 20), (2, 20)):
+                    be.rope_append(pool, [(slot, n, later)], more, more)
+        k.copy_(rows_of(rng, 40, 1, 64, False))
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        step(pools[1])
+        a = state(pools[0])
+        same(a, state(pools[1]))
+        for slot, n in ((0, 25), (1, 20), (2, 20)):
+            table, held = a["page_table"].reshape(4, 8)[slot], n + (later if i else 0)
+            ntok = [a["ntok"][p] for p in table[:-(-held // PAGE)]]
+            want = [min(PAGE, held - PAGE * j) for j in range(len(ntok))]
+            want[(n - 1) // PAGE] = (n - 1) % PAGE + 1
+            assert ntok == want and a["n_logical"][slot] == len(want) and a["n_indexed"][slot] == held // PAGE

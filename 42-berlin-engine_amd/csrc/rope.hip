@@ -40,8 +40,9 @@ struct RopeIn {
     int n_heads, rope_len, rope_dim, interleaved;
     float eps;
 };
-// (arguments of a kernel are at most 4 KB)
-static_assert(sizeof(be42_kv_pool) + sizeof(RopeArgs) + sizeof(RopeIn) <= 4096 - 16, "arguments of a launch");
+// (arguments of a kernel are at most 4 KB, with the padding between them)
+constexpr size_t kMostArgs = 4096 - 16;
+static_assert(sizeof(be42_kv_pool) + sizeof(RopeArgs) + sizeof(RopeIn) <= kMostArgs, "arguments of a launch");
 
 // The entry of page j of a piece: its physical page, and kNewPage.
 __device__ __forceinline__ int page_entry(const RopeArgs &a, const Piece &p, int j)
@@ -438,7 +439,7 @@ __global__ __launch_bounds__(256) void k_rope_append(const be42_kv_pool P, const
 // to take.  Pages that are old in every layer are looked up in the page tables; the
 // others are listed, layer after layer (a page for every one of 28 layers x 25 pages
 // would take two launches).
-constexpr int kTakes = 64, kTaken = 256, kTakePages = 352;
+constexpr int kTakes = 64, kTaken = 248, kTakePages = 352;
 struct TakeArgs {
     int n, n_pages, n_listed, layer0, from_step, to_step;
     struct {
@@ -449,6 +450,8 @@ struct TakeArgs {
     int index[kTaken];
     int pages[kTakePages];
 };
+static_assert(sizeof(be42_kv_pool) + sizeof(TakeArgs) <= kMostArgs, "arguments of a launch");
+static_assert(kTaken <= 16 * kPage, "at most 17 pages of a piece");
 
 template <bool KV8>
 __global__ __launch_bounds__(256) void k_kv_accept(const be42_kv_pool P, const TakeArgs a)

@@ -119,3 +119,33 @@ def test_a_replay_leaves_what_the_call_leaves(be, kind, later):
             want = [min(PAGE, held - PAGE * j) for j in range(len(ntok))]
             want[(n - 1) // PAGE] = (n - 1) % PAGE + 1
             assert ntok == want and a["n_logical"][slot] == len(want) and a["n_indexed"][slot] == held // PAGE
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("counts", [[248], [249], [265], [240, 8], [240, 9, 30], [3] * 64, [4] * 65, [100, 200, 300]])
+@pytest.mark.parametrize("first", [15, 16])
+def test_accepts_past_what_a_launch_takes(be, kind, counts, first):
+    """248 tokens or 64 runs: rows, counts and seals of every slot."""
+    rng = np.random.default_rng(len(counts) + first)
+    n, batch = sum(counts), len(counts)
+    pages = -(-(max(n, max(counts) + first)) // PAGE)
+    pool = make(be, kind, batch + 1, 1, 64, pages)
+    k = rows_of(rng, n + batch * first, 1, 64, False).cuda()
+    be.rope_append(pool, [(s, 0, first) for s in range(batch)] + [(batch, 0, n)], k, k)
+    index = rng.permutation(n)
+    src = held_rows(pool, batch, n)
+    be.kv_accept(pool, [(batch, s, first, c) for s, c in enumerate(counts)], index)
+    a, at = state(pool), 0
+    for s, c in enumerate(counts):
+        got = held_rows(pool, s, first + c)
+        for name in got:
+            assert (got[name][first:] == src[name][torch.from_numpy(index[at:at + c]).cuda()]).all(), (s, name)
+        at += c
+        assert a["n_logical"][s] == a["length"][s] == -(-(first + c) // PAGE) and a["n_indexed"][s] == (first + c) // PAGE
+        table = a["page_table"].reshape(-1, pages)[s]
+        assert [a["ntok"][p] for p in table[:a["length"][s]]] == [min(PAGE, first + c - PAGE * j) for j in range(a["length"][s])]
+        rows = got["k"].double() * (got["k_scale"].double()[..., None] if kind == "int8" else 1.0)
+        for j in range((first + c) // PAGE):
+            x = rows[PAGE * j:PAGE * j + PAGE, 0].cpu().numpy()
+            # sixteen products and fifteen sums, each half a step of at most the sum of sizes
+            assert (np.abs(a["centroid"][table[j]] - x.mean(0)) <= 31 * 2.0 ** -24 * np.abs(x).mean(0)).all()

@@ -562,7 +562,7 @@ static int rope_append(be42_kv_pool *pool, const be42_kv_run *runs, int n_runs, 
             const bool listed = take < kInOrder;
             if (listed) {
                 // up to where some follow one another, as many as the launch has room for
-                const int room = std::min(want, kPiecePages - a.n_listed);
+                const int room = std::min({want, kPiecePages - a.n_listed, kMaxBlocks - a.n_pages});
                 for (step = 0; take < room;) {
                     int by;
                     const int n = in_order(at + take, want - take, by);

@@ -149,3 +149,22 @@ def test_accepts_past_what_a_launch_takes(be, kind, counts, first):
             x = rows[PAGE * j:PAGE * j + PAGE, 0].cpu().numpy()
             # sixteen products and fifteen sums, each half a step of at most the sum of sizes
             assert (np.abs(a["centroid"][table[j]] - x.mean(0)) <= 31 * 2.0 ** -24 * np.abs(x).mean(0)).all()
+
+
+def test_more_pages_than_a_grid_holds(be):
+    """2^24 - 1 pages in a row, and three more, which go into another launch."""
+    most = (1 << 24) - 1
+    n, hd = most * PAGE, 8
+    pool = make(be, "int8", 2, 1, hd, most)
+    t = pool.tensors()
+    k = torch.zeros(n + 40, 1, hd, dtype=torch.bfloat16, device="cuda")
+    for i in (0, 5, n - 1, n, n + 39):
+        k[i] = 1.0 + i % 7
+    be.rope_append(pool, [(0, 0, n), (1, 0, 40)], k, k)
+    assert list(pool.fetch("n_logical", 2, np.int32)) == [most, 3] and list(pool.fetch("n_indexed", 2, np.int32)) == [most, 2]
+    pages = [pool.layer_pages(s) for s in range(2)]
+    for i in (0, 5, 6, n - 1, n, n + 1, n + 39):
+        page, off = pages[int(i >= n)][i % n // PAGE], i % n % PAGE
+        want = k[i, 0].float()
+        assert (t["k"][page, 0, off] == (127 if float(want[0]) else 0)).all()
+        assert float(t["k_scale"][page, 0, off]) == (np.float32(want[0].item()) / np.float32(127) if float(want[0]) else 1.0)

@@ -579,11 +579,7 @@ __global__ __launch_bounds__(512) void k_block_few(void *__restrict__ Y, const v
                 const float mine = r ? c : a;                   // the token of the lane's column
                 s[i] *= mine > 0.0f ? mine / 224.0f : 1.0f;
                 const float e[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-                uint32_t code = 0;
-#pragma unroll
-                for (int d = 0; d < 4; d++)
-                    code |= (uint32_t)finite_to_fp8(e[d] * inv) << (8 * d);
-                own[wave][i][lane >> 5][lane & 31] = code;
+                own[wave][i][lane >> 5][lane & 31] = scaled_to_fp8(e, inv);
             }
             // (the wave's own: what it wrote is there once its writes are)
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");

@@ -57,4 +57,24 @@ __device__ __forceinline__ uint8_t finite_to_fp8(float v)
     return (uint8_t)(a == 0.0f ? 0u : c | (__float_as_uint(v) >> 24 & 0x80u));
 }
 
+// f32_to_fp8's code of NaN: what a row's zeros become where 1 / scale is infinite (its
+// largest magnitude is above 0, but below 224 * 2^-128).
+constexpr uint32_t kFp8OfNan = 0x78;
+
+// Codes of four elements e times inv = 1 / scale, as f32_to_fp8 of the products gives them
+// for finite e.
+__device__ __forceinline__ uint32_t scaled_to_fp8(const float *e, float inv)
+{
+    uint32_t code = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        code |= (uint32_t)finite_to_fp8(e[j] * inv) << (8 * j);
+    if (inv == INFINITY)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (e[j] == 0.0f)
+                code = (code & ~(0xFFu << (8 * j))) | kFp8OfNan << (8 * j);
+    return code;
+}
+
 }  // namespace be42

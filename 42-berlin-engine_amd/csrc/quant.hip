@@ -186,10 +186,10 @@ __global__ __launch_bounds__(256) void k_quant_blocks(uint8_t *__restrict__ q, f
     const float scale = m > 0.0f ? m / 224.0f : 1.0f, inv = m > 0.0f ? 1.0f / scale : 1.0f;
     if (threadIdx.x % L == 0)
         scales[at] = scale;
-    uint32_t code[VE / 4] = {};
+    uint32_t code[VE / 4];
 #pragma unroll
-    for (int j = 0; j < VE; j++)
-        code[j / 4] |= (uint32_t)finite_to_fp8(v[j] * inv) << (8 * (j % 4));
+    for (int j = 0; j < VE / 4; j++)
+        code[j] = scaled_to_fp8(v + 4 * j, inv);
     uint8_t *to = q + row * cols + c0;
     if constexpr (WORDS) {
         if (c0 < cols)

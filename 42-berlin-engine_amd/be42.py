@@ -635,7 +635,9 @@ class Lib:
         """A dense int32 array of host integers, [n] or [n][cols], and its address."""
         import numpy as np
         if not (isinstance(x, np.ndarray) and x.dtype == np.int32 and x.flags.c_contiguous):
-            a = np.asarray(x, np.int64)
+            a = np.asarray(x)
+            if a.size and a.dtype.kind not in "iu":     # (truth values and fractions would be cut to integers)
+                raise Be42Error(f"{name}: {what} of type {a.dtype}")
             if a.size and (a.min() < -(1 << 31) or a.max() >= 1 << 31):
                 raise Be42Error(f"{name}: {what} past 32 bits")
             x = np.ascontiguousarray(a, np.int32)

@@ -449,6 +449,9 @@ class Lib:
         """Y [m][n] (float32 or bfloat16) = codes xq [m][k] with scales sx
         [m][k / 128] x codes wq [n][k] with scales sw [n / 128][k / 128], the
         last blocks short where 128 does not divide (quant_blocks_fp8).
+        bfloat16 outputs of more than 16 tokens are formed by the 8-bit matrix
+        instructions, which cut small products beside large ones
+        (include/be42_hip.h); float32 ones are not.
         workspace: be42_gemm_fp8_block_workspace_bytes bytes (uint8) to use
         instead of a new tensor."""
         t, name = self.torch, "be42_gemm_fp8_block"

@@ -44,9 +44,15 @@ union Codes {
     uint2 d[4];
 };
 
-// One 16x16 tile's sum over a block: the 8-bit instruction takes all 128 at once; for
-// exact sums four bf16 ones take the lane's codes eight at a time (either operand's
-// the same way, so that equal k meet).
+// One 16x16 tile's sum over a block.  The 8-bit instruction takes all 128 at once, at
+// twice the bf16 rate (4096 x 14336 x 4096 to bf16 275 us); it aligns the products of
+// eight elements to the largest's power of two and cuts each towards zero below 2^-13
+// of it, then adds the eights in fp32 (seen with codes of single bits, the same for any
+// eight).  A bf16 output keeps 8 bits: for normal values 1.5% of the outputs become a
+// neighbouring one and the relative error against 64 bits is 1.65763e-3, with exact sums
+// 1.65756e-3; large terms that cancel leave more of it.  fp32 outputs take four bf16
+// instructions of the lane's codes eight at a time (either operand's the same way, so
+// that equal k meet), in which products are exact and sums fp32.
 struct Wide {
     bf16x8 v[4];
 };

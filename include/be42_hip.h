@@ -173,9 +173,14 @@ int    be42_gemm_prepared_multi(const be42_gemv_seg *segs, int nseg, const void 
  * [n][k] with scales sw [ceil(n / 128)][blocks], one for 128 x 128, blocks =
  * ceil(k / 128); the last block of either may be short.
  *   y[m][n] = sum_b sx[m][b] * sw[n / 128][b] * sum_{k in block b} xq[m][k] * wq[n][k]
- * y [m][n] is fp32, or bf16 with y_bf16.  Sums are fp32; for fp32 outputs the codes
- * go through the bf16 matrix cores (exact), for bf16 ones through the 8-bit ones,
- * whose sums keep about 16 bits.  Codes are E4M3 (bias 7); 0x7F and 0xFF, which the
+ * y [m][n] is fp32, or bf16 with y_bf16.  Sums are fp32.  For fp32 outputs the codes
+ * go through the bf16 matrix cores, which lose nothing of a product (nor do up to 16
+ * tokens' bf16 outputs).  For bf16 outputs of more they go through the 8-bit ones, at
+ * twice the rate: of the products of eight elements (k = 8 i .. 8 i + 7) each is cut
+ * towards zero below 2^-13 of the largest's power of two before they are added, so that
+ * y is off by less than 7 * 2^-13 of the largest of each eight, added up (1.5e-5 of
+ * itself for normal values), before it is rounded.  Who needs bf16 outputs of sums
+ * without that takes fp32 outputs and rounds them.  Codes are E4M3 (bias 7); 0x7F and 0xFF, which the
  * codecs never give, are NaN.  k % 16 == 0, at most 2^22; xq, wq and y 16-byte aligned.
  * A NaN or an infinity among the scales reaches the outputs of its rows (or features)
  * only.  workspace NULL: the library's (grow-only; refused while the stream is

@@ -45,7 +45,7 @@ union Codes {
 };
 
 // One 16x16 tile's sum over a block.  The 8-bit instruction takes all 128 at once, at
-// twice the bf16 rate (4096 x 14336 x 4096 to bf16 275 us); it aligns the products of
+// twice the bf16 rate (4096 x 14336 x 4096 to bf16 272 us); it aligns the products of
 // eight elements to the largest's power of two and cuts each towards zero below 2^-13
 // of it, then adds the eights in fp32 (seen with codes of single bits, the same for any
 // eight).  A bf16 output keeps 8 bits: for normal values 1.5% of the outputs become a
@@ -706,8 +706,8 @@ struct Plan {
 // 10.7, in one 13.2; 261 x 2064 x 14352 30.9 in 3 parts of 64 x 128, 52.6 in one of 64 x
 // 64, 67.5 in 2 of 128 x 128; 512 x 4096 x 4096 19.4, 26.4 in 128 x 128; 1024 30.0 in
 // deep 128 x 128, 34.9 in 64 x 128; 2048 x 14336 x 4096 141 in 256 x 256, 168 in 128 x
-// 128; 8192^3 532, 648; 4096 x 14336 x 4096 282, with the codes, in three rounds of 256 x
-// 256 and 2048 features in 128 x 128, all in 256 x 256 293.)
+// 128; 8192^3 532, 648; 4096 x 14336 x 4096 272, with the codes, in three rounds of 256 x
+// 256 and 2048 features in 128 x 128, all in 256 x 256 283.)
 static Plan plan_block(long m, long n, long k, bool yb)
 {
     const long blocks = (k + kBlock - 1) / kBlock;
